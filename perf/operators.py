@@ -276,12 +276,13 @@ def _rotate(x, rope, pos):
 
 
 def _quantise(x, store):
-    top, a = _TOP[store], x.abs().amax(-1, keepdim=True)
+    a = x.abs().amax(-1, keepdim=True)
+    top = torch.full_like(a, _TOP[store])  # a division by a number would be a product with its inverse
     y = torch.where(a < _TINY, 0.0, x * (top / a))
     scale = torch.where(a < _TINY, 0.0, a / top)[..., 0]
     if store == "int8":
-        return y.round().clamp(-top, top).to(torch.int8), scale
-    return y.clamp(-top, top).to(torch.float8_e4m3fn), scale
+        return y.round().clamp(-127, 127).to(torch.int8), scale
+    return y.clamp(-448, 448).to(torch.float8_e4m3fn), scale
 
 
 def _put(s, seq, pos):
