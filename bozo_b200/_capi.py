@@ -17,8 +17,10 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib",
 
 OK = 0
 ERR_SCRATCH_LIMIT = 9
+ERR_DEVICE_INDEX = 10
 NOALLOC_SCRATCH_BYTES = 8 << 20  # BOZO_NOALLOC_SCRATCH_BYTES
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
+DT_F8E4M3, DT_I8 = 3, 4  # paged-cache rows only
 MODE_LOCAL, MODE_GLOBAL = 0, 1
 NORM_NONE, NORM_MASS, NORM_COUNT = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05 = 0, 1, 2
@@ -37,6 +39,7 @@ EXPORTED = (
     "bozo_tension_error_async", "bozo_tension_wait_selftest", "bozo_tension_fwd_needs_lp",
     "bozo_wo_add_rmsnorm_fwd", "bozo_wo_add_rmsnorm_supported",
     "bozo_embedding_bwd",
+    "bozo_paged_write", "bozo_paged_read", "bozo_paged_decode", "bozo_paged_decode_workspace",
 )
 TAU_AUX_MAX_LAYERS = 64  # BOZO_TAU_AUX_MAX_LAYERS
 
@@ -89,6 +92,43 @@ class DecodeArgs(C.Structure):
         ("v_cache", C.c_void_p), ("v_cache_dtype", C.c_int32),
         ("out", C.c_void_p), ("out_dtype", C.c_int32),
         ("tau", C.c_void_p), ("tau_dtype", C.c_int32),
+    ]
+
+
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p), ("dtype", C.c_int32), ("pages", C.c_int32),
+        ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("HD", C.c_int32),
+        ("batch", C.c_int32), ("width", C.c_int32), ("_pad", C.c_int32),
+        ("table", C.c_void_p), ("table_stride", C.c_int64), ("lengths", C.c_void_p),
+    ]
+
+
+class PagedWriteArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("rows", C.c_int64), ("cu_rows", C.c_void_p),
+        ("rope_len", C.c_int32), ("_pad", C.c_int32), ("rope_cos", C.c_void_p),
+        ("rope_sin", C.c_void_p), ("k", Tensor4), ("v", Tensor4),
+    ]
+
+
+class PagedReadArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("rows", C.c_int64), ("cu_rows", C.c_void_p),
+        ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("out_dtype", C.c_int32),
+        ("_pad", C.c_int32),
+    ]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache), ("H", C.c_int32), ("mode", C.c_int32), ("window", C.c_int32),
+        ("normalize", C.c_int32), ("tau_width", C.c_int32), ("scale", C.c_float),
+        ("rope_len", C.c_int32), ("_pad", C.c_int32), ("rope_cos", C.c_void_p),
+        ("rope_sin", C.c_void_p), ("q", Tensor4), ("k", Tensor4), ("v", Tensor4),
+        ("out", C.c_void_p), ("tau", C.c_void_p), ("out_dtype", C.c_int32),
+        ("tau_dtype", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -205,6 +245,14 @@ def lib():
                 L.bozo_graph_bias_build.restype = C.c_int
                 L.bozo_tension_decode.argtypes = [C.POINTER(DecodeArgs), C.c_void_p]
                 L.bozo_tension_decode.restype = C.c_int
+                L.bozo_paged_write.argtypes = [C.POINTER(PagedWriteArgs), C.c_void_p]
+                L.bozo_paged_write.restype = C.c_int
+                L.bozo_paged_read.argtypes = [C.POINTER(PagedReadArgs), C.c_void_p]
+                L.bozo_paged_read.restype = C.c_int
+                L.bozo_paged_decode.argtypes = [C.POINTER(PagedDecodeArgs), C.c_void_p]
+                L.bozo_paged_decode.restype = C.c_int
+                L.bozo_paged_decode_workspace.argtypes = [C.POINTER(PagedDecodeArgs)]
+                L.bozo_paged_decode_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_workspace.argtypes = [C.POINTER(TauAuxFwdArgs)]
                 L.bozo_tau_aux_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_fwd.argtypes = [C.POINTER(TauAuxFwdArgs), C.c_void_p]

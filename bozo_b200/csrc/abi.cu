@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "paged.cuh"
 #include "tc.cuh"
 #include "tc_host.cuh"
 
@@ -172,6 +173,8 @@ const char* bozo_status_string(int s) {
     case BOZO_ERR_WORKSPACE: return "workspace missing or too small";
     case BOZO_ERR_SCRATCH_LIMIT:
       return "problem needs more than the fixed 8 MiB no-alloc scratch; use bozo_tension_bwd";
+    case BOZO_ERR_DEVICE_INDEX:
+      return "a paged-cache kernel skipped a position outside the RoPE tables or a page outside the pool";
     default: return "unknown status";
   }
 }
@@ -497,6 +500,147 @@ int bozo_tension_decode(const bozo_tension_decode_args* a, void* stream) {
   return BOZO_OK;
 }
 
+static int check_paged(const bozo_paged_cache& c) {
+  if (c.pages <= 0 || c.kv_heads <= 0 || c.page_size <= 0 || c.HD <= 0 || c.batch <= 0 ||
+      c.width <= 0 || c.table_stride < 0)
+    return BOZO_ERR_BAD_SHAPE;
+  const bool eight = c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
+  if (!eight && !dtype_ok(c.dtype)) return BOZO_ERR_BAD_DTYPE;
+  if (c.HD > 128) return BOZO_ERR_UNSUPPORTED;
+  // rows are numbered in 32 bits, and so are a sequence's positions
+  if ((double)c.pages * c.kv_heads * c.page_size >= 4294967295.0 ||
+      (long long)c.width * c.page_size > 0x7fffffffLL)
+    return BOZO_ERR_UNSUPPORTED;
+  if (!c.k_pages || !c.v_pages || !c.table || !c.lengths) return BOZO_ERR_NULL;
+  if (eight && (!c.k_scale || !c.v_scale)) return BOZO_ERR_NULL;
+  if (!eight && (c.k_scale || c.v_scale)) return BOZO_ERR_BAD_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages)) & 15)
+    return BOZO_ERR_ALIGNMENT;
+  return BOZO_OK;
+}
+
+static int check_rope(int len, const float* cos, const float* sin, int HD) {
+  if (len < 0) return BOZO_ERR_BAD_SHAPE;
+  if (len == 0) return BOZO_OK;
+  if (!cos || !sin) return BOZO_ERR_NULL;
+  return HD % 2 ? BOZO_ERR_UNSUPPORTED : BOZO_OK;
+}
+
+int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
+  if (!a) return BOZO_ERR_NULL;
+  int st;
+  if ((st = check_paged(a->cache))) return st;
+  if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
+    return BOZO_ERR_BAD_SHAPE;
+  if ((st = check_rope(a->rope_len, a->rope_cos, a->rope_sin, a->cache.HD))) return st;
+  if (a->rows == 0) return BOZO_OK;
+  if ((st = check_t4(a->k)) || (st = check_t4(a->v))) return st;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  PagedP p = paged_params(a->cache);
+  p.rows = a->rows; p.cu = a->cu_rows;
+  p.rope_len = a->rope_len;
+  p.cos = a->rope_len ? a->rope_cos : nullptr;
+  p.sin = a->rope_len ? a->rope_sin : nullptr;
+  p.kn = dev_t4(a->k); p.vn = dev_t4(a->v);
+  if (!(p.err = error_word(&e))) return cuda_fail(e);
+  e = launch_paged_write(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = 1;
+  return BOZO_OK;
+}
+
+int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
+  if (!a) return BOZO_ERR_NULL;
+  int st;
+  if ((st = check_paged(a->cache))) return st;
+  if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
+    return BOZO_ERR_BAD_SHAPE;
+  if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
+  if (a->rows == 0) return BOZO_OK;
+  if (!a->k_out || !a->v_out) return BOZO_ERR_NULL;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  PagedP p = paged_params(a->cache);
+  p.rows = a->rows; p.cu = a->cu_rows;
+  p.k_out = a->k_out; p.v_out = a->v_out; p.out_dt = a->out_dtype;
+  if (!(p.err = error_word(&e))) return cuda_fail(e);
+  e = launch_paged_read(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = 1;
+  return BOZO_OK;
+}
+
+// The decode step's parameters (no device needed): checks first.
+static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
+  if (!a) return BOZO_ERR_NULL;
+  int st;
+  if ((st = check_paged(a->cache))) return st;
+  const bozo_paged_cache& c = a->cache;
+  if (a->H <= 0 || a->H % c.kv_heads) return BOZO_ERR_BAD_SHAPE;
+  if ((long long)c.batch * a->H > 0x7fffffffLL / 4096) return BOZO_ERR_UNSUPPORTED;
+  if (a->mode != BOZO_MODE_LOCAL && a->mode != BOZO_MODE_GLOBAL) return BOZO_ERR_BAD_SHAPE;
+  if (a->mode == BOZO_MODE_LOCAL &&
+      (a->window < 1 || (long long)c.width * c.page_size < (long long)a->window + 1))
+    return BOZO_ERR_BAD_SHAPE;
+  if (a->normalize != BOZO_NORM_NONE && a->normalize != BOZO_NORM_MASS &&
+      a->normalize != BOZO_NORM_COUNT)
+    return BOZO_ERR_BAD_SHAPE;
+  if (!(a->scale != 0.f)) return BOZO_ERR_BAD_SHAPE;
+  if ((st = check_rope(a->rope_len, a->rope_cos, a->rope_sin, c.HD))) return st;
+  if ((st = check_t4(a->q))) return st;
+  if ((a->k.ptr == nullptr) != (a->v.ptr == nullptr)) return BOZO_ERR_NULL;
+  if (a->k.ptr && ((st = check_t4(a->k)) || (st = check_t4(a->v)))) return st;
+  if (!a->out) return BOZO_ERR_NULL;
+  if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
+  if (a->tau && (!dtype_ok(a->tau_dtype) || a->tau_width < 1)) return BOZO_ERR_BAD_SHAPE;
+  if (a->mode == BOZO_MODE_LOCAL && a->tau && a->tau_width != a->window) return BOZO_ERR_BAD_SHAPE;
+  p = paged_params(c);
+  p.rows = c.batch;
+  p.rope_len = a->rope_len;
+  p.cos = a->rope_len ? a->rope_cos : nullptr;
+  p.sin = a->rope_len ? a->rope_sin : nullptr;
+  p.q = dev_t4(a->q); p.kn = dev_t4(a->k); p.vn = dev_t4(a->v);
+  p.H = a->H; p.mode = a->mode; p.W = a->mode == BOZO_MODE_LOCAL ? a->window : 0;
+  p.norm = a->normalize;
+  p.inv_scale = 1.0f / a->scale;
+  p.out = a->out; p.out_dt = a->out_dtype;
+  p.tau = a->tau; p.tau_dt = a->tau_dtype; p.tw = a->tau ? a->tau_width : 0;
+  return BOZO_OK;
+}
+
+size_t bozo_paged_decode_workspace(const bozo_paged_decode_args* a) {
+  PagedP p;
+  if (paged_decode_params(a, p) != BOZO_OK) return 0;
+  DeviceRestore restore;
+  if (bind_device(a->cache.k_pages, restore) != cudaSuccess) return 0;
+  return paged_decode_bytes(p, num_sms());
+}
+
+int bozo_paged_decode(const bozo_paged_decode_args* a, void* stream) {
+  PagedP p;
+  const int st = paged_decode_params(a, p);
+  if (st) return st;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  const size_t need = paged_decode_bytes(p, num_sms());
+  if (need && (!a->workspace || a->workspace_bytes < need)) return BOZO_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return BOZO_ERR_ALIGNMENT;
+  p.ws = static_cast<float*>(a->workspace);
+  if (!(p.err = error_word(&e))) return cuda_fail(e);
+  int launches = 0;
+  e = launch_paged_decode(p, num_sms(), static_cast<cudaStream_t>(stream), &launches);
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = launches;
+  return BOZO_OK;
+}
+
 int bozo_graph_bias_build(const bozo_graph_bias_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
   if (a->T <= 0 || a->window < 0 || a->n_edges < 0) return BOZO_ERR_BAD_SHAPE;
@@ -694,7 +838,7 @@ int bozo_tension_poll_error(void* stream) {
   if (v) {
     const int zero = 0;
     if (cudaMemcpy(ptr, &zero, sizeof(int), cudaMemcpyHostToDevice) != cudaSuccess) return BOZO_ERR_CUDA;
-    return BOZO_ERR_DEVICE_TIMEOUT;
+    return (v & ~0xff) == kErrPaged ? BOZO_ERR_DEVICE_INDEX : BOZO_ERR_DEVICE_TIMEOUT;
   }
   return BOZO_OK;
 }

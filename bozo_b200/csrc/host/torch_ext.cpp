@@ -257,6 +257,201 @@ std::vector<at::Tensor> tension_decode(const at::Tensor& q, const at::Tensor& k,
   return {out, tau};
 }
 
+// ── paged caches ──
+
+const at::Tensor* given(const c10::optional<at::Tensor>& t) {
+  return t && t->defined() ? &*t : nullptr;
+}
+
+// The cache argument block; every shape, type and device is checked here (the
+// C ABI sees pointers only).
+bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const at::Tensor& v_pages,
+                             const at::Tensor& table, const at::Tensor& lengths,
+                             const c10::optional<at::Tensor>& k_scale,
+                             const c10::optional<at::Tensor>& v_scale) {
+  auto bad = [&](const char* msg) { return std::invalid_argument(std::string(what) + ": " + msg); };
+  const auto dev = k_pages.device();
+  if (!dev.is_cuda())
+    throw std::runtime_error(std::string(what) + ": paged caches live on CUDA only (no CPU fallback)");
+  bozo_paged_cache c{};
+  switch (k_pages.scalar_type()) {
+    case at::kFloat8_e4m3fn: c.dtype = BOZO_DT_F8E4M3; break;
+    case at::kChar: c.dtype = BOZO_DT_I8; break;
+    default: c.dtype = dtype_code(k_pages.scalar_type());
+  }
+  if (k_pages.dim() != 4 || !k_pages.is_contiguous() || !v_pages.is_contiguous() ||
+      v_pages.sizes() != k_pages.sizes() || v_pages.scalar_type() != k_pages.scalar_type() ||
+      v_pages.device() != dev)
+    throw bad("k_pages and v_pages must be contiguous [pages, kv_heads, page_size, HD] tensors of one type and device");
+  if (table.dim() != 2 || table.scalar_type() != at::kInt || table.device() != dev ||
+      (table.size(1) > 1 && table.stride(1) != 1))
+    throw bad("page_table must be an int32 [B, width] tensor on the pages' device");
+  if (lengths.dim() != 1 || lengths.scalar_type() != at::kInt || lengths.device() != dev ||
+      lengths.size(0) != table.size(0) || !lengths.is_contiguous())
+    throw bad("lengths must be an int32 [B] tensor on the pages' device");
+  const at::Tensor* sc[2] = {given(k_scale), given(v_scale)};
+  const bool eight = c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
+  for (const at::Tensor* t : sc) {
+    if (eight != (t != nullptr))
+      throw bad("k_scale and v_scale go with 8-bit pages, and only with them");
+    if (t && (t->scalar_type() != at::kFloat || t->device() != dev || !t->is_contiguous() ||
+              t->sizes() != k_pages.sizes().slice(0, 3)))
+      throw bad("scales must be contiguous float32 [pages, kv_heads, page_size] tensors on the pages' device");
+  }
+  c.k_pages = k_pages.data_ptr();
+  c.v_pages = v_pages.data_ptr();
+  if (eight) {
+    c.k_scale = sc[0]->data_ptr<float>();
+    c.v_scale = sc[1]->data_ptr<float>();
+  }
+  if (k_pages.size(0) > INT32_MAX || table.size(1) > INT32_MAX) throw bad("too many pages");
+  c.pages = (int32_t)k_pages.size(0);
+  c.kv_heads = (int32_t)k_pages.size(1);
+  c.page_size = (int32_t)k_pages.size(2);
+  c.HD = (int32_t)k_pages.size(3);
+  c.batch = (int32_t)table.size(0);
+  c.width = (int32_t)table.size(1);
+  c.table = table.data_ptr<int32_t>();
+  c.table_stride = table.stride(0);
+  c.lengths = lengths.data_ptr<int32_t>();
+  return c;
+}
+
+// [rows, heads, HD] (any strides) as the ABI's [rows, 1, heads, HD] view
+bozo_tensor4 rows_view(const char* what, const char* name, const at::Tensor& t, const bozo_paged_cache& c,
+                       int64_t rows, int64_t heads, const at::Device& dev) {
+  if (t.dim() != 3 || t.size(0) != rows || t.size(1) != heads || t.size(2) != c.HD || t.device() != dev)
+    throw std::invalid_argument(std::string(what) + ": " + name + " must be a [" + std::to_string(rows) +
+                                ", " + std::to_string(heads) + ", " + std::to_string(c.HD) +
+                                "] tensor on the pages' device");
+  bozo_tensor4 s{};
+  s.ptr = t.data_ptr();
+  s.dtype = dtype_code(t.scalar_type());
+  s.stride[0] = t.stride(0);
+  s.stride[2] = t.stride(1);
+  s.stride[3] = t.stride(2);
+  return s;
+}
+
+const int32_t* rows_of(const char* what, const at::Tensor* cu, const bozo_paged_cache& c, int64_t rows,
+                       const at::Device& dev) {
+  if (!cu) {
+    if (rows != c.batch)
+      throw std::invalid_argument(std::string(what) + ": without cu_rows there is one row a sequence");
+    return nullptr;
+  }
+  if (cu->dim() != 1 || cu->scalar_type() != at::kInt || cu->size(0) != c.batch + 1 ||
+      cu->device() != dev || !cu->is_contiguous())
+    throw std::invalid_argument(std::string(what) + ": cu_rows must be an int32 [B + 1] tensor on the pages' device");
+  return cu->data_ptr<int32_t>();
+}
+
+template <typename A>
+void rope_of(const char* what, A& a, const at::Tensor* cos, const at::Tensor* sin, const bozo_paged_cache& c,
+             const at::Device& dev) {
+  if (!cos) return;
+  for (const at::Tensor* t : {cos, sin})
+    if (!t || t->dim() != 2 || t->size(0) != cos->size(0) || t->size(1) * 2 != c.HD ||
+        t->scalar_type() != at::kFloat || t->device() != dev || !t->is_contiguous())
+      throw std::invalid_argument(std::string(what) + ": rope must be float32 (cos, sin) tables [length, HD/2] on the pages' device");
+  a.rope_len = (int32_t)cos->size(0);
+  a.rope_cos = cos->data_ptr<float>();
+  a.rope_sin = sin->data_ptr<float>();
+}
+
+void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_pages,
+                 const at::Tensor& v_pages, const at::Tensor& table, const at::Tensor& lengths,
+                 const c10::optional<at::Tensor>& cu_rows, const c10::optional<at::Tensor>& cos,
+                 const c10::optional<at::Tensor>& sin, const c10::optional<at::Tensor>& k_scale,
+                 const c10::optional<at::Tensor>& v_scale) {
+  const char* what = "write_kv";
+  bozo_paged_write_args a{};
+  a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  const auto dev = k_pages.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  a.rows = k.size(0);
+  a.k = rows_view(what, "k", k, a.cache, a.rows, a.cache.kv_heads, dev);
+  a.v = rows_view(what, "v", v, a.cache, a.rows, a.cache.kv_heads, dev);
+  a.cu_rows = rows_of(what, given(cu_rows), a.cache, a.rows, dev);
+  rope_of(what, a, given(cos), given(sin), a.cache, dev);
+  check(bozo_paged_write(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_write");
+}
+
+std::vector<at::Tensor> paged_read(const at::Tensor& k_pages, const at::Tensor& v_pages,
+                                   const at::Tensor& table, const at::Tensor& lengths,
+                                   const c10::optional<at::Tensor>& cu_rows, int64_t rows,
+                                   const c10::optional<at::Tensor>& k_scale,
+                                   const c10::optional<at::Tensor>& v_scale, int64_t out_dtype) {
+  const char* what = "read_kv";
+  bozo_paged_read_args a{};
+  a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  const auto dev = k_pages.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  if (rows < 0) throw std::invalid_argument("read_kv: rows must not be negative");
+  a.rows = rows;
+  a.cu_rows = rows_of(what, given(cu_rows), a.cache, rows, dev);
+  auto opts = k_pages.options().dtype(scalar_type(out_dtype));
+  at::Tensor k = at::empty({rows, a.cache.kv_heads, a.cache.HD}, opts), v = at::empty_like(k);
+  a.k_out = k.data_ptr();
+  a.v_out = v.data_ptr();
+  a.out_dtype = (int32_t)out_dtype;
+  check(bozo_paged_read(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_read");
+  return {k, v};
+}
+
+// Returns [out [B, H, HD], tau [B, H, tau_width] (undefined unless tau_width > 0)] in q's dtype.
+std::vector<at::Tensor> paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
+                                     const at::Tensor& v_pages, const at::Tensor& table,
+                                     const at::Tensor& lengths, int64_t mode, int64_t window,
+                                     int64_t norm, double scale, const c10::optional<at::Tensor>& cos,
+                                     const c10::optional<at::Tensor>& sin,
+                                     const c10::optional<at::Tensor>& k,
+                                     const c10::optional<at::Tensor>& v,
+                                     const c10::optional<at::Tensor>& k_scale,
+                                     const c10::optional<at::Tensor>& v_scale, int64_t tau_width) {
+  const char* what = "paged_tension";
+  bozo_paged_decode_args a{};
+  a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  const auto dev = k_pages.device();
+  const c10::cuda::CUDAGuard guard(dev);
+  const int64_t B = a.cache.batch, H = q.dim() == 3 ? q.size(1) : 0;
+  if (H <= 0 || H % a.cache.kv_heads)
+    throw std::invalid_argument("paged_tension: q must be [B, H, HD] with H a multiple of the pages' heads");
+  if (window < 0 || window > INT32_MAX || tau_width < 0 || tau_width > INT32_MAX ||
+      (mode == BOZO_MODE_LOCAL && (int64_t)a.cache.width * a.cache.page_size < window + 1))
+    throw std::invalid_argument("paged_tension: a window of W needs a page table of at least W + 1 positions");
+  a.q = rows_view(what, "q", q, a.cache, B, H, dev);
+  const at::Tensor *nk = given(k), *nv = given(v);
+  if ((nk == nullptr) != (nv == nullptr))
+    throw std::invalid_argument("paged_tension: k and v go together");
+  if (nk) {
+    a.k = rows_view(what, "k", *nk, a.cache, B, a.cache.kv_heads, dev);
+    a.v = rows_view(what, "v", *nv, a.cache, B, a.cache.kv_heads, dev);
+  }
+  rope_of(what, a, given(cos), given(sin), a.cache, dev);
+  a.H = (int32_t)H;
+  a.mode = (int32_t)mode;
+  a.window = (int32_t)window;
+  a.normalize = (int32_t)norm;
+  a.scale = (float)scale;
+  a.tau_width = (int32_t)tau_width;
+  a.out_dtype = a.tau_dtype = a.q.dtype;
+  at::Tensor out = at::empty({B, H, (int64_t)a.cache.HD}, q.options()), tau, ws;
+  a.out = out.data_ptr();
+  if (tau_width > 0) {
+    tau = at::empty({B, H, tau_width}, q.options());
+    a.tau = tau.data_ptr();
+  }
+  const size_t bytes = bozo_paged_decode_workspace(&a);
+  if (bytes) {
+    ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  check(bozo_paged_decode(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_decode");
+  return {out, tau};
+}
+
 // Graph bias [T, W] (window > 0) or [T, T] (window 0) from the context's
 // content ids and the sorted edge table; stats [3] (pairs, Σ weight, max)
 // as float64.  Returns [bias, stats].
@@ -585,6 +780,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tension_fwd", &tension_fwd, "forward through bozo_tension_fwd");
   m.def("tension_bwd", &tension_bwd, "backward through bozo_tension_bwd");
   m.def("tension_decode", &tension_decode, "one decode step through bozo_tension_decode");
+  m.def("paged_write", &paged_write, "rows into a paged cache through bozo_paged_write");
+  m.def("paged_read", &paged_read, "rows of a paged cache through bozo_paged_read");
+  m.def("paged_decode", &paged_decode, "one decode step over a paged cache through bozo_paged_decode");
   m.def("graph_bias", &graph_bias, "graph bias through bozo_graph_bias_build");
   m.def("add_rmsnorm_fwd", &add_rmsnorm_fwd, "residual add + RMSNorm through bozo_add_rmsnorm_fwd");
   m.def("add_rmsnorm_bwd", &add_rmsnorm_bwd, "its backward through bozo_add_rmsnorm_bwd");

@@ -52,8 +52,11 @@ typedef enum {
   BOZO_ERR_DEVICE_TIMEOUT = 6, /* a bounded device-side wait gave up */
   BOZO_ERR_CUDA = 7,           /* a CUDA runtime call failed */
   BOZO_ERR_WORKSPACE = 8,      /* workspace NULL or smaller than required */
-  BOZO_ERR_SCRATCH_LIMIT = 9   /* bozo_tension_bwd_noalloc: problem needs more
+  BOZO_ERR_SCRATCH_LIMIT = 9,  /* bozo_tension_bwd_noalloc: problem needs more
                                   than BOZO_NOALLOC_SCRATCH_BYTES of scratch */
+  BOZO_ERR_DEVICE_INDEX = 10   /* a paged-cache kernel met a position outside the
+                                  RoPE tables or a page outside the pool and
+                                  skipped it (bozo_tension_poll_error) */
 } bozo_status;
 
 /* Size of the library's fixed device scratch array used by
@@ -61,6 +64,9 @@ typedef enum {
 #define BOZO_NOALLOC_SCRATCH_BYTES (8u << 20)
 
 typedef enum { BOZO_DT_F32 = 0, BOZO_DT_BF16 = 1, BOZO_DT_F16 = 2 } bozo_dtype;
+/* Types of paged-cache rows beside the bozo_dtype ones: 8-bit codes with one
+ * fp32 scale a row (the row stands for code · scale). */
+enum { BOZO_DT_F8E4M3 = 3, BOZO_DT_I8 = 4 };
 typedef enum { BOZO_MODE_LOCAL = 0, BOZO_MODE_GLOBAL = 1 } bozo_mode;
 typedef enum { BOZO_NORM_NONE = 0, BOZO_NORM_MASS = 1, BOZO_NORM_COUNT = 2 } bozo_norm;
 
@@ -200,6 +206,103 @@ typedef struct {
  * forward. */
 int bozo_tension_decode(const bozo_tension_decode_args* args, void* stream);
 
+/* ── paged caches ──
+ * Keys and values of many sequences of different lengths in pages of a shared
+ * pool, each sequence at a position of its own.  A row is one token's key (or
+ * value) of one head: HD elements of `dtype`; the rows of a (page, head) are
+ * contiguous.  Position s of sequence b lies in page
+ *     table[b][(s mod C) / page_size], row s mod page_size,  C = width·page_size,
+ * so a table narrower than a sequence is a ring that keeps its last C tokens
+ * (a local layer needs C ≥ W + 1).  Keys are held RoPE-rotated.
+ *
+ * 8-bit rows (BOZO_DT_F8E4M3, BOZO_DT_I8) have a scale each: with a = max |x|
+ * over the row and top = 448 (e4m3) or 127, scale = a / top and
+ * code = round(x · (top / a)), ties to even (the scale is held down where
+ * top · scale would overflow); a row with a < 2^-100 is held as zeros (scale
+ * 0), a row with an infinity or a NaN as zeros with scale NaN, so that
+ * everything read from it is NaN.
+ *
+ * lengths[b] < 0 marks an inactive sequence: its rows are not written, and its
+ * outputs are zeros.  A position outside the RoPE tables or a needed page
+ * outside [0, pages) is skipped (rows unwritten, values read as zeros, keys
+ * left out) and sets the device error word (BOZO_ERR_DEVICE_INDEX from
+ * bozo_tension_poll_error).  No counterpart in the reference, whose
+ * generate_cached (model.py:718-768) keeps no keys. */
+typedef struct {
+  void* k_pages;          /* [pages, kv_heads, page_size, HD] contiguous, 16-byte aligned */
+  void* v_pages;
+  float* k_scale;         /* [pages, kv_heads, page_size] for 8-bit rows, else NULL */
+  float* v_scale;
+  int32_t dtype;          /* bozo_dtype, BOZO_DT_F8E4M3 or BOZO_DT_I8 */
+  int32_t pages, kv_heads, page_size, HD;
+  int32_t batch;          /* sequences B */
+  int32_t width;          /* pages of a sequence in the table */
+  int32_t _pad;
+  const int32_t* table;   /* [B, width] page numbers, rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* lengths; /* [B] device: position of each sequence's first new token */
+} bozo_paged_cache;
+
+/* Write new tokens' keys (rotated) and values.  Rows n with
+ * cu_rows[b] ≤ n < cu_rows[b+1] are sequence b's tokens at positions
+ * lengths[b] + n − cu_rows[b]; rows from cu_rows[B] on are padding.  Of more
+ * than C tokens of one sequence the last C are written.  cu_rows NULL: one row
+ * a sequence (rows = B).  `lengths` is not advanced. */
+typedef struct {
+  bozo_paged_cache cache;
+  int64_t rows;
+  const int32_t* cu_rows; /* [B+1] device, non-decreasing from 0, or NULL */
+  int32_t rope_len;       /* rows of the RoPE tables or 0 for no RoPE */
+  int32_t _pad;
+  const float* rope_cos;  /* [rope_len, HD/2] fp32 contiguous, or NULL */
+  const float* rope_sin;
+  bozo_tensor4 k, v;      /* [rows, 1, kv_heads, HD] views */
+} bozo_paged_write_args;
+int bozo_paged_write(const bozo_paged_write_args* args, void* stream);
+
+/* Read rows back: out row n of sequence b is position lengths[b] + n −
+ * cu_rows[b] (as for writing; padding rows come out as zeros), code · scale
+ * rounded once to out_dtype. */
+typedef struct {
+  bozo_paged_cache cache;
+  int64_t rows;
+  const int32_t* cu_rows;
+  void* k_out;            /* [rows, kv_heads, HD] contiguous */
+  void* v_out;
+  int32_t out_dtype;
+  int32_t _pad;
+} bozo_paged_read_args;
+int bozo_paged_read(const bozo_paged_read_args* args, void* stream);
+
+/* One decode step over a paged cache: bozo_tension_decode with t = lengths[b]
+ * per sequence, H query heads over kv_heads key heads (H a multiple; query
+ * head h reads key head h / (H / kv_heads)).  With k and v given the new
+ * token's row is written first (as bozo_paged_write does); without them
+ * (ptr NULL) a GLOBAL step expects it in the cache already.
+ *   LOCAL : keys s ∈ [max(0, t−W), t−1];  GLOBAL: s ∈ [max(0, t−C+1), t].
+ * Long rows are split over blocks, and their partial sums joined in a fixed
+ * order (the same bits on every call) from `workspace`. */
+typedef struct {
+  bozo_paged_cache cache;
+  int32_t H;
+  int32_t mode, window, normalize; /* as in bozo_tension_decode_args */
+  int32_t tau_width;
+  float scale;            /* divisor of the dot product */
+  int32_t rope_len;
+  int32_t _pad;
+  const float* rope_cos;
+  const float* rope_sin;
+  bozo_tensor4 q;         /* [B, 1, H, HD] view */
+  bozo_tensor4 k, v;      /* [B, 1, kv_heads, HD] views, or ptr NULL */
+  void* out;              /* [B, H, HD] contiguous */
+  void* tau;              /* [B, H, tau_width] contiguous, or NULL */
+  int32_t out_dtype, tau_dtype;
+  void* workspace;        /* bozo_paged_decode_workspace() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} bozo_paged_decode_args;
+size_t bozo_paged_decode_workspace(const bozo_paged_decode_args* args);
+int bozo_paged_decode(const bozo_paged_decode_args* args, void* stream);
+
 /* 1 when this forward, given q_lp / k_lp, runs on the tensor-core kernels
  * from bf16 copies of fp32 q and k: the reference's mixed-dtype call
  * (model.py:248-264 under bf16 autocast — RoPE-promoted fp32 Q/K, bf16 V,
@@ -244,8 +347,9 @@ int bozo_tension_bwd(const bozo_tension_bwd_args* args, void* stream);
 int bozo_tension_bwd_noalloc(const bozo_tension_bwd_args* args, void* stream);
 
 /* Synchronise `stream`, then read and clear the device error word that
- * bounded waits inside the tensor-core kernels set when they give up.
- * Returns BOZO_OK or BOZO_ERR_DEVICE_TIMEOUT (or BOZO_ERR_CUDA). */
+ * bounded waits inside the tensor-core kernels set when they give up (and the
+ * paged-cache kernels when they skip an index out of range).  Returns BOZO_OK,
+ * BOZO_ERR_DEVICE_TIMEOUT or BOZO_ERR_DEVICE_INDEX (or BOZO_ERR_CUDA). */
 int bozo_tension_poll_error(void* stream);
 
 /* Enqueue on `stream` an asynchronous copy of the device error word of the
