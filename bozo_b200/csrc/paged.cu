@@ -13,8 +13,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ unsigned warp_max(unsigned v) { return __reduce_max_sync(0xffffffffu, v); }
-
 // One warp per (row, head): any head width, types and strides.
 __global__ void __launch_bounds__(kThreads) paged_write_any(PagedP p) {
   const int lane = threadIdx.x & 31;
@@ -31,46 +29,9 @@ __global__ void __launch_bounds__(kThreads) paged_write_any(PagedP p) {
   }
   const unsigned row0 = paged_row(p, b, pos);
   if (row0 == kNoRow) return;
-  const size_t row = row0 + (size_t)h * p.page, at = row * p.HD;
-  const int HD = p.HD, half = HD / 2;
-  const long long ko = n * p.kn.sb + h * p.kn.sh, vo = n * p.vn.sb + h * p.vn.sh;
-  const float* c = p.cos + (size_t)pos * half;
-  const float* s = p.sin + (size_t)pos * half;
-  auto key = [&](int d) {
-    const float x = ldf(p.kn.p, ko + d * p.kn.sd, p.kn.dt);
-    if (!p.cos) return x;
-    if (d < half) {
-      const float y = ldf(p.kn.p, ko + (d + half) * p.kn.sd, p.kn.dt);
-      return __fsub_rn(__fmul_rn(x, c[d]), __fmul_rn(y, s[d]));
-    }
-    const float y = ldf(p.kn.p, ko + (d - half) * p.kn.sd, p.kn.dt);
-    return __fadd_rn(__fmul_rn(y, s[d - half]), __fmul_rn(x, c[d - half]));
-  };
-  auto val = [&](int d) { return ldf(p.vn.p, vo + d * p.vn.sd, p.vn.dt); };
-  if (p.dt <= BOZO_DT_F16) {
-    for (int d = lane; d < HD; d += 32) {
-      stf(p.k, (long long)(at + d), p.dt, key(d));
-      stf(p.v, (long long)(at + d), p.dt, val(d));
-    }
-    return;
-  }
-  const float top = p.dt == BOZO_DT_I8 ? 127.f : 448.f;
-  unsigned ka = 0, va = 0;
-  for (int d = lane; d < HD; d += 32) {
-    ka = max(ka, __float_as_uint(key(d)) & 0x7fffffffu);
-    va = max(va, __float_as_uint(val(d)) & 0x7fffffffu);
-  }
-  float ksc, kinv, vsc, vinv;
-  quant_scale(warp_max(ka), top, ksc, kinv);
-  quant_scale(warp_max(va), top, vsc, vinv);
-  for (int d = lane; d < HD; d += 32) {
-    static_cast<unsigned char*>(p.k)[at + d] = quant_code(key(d), kinv, p.dt);
-    static_cast<unsigned char*>(p.v)[at + d] = quant_code(val(d), vinv, p.dt);
-  }
-  if (lane == 0) {
-    p.ks[row] = ksc;
-    p.vs[row] = vsc;
-  }
+  const size_t row = row0 + (size_t)h * p.page;
+  put_row(p, p.kn, p.k, p.ks, n, h, pos, row, p.cos != nullptr, lane);
+  put_row(p, p.vn, p.v, p.vs, n, h, pos, row, false, lane);
 }
 
 // One warp per (row, head).
