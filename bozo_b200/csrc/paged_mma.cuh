@@ -1,0 +1,625 @@
+// paged_mma.cuh — the tensor-core kernel of a decode step over a paged cache:
+// 16- and 8-bit pages, head widths 32, 64 and 128.
+//
+// One block per (b, key head, up to 8 of its query heads, piece).  Each warp walks
+// tiles of its own through a ring in shared memory that 16-byte asynchronous
+// copies fill a few tiles ahead (rows out of reach are filled with zeros), and
+// feeds mma.m16n8k16 from it; nothing is shared between warps before the end.
+//   Sᵀ = K·Qᵀ  16 keys by 8 columns: a column is a query head's q rounded to 16
+//              bits or what that rounding left of it, side by side, so the sum
+//              of two neighbouring accumulators (in one lane) has q to 16 bits
+//              and more.  Up to 4 heads fit; where there are fewer, the columns
+//              repeat them and each group of lanes takes its scores from a tile
+//              of its own, so that every lane computes different τ.
+//   O  = P·V   rows 0-7 the heads' τ (· the value row's scale) in 16 bits, rows
+//              8-15 what that left; τ goes from lanes to operands through a few
+//              words of shared memory.
+// Scores, τ, both sums and what is joined are fp32.
+#pragma once
+
+#include <algorithm>
+
+#include "paged_decode.cuh"
+
+namespace bozo {
+namespace {
+
+template <int DT> struct Fmt;
+template <> struct Fmt<BOZO_DT_BF16> { static constexpr int size = 2; static constexpr bool bf = true, scaled = false; };
+template <> struct Fmt<BOZO_DT_F16> { static constexpr int size = 2; static constexpr bool bf = false, scaled = false; };
+template <> struct Fmt<BOZO_DT_F8E4M3> { static constexpr int size = 1; static constexpr bool bf = false, scaled = true; };
+template <> struct Fmt<BOZO_DT_I8> { static constexpr int size = 1; static constexpr bool bf = false, scaled = true; };
+
+template <bool BF>
+__device__ __forceinline__ void mma16816(float* d, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+  if constexpr (BF)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// x as a 16-bit number (high half) and what that left of it (low half)
+template <bool BF>
+__device__ __forceinline__ unsigned split(float x) {
+  unsigned w;
+  if constexpr (BF) {
+    unsigned h;  // bf16(x) in the high half is that number in fp32
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(x), "f"(0.f));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x), "f"(x - __uint_as_float(h)));
+  } else {
+    const float h = __half2float(__float2half_rn(x));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x), "f"(x - h));
+  }
+  return w;
+}
+
+// Four 8-bit codes as two pairs of halfs (exact).
+template <int DT>
+__device__ __forceinline__ void widen4(unsigned x, unsigned& p01, unsigned& p23) {
+  if constexpr (DT == BOZO_DT_F8E4M3) {
+    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x & 0xffffu), __NV_E4M3);
+    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x >> 16), __NV_E4M3);
+    p01 = *reinterpret_cast<const unsigned*>(&a);
+    p23 = *reinterpret_cast<const unsigned*>(&b);
+  } else {
+    // 1024 + (code + 128) is the half with those low bits; less 1152 it is the code
+    const unsigned u = x ^ 0x80808080u;
+    unsigned a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    p01 = *reinterpret_cast<const unsigned*>(&ha);
+    p23 = *reinterpret_cast<const unsigned*>(&hb);
+  }
+}
+
+// σ(z) from −z·log2 e: one exponential and one reciprocal, each with a relative
+// error of about 2^-22; results below 2^-126 are zero.
+__device__ __forceinline__ float sigmoid_exp2(float y) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return r;
+}
+
+__device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ uint4 lds128(unsigned a) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
+  return x;
+}
+__device__ __forceinline__ uint2 lds64(unsigned a) {
+  uint2 x;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(a) : "memory");
+  return x;
+}
+template <int N>  // N 32-bit words
+__device__ __forceinline__ void lds_words(unsigned a, unsigned* w) {
+  if constexpr (N == 4) {
+    const uint4 x = lds128(a);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (N == 2) {
+    const uint2 x = lds64(a);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
+  }
+}
+template <bool T>
+__device__ __forceinline__ void ldmatrix4(unsigned a, unsigned* w) {
+  if constexpr (T)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+}
+
+// Asynchronous copies to shared memory; `bytes` 0 fills with zeros.
+__device__ __forceinline__ void copy16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(unsigned dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_peer(unsigned addr, unsigned rank) {
+  unsigned a;
+  float x;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(a) : "memory");
+  return x;
+}
+
+constexpr int kWarps = 4;
+constexpr int kStages = 3;
+
+// Geometry of the kernel for one page type, head width and count of heads.
+template <int DT, int HD, int GP> struct Geo {
+  static constexpr int row = HD * Fmt<DT>::size;             // bytes of a row
+  static constexpr int keys = row >= 256 ? 16 : row >= 128 ? 32 : 64;  // keys of a tile of the ring
+  static constexpr int kv = keys * row;                      // bytes of its K (or V): 4 KB, 2 KB at 32-byte rows
+  static constexpr int scales = Fmt<DT>::scaled ? 2 * keys * 4 : 0;
+  static constexpr int meta = scales + 16;                   // scales, and 16 bits a 16 keys: which are in reach
+  static constexpr int pstride = keys + 8;                   // words of a head's τ
+  static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * 4;
+};
+
+// Byte offset of 16-byte piece ch of row r of a K or V tile with R-byte rows.  The
+// pieces of a 128-byte line are permuted so that reading is free of bank
+// conflicts: 16-bit rows are read as 8×8 matrices (8 rows' pieces of one number),
+// 8-bit K rows two at a time, 8-bit V rows four at a time in steps of two.
+template <int SIZE, int R, bool V> __device__ __forceinline__ int ring_at(int r, int ch) {
+  if constexpr (SIZE == 2) {
+    if constexpr (R >= 128) return r * R + ((ch ^ (r & 7)) << 4);
+    else return (r >> 1) * 128 + (((((r & 1) << 2) | ch) ^ ((r >> 1) & 3)) << 4);
+  } else if constexpr (R >= 128) {
+    return r * R + ((ch ^ (V ? ((r >> 1) & 3) << 1 : (r & 1) << 2)) << 4);
+  } else if constexpr (V) {
+    constexpr int per = 128 / R;  // rows of a line
+    const int line = r / per, c8 = (r % per) * (R / 16) + ch;
+    return line * 128 + ((c8 ^ (R == 64 ? (line & 3) << 1 : (line & 1) << 1)) << 4);
+  } else {
+    return r * R + (ch << 4);
+  }
+}
+
+template <int DT, int HD, int GP, bool AL>
+__global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S, int HG, bool clustered) {
+  using F = Fmt<DT>;
+  using Z = Geo<DT, HD, GP>;
+  constexpr bool BF = F::bf;
+  constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size;
+  constexpr int GQ = GP < 4 ? GP : 4, NS = GP == 8 ? 2 : 1;        // heads of an 8-column operand, operands
+  constexpr int T = GP == 8 ? 1 : (NT < 4 / GQ ? NT : 4 / GQ);     // 16-key tiles whose scores the lanes share out
+  constexpr int kSteps = HD / 16, kTiles = HD / 8;
+  // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
+  constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
+  constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB / 4;
+  extern __shared__ __align__(256) char smb[];
+  __shared__ float sq[kHeads][HD + 4];
+  __shared__ float sback[kHeads];  // what undoes the power of two that q was multiplied by (halfs)
+  __shared__ float smass[kWarps][kHeads];
+  const int G = p.H / p.Hk;
+  int x = blockIdx.x;
+  const int piece = x % S;
+  x /= S;
+  const int hg = x % HG;
+  x /= HG;
+  const int hk = x % p.Hk, b = x / p.Hk;
+  const int h0 = hk * G + hg * kHeads, Gh = min(kHeads, G - hg * kHeads);  // query heads h0 … h0+Gh−1
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const Reach rc = reach(p, b, S);
+  const bool mine = (unsigned)piece < rc.count;
+  if (!mine && !clustered) return;
+  const unsigned p0 = rc.first(piece), p1 = mine ? rc.last(piece) : p0;  // this block's positions
+  const unsigned nk = p1 > p0 ? p1 - p0 : 0u;
+  float mass[NS], unit[NS], lim[NS];  // P operand: p · unit, renewed where p passes lim (halfs)
+  float acc[kTiles][4];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) mass[s] = lim[s] = 0.f, unit[s] = 1.f;
+#pragma unroll
+  for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+
+  if (writes_row(p, rc, piece, hg == 0)) {
+    append_row(p, b, hk, rc.t, warp, lane);
+    __syncthreads();
+  }
+  const unsigned ring = smem_u32(smb) + warp * kStages * 2 * Z::kv;
+  char* meta = smb + kWarps * kStages * 2 * Z::kv + warp * kStages * Z::meta;
+  unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * kStages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
+  const char* kpages = static_cast<const char*>(p.k);
+  const char* vpages = static_cast<const char*>(p.v);
+  // Row numbers: AL (16 positions from a multiple of 16 on lie in one page): lane
+  // L looks up 16 keys, those of tile (batch + L / NT), part L % NT; else one key
+  // each of the next tile.
+  constexpr int RR = AL ? 1 : (KT > 32 ? KT / 32 : 1), kBatch = 32 / NT;
+  unsigned cur[RR], nxt[RR];
+  auto start = [&](int k) { return (unsigned)(warp + k * kWarps) * KT; };  // first key of the warp's tile k
+  auto find = [&](int k, unsigned* rows) {
+#pragma unroll
+    for (int r = 0; r < RR; ++r) {
+      const unsigned j = AL ? start(k + lane / NT) + lane % NT * 16 : start(k) + r * 32 + (KT < 32 ? lane % KT : lane);
+      rows[r] = kNoRow;
+      if (j < nk && (AL || p0 + j >= rc.lo)) {
+        const unsigned row = paged_row(p, b, p0 + j);
+        if (row != kNoRow) rows[r] = row + (unsigned)hk * p.page;
+      }
+    }
+  };
+  auto fill = [&](int slot, int k) {
+    const unsigned kd = ring + slot * 2 * Z::kv, vd = kd + Z::kv;
+    char* md = meta + slot * Z::meta;
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const int src = AL ? k % kBatch * NT + u : 0;
+      const unsigned row = AL ? __shfl_sync(0xffffffffu, cur[0], src) : 0u;
+      const unsigned pos = p0 + start(k) + u * 16;
+      // the row of key r of these 16, or kNoRow
+      auto row_of = [&](int r) {
+        if constexpr (AL) return row == kNoRow || pos + r < rc.lo || pos + r >= p1 ? kNoRow : row + r;
+        else return __shfl_sync(0xffffffffu, cur[u / 2], (u * 16 + r) % 32);
+      };
+      if (AL && row != kNoRow && pos >= rc.lo && pos + 16 <= p1) {
+        const size_t at = (size_t)row * R + lane * 16;
+        const char *ka = kpages + at, *va = vpages + at;
+#pragma unroll
+        for (int it = 0; it < (NCH + 1) / 2; ++it) {
+          const int r = u * 16 + (it * 32 + lane) / NCH, ch = lane % NCH;
+          copy16(kd + ring_at<SZ, R, false>(r, ch), ka + it * 512);
+          copy16(vd + ring_at<SZ, R, true>(r, ch), va + it * 512);
+        }
+        if (F::scaled) copy4(smem_u32(md) + (((lane >> 4) * KT + u * 16 + (lane & 15)) << 2),
+                             (lane < 16 ? p.ks : p.vs) + row + (lane & 15), 4);
+        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = 0xffffu;
+      } else {
+#pragma unroll
+        for (int it = 0; it < (NCH + 1) / 2; ++it) {
+          const int r = (it * 32 + lane) / NCH, ch = lane % NCH;
+          const unsigned rr = row_of(r);
+          const size_t at = rr == kNoRow ? 0 : (size_t)rr * R + ch * 16;
+          copy16(kd + ring_at<SZ, R, false>(u * 16 + r, ch), kpages + at, rr == kNoRow ? 0 : 16);
+          copy16(vd + ring_at<SZ, R, true>(u * 16 + r, ch), vpages + at, rr == kNoRow ? 0 : 16);
+        }
+        const unsigned rr = row_of(lane & 15);
+        if (F::scaled) copy4(smem_u32(md) + (((lane >> 4) * KT + u * 16 + (lane & 15)) << 2),
+                             (lane < 16 ? p.ks : p.vs) + (rr == kNoRow ? 0u : rr), rr == kNoRow ? 0 : 4);
+        const unsigned m = __ballot_sync(0xffffffffu, rr != kNoRow);
+        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = (unsigned short)m;
+      }
+    }
+  };
+  // Fills the ring with tile k, if there is one, and looks ahead for the next rows.
+  auto feed = [&](int slot, int k) {
+    if (start(k) < nk) fill(slot, k);
+    copy_commit();
+    if (!AL) {
+#pragma unroll
+      for (int r = 0; r < RR; ++r) cur[r] = nxt[r];
+      find(k + 2, nxt);
+    } else if ((k + 1) % kBatch == 0) {
+      cur[0] = nxt[0];
+      find(k + 1 + kBatch, nxt);
+    }
+  };
+  if (nk) {
+    find(0, cur);
+    find(AL ? kBatch : 1, nxt);
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
+  }
+  if (mine && rc.active)
+    for (int i = tid; i < GP * HD; i += kWarps * 32) {
+      const int h = i / HD, d = i - h * HD;
+      sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
+    }
+  __syncthreads();
+  if (nk) {
+    // columns of S: lane (g, c) holds k-pairs of column g, that is of head
+    // (g/2) mod GQ (of each operand), its 16-bit part (g even) or the rest
+    unsigned qb[NS][kSteps][2];
+    float back[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      const int h = s * 4 + (g >> 1) % GQ;
+      float qs = 1.f;
+      if constexpr (!BF) {  // as halfs, brought near 1 by a power of two
+        float m = 0.f;
+        for (int d = c; d < HD; d += 4) m = fmaxf(m, fabsf(sq[h][d]));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        const int e = m > 0.f ? min(126, max(-126, (int)(__float_as_uint(m) >> 23) - 127)) : 0;
+        qs = __uint_as_float((unsigned)(127 - e) << 23);
+        if (c == 0) sback[h] = __uint_as_float((unsigned)(127 + e) << 23);  // every warp the same
+      }
+      auto pair = [&](int d) {
+        const unsigned u = split<BF>(sq[h][d] * qs), v = split<BF>(sq[h][d + 1] * qs);
+        return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
+      };
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        if constexpr (SZ == 2) {
+          qb[s][k][0] = pair(16 * k + 2 * c);
+          qb[s][k][1] = pair(16 * k + 8 + 2 * c);
+        } else {
+          const int d = k / kKW * 4 * kKB + c * kKB + k % kKW * 4;
+          qb[s][k][0] = pair(d);
+          qb[s][k][1] = pair(d + 2);
+        }
+      }
+    }
+    __syncwarp();
+    // exponent of the sigmoid: −log2 e · score
+#pragma unroll
+    for (int s = 0; s < NS; ++s) back[s] = (BF ? 1.f : sback[s * 4 + c % GQ]) * p.inv_scale * -1.4426950408889634f;
+    const int tsel = c / GQ % T;  // the tile (of T) whose τ this lane computes
+    const int mrow = (lane & 7) + (lane & 8), mch = lane >> 4;  // row and piece of an 8×8 matrix's row
+
+    int slot = 0;
+#pragma unroll 1
+    for (int k = 0; start(k) < nk; ++k) {
+      copy_wait<kStages - 2>();
+      __syncwarp();
+      feed(slot == 0 ? kStages - 1 : slot - 1, k + kStages - 1);
+      const unsigned kt = ring + slot * 2 * Z::kv, vt = kt + Z::kv;
+      const char* md = meta + slot * Z::meta;
+      const float* sc = reinterpret_cast<const float*>(md);
+      slot = slot == kStages - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < NT / T; ++q) {
+        float s[T][NS][4];
+#pragma unroll
+        for (int u = 0; u < T; ++u) {
+#pragma unroll
+          for (int e = 0; e < NS; ++e) s[u][e][0] = s[u][e][1] = s[u][e][2] = s[u][e][3] = 0.f;
+          const int r0 = (q * T + u) * 16;
+          if constexpr (SZ == 2) {
+            const unsigned a = kt + ring_at<SZ, R, false>(r0 + mrow, mch);
+#pragma unroll
+            for (int st = 0; st < kSteps; ++st) {
+              unsigned w[4];
+              ldmatrix4<false>(a ^ (st << 5), w);
+#pragma unroll
+              for (int e = 0; e < NS; ++e) mma16816<BF>(s[u][e], w[0], w[1], w[2], w[3], qb[e][st][0], qb[e][st][1]);
+            }
+          } else {
+#pragma unroll
+            for (int l = 0; l < kKL; ++l) {
+              unsigned ka[kKW], kb[kKW];
+              const int byte = l * 4 * kKB + c * kKB;
+              lds_words<kKW>(kt + ring_at<SZ, R, false>(r0 + g, byte >> 4) + (byte & 15), ka);
+              lds_words<kKW>(kt + ring_at<SZ, R, false>(r0 + g + 8, byte >> 4) + (byte & 15), kb);
+#pragma unroll
+              for (int w = 0; w < kKW; ++w) {
+                unsigned a0, a1, a2, a3;
+                widen4<DT>(ka[w], a0, a2);
+                widen4<DT>(kb[w], a1, a3);
+#pragma unroll
+                for (int e = 0; e < NS; ++e)
+                  mma16816<BF>(s[u][e], a0, a1, a2, a3, qb[e][l * kKW + w][0], qb[e][l * kKW + w][1]);
+              }
+            }
+          }
+        }
+        // τ of the keys g, g + 8 of tile tsel and head c mod GQ of each operand
+        const int tile = q * T + tsel;
+        const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::scales)[tile] >> g;
+        float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+        if constexpr (F::scaled) {
+          ks[0] = sc[tile * 16 + g];
+          ks[1] = sc[tile * 16 + g + 8];
+          vs[0] = sc[KT + tile * 16 + g];
+          vs[1] = sc[KT + tile * 16 + g + 8];
+        }
+#pragma unroll
+        for (int e = 0; e < NS; ++e) {
+          float pr[2];
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            float z = s[0][e][2 * o] + s[0][e][2 * o + 1];
+#pragma unroll
+            for (int u = 1; u < T; ++u) z = tsel == u ? s[u][e][2 * o] + s[u][e][2 * o + 1] : z;
+            z *= back[e];
+            if constexpr (F::scaled) z *= ks[o];
+            const bool on = (live >> (8 * o)) & 1;
+            const float tau = on ? sigmoid_exp2(z) : 0.f;
+            mass[e] += tau;
+            if (p.tau && on && c / GQ < T && e * 4 + c % GQ < Gh)
+              put_tau(p, (size_t)b * p.H + h0 + e * 4 + c % GQ, rc.t, p0 + start(k) + tile * 16 + g + 8 * o, tau);
+            pr[o] = F::scaled ? tau * vs[o] : tau;
+          }
+          if constexpr (!BF) {
+            // halfs reach from 2^-24 to 65504: keep the largest p of a head between 1
+            // and 4096 by a power of two, what was summed before following it
+            const float pm = fmaxf(pr[0], pr[1]);
+            if (__any_sync(0xffffffffu, pm > lim[e])) {
+              float m = pm;
+#pragma unroll
+              for (int o = GQ; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+              float f = 1.f;
+              if (m > lim[e]) {
+                const int ex = min(113, max(-126, (int)(__float_as_uint(m) >> 23) - 127));
+                const float nu = __uint_as_float((unsigned)(127 - ex) << 23);
+                f = lim[e] == 0.f ? 0.f : nu / unit[e];
+                unit[e] = nu;
+                lim[e] = __uint_as_float((unsigned)(127 + ex + 12) << 23);
+              }
+              f = __shfl_sync(0xffffffffu, f, g % 4 % GQ);  // of this lane's row of O
+              if (g / 4 == e || GP <= 4) {
+#pragma unroll
+                for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) acc[j][i] *= f;
+              }
+            }
+            pr[0] *= unit[e];
+            pr[1] *= unit[e];
+          }
+          unsigned* pw = ps + (e * 4 + c % GQ) * Z::pstride + tile * 16 + g;
+          pw[0] = split<BF>(pr[0]);
+          pw[8] = split<BF>(pr[1]);
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0;
+        if (g < GP) {
+          const unsigned at = smem_u32(ps + g * Z::pstride + u * 16 + 2 * c);
+          const uint2 x = lds64(at), y = lds64(at + 32);
+          a0 = __byte_perm(x.x, x.y, 0x7632);
+          a1 = __byte_perm(x.x, x.y, 0x5410);
+          a2 = __byte_perm(y.x, y.y, 0x7632);
+          a3 = __byte_perm(y.x, y.y, 0x5410);
+        }
+        if constexpr (SZ == 2) {
+          const unsigned a = vt + ring_at<SZ, R, true>(u * 16 + mrow, mch);
+#pragma unroll
+          for (int j = 0; j < kTiles; j += 2) {
+            unsigned w[4];
+            ldmatrix4<true>(a ^ (j << 4), w);
+            mma16816<BF>(acc[j], a0, a1, a2, a3, w[0], w[1]);
+            mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
+          }
+        } else {
+#pragma unroll
+          for (int l = 0; l < kVL; ++l) {
+            unsigned vw[4][kVW];
+            const int byte = l * 8 * kVB + g * kVB;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              lds_words<kVW>(vt + ring_at<SZ, R, true>(u * 16 + 8 * (i >> 1) + 2 * c + (i & 1), byte >> 4) + (byte & 15),
+                             vw[i]);
+#pragma unroll
+            for (int w = 0; w < kVW; ++w)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const unsigned sel = i ? 0x7362 : 0x5140;  // two keys' codes side by side
+                unsigned x0, x1, y0, y1;
+                widen4<DT>(__byte_perm(vw[0][w], vw[1][w], sel), x0, x1);
+                widen4<DT>(__byte_perm(vw[2][w], vw[3][w], sel), y0, y1);
+                const int j = l * kVB + 4 * w + 2 * i;
+                mma16816<BF>(acc[j], a0, a1, a2, a3, x0, y0);
+                mma16816<BF>(acc[j + 1], a0, a1, a2, a3, x1, y1);
+              }
+          }
+        }
+      }
+    }
+    copy_wait<0>();
+  }
+
+  // the warps' sums, added in order
+  __syncthreads();  // the rings and the queries are done with
+  float* part = reinterpret_cast<float*>(smb);  // [warps][Gh][HD], then the block's [Gh][HD]
+#pragma unroll
+  for (int e = 0; e < NS; ++e) {
+    float m = c / GQ < T ? mass[e] : 0.f;
+#pragma unroll
+    for (int o = GQ; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+    if (lane < GQ) smass[warp][e * 4 + lane] = m;
+  }
+  float un = 1.f;  // of head g
+  if constexpr (!BF) {
+    un = __shfl_sync(0xffffffffu, unit[0], g % 4 % GQ);
+    if constexpr (NS == 2) {
+      const float u1 = __shfl_sync(0xffffffffu, unit[1], g % 4);
+      un = g < 4 ? un : u1;
+    }
+  }
+  if (g < Gh) {
+    const float back = 1.f / un;
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int d = SZ == 2 ? 8 * j + 2 * c + e : j / kVB * 8 * kVB + (2 * c + e) * kVB + j % kVB;
+        part[(warp * Gh + g) * HD + d] = (acc[j][e] + acc[j][2 + e]) * back;
+      }
+  }
+  __syncthreads();
+  float* sum = part + kWarps * Gh * HD;
+  for (int i = tid; i < Gh * HD; i += kWarps * 32) {
+    const int h = i / HD, d = i - h * HD;
+    float o = 0.f, m = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      o += part[w * Gh * HD + i];
+      m += smass[w][h];
+    }
+    const size_t bh = (size_t)b * p.H + h0 + h;
+    if (rc.count == 1) {
+      if (piece == 0) stf(p.out, (long long)(bh * HD + d), p.out_dt, o / norm_divisor(p, m, rc.n));
+    } else if (clustered) {
+      sum[i] = o;
+      if (d == 0) sq[0][h] = m;
+    } else {
+      p.ws[(bh * S + piece) * HD + d] = o;
+      if (d == 0) piece_mass(p, S)[bh * S + piece] = m;
+    }
+  }
+  if (p.tau && piece == 0)
+    for (int h = warp; h < Gh; h += kWarps) clear_tau(p, (size_t)b * p.H + h0 + h, rc.n, lane, 32);
+  if (clustered) {
+    // the pieces' sums through the cluster's shared memory, each block a part of
+    // the elements, in the order of the pieces
+    cluster_sync();
+    if (rc.count > 1)
+      for (int i = tid + piece * kWarps * 32; i < Gh * HD; i += S * kWarps * 32) {
+        const int h = i / HD, d = i - h * HD;
+        float o = 0.f, m = 0.f;
+        for (unsigned r = 0; r < rc.count; ++r) {
+          o += ld_peer(smem_u32(sum + i), r);
+          m += ld_peer(smem_u32(&sq[0][h]), r);
+        }
+        const size_t bh = (size_t)b * p.H + h0 + h;
+        stf(p.out, (long long)(bh * HD + d), p.out_dt, o / norm_divisor(p, m, rc.n));
+      }
+    cluster_sync();
+  }
+}
+
+template <int DT, int HD, int GP, bool AL>
+cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  const int G = p.H / p.Hk, HG = (G + kHeads - 1) / kHeads;
+  const size_t ring = (size_t)kWarps * Geo<DT, HD, GP>::warp;
+  const size_t part = (size_t)(kWarps + 1) * std::min(G, kHeads) * HD * sizeof(float);
+  const size_t smem = std::max(ring, part);
+  auto kern = paged_decode_mma<DT, HD, GP, AL>;
+  if (smem > 32 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hk * HG * pl.S));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {(unsigned)pl.S, 1, 1};
+  cfg.attrs = &at;
+  cfg.numAttrs = pl.clustered ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, p, pl.S, HG, pl.clustered);
+}
+template <int DT, int HD, int GP>
+cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  return p.page % 16 == 0 ? launch_paged_mma<DT, HD, GP, true>(p, pl, st)
+                          : launch_paged_mma<DT, HD, GP, false>(p, pl, st);
+}
+template <int DT, int HD>
+cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  const int G = p.H / p.Hk;
+  if (G == 1) return launch_paged_mma<DT, HD, 1>(p, pl, st);
+  if (G == 2) return launch_paged_mma<DT, HD, 2>(p, pl, st);
+  if (G <= 4) return launch_paged_mma<DT, HD, 4>(p, pl, st);
+  return launch_paged_mma<DT, HD, 8>(p, pl, st);
+}
+template <int DT>
+cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  switch (p.HD) {
+    case 32: return launch_paged_mma<DT, 32>(p, pl, st);
+    case 64: return launch_paged_mma<DT, 64>(p, pl, st);
+    default: return launch_paged_mma<DT, 128>(p, pl, st);
+  }
+}
+
+}  // namespace
+}  // namespace bozo
