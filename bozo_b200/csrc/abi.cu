@@ -545,7 +545,7 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   p.sin = a->rope_len ? a->rope_sin : nullptr;
   p.kn = dev_t4(a->k); p.vn = dev_t4(a->v);
   if (!(p.err = error_word(&e))) return cuda_fail(e);
-  e = launch_paged_write(p, static_cast<cudaStream_t>(stream));
+  e = launch_paged_write(p, num_sms(), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = BOZO_PATH_SIMT;
   t_last_launches = 1;
@@ -568,7 +568,7 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   p.rows = a->rows; p.cu = a->cu_rows;
   p.k_out = a->k_out; p.v_out = a->v_out; p.out_dt = a->out_dtype;
   if (!(p.err = error_word(&e))) return cuda_fail(e);
-  e = launch_paged_read(p, static_cast<cudaStream_t>(stream));
+  e = launch_paged_read(p, num_sms(), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = BOZO_PATH_SIMT;
   t_last_launches = 1;

@@ -60,10 +60,11 @@ __global__ void __launch_bounds__(kThreads) paged_read_any(PagedP p) {
 }
 
 // ─────────────── vector path: HD 32, 64, 128, unit element stride, aligned rows ───────────────
-// HD/8 lanes hold one row: of a key the dimensions 4l … 4l+3 and HD/2 + 4l …, so a
-// lane has both halves of its rotations, of a value 8l … 8l+7.  A group of lanes
-// takes NH heads of its token: their loads are in flight together and the
-// token's place is looked up once for all of them.
+// A block takes `rows` consecutive rows.  Their sequence is found by all its threads
+// at once (one of B compares holds), each row's place by one thread; then groups of
+// HD/16 lanes go through the heads' keys and values of one row, sixteen elements a
+// lane: dimensions 8l … 8l+7 of either half of the row, so a lane has both halves of
+// its rotations, whose cosines and sines it loads once for all heads.
 template <int DT> struct PageT;
 template <> struct PageT<BOZO_DT_F32> { using type = float; };
 template <> struct PageT<BOZO_DT_BF16> { using type = __nv_bfloat16; };
@@ -71,249 +72,327 @@ template <> struct PageT<BOZO_DT_F16> { using type = __half; };
 template <> struct PageT<BOZO_DT_F8E4M3> { using type = unsigned char; };
 template <> struct PageT<BOZO_DT_I8> { using type = unsigned char; };
 
-template <int BYTES> struct Bytes;
-template <> struct Bytes<4> { using type = unsigned; };
-template <> struct Bytes<8> { using type = uint2; };
-template <> struct Bytes<16> { using type = uint4; };
-
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
-__device__ __forceinline__ void from_f(float& y, float x) { y = x; }
-__device__ __forceinline__ void from_f(__nv_bfloat16& y, float x) { y = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void from_f(__half& y, float x) { y = __float2half_rn(x); }
-
-// N elements of type T, N·sizeof(T) bytes aligned to themselves (at most 16)
-template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack { T e[N]; };
-
-template <typename T, int N>
-__device__ __forceinline__ Pack<T, N> ld_pack(const T* p) {
-  Pack<T, N> x;
-  constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16;
-  using V = typename Bytes<B>::type;
+// Eight elements of type T: 8, 16 or 32 bytes, moved in pieces of up to 16.
+template <typename T> struct Eight {
+  static constexpr int words = 8 * sizeof(T) / 4;
+  unsigned w[words];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> ld8(const T* p) {
+  Eight<T> x;
+  if constexpr (sizeof(T) == 1) {
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+    x.w[0] = v.x; x.w[1] = v.y;
+  } else {
 #pragma unroll
-  for (int i = 0; i < (int)(N * sizeof(T)) / B; ++i)
-    reinterpret_cast<V*>(&x)[i] = __ldg(reinterpret_cast<const V*>(p) + i);
+    for (int i = 0; i < Eight<T>::words / 4; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      x.w[4 * i] = v.x; x.w[4 * i + 1] = v.y; x.w[4 * i + 2] = v.z; x.w[4 * i + 3] = v.w;
+    }
+  }
   return x;
 }
-template <typename T, int N>
-__device__ __forceinline__ void st_pack(T* p, const Pack<T, N>& x) {
-  constexpr int B = N * sizeof(T) < 16 ? N * sizeof(T) : 16;
-  using V = typename Bytes<B>::type;
+template <typename T>
+__device__ __forceinline__ void st8(T* p, const Eight<T>& x) {
+  if constexpr (sizeof(T) == 1) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(x.w[0], x.w[1]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < (int)(N * sizeof(T)) / B; ++i)
-    reinterpret_cast<V*>(p)[i] = reinterpret_cast<const V*>(&x)[i];
-}
-
-// N fp32 numbers as a page holds them (for codes: times inv; |x·inv| ≤ top up to
-// rounding, which no code passes)
-template <int DT, int N>
-__device__ __forceinline__ void st_page(typename PageT<DT>::type* p, const float* x, float inv) {
-  using T = typename PageT<DT>::type;
-  Pack<T, N> y;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    if constexpr (DT == BOZO_DT_F8E4M3 || DT == BOZO_DT_I8) y.e[i] = quant_code(x[i], inv, DT);
-    else from_f(y.e[i], x[i]);
+    for (int i = 0; i < Eight<T>::words / 4; ++i)
+      reinterpret_cast<uint4*>(p)[i] = make_uint4(x.w[4 * i], x.w[4 * i + 1], x.w[4 * i + 2], x.w[4 * i + 3]);
   }
-  st_pack(p, y);
 }
-
-template <int DT, typename I, int NH>
-__global__ void __launch_bounds__(kThreads) paged_write_vec(PagedP p, int lanes, FastDiv units) {
-  using T = typename PageT<DT>::type;
-  constexpr bool Q = DT == BOZO_DT_F8E4M3 || DT == BOZO_DT_I8;
-  const int L = 1 << lanes, l = threadIdx.x & (L - 1);
-  const unsigned nu = (unsigned)(p.Hk + NH - 1) / NH;  // units of a token
-  const unsigned g = (blockIdx.x * kThreads + threadIdx.x) >> lanes;
-  const unsigned n = fast_div(g, units);
-  const int h0 = (int)(g - n * nu) * NH;
-  int b = 0;
-  unsigned pos = 0, end = 0, row0 = kNoRow;
-  if (n < (unsigned)p.rows && paged_place(p, (int)n, b, pos, end) && !(end > p.cap && pos < end - p.cap)) {
-    if (p.cos && pos >= (unsigned)p.rope_len) {
-      if (l == 0) atomicCAS(p.err, 0, kErrPaged | 1);
+__device__ __forceinline__ void widen(const Eight<float>& x, float* y) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = __uint_as_float(x.w[i]);
+}
+__device__ __forceinline__ void widen(const Eight<__nv_bfloat16>& x, float* y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[2 * i] = __uint_as_float(x.w[i] << 16);
+    y[2 * i + 1] = __uint_as_float(x.w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void widen(const Eight<__half>& x, float* y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x.w[i]));
+    y[2 * i] = f.x;
+    y[2 * i + 1] = f.y;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void widen_codes(const Eight<unsigned char>& x, float* y) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (DT == BOZO_DT_F8E4M3) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x.w[i] >> (16 * j)), __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        y[4 * i + 2 * j] = f.x;
+        y[4 * i + 2 * j + 1] = f.y;
+      }
     } else {
-      row0 = paged_row(p, b, pos);
-    }
-  }
-  const bool live = row0 != kNoRow;
-  const int HD = L * 8, half = L * 4;
-  Pack<I, 4> ka[NH], kb[NH];
-  Pack<I, 8> va[NH];
-  float4 cs{}, sn{};
+      // 2^23 + (code + 128) has those low bits
+      const unsigned u = x.w[i] ^ 0x80808080u;
 #pragma unroll
-  for (int i = 0; i < NH; ++i)
-    if (live && h0 + i < p.Hk) {
-      const I* k = static_cast<const I*>(p.kn.p) + n * p.kn.sb + (h0 + i) * p.kn.sh;
-      const I* v = static_cast<const I*>(p.vn.p) + n * p.vn.sb + (h0 + i) * p.vn.sh;
-      ka[i] = ld_pack<I, 4>(k + 4 * l);
-      kb[i] = ld_pack<I, 4>(k + half + 4 * l);
-      va[i] = ld_pack<I, 8>(v + 8 * l);
-    }
-  if (live && p.cos) {
-    cs = __ldg(reinterpret_cast<const float4*>(p.cos + (size_t)pos * half) + l);
-    sn = __ldg(reinterpret_cast<const float4*>(p.sin + (size_t)pos * half) + l);
-  }
-  const float c[4] = {cs.x, cs.y, cs.z, cs.w}, s[4] = {sn.x, sn.y, sn.z, sn.w};
-#pragma unroll
-  for (int i = 0; i < NH; ++i) {
-    const bool on = live && h0 + i < p.Hk;
-    float k[8], v[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = to_f(ka[i].e[e]), y = to_f(kb[i].e[e]);
-      k[e] = p.cos ? __fsub_rn(__fmul_rn(x, c[e]), __fmul_rn(y, s[e])) : x;
-      k[4 + e] = p.cos ? __fadd_rn(__fmul_rn(x, s[e]), __fmul_rn(y, c[e])) : y;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = to_f(va[i].e[e]);
-    const size_t row = (size_t)row0 + (size_t)(h0 + i) * p.page;
-    float kinv = 1.f, vinv = 1.f;
-    if constexpr (Q) {
-      constexpr float top = DT == BOZO_DT_I8 ? 127.f : 448.f;
-      unsigned km = 0, vm = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        km = max(km, __float_as_uint(k[e]) & 0x7fffffffu);
-        vm = max(vm, __float_as_uint(v[e]) & 0x7fffffffu);
-      }
-      for (int o = L / 2; o; o >>= 1) {
-        km = max(km, __shfl_xor_sync(0xffffffffu, km, o));
-        vm = max(vm, __shfl_xor_sync(0xffffffffu, vm, o));
-      }
-      float ksc, vsc;
-      quant_scale(km, top, ksc, kinv);
-      quant_scale(vm, top, vsc, vinv);
-      if (on && l == 0) {
-        p.ks[row] = ksc;
-        p.vs[row] = vsc;
-      }
-    }
-    if (on) {
-      T* kp = static_cast<T*>(p.k) + row * HD;
-      st_page<DT, 4>(kp + 4 * l, k, kinv);
-      st_page<DT, 4>(kp + half + 4 * l, k + 4, kinv);
-      st_page<DT, 8>(static_cast<T*>(p.v) + row * HD + 8 * l, v, vinv);
+      for (int j = 0; j < 4; ++j)
+        y[4 * i + j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 + j)) - 8388736.f;
     }
   }
 }
-
-template <int DT, typename O, int NH>
-__global__ void __launch_bounds__(kThreads) paged_read_vec(PagedP p, int lanes, FastDiv units) {
-  using T = typename PageT<DT>::type;
-  constexpr bool Q = DT == BOZO_DT_F8E4M3 || DT == BOZO_DT_I8;
-  const int L = 1 << lanes, l = threadIdx.x & (L - 1), HD = L * 8;
-  const unsigned nu = (unsigned)(p.Hk + NH - 1) / NH;
-  const unsigned g = (blockIdx.x * kThreads + threadIdx.x) >> lanes;
-  const unsigned n = fast_div(g, units);
-  const int h0 = (int)(g - n * nu) * NH;
-  if (n >= (unsigned)p.rows) return;
-  int b = 0;
-  unsigned pos = 0, end = 0, row0 = kNoRow;
-  if (paged_place(p, (int)n, b, pos, end)) row0 = paged_row(p, b, pos);
-  Pack<T, 8> k[NH], v[NH];
-  float ks[NH], vs[NH];
+__device__ __forceinline__ void narrow(Eight<float>& x, const float* y) {
 #pragma unroll
-  for (int i = 0; i < NH; ++i) {
-    ks[i] = vs[i] = 1.f;
-    if (row0 != kNoRow && h0 + i < p.Hk) {
-      const size_t row = (size_t)row0 + (size_t)(h0 + i) * p.page;
-      k[i] = ld_pack<T, 8>(static_cast<const T*>(p.k) + row * HD + 8 * l);
-      v[i] = ld_pack<T, 8>(static_cast<const T*>(p.v) + row * HD + 8 * l);
-      if constexpr (Q) {
-        ks[i] = __ldg(p.ks + row);
-        vs[i] = __ldg(p.vs + row);
-      }
-    }
+  for (int i = 0; i < 8; ++i) x.w[i] = __float_as_uint(y[i]);
+}
+__device__ __forceinline__ void narrow(Eight<__nv_bfloat16>& x, const float* y) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+    x.w[i] = *reinterpret_cast<const unsigned*>(&h);
   }
+}
+__device__ __forceinline__ void narrow(Eight<__half>& x, const float* y) {
 #pragma unroll
-  for (int i = 0; i < NH; ++i) {
-    if (h0 + i >= p.Hk) break;
-    Pack<O, 8> x, y;
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(y[2 * i], y[2 * i + 1]);
+    x.w[i] = *reinterpret_cast<const unsigned*>(&h);
+  }
+}
+// Codes of y · inv (|y·inv| ≤ top up to a rounding that no code passes); all zero
+// where inv is.
+template <int DT>
+__device__ __forceinline__ void narrow_codes(Eight<unsigned char>& x, const float* y, float inv) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float a = 0.f, d = 0.f;
-      if (row0 != kNoRow) {
-        if constexpr (Q) {
-          a = __fmul_rn(code_value(k[i].e[e], DT), ks[i]);
-          d = __fmul_rn(code_value(v[i].e[e], DT), vs[i]);
-        } else {
-          a = to_f(k[i].e[e]);
-          d = to_f(v[i].e[e]);
+  for (int i = 0; i < 2; ++i) {
+    unsigned w;
+    if constexpr (DT == BOZO_DT_F8E4M3) {
+      const float* z = y + 4 * i;
+      const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(z[0], inv), __fmul_rn(z[1], inv)), __NV_SATFINITE, __NV_E4M3);
+      const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(z[2], inv), __fmul_rn(z[3], inv)), __NV_SATFINITE, __NV_E4M3);
+      w = lo | hi << 16;
+    } else {
+      unsigned c[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)  // 1.5·2^23 + z: the low byte is z rounded to even
+        c[j] = __float_as_uint(__fadd_rn(__fmul_rn(y[4 * i + j], inv), 12582912.f));
+      w = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    }
+    x.w[i] = inv == 0.f ? 0u : w;
+  }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // of |a|, |b|; a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
+// The places of a block's rows n0 … n0 + rows − 1: row numbers (head 0) and
+// positions in shared memory.
+template <bool WRITE>
+__device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int rows, unsigned* srow, unsigned* spos) {
+  __shared__ int found;
+  if (p.cu) {
+    if (threadIdx.x == 0) found = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.B; i += kThreads)
+      if (__ldg(p.cu + i) <= (int)n0 && (int)n0 < __ldg(p.cu + i + 1)) found = i;
+    __syncthreads();
+  }
+  for (int r = threadIdx.x; r < rows; r += kThreads) {
+    const unsigned n = n0 + r;
+    unsigned row = kNoRow, pos = 0;
+    if (n < (unsigned)p.rows) {
+      int b = (int)n, first = (int)n, next = (int)n + 1;
+      if (p.cu) {
+        b = found;
+        if (b >= 0) {
+          while (b < p.B && (next = __ldg(p.cu + b + 1)) <= (int)n) ++b;
+          if (b < p.B) first = __ldg(p.cu + b);
+          else b = -1;
         }
       }
-      from_f(x.e[e], a);
-      from_f(y.e[e], d);
+      const int t = b < 0 ? -1 : __ldg(p.len + b);
+      if (t >= 0) {
+        pos = (unsigned)t + (n - (unsigned)first);
+        const unsigned end = (unsigned)t + (unsigned)(next - first);
+        if (pos <= 0x7fffffffu && !(WRITE && end > p.cap && pos < end - p.cap)) {
+          if (WRITE && p.cos && pos >= (unsigned)p.rope_len) atomicCAS(p.err, 0, kErrPaged | 1);
+          else row = paged_row(p, b, pos);
+        }
+      }
     }
-    const size_t at = ((size_t)n * p.Hk + h0 + i) * HD + 8 * l;
-    st_pack(static_cast<O*>(p.k_out) + at, x);
-    st_pack(static_cast<O*>(p.v_out) + at, y);
+    srow[r] = row;
+    if (WRITE) spos[r] = pos;
+  }
+  __syncthreads();
+}
+
+constexpr int kMaxRows = kThreads / 2;  // rows of a block, at most
+
+template <int DT, typename I>
+__global__ void __launch_bounds__(kThreads) paged_write_vec(PagedP p, int lanes, int rows) {
+  using T = typename PageT<DT>::type;
+  constexpr bool Q = sizeof(T) == 1;
+  __shared__ unsigned srow[kMaxRows], spos[kMaxRows];
+  const int L = 1 << lanes, l = threadIdx.x & (L - 1), half = L * 8, HD = half * 2;
+  const int per = (kThreads >> lanes) / rows;  // groups of a row
+  const int g = threadIdx.x >> lanes, r = g / per, sub = g - r * per;
+  const unsigned n0 = blockIdx.x * rows, n = n0 + r;
+  block_places<true>(p, n0, rows, srow, spos);
+  const unsigned row0 = srow[r];
+  float c[8], s[8];
+  if (p.cos && row0 != kNoRow) {
+    const size_t at = (size_t)spos[r] * half + 8 * l;
+    widen(ld8(p.cos + at), c);
+    widen(ld8(p.sin + at), s);
+  }
+  // every lane goes through the loop (the maxima are shuffled in full warps)
+  for (int u = sub; u < 2 * p.Hk + sub; u += per) {
+    const bool on = u < 2 * p.Hk && row0 != kNoRow, key = u < p.Hk;
+    const int h = key ? u : u - p.Hk;
+    float x[16];
+    if (on) {
+      const DevT4& src = key ? p.kn : p.vn;
+      const I* at = static_cast<const I*>(src.p) + n * src.sb + h * src.sh;
+      const Eight<I> lo = ld8(at + 8 * l), hi = ld8(at + half + 8 * l);
+      widen(lo, x);
+      widen(hi, x + 8);
+      if (key && p.cos) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float y = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(x[8 + i], s[i]));
+          x[8 + i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(x[8 + i], c[i]));
+          x[i] = y;
+        }
+      }
+    }
+    const size_t row = (size_t)row0 + (size_t)h * p.page;
+    Eight<T> lo, hi;
+    if constexpr (Q) {
+      float a = 0.f;
+      if (on) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) a = max_nan(a, x[i]);
+      }
+      for (int o = L / 2; o; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+      float scale, inv;
+      quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+      if (on) {
+        if (l == 0) (key ? p.ks : p.vs)[row] = scale;
+        narrow_codes<DT>(lo, x, inv);
+        narrow_codes<DT>(hi, x + 8, inv);
+      }
+    } else if (on) {
+      narrow(lo, x);
+      narrow(hi, x + 8);
+    }
+    if (on) {
+      T* to = static_cast<T*>(key ? p.k : p.v) + row * HD + 8 * l;
+      st8(to, lo);
+      st8(to + half, hi);
+    }
+  }
+}
+
+template <int DT, typename O>
+__global__ void __launch_bounds__(kThreads) paged_read_vec(PagedP p, int lanes, int rows) {
+  using T = typename PageT<DT>::type;
+  constexpr bool Q = sizeof(T) == 1;
+  __shared__ unsigned srow[kMaxRows];
+  const int L = 1 << lanes, l = threadIdx.x & (L - 1), half = L * 8, HD = half * 2;
+  const int per = (kThreads >> lanes) / rows;
+  const int g = threadIdx.x >> lanes, r = g / per, sub = g - r * per;
+  const unsigned n0 = blockIdx.x * rows, n = n0 + r;
+  block_places<false>(p, n0, rows, srow, nullptr);
+  const unsigned row0 = srow[r];
+  if (n >= (unsigned)p.rows) return;
+#pragma unroll 2
+  for (int u = sub; u < 2 * p.Hk; u += per) {
+    const bool key = u < p.Hk;
+    const int h = key ? u : u - p.Hk;
+    float x[16];
+    if (row0 != kNoRow) {
+      const size_t row = (size_t)row0 + (size_t)h * p.page;
+      const T* at = static_cast<const T*>(key ? p.k : p.v) + row * HD + 8 * l;
+      const Eight<T> lo = ld8(at), hi = ld8(at + half);
+      if constexpr (Q) {
+        const float scale = __ldg((key ? p.ks : p.vs) + row);
+        widen_codes<DT>(lo, x);
+        widen_codes<DT>(hi, x + 8);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __fmul_rn(x[i], scale);
+      } else {
+        widen(lo, x);
+        widen(hi, x + 8);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    }
+    Eight<O> lo, hi;
+    narrow(lo, x);
+    narrow(hi, x + 8);
+    O* to = static_cast<O*>(key ? p.k_out : p.v_out) + ((size_t)n * p.Hk + h) * HD + 8 * l;
+    st8(to, lo);
+    st8(to + half, hi);
   }
 }
 
 // log2 of the lanes a row takes, or −1 where the vector kernels do not apply
-int vec_lanes(const PagedP& p) { return p.HD == 32 ? 2 : p.HD == 64 ? 3 : p.HD == 128 ? 4 : -1; }
+int vec_lanes(const PagedP& p) { return p.HD == 32 ? 1 : p.HD == 64 ? 2 : p.HD == 128 ? 3 : -1; }
 
 bool vec_input(const DevT4& t, int dt) {
   const long long e = dt == BOZO_DT_F32 ? 4 : 2;
   return t.dt == dt && t.sd == 1 && !((reinterpret_cast<uintptr_t>(t.p) | (t.sb * e) | (t.sh * e)) & 15);
 }
 
-// Heads of a group: one while the rows do not fill the device, else four
-constexpr int kGroupHeads = 4;
-bool few_rows(const PagedP& p, int lanes) { return ((p.rows * p.Hk) << lanes) <= 148LL * 2048; }
+// Rows of a block: as many as leave each group at most 8 keys or values, fewer
+// where that gives less than six blocks an SM, down to one for each.
+int block_rows(const PagedP& p, int lanes, int sms) {
+  const int groups = kThreads >> lanes;
+  int per = 1;
+  while (per < groups && per < 2 * p.Hk && (per * 8 < 2 * p.Hk || p.rows * per < 6LL * sms * groups)) per *= 2;
+  return groups / per;
+}
 
 template <typename F>
-cudaError_t launch_vec(const PagedP& p, int lanes, int nh, cudaStream_t st, F kern) {
-  const unsigned nu = (unsigned)((p.Hk + nh - 1) / nh);
-  const long long groups = p.rows * nu;
-  const long long per = kThreads >> lanes;
-  kern<<<(unsigned)((groups + per - 1) / per), kThreads, 0, st>>>(p, lanes, make_fastdiv(nu));
+cudaError_t launch_vec(const PagedP& p, int lanes, int sms, cudaStream_t st, F kern) {
+  const int rows = block_rows(p, lanes, sms);
+  kern<<<(unsigned)((p.rows + rows - 1) / rows), kThreads, 0, st>>>(p, lanes, rows);
   return cudaGetLastError();
 }
 
-template <int DT, typename I>
-cudaError_t write_vec(const PagedP& p, int lanes, cudaStream_t st) {
-  if (few_rows(p, lanes)) return launch_vec(p, lanes, 1, st, paged_write_vec<DT, I, 1>);
-  return launch_vec(p, lanes, kGroupHeads, st, paged_write_vec<DT, I, kGroupHeads>);
-}
 template <int DT>
-cudaError_t write_vec(const PagedP& p, int lanes, cudaStream_t st) {
+cudaError_t write_vec(const PagedP& p, int lanes, int sms, cudaStream_t st) {
   switch (p.kn.dt) {
-    case BOZO_DT_F32: return write_vec<DT, float>(p, lanes, st);
-    case BOZO_DT_BF16: return write_vec<DT, __nv_bfloat16>(p, lanes, st);
-    default: return write_vec<DT, __half>(p, lanes, st);
+    case BOZO_DT_F32: return launch_vec(p, lanes, sms, st, paged_write_vec<DT, float>);
+    case BOZO_DT_BF16: return launch_vec(p, lanes, sms, st, paged_write_vec<DT, __nv_bfloat16>);
+    default: return launch_vec(p, lanes, sms, st, paged_write_vec<DT, __half>);
   }
 }
-template <int DT, typename O>
-cudaError_t read_vec(const PagedP& p, int lanes, cudaStream_t st) {
-  if (few_rows(p, lanes)) return launch_vec(p, lanes, 1, st, paged_read_vec<DT, O, 1>);
-  return launch_vec(p, lanes, kGroupHeads, st, paged_read_vec<DT, O, kGroupHeads>);
-}
 template <int DT>
-cudaError_t read_vec(const PagedP& p, int lanes, cudaStream_t st) {
+cudaError_t read_vec(const PagedP& p, int lanes, int sms, cudaStream_t st) {
   switch (p.out_dt) {
-    case BOZO_DT_F32: return read_vec<DT, float>(p, lanes, st);
-    case BOZO_DT_BF16: return read_vec<DT, __nv_bfloat16>(p, lanes, st);
-    default: return read_vec<DT, __half>(p, lanes, st);
+    case BOZO_DT_F32: return launch_vec(p, lanes, sms, st, paged_read_vec<DT, float>);
+    case BOZO_DT_BF16: return launch_vec(p, lanes, sms, st, paged_read_vec<DT, __nv_bfloat16>);
+    default: return launch_vec(p, lanes, sms, st, paged_read_vec<DT, __half>);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_write(const PagedP& p, cudaStream_t st) {
+cudaError_t launch_paged_write(const PagedP& p, int sms, cudaStream_t st) {
   const int lanes = vec_lanes(p);
   const bool tables = !p.cos || !((reinterpret_cast<uintptr_t>(p.cos) | reinterpret_cast<uintptr_t>(p.sin)) & 15);
-  // groups are numbered in 32 bits
-  if (lanes >= 0 && tables && vec_input(p.kn, p.kn.dt) && vec_input(p.vn, p.kn.dt) &&
-      ((p.rows * p.Hk) << lanes) < (1LL << 31)) {
+  if (lanes >= 0 && tables && vec_input(p.kn, p.kn.dt) && vec_input(p.vn, p.kn.dt)) {
     switch (p.dt) {
-      case BOZO_DT_F32: return write_vec<BOZO_DT_F32>(p, lanes, st);
-      case BOZO_DT_BF16: return write_vec<BOZO_DT_BF16>(p, lanes, st);
-      case BOZO_DT_F16: return write_vec<BOZO_DT_F16>(p, lanes, st);
-      case BOZO_DT_F8E4M3: return write_vec<BOZO_DT_F8E4M3>(p, lanes, st);
-      default: return write_vec<BOZO_DT_I8>(p, lanes, st);
+      case BOZO_DT_F32: return write_vec<BOZO_DT_F32>(p, lanes, sms, st);
+      case BOZO_DT_BF16: return write_vec<BOZO_DT_BF16>(p, lanes, sms, st);
+      case BOZO_DT_F16: return write_vec<BOZO_DT_F16>(p, lanes, sms, st);
+      case BOZO_DT_F8E4M3: return write_vec<BOZO_DT_F8E4M3>(p, lanes, sms, st);
+      default: return write_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
   const long long warps = p.rows * p.Hk;
@@ -321,16 +400,15 @@ cudaError_t launch_paged_write(const PagedP& p, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_paged_read(const PagedP& p, cudaStream_t st) {
+cudaError_t launch_paged_read(const PagedP& p, int sms, cudaStream_t st) {
   const int lanes = vec_lanes(p);
-  if (lanes >= 0 && !((reinterpret_cast<uintptr_t>(p.k_out) | reinterpret_cast<uintptr_t>(p.v_out)) & 15) &&
-      ((p.rows * p.Hk) << lanes) < (1LL << 31)) {
+  if (lanes >= 0 && !((reinterpret_cast<uintptr_t>(p.k_out) | reinterpret_cast<uintptr_t>(p.v_out)) & 15)) {
     switch (p.dt) {
-      case BOZO_DT_F32: return read_vec<BOZO_DT_F32>(p, lanes, st);
-      case BOZO_DT_BF16: return read_vec<BOZO_DT_BF16>(p, lanes, st);
-      case BOZO_DT_F16: return read_vec<BOZO_DT_F16>(p, lanes, st);
-      case BOZO_DT_F8E4M3: return read_vec<BOZO_DT_F8E4M3>(p, lanes, st);
-      default: return read_vec<BOZO_DT_I8>(p, lanes, st);
+      case BOZO_DT_F32: return read_vec<BOZO_DT_F32>(p, lanes, sms, st);
+      case BOZO_DT_BF16: return read_vec<BOZO_DT_BF16>(p, lanes, sms, st);
+      case BOZO_DT_F16: return read_vec<BOZO_DT_F16>(p, lanes, sms, st);
+      case BOZO_DT_F8E4M3: return read_vec<BOZO_DT_F8E4M3>(p, lanes, sms, st);
+      default: return read_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
   const long long warps = p.rows * p.Hk;
