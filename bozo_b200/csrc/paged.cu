@@ -30,8 +30,8 @@ __global__ void __launch_bounds__(kThreads) paged_write_any(PagedP p) {
   const unsigned row0 = paged_row(p, b, pos);
   if (row0 == kNoRow) return;
   const size_t row = row0 + (size_t)h * p.page;
-  put_row(p, p.kn, p.k, p.ks, n, h, pos, row, p.cos != nullptr, lane);
-  put_row(p, p.vn, p.v, p.vs, n, h, pos, row, false, lane);
+  NewRow(p, p.kn, n, h, pos, p.cos != nullptr, lane).put(p, p.k, p.ks, row, lane);
+  NewRow(p, p.vn, n, h, pos, false, lane).put(p, p.v, p.vs, row, lane);
 }
 
 // One warp per (row, head).

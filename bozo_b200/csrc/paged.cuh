@@ -131,36 +131,47 @@ __device__ __forceinline__ float ld_page(const void* p, size_t i, int dt) {
   return code_value(static_cast<const unsigned char*>(p)[i], dt);
 }
 
-// One warp writes row `row` of the pages from the new key (or value) of head h in
-// input row n: any head width, types and strides.
-__device__ __forceinline__ void put_row(const PagedP& p, const DevT4& src, void* pages, float* scales, int n,
-                                        int h, unsigned pos, size_t row, bool turn, int lane) {
-  const int HD = p.HD, half = HD / 2;
-  const long long o = (long long)n * src.sb + (long long)h * src.sh;
-  const float* c = p.cos + (size_t)pos * half;
-  const float* s = p.sin + (size_t)pos * half;
-  auto get = [&](int d) {
-    const float x = ldf(src.p, o + d * src.sd, src.dt);
-    if (!turn) return x;
-    if (d < half) {
-      const float y = ldf(src.p, o + (d + half) * src.sd, src.dt);
-      return __fsub_rn(__fmul_rn(x, c[d]), __fmul_rn(y, s[d]));
+// One warp holds a new row in its registers: element lane + 32·i of key (turned at
+// `pos`) or value h of input row n; any head width up to 128, types and strides.
+struct NewRow {
+  float x[4];
+  __device__ __forceinline__ NewRow(const PagedP& p, const DevT4& src, int n, int h, unsigned pos, bool turn,
+                                    int lane) {
+    const int half = p.HD / 2;
+    const long long o = (long long)n * src.sb + (long long)h * src.sh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = lane + 32 * i;
+      x[i] = 0.f;
+      if (d >= p.HD) continue;
+      x[i] = ldf(src.p, o + d * src.sd, src.dt);
+      if (!turn) continue;
+      const int f = d < half ? d : d - half;
+      const float c = __ldg(p.cos + (size_t)pos * half + f), s = __ldg(p.sin + (size_t)pos * half + f);
+      const float y = ldf(src.p, o + (d < half ? d + half : f) * src.sd, src.dt);
+      x[i] = d < half ? __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(y, s))
+                      : __fadd_rn(__fmul_rn(y, s), __fmul_rn(x[i], c));
     }
-    const float y = ldf(src.p, o + (d - half) * src.sd, src.dt);
-    return __fadd_rn(__fmul_rn(y, s[d - half]), __fmul_rn(x, c[d - half]));
-  };
-  const size_t at = row * HD;
-  if (p.dt <= BOZO_DT_F16) {
-    for (int d = lane; d < HD; d += 32) stf(pages, (long long)(at + d), p.dt, get(d));
-    return;
   }
-  unsigned a = 0;
-  for (int d = lane; d < HD; d += 32) a = max(a, __float_as_uint(get(d)) & 0x7fffffffu);
-  float scale, inv;
-  quant_scale(__reduce_max_sync(0xffffffffu, a), p.dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
-  for (int d = lane; d < HD; d += 32)
-    static_cast<unsigned char*>(pages)[at + d] = quant_code(get(d), inv, p.dt);
-  if (lane == 0) scales[row] = scale;
-}
+  // … into row `row` of the pages.
+  __device__ __forceinline__ void put(const PagedP& p, void* pages, float* scales, size_t row, int lane) const {
+    float inv = 1.f;
+    if (p.dt > BOZO_DT_F16) {
+      unsigned a = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
+      float scale;
+      quant_scale(__reduce_max_sync(0xffffffffu, a), p.dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+      if (lane == 0) scales[row] = scale;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = lane + 32 * i;
+      if (d >= p.HD) continue;
+      if (p.dt <= BOZO_DT_F16) stf(pages, (long long)(row * p.HD + d), p.dt, x[i]);
+      else static_cast<unsigned char*>(pages)[row * p.HD + d] = quant_code(x[i], inv, p.dt);
+    }
+  }
+};
 
 }  // namespace bozo

@@ -14,7 +14,8 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kMaxPiece = 8192;     // positions of a piece of paged_decode_any, which holds their τ in shared memory
-constexpr int kCluster = 8;         // pieces that are joined inside a cluster
+constexpr int kRowWarps = 8;        // warps of a block of paged_decode_rows
+constexpr int kRowHeads = 4;        // and its query heads, at most
 
 // One block per (b, h, piece), one warp per key: any head width and types.
 __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
@@ -73,15 +74,155 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
   }
 }
 
+// Four consecutive elements of a page (at a multiple of 4).
+template <int DT>
+__device__ __forceinline__ void ld4(const void* pages, size_t at, float* x) {
+  if constexpr (DT == BOZO_DT_F32) {
+    const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(pages) + at);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else if constexpr (DT == BOZO_DT_BF16) {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(pages) + at);
+    x[0] = __uint_as_float(v.x << 16); x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16); x[3] = __uint_as_float(v.y & 0xffff0000u);
+  } else if constexpr (DT == BOZO_DT_F16) {
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const __half*>(pages) + at);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
+    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
+    x[0] = a.x; x[1] = a.y; x[2] = c.x; x[3] = c.y;
+  } else {
+    const unsigned v = *reinterpret_cast<const unsigned*>(static_cast<const unsigned char*>(pages) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = code_value((unsigned char)(v >> (8 * i)), DT);
+  }
+}
+
+// fp32 pages, and head widths without a tensor-core kernel (multiples of 4): one
+// block per (b, key head, NH of its query heads, piece).  A row is held by 8, 16 or
+// 32 lanes, four elements each; a warp takes 4, 2 or 1 rows at a time and has
+// kUnroll such steps' keys and values in flight.  τ with the exact sigmoid, in
+// fp32 throughout.
+template <int DT, int NH>
+__global__ void __launch_bounds__(kRowWarps * 32) paged_decode_rows(PagedP p, int S, int HG, int lanes) {
+  constexpr int kUnroll = 4;
+  __shared__ float sq[NH][132];
+  __shared__ float part[kRowWarps][NH][132];
+  __shared__ float smass[kRowWarps][NH];
+  const int G = p.H / p.Hk, HD = p.HD;
+  int x = blockIdx.x;
+  const int piece = x % S;
+  x /= S;
+  const int hg = x % HG;
+  x /= HG;
+  const int hk = x % p.Hk, b = x / p.Hk;
+  const int h0 = hk * G + hg * NH, Gh = min(NH, G - hg * NH);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int L = 1 << lanes, l = lane & (L - 1), per = 32 >> lanes;  // rows of a warp's step
+  const Reach rc = reach(p, b, S);
+  if ((unsigned)piece >= rc.count) return;
+  const unsigned j0 = max(rc.first(piece), rc.lo), j1 = rc.last(piece);
+  if (rc.active)
+    for (int i = tid; i < NH * HD; i += kRowWarps * 32) {
+      const int h = i / HD, d = i - h * HD;
+      sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
+    }
+  if (writes_row(p, rc, piece, hg == 0)) append_row(p, b, hk, rc.t, warp, lane);
+  __syncthreads();
+  const bool on = 4 * l < HD;
+  float q[NH][4], acc[NH][4], mass[NH];
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    mass[h] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[h][i] = rc.active && on ? sq[h][4 * l + i] : 0.f;
+      acc[h][i] = 0.f;
+    }
+  }
+  const unsigned step = kRowWarps * per;
+  for (unsigned j = j0 + warp * per + (lane >> lanes); j - (lane >> lanes) < j1; j += kUnroll * step) {
+    float k[kUnroll][4], v[kUnroll][4], ks[kUnroll], vs[kUnroll];
+    bool live[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const unsigned pos = j + u * step;
+      const unsigned row0 = pos < j1 ? paged_row(p, b, pos) : kNoRow;
+      const size_t row = (size_t)row0 + (size_t)hk * p.page;
+      live[u] = row0 != kNoRow;
+      ks[u] = vs[u] = 1.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[u][i] = v[u][i] = 0.f;
+      if (live[u] && on) {
+        ld4<DT>(p.k, row * HD + 4 * l, k[u]);
+        ld4<DT>(p.v, row * HD + 4 * l, v[u]);
+      }
+      if (live[u] && DT > BOZO_DT_F16) {
+        ks[u] = p.ks[row];
+        vs[u] = p.vs[row];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z = fmaf(q[h][i], k[u][i], z);
+        for (int o = L / 2; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        const float tau = live[u] ? sigmoid_exact(z * ks[u] * p.inv_scale) : 0.f;
+        mass[h] += tau;
+        if (p.tau && live[u] && l == 0 && h < Gh)
+          put_tau(p, (size_t)b * p.H + h0 + h, rc.t, j + u * step, tau);
+        const float w = tau * vs[u];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[h][i] = fmaf(w, v[u][i], acc[h][i]);
+      }
+  }
+  grid_release();
+  // the warp's rows, then the warps, each in a fixed order
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    for (int o = L; o < 32; o <<= 1) {
+      mass[h] += __shfl_xor_sync(0xffffffffu, mass[h], o);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[h][i] += __shfl_xor_sync(0xffffffffu, acc[h][i], o);
+    }
+    if (lane < L && on)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) part[warp][h][4 * l + i] = acc[h][i];
+    if (lane == 0) smass[warp][h] = mass[h];
+  }
+  __syncthreads();
+  for (int i = tid; i < Gh * HD; i += kRowWarps * 32) {
+    const int h = i / HD, d = i - h * HD;
+    float o = 0.f, m = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      o += part[w][h][d];
+      m += smass[w][h];
+    }
+    const size_t bh = (size_t)b * p.H + h0 + h;
+    if (rc.count == 1) {
+      stf(p.out, (long long)(bh * HD + d), p.out_dt, o / norm_divisor(p, m, rc.n));
+    } else {
+      p.ws[(bh * S + piece) * HD + d] = o;
+      if (d == 0) piece_mass(p, S)[bh * S + piece] = m;
+    }
+  }
+  if (p.tau && piece == 0)
+    for (int h = warp; h < Gh; h += kRowWarps) clear_tau(p, (size_t)b * p.H + h0 + h, rc.n, lane, 32);
+}
+
 // Rows cut into more than one piece: one block per (b, h).
 __global__ void __launch_bounds__(kThreads) paged_join(PagedP p, int S) {
   const int bh = blockIdx.x, HD = p.HD;
+  grid_wait();
   const Reach r = reach(p, bh / p.H, S);
   if (r.count < 2) return;
   const float* w = p.ws + (size_t)bh * S * HD;
   const float* wm = piece_mass(p, S) + (size_t)bh * S;
   for (int d = threadIdx.x; d < HD; d += kThreads) {
     float acc = 0.f, m = 0.f;
+#pragma unroll 8
     for (unsigned i = 0; i < r.count; ++i) {
       acc += w[i * HD + d];
       m += wm[i];
@@ -94,16 +235,53 @@ bool mma_path(const PagedP& p) {
   return p.dt != BOZO_DT_F32 && (p.HD == 32 || p.HD == 64 || p.HD == 128);
 }
 
-PagedPlan plan(const PagedP& p, int sms) {
-  const bool mma = mma_path(p);
-  const long long keys = (p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap) + 15;
+bool rows_path(const PagedP& p) { return p.HD % 4 == 0; }
+
+// Blocks of a row's heads.
+int head_groups(const PagedP& p) {
   const int G = p.H / p.Hk;
-  const long long rows = (long long)p.B * (mma ? (long long)p.Hk * ((G + kHeads - 1) / kHeads) : p.H);
-  long long s = (sms * (mma ? 16 : 8) + rows - 1) / rows;
+  return mma_path(p) ? (G + kHeads - 1) / kHeads : rows_path(p) ? (G + kRowHeads - 1) / kRowHeads : G;
+}
+
+// Pieces of a row.  About three blocks an SM keep the memory busy (16 rows of
+// 120001 keys: 95 µs at 12 pieces, 78 at 18-28, 82 at 37, 86 at 74; 192 rows of
+// 1024 keys: 15.2 µs whole, 12.7 in two, 17 in four).  Sequences of different
+// lengths want smaller pieces to even out — twelve an SM, of 2048 keys at least
+// (1024 rows of up to 8192 keys: 185 µs whole, 167 in two to four, 171 in
+// eight; 512 rows of up to 16384 keys in e4m3: 239, 215 in two, 197 in four, 201 in
+// eight).  Two pieces are joined inside a cluster; a cluster of more waits
+// longer for its place than a second kernel takes (192 rows in three: 16.7 against 13.9 µs).
+PagedPlan plan(const PagedP& p, int sms) {
+  const long long keys = (p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap) + 15;
+  const long long rows = (long long)p.B * p.Hk * head_groups(p);
+  long long s = (3LL * sms + rows / 2) / rows;
+  if (p.B > 1) s = std::max(s, std::min((12LL * sms + rows - 1) / rows, keys / 2048));
   s = std::min(s, (keys + kMinPiece - 1) / kMinPiece);
-  if (!mma) s = std::max(s, (keys + kMaxPiece - 1) / kMaxPiece);
+  if (!mma_path(p) && !rows_path(p)) s = std::max(s, (keys + kMaxPiece - 1) / kMaxPiece);
   s = std::max(s, 1LL);
-  return {(int)s, mma && s > 1 && s <= kCluster};
+  return {(int)s, mma_path(p) && s == 2};
+}
+
+template <int DT>
+cudaError_t launch_rows(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  const int lanes = p.HD <= 32 ? 3 : p.HD <= 64 ? 4 : 5, HG = head_groups(p);
+  const unsigned grid = (unsigned)((long long)p.B * p.Hk * HG * pl.S);
+  if (p.H == p.Hk) paged_decode_rows<DT, 1><<<grid, kRowWarps * 32, 0, st>>>(p, pl.S, HG, lanes);
+  else paged_decode_rows<DT, kRowHeads><<<grid, kRowWarps * 32, 0, st>>>(p, pl.S, HG, lanes);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_join(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.B * p.H));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join, p, pl.S);
 }
 
 }  // namespace
@@ -124,6 +302,14 @@ cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* 
       case BOZO_DT_F8E4M3: e = launch_paged_mma_f8(p, pl, st); break;
       default: e = launch_paged_mma_i8(p, pl, st);
     }
+  } else if (rows_path(p)) {
+    switch (p.dt) {
+      case BOZO_DT_F32: e = launch_rows<BOZO_DT_F32>(p, pl, st); break;
+      case BOZO_DT_BF16: e = launch_rows<BOZO_DT_BF16>(p, pl, st); break;
+      case BOZO_DT_F16: e = launch_rows<BOZO_DT_F16>(p, pl, st); break;
+      case BOZO_DT_F8E4M3: e = launch_rows<BOZO_DT_F8E4M3>(p, pl, st); break;
+      default: e = launch_rows<BOZO_DT_I8>(p, pl, st);
+    }
   } else {
     const long long keys = p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap;
     const size_t smem = (size_t)(p.HD + std::min<long long>(keys, kMaxPiece) + 16) * sizeof(float);
@@ -133,10 +319,10 @@ cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* 
   if (e != cudaSuccess) return e;
   *launches = 1;
   if (pl.S > 1 && !pl.clustered) {
-    paged_join<<<(unsigned)(p.B * p.H), kThreads, 0, st>>>(p, pl.S);
+    e = launch_join(p, pl, st);
     *launches = 2;
   }
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace bozo

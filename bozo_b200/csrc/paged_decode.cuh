@@ -8,7 +8,12 @@
 namespace bozo {
 
 constexpr int kMinPiece = 128;  // positions of a piece, at least (where there are two)
-constexpr int kHeads = 8;       // query heads of a block in the tensor-core kernel
+constexpr int kHeads = 8;       // query heads of a block in the tensor-core kernel, at most
+
+// A join that is launched before its pieces are done waits for them here; a block
+// that has no more to start lets it be launched.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 struct PagedPlan {
   int S;           // pieces a row may be cut into
@@ -69,11 +74,11 @@ __device__ __forceinline__ bool writes_row(const PagedP& p, const Reach& r, unsi
 }
 __device__ __forceinline__ void append_row(const PagedP& p, int b, int hk, int t, int warp, int lane) {
   if (warp > 1) return;
+  const bool key = warp == 0;
+  const NewRow x(p, key ? p.kn : p.vn, b, hk, (unsigned)t, key && p.cos, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
-  if (row0 == kNoRow) return;
-  const size_t row = (size_t)row0 + (size_t)hk * p.page;
-  if (warp == 0) put_row(p, p.kn, p.k, p.ks, b, hk, (unsigned)t, row, p.cos != nullptr, lane);
-  else put_row(p, p.vn, p.v, p.vs, b, hk, (unsigned)t, row, false, lane);
+  if (row0 != kNoRow)
+    x.put(p, key ? p.k : p.v, key ? p.ks : p.vs, (size_t)row0 + (size_t)hk * p.page, lane);
 }
 
 // Rotated query element i of head h.

@@ -18,6 +18,7 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 
 #include "paged_decode.cuh"
 
@@ -154,8 +155,8 @@ constexpr int kStages = 3;
 // Geometry of the kernel for one page type, head width and count of heads.
 template <int DT, int HD, int GP> struct Geo {
   static constexpr int row = HD * Fmt<DT>::size;             // bytes of a row
-  static constexpr int keys = row >= 256 ? 16 : row >= 128 ? 32 : 64;  // keys of a tile of the ring
-  static constexpr int kv = keys * row;                      // bytes of its K (or V): 4 KB, 2 KB at 32-byte rows
+  static constexpr int keys = row >= 128 ? 16 : 2048 / row;  // keys of a tile of the ring
+  static constexpr int kv = keys * row;                      // bytes of its K (or V): 2 KB, 4 KB at 256-byte rows
   static constexpr int scales = Fmt<DT>::scaled ? 2 * keys * 4 : 0;
   static constexpr int meta = scales + 16;                   // scales, and 16 bits a 16 keys: which are in reach
   static constexpr int pstride = keys + 8;                   // words of a head's τ
@@ -218,10 +219,6 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
 #pragma unroll
   for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
-  if (writes_row(p, rc, piece, hg == 0)) {
-    append_row(p, b, hk, rc.t, warp, lane);
-    __syncthreads();
-  }
   const unsigned ring = smem_u32(smb) + warp * kStages * 2 * Z::kv;
   char* meta = smb + kWarps * kStages * 2 * Z::kv + warp * kStages * Z::meta;
   unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * kStages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
@@ -302,14 +299,21 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
   if (nk) {
     find(0, cur);
     find(AL ? kBatch : 1, nxt);
-#pragma unroll
-    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
   }
   if (mine && rc.active)
     for (int i = tid; i < GP * HD; i += kWarps * 32) {
       const int h = i / HD, d = i - h * HD;
       sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
     }
+  const bool writes = writes_row(p, rc, piece, hg == 0);
+  if (writes && p.mode == BOZO_MODE_GLOBAL) {  // these keys end with the new one
+    append_row(p, b, hk, rc.t, warp, lane);
+    __syncthreads();
+  }
+  if (nk)
+#pragma unroll
+    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
+  if (writes && p.mode == BOZO_MODE_LOCAL) append_row(p, b, hk, rc.t, warp, lane);
   __syncthreads();
   if (nk) {
     // columns of S: lane (g, c) holds k-pairs of column g, that is of head
@@ -507,6 +511,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
   }
 
   // the warps' sums, added in order
+  grid_release();
   __syncthreads();  // the rings and the queries are done with
   float* part = reinterpret_cast<float*>(smb);  // [warps][Gh][HD], then the block's [Gh][HD]
 #pragma unroll
@@ -583,9 +588,15 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
   const size_t part = (size_t)(kWarps + 1) * std::min(G, kHeads) * HD * sizeof(float);
   const size_t smem = std::max(ring, part);
   auto kern = paged_decode_mma<DT, HD, GP, AL>;
-  if (smem > 32 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+    const int most = (int)std::max(ring, (size_t)(kWarps + 1) * kHeads * HD * sizeof(float));
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
+    if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hk * HG * pl.S));
