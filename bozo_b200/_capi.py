@@ -100,7 +100,7 @@ class PagedCache(C.Structure):
         ("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p),
         ("v_scale", C.c_void_p), ("dtype", C.c_int32), ("pages", C.c_int32),
         ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("HD", C.c_int32),
-        ("batch", C.c_int32), ("width", C.c_int32), ("_pad", C.c_int32),
+        ("batch", C.c_int32), ("width", C.c_int32), ("device_current", C.c_int32),
         ("table", C.c_void_p), ("table_stride", C.c_int64), ("lengths", C.c_void_p),
     ]
 

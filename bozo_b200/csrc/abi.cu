@@ -536,7 +536,7 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   if (a->rows == 0) return BOZO_OK;
   if ((st = check_t4(a->k)) || (st = check_t4(a->v))) return st;
   DeviceRestore restore;
-  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
   PagedP p = paged_params(a->cache);
   p.rows = a->rows; p.cu = a->cu_rows;
@@ -562,7 +562,7 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   if (a->rows == 0) return BOZO_OK;
   if (!a->k_out || !a->v_out) return BOZO_ERR_NULL;
   DeviceRestore restore;
-  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
   PagedP p = paged_params(a->cache);
   p.rows = a->rows; p.cu = a->cu_rows;
@@ -616,8 +616,6 @@ static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
 size_t bozo_paged_decode_workspace(const bozo_paged_decode_args* a) {
   PagedP p;
   if (paged_decode_params(a, p) != BOZO_OK) return 0;
-  DeviceRestore restore;
-  if (bind_device(a->cache.k_pages, restore) != cudaSuccess) return 0;
   return paged_decode_bytes(p, num_sms());
 }
 
@@ -626,15 +624,16 @@ int bozo_paged_decode(const bozo_paged_decode_args* a, void* stream) {
   const int st = paged_decode_params(a, p);
   if (st) return st;
   DeviceRestore restore;
-  cudaError_t e = bind_device(a->cache.k_pages, restore);
+  cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
-  const size_t need = paged_decode_bytes(p, num_sms());
+  const int sms = num_sms();
+  const size_t need = paged_decode_bytes(p, sms);
   if (need && (!a->workspace || a->workspace_bytes < need)) return BOZO_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return BOZO_ERR_ALIGNMENT;
   p.ws = static_cast<float*>(a->workspace);
   if (!(p.err = error_word(&e))) return cuda_fail(e);
   int launches = 0;
-  e = launch_paged_decode(p, num_sms(), static_cast<cudaStream_t>(stream), &launches);
+  e = launch_paged_decode(p, sms, static_cast<cudaStream_t>(stream), &launches);
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = BOZO_PATH_SIMT;
   t_last_launches = launches;

@@ -9,6 +9,7 @@
 // (triton_tension/ops.py:75-124, 126-187), in C++ so a call costs a few
 // microseconds of host time instead of a Python-level struct build.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -263,6 +264,13 @@ const at::Tensor* given(const c10::optional<at::Tensor>& t) {
   return t && t->defined() ? &*t : nullptr;
 }
 
+void no_grad(const char* what, std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : ts)
+    if (t && t->requires_grad())
+      throw std::runtime_error(std::string(what) + " has no gradient: call it under torch.no_grad()");
+}
+
 // The cache argument block; every shape, type and device is checked here (the
 // C ABI sees pointers only).
 bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const at::Tensor& v_pages,
@@ -314,7 +322,12 @@ bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const 
   c.table = table.data_ptr<int32_t>();
   c.table_stride = table.stride(0);
   c.lengths = lengths.data_ptr<int32_t>();
+  c.device_current = 1;  // every caller holds a guard of the pages' device
   return c;
+}
+
+at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
+  return at::detail::empty_cuda(shape, type, dev, c10::nullopt);
 }
 
 // [rows, heads, HD] (any strides) as the ABI's [rows, 1, heads, HD] view
@@ -365,6 +378,7 @@ void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_p
                  const c10::optional<at::Tensor>& sin, const c10::optional<at::Tensor>& k_scale,
                  const c10::optional<at::Tensor>& v_scale) {
   const char* what = "write_kv";
+  no_grad(what, {&k, &v});
   bozo_paged_write_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
   const auto dev = k_pages.device();
@@ -377,11 +391,11 @@ void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_p
   check(bozo_paged_write(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_write");
 }
 
-std::vector<at::Tensor> paged_read(const at::Tensor& k_pages, const at::Tensor& v_pages,
-                                   const at::Tensor& table, const at::Tensor& lengths,
-                                   const c10::optional<at::Tensor>& cu_rows, int64_t rows,
-                                   const c10::optional<at::Tensor>& k_scale,
-                                   const c10::optional<at::Tensor>& v_scale, int64_t out_dtype) {
+std::tuple<at::Tensor, at::Tensor> paged_read(
+    const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
+    const at::Tensor& lengths, const c10::optional<at::Tensor>& cu_rows, int64_t rows,
+    const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale,
+    int64_t out_dtype) {
   const char* what = "read_kv";
   bozo_paged_read_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
@@ -390,17 +404,17 @@ std::vector<at::Tensor> paged_read(const at::Tensor& k_pages, const at::Tensor& 
   if (rows < 0) throw std::invalid_argument("read_kv: rows must not be negative");
   a.rows = rows;
   a.cu_rows = rows_of(what, given(cu_rows), a.cache, rows, dev);
-  auto opts = k_pages.options().dtype(scalar_type(out_dtype));
-  at::Tensor k = at::empty({rows, a.cache.kv_heads, a.cache.HD}, opts), v = at::empty_like(k);
+  const int64_t shape[3] = {rows, a.cache.kv_heads, a.cache.HD};
+  at::Tensor k = empty(shape, scalar_type(out_dtype), dev), v = empty(shape, scalar_type(out_dtype), dev);
   a.k_out = k.data_ptr();
   a.v_out = v.data_ptr();
   a.out_dtype = (int32_t)out_dtype;
   check(bozo_paged_read(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_read");
-  return {k, v};
+  return {std::move(k), std::move(v)};
 }
 
-// Returns [out [B, H, HD], tau [B, H, tau_width] (undefined unless tau_width > 0)] in q's dtype.
-std::vector<at::Tensor> paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
+// Returns out [B, H, HD] in q's dtype, or with tau_width > 0 (out, tau [B, H, tau_width]).
+pybind11::object paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
                                      const at::Tensor& v_pages, const at::Tensor& table,
                                      const at::Tensor& lengths, int64_t mode, int64_t window,
                                      int64_t norm, double scale, const c10::optional<at::Tensor>& cos,
@@ -410,6 +424,7 @@ std::vector<at::Tensor> paged_decode(const at::Tensor& q, const at::Tensor& k_pa
                                      const c10::optional<at::Tensor>& k_scale,
                                      const c10::optional<at::Tensor>& v_scale, int64_t tau_width) {
   const char* what = "paged_tension";
+  no_grad(what, {&q, given(k), given(v)});
   bozo_paged_decode_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
   const auto dev = k_pages.device();
@@ -436,20 +451,22 @@ std::vector<at::Tensor> paged_decode(const at::Tensor& q, const at::Tensor& k_pa
   a.scale = (float)scale;
   a.tau_width = (int32_t)tau_width;
   a.out_dtype = a.tau_dtype = a.q.dtype;
-  at::Tensor out = at::empty({B, H, (int64_t)a.cache.HD}, q.options()), tau, ws;
+  const int64_t shape[3] = {B, H, a.cache.HD}, tau_shape[3] = {B, H, tau_width};
+  at::Tensor out = empty(shape, q.scalar_type(), dev), tau, ws;
   a.out = out.data_ptr();
   if (tau_width > 0) {
-    tau = at::empty({B, H, tau_width}, q.options());
+    tau = empty(tau_shape, q.scalar_type(), dev);
     a.tau = tau.data_ptr();
   }
-  const size_t bytes = bozo_paged_decode_workspace(&a);
+  const int64_t bytes = (int64_t)bozo_paged_decode_workspace(&a);
   if (bytes) {
-    ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    ws = empty(bytes, at::kByte, dev);
     a.workspace = ws.data_ptr();
-    a.workspace_bytes = bytes;
+    a.workspace_bytes = (size_t)bytes;
   }
   check(bozo_paged_decode(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_decode");
-  return {out, tau};
+  if (tau_width > 0) return pybind11::make_tuple(std::move(out), std::move(tau));
+  return pybind11::cast(std::move(out));
 }
 
 // Graph bias [T, W] (window > 0) or [T, T] (window 0) from the context's

@@ -41,11 +41,6 @@ from . import _capi, ops
 __all__ = ["write_kv", "read_kv", "paged_tension"]
 
 
-def _no_grad(what: str, *ts: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad()")
-
-
 def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
              lengths: Tensor, *, cu_rows: Optional[Tensor] = None, rope=None,
              k_scale: Optional[Tensor] = None, v_scale: Optional[Tensor] = None) -> None:
@@ -61,7 +56,6 @@ def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table:
     ``lengths`` is not advanced (all layers of a step share it).  Of more than C
     tokens of one sequence the last C are kept.
     """
-    _no_grad("write_kv", k, v)
     cos, sin = (rope[0], rope[1]) if rope is not None else (None, None)
     _capi.ext().paged_write(k, v, k_pages, v_pages, page_table, lengths, cu_rows, cos, sin,
                             k_scale, v_scale)
@@ -75,8 +69,8 @@ def read_kv(k_pages: Tensor, v_pages: Tensor, page_table: Tensor, start: Tensor,
     ``[rows, Hk, HD]`` in ``dtype``: rows ``cu_rows[b]:cu_rows[b+1]`` are sequence
     b's positions ``start[b]``, …; padding rows and inactive sequences are zeros.
     8-bit rows come back as code · scale."""
-    return tuple(_capi.ext().paged_read(k_pages, v_pages, page_table, start, cu_rows, int(rows),
-                                        k_scale, v_scale, ops._dt(dtype)))
+    return _capi.ext().paged_read(k_pages, v_pages, page_table, start, cu_rows, rows, k_scale,
+                                  v_scale, ops._dt(dtype))
 
 
 def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tensor,
@@ -103,18 +97,18 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
 
     Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.
     """
-    _no_grad("paged_tension", q, k, v)
-    if normalize not in ops._NORM:
+    norm = ops._NORM.get(normalize, -1)
+    if norm < 0:
         raise ValueError(f"normalize must be 'mass', 'count' or None, got {normalize!r}")
     if window is None:
-        mode, win, tw = _capi.MODE_GLOBAL, 0, int(tau_window or 0)
-        if normalize == "count":
+        mode, win, tw = _capi.MODE_GLOBAL, 0, int(tau_window or 0) if return_tau else 0
+        if norm == _capi.NORM_COUNT:
             raise ValueError("normalize='count' is defined for local windows only")
         if return_tau and tw < 1:
             raise ValueError("global mode exports τ over the model's local window: pass tau_window")
     else:
         mode, win = _capi.MODE_LOCAL, int(window)
-        tw = win
+        tw = win if return_tau else 0
         if win < 1:
             raise ValueError("window must be >= 1")
         if return_tau and tau_window is not None and int(tau_window) != win:
@@ -122,7 +116,5 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
     cos, sin = (rope[0], rope[1]) if rope is not None else (None, None)
     if scale is None:
         scale = math.sqrt(k_pages.shape[-1])
-    out, tau = _capi.ext().paged_decode(
-        q, k_pages, v_pages, page_table, lengths, mode, win, ops._NORM[normalize], float(scale),
-        cos, sin, k, v, k_scale, v_scale, tw if return_tau else 0)
-    return (out, tau) if return_tau else out
+    return _capi.ext().paged_decode(q, k_pages, v_pages, page_table, lengths, mode, win, norm, scale,
+                                    cos, sin, k, v, k_scale, v_scale, tw)

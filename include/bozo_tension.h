@@ -237,7 +237,8 @@ typedef struct {
   int32_t pages, kv_heads, page_size, HD;
   int32_t batch;          /* sequences B */
   int32_t width;          /* pages of a sequence in the table */
-  int32_t _pad;
+  int32_t device_current; /* 1: the pages' device is current on the calling thread;
+                             0: it is looked up and made current for the call */
   const int32_t* table;   /* [B, width] page numbers, rows table_stride apart */
   int64_t table_stride;
   const int32_t* lengths; /* [B] device: position of each sequence's first new token */
@@ -300,6 +301,8 @@ typedef struct {
   void* workspace;        /* bozo_paged_decode_workspace() bytes, 16-byte aligned */
   size_t workspace_bytes;
 } bozo_paged_decode_args;
+/* Bytes for the current device, which has to be the pages' (its count of SMs
+ * decides how far a row is split); 0 is possible. */
 size_t bozo_paged_decode_workspace(const bozo_paged_decode_args* args);
 int bozo_paged_decode(const bozo_paged_decode_args* args, void* stream);
 
