@@ -182,9 +182,9 @@ __device__ __forceinline__ void narrow_codes(Eight<unsigned char>& x, const floa
     x.w[i] = inv == 0.f ? 0u : w;
   }
 }
-__device__ __forceinline__ float max_nan(float a, float b) {  // of |a|, |b|; a NaN stays
+__device__ __forceinline__ float max_abs(float a, float b) {  // ± max(|a|, |b|); a NaN stays
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(kThreads) paged_write_vec(PagedP p, int lanes,
       float a = 0.f;
       if (on) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) a = max_nan(a, x[i]);
+        for (int i = 0; i < 16; ++i) a = max_abs(a, x[i]);
       }
-      for (int o = L / 2; o; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+      for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
       float scale, inv;
       quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
       if (on) {
@@ -348,12 +348,17 @@ bool vec_input(const DevT4& t, int dt) {
   return t.dt == dt && t.sd == 1 && !((reinterpret_cast<uintptr_t>(t.p) | (t.sb * e) | (t.sh * e)) & 15);
 }
 
-// Rows of a block: as many as leave each group at most 8 keys or values, fewer
-// where that gives less than six blocks an SM, down to one for each.
+// Rows of a block: as many as leave each group at most kGroupHeads heads, fewer
+// where that gives less than six blocks an SM, down to one.
+#ifndef KGH
+#define KGH 8
+#define KBS 6
+#endif
+constexpr int kGroupHeads = KGH;
 int block_rows(const PagedP& p, int lanes, int sms) {
   const int groups = kThreads >> lanes;
   int per = 1;
-  while (per < groups && per < 2 * p.Hk && (per * 8 < 2 * p.Hk || p.rows * per < 6LL * sms * groups)) per *= 2;
+  while (per < groups && per < 2 * p.Hk && (per * kGroupHeads < 2 * p.Hk || p.rows * per < (long long)KBS * sms * groups)) per *= 2;
   return groups / per;
 }
 
