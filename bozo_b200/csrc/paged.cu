@@ -11,7 +11,7 @@
 namespace bozo {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // One warp per (row, head): any head width, types and strides.
 __global__ void __launch_bounds__(kThreads) paged_write_any(PagedP p) {
@@ -230,9 +230,15 @@ __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int r
 }
 
 constexpr int kMaxRows = kThreads / 2;  // rows of a block, at most
+// What hides the chain from a sequence's offset to its rows is other blocks, so the
+// kernels keep to the registers that let this many stay on an SM (36 rows · 2^10 of
+// 16 heads from bf16 to e4m3 and back: 113 µs; 118 with half as many blocks of twice
+// the threads, 128 where each group has two rows' loads in flight at the price of
+// a third of the blocks).
+constexpr int kWriteBlocks = 10, kReadBlocks = 16;
 
 template <int DT, typename I>
-__global__ void __launch_bounds__(kThreads) paged_write_vec(PagedP p, int lanes, int rows) {
+__global__ void __launch_bounds__(kThreads, kWriteBlocks) paged_write_vec(PagedP p, int lanes, int rows) {
   using T = typename PageT<DT>::type;
   constexpr bool Q = sizeof(T) == 1;
   __shared__ unsigned srow[kMaxRows], spos[kMaxRows];
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) paged_write_vec(PagedP p, int lanes,
 }
 
 template <int DT, typename O>
-__global__ void __launch_bounds__(kThreads) paged_read_vec(PagedP p, int lanes, int rows) {
+__global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p, int lanes, int rows) {
   using T = typename PageT<DT>::type;
   constexpr bool Q = sizeof(T) == 1;
   __shared__ unsigned srow[kMaxRows];
@@ -308,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) paged_read_vec(PagedP p, int lanes, 
   block_places<false>(p, n0, rows, srow, nullptr);
   const unsigned row0 = srow[r];
   if (n >= (unsigned)p.rows) return;
-#pragma unroll 2
+#pragma unroll 1
   for (int u = sub; u < 2 * p.Hk; u += per) {
     const bool key = u < p.Hk;
     const int h = key ? u : u - p.Hk;
@@ -348,17 +354,14 @@ bool vec_input(const DevT4& t, int dt) {
   return t.dt == dt && t.sd == 1 && !((reinterpret_cast<uintptr_t>(t.p) | (t.sb * e) | (t.sh * e)) & 15);
 }
 
-// Rows of a block: as many as leave each group at most kGroupHeads heads, fewer
-// where that gives less than six blocks an SM, down to one.
-#ifndef KGH
-#define KGH 8
-#define KBS 6
-#endif
-constexpr int kGroupHeads = KGH;
+// Rows of a block: as many as leave each group at most 8 keys or values, fewer
+// where that gives less than six blocks an SM, down to one (the same prompts: 113.5 µs
+// at 8, 115.6 at 4, 115.2 at 12).
+constexpr int kGroupHeads = 8;
 int block_rows(const PagedP& p, int lanes, int sms) {
   const int groups = kThreads >> lanes;
   int per = 1;
-  while (per < groups && per < 2 * p.Hk && (per * kGroupHeads < 2 * p.Hk || p.rows * per < (long long)KBS * sms * groups)) per *= 2;
+  while (per < groups && per < 2 * p.Hk && (per * kGroupHeads < 2 * p.Hk || p.rows * per < 6LL * sms * groups)) per *= 2;
   return groups / per;
 }
 
