@@ -97,13 +97,13 @@ __device__ __forceinline__ void ld4(const void* pages, size_t at, float* x) {
 }
 
 // fp32 pages, and head widths without a tensor-core kernel (multiples of 4): one
-// block per (b, key head, NH of its query heads, piece).  A row is held by 8, 16 or
-// 32 lanes, four elements each; a warp takes 4, 2 or 1 rows at a time and has
-// kUnroll such steps' keys and values in flight.  τ with the exact sigmoid, in
-// fp32 throughout.
+// block per (b, key head, NH of its query heads, piece).  A row is held by L = 4, 8
+// or 16 lanes, eight elements each (the 4-element pieces l and l + L); a warp takes
+// 8, 4 or 2 rows at a time and has kUnroll such steps' keys and values in flight.
+// τ with the exact sigmoid, in fp32 throughout.
 template <int DT, int NH>
-__global__ void __launch_bounds__(kRowWarps * 32) paged_decode_rows(PagedP p, int S, int HG, int lanes) {
-  constexpr int kUnroll = 4;
+__global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p, int S, int HG, int lanes) {
+  constexpr int kUnroll = NH == 1 ? 4 : 2;
   __shared__ float sq[NH][132];
   __shared__ float part[kRowWarps][NH][132];
   __shared__ float smass[kRowWarps][NH];
@@ -127,20 +127,20 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_decode_rows(PagedP p, in
     }
   if (writes_row(p, rc, piece, hg == 0)) append_row(p, b, hk, rc.t, warp, lane);
   __syncthreads();
-  const bool on = 4 * l < HD;
-  float q[NH][4], acc[NH][4], mass[NH];
+  const bool on[2] = {4 * l < HD, 4 * (l + L) < HD};
+  const int own = NH == 1 ? 0 : l / (L / 4);  // the head whose τ this lane computes
+  float q[NH][8], acc[NH][8], mass = 0.f;
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
-    mass[h] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      q[h][i] = rc.active && on ? sq[h][4 * l + i] : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      q[h][i] = rc.active && on[i / 4] ? sq[h][4 * (l + i / 4 * L) + i % 4] : 0.f;
       acc[h][i] = 0.f;
     }
   }
   const unsigned step = kRowWarps * per;
   for (unsigned j = j0 + warp * per + (lane >> lanes); j - (lane >> lanes) < j1; j += kUnroll * step) {
-    float k[kUnroll][4], v[kUnroll][4], ks[kUnroll], vs[kUnroll];
+    float k[kUnroll][8], v[kUnroll][8], ks[kUnroll], vs[kUnroll];
     bool live[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -150,47 +150,66 @@ __global__ void __launch_bounds__(kRowWarps * 32) paged_decode_rows(PagedP p, in
       live[u] = row0 != kNoRow;
       ks[u] = vs[u] = 1.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[u][i] = v[u][i] = 0.f;
-      if (live[u] && on) {
-        ld4<DT>(p.k, row * HD + 4 * l, k[u]);
-        ld4<DT>(p.v, row * HD + 4 * l, v[u]);
-      }
+      for (int i = 0; i < 8; ++i) k[u][i] = v[u][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (live[u] && on[i]) {
+          ld4<DT>(p.k, row * HD + 4 * (l + i * L), k[u] + 4 * i);
+          ld4<DT>(p.v, row * HD + 4 * (l + i * L), v[u] + 4 * i);
+        }
       if (live[u] && DT > BOZO_DT_F16) {
         ks[u] = p.ks[row];
         vs[u] = p.vs[row];
       }
     }
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
+    for (int u = 0; u < kUnroll; ++u) {
+      float z[NH];
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        float z = 0.f;
+        z[h] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z = fmaf(q[h][i], k[u][i], z);
-        for (int o = L / 2; o; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        const float tau = live[u] ? sigmoid_exact(z * ks[u] * p.inv_scale) : 0.f;
-        mass[h] += tau;
-        if (p.tau && live[u] && l == 0 && h < Gh)
-          put_tau(p, (size_t)b * p.H + h0 + h, rc.t, j + u * step, tau);
-        const float w = tau * vs[u];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[h][i] = fmaf(w, v[u][i], acc[h][i]);
+        for (int i = 0; i < 8; ++i) z[h] = fmaf(q[h][i], k[u][i], z[h]);
       }
+      // over the row's lanes; of four heads each lane keeps one, head `own`
+      float y = z[0];
+      int o = L / 2;
+      if constexpr (NH == 4) {
+        const bool up = l & o, odd = l & (o / 2);
+        const float a = (up ? z[2] : z[0]) + __shfl_xor_sync(0xffffffffu, up ? z[0] : z[2], o);
+        const float c = (up ? z[3] : z[1]) + __shfl_xor_sync(0xffffffffu, up ? z[1] : z[3], o);
+        o /= 2;
+        y = (odd ? c : a) + __shfl_xor_sync(0xffffffffu, odd ? a : c, o);
+        o /= 2;
+      }
+      for (; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
+      const float tau = live[u] ? sigmoid_exact(y * ks[u] * p.inv_scale) : 0.f;
+      mass += tau;
+      if (p.tau && live[u] && (l & (L / NH - 1)) == 0 && own < Gh)
+        put_tau(p, (size_t)b * p.H + h0 + own, rc.t, j + u * step, tau);
+      const float w = tau * vs[u];
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const float wh = NH == 1 ? w : __shfl_sync(0xffffffffu, w, (lane & ~(L - 1)) + h * (L / 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[h][i] = fmaf(wh, v[u][i], acc[h][i]);
+      }
+    }
   }
   grid_release();
   // the warp's rows, then the warps, each in a fixed order
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
-    for (int o = L; o < 32; o <<= 1) {
-      mass[h] += __shfl_xor_sync(0xffffffffu, mass[h], o);
+    for (int o = L; o < 32; o <<= 1)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[h][i] += __shfl_xor_sync(0xffffffffu, acc[h][i], o);
-    }
-    if (lane < L && on)
+      for (int i = 0; i < 8; ++i) acc[h][i] += __shfl_xor_sync(0xffffffffu, acc[h][i], o);
+    if (lane < L)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) part[warp][h][4 * l + i] = acc[h][i];
-    if (lane == 0) smass[warp][h] = mass[h];
+      for (int i = 0; i < 8; ++i)
+        if (on[i / 4]) part[warp][h][4 * (l + i / 4 * L) + i % 4] = acc[h][i];
   }
+  for (int o = L; o < 32; o <<= 1) mass += __shfl_xor_sync(0xffffffffu, mass, o);
+  if (lane < L && (l & (L / NH - 1)) == 0) smass[warp][own] = mass;
   __syncthreads();
   for (int i = tid; i < Gh * HD; i += kRowWarps * 32) {
     const int h = i / HD, d = i - h * HD;
@@ -264,7 +283,7 @@ PagedPlan plan(const PagedP& p, int sms) {
 
 template <int DT>
 cudaError_t launch_rows(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
-  const int lanes = p.HD <= 32 ? 3 : p.HD <= 64 ? 4 : 5, HG = head_groups(p);
+  const int lanes = p.HD <= 32 ? 2 : p.HD <= 64 ? 3 : 4, HG = head_groups(p);
   const unsigned grid = (unsigned)((long long)p.B * p.Hk * HG * pl.S);
   if (p.H == p.Hk) paged_decode_rows<DT, 1><<<grid, kRowWarps * 32, 0, st>>>(p, pl.S, HG, lanes);
   else paged_decode_rows<DT, kRowHeads><<<grid, kRowWarps * 32, 0, st>>>(p, pl.S, HG, lanes);
