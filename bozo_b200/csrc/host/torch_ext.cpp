@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <stdexcept>
 #include <string>
 
@@ -417,7 +418,8 @@ std::tuple<at::Tensor, at::Tensor> paged_read(
 pybind11::object paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
                                      const at::Tensor& v_pages, const at::Tensor& table,
                                      const at::Tensor& lengths, int64_t mode, int64_t window,
-                                     int64_t norm, double scale, const c10::optional<at::Tensor>& cos,
+                                     int64_t norm, c10::optional<double> scale,
+                                     const c10::optional<at::Tensor>& cos,
                                      const c10::optional<at::Tensor>& sin,
                                      const c10::optional<at::Tensor>& k,
                                      const c10::optional<at::Tensor>& v,
@@ -448,7 +450,7 @@ pybind11::object paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
   a.mode = (int32_t)mode;
   a.window = (int32_t)window;
   a.normalize = (int32_t)norm;
-  a.scale = (float)scale;
+  a.scale = scale ? (float)*scale : std::sqrt((float)a.cache.HD);
   a.tau_width = (int32_t)tau_width;
   a.out_dtype = a.tau_dtype = a.q.dtype;
   const int64_t shape[3] = {B, H, a.cache.HD}, tau_shape[3] = {B, H, tau_width};

@@ -160,6 +160,18 @@ __device__ __forceinline__ void narrow(Eight<__half>& x, const float* y) {
     x.w[i] = *reinterpret_cast<const unsigned*>(&h);
   }
 }
+// Two products (sums) in one instruction, each rounded as on its own.  A pair of
+// products must not run into a pair of sums, which would contract them: where one
+// follows, the products are single instructions.
+__device__ __forceinline__ void mul2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{.reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; mul.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b, float c, float d) {
+  asm("{.reg .b64 p, q; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %5}; add.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}"
+      : "=f"(x), "=f"(y) : "f"(a), "f"(b), "f"(c), "f"(d));
+}
+
 // Codes of y · inv (|y·inv| ≤ top up to a rounding that no code passes); all zero
 // where inv is.
 template <int DT>
@@ -167,17 +179,21 @@ __device__ __forceinline__ void narrow_codes(Eight<unsigned char>& x, const floa
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     unsigned w;
+    float z[4];
     if constexpr (DT == BOZO_DT_F8E4M3) {
-      const float* z = y + 4 * i;
-      const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(z[0], inv), __fmul_rn(z[1], inv)), __NV_SATFINITE, __NV_E4M3);
-      const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(__fmul_rn(z[2], inv), __fmul_rn(z[3], inv)), __NV_SATFINITE, __NV_E4M3);
+      mul2(z[0], z[1], y[4 * i], y[4 * i + 1], inv, inv);
+      mul2(z[2], z[3], y[4 * i + 2], y[4 * i + 3], inv, inv);
+      const unsigned lo = __nv_cvt_float2_to_fp8x2(make_float2(z[0], z[1]), __NV_SATFINITE, __NV_E4M3);
+      const unsigned hi = __nv_cvt_float2_to_fp8x2(make_float2(z[2], z[3]), __NV_SATFINITE, __NV_E4M3);
       w = lo | hi << 16;
     } else {
-      unsigned c[4];
+      // 1.5·2^23 + z: the low byte is z rounded to even
 #pragma unroll
-      for (int j = 0; j < 4; ++j)  // 1.5·2^23 + z: the low byte is z rounded to even
-        c[j] = __float_as_uint(__fadd_rn(__fmul_rn(y[4 * i + j], inv), 12582912.f));
-      w = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+      for (int j = 0; j < 4; ++j) z[j] = __fmul_rn(y[4 * i + j], inv);
+      add2(z[0], z[1], z[0], z[1], 12582912.f, 12582912.f);
+      add2(z[2], z[3], z[2], z[3], 12582912.f, 12582912.f);
+      w = __byte_perm(__byte_perm(__float_as_uint(z[0]), __float_as_uint(z[1]), 0x0040),
+                      __byte_perm(__float_as_uint(z[2]), __float_as_uint(z[3]), 0x0040), 0x5410);
     }
     x.w[i] = inv == 0.f ? 0u : w;
   }
@@ -267,10 +283,12 @@ __global__ void __launch_bounds__(kThreads, kWriteBlocks) paged_write_vec(PagedP
       widen(hi, x + 8);
       if (key && p.cos) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float y = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(x[8 + i], s[i]));
-          x[8 + i] = __fadd_rn(__fmul_rn(x[i], s[i]), __fmul_rn(x[8 + i], c[i]));
-          x[i] = y;
+        for (int i = 0; i < 8; i += 2) {
+          const float d0 = __fmul_rn(x[i], s[i]), d1 = __fmul_rn(x[i + 1], s[i + 1]);
+          const float e0 = __fmul_rn(x[8 + i], c[i]), e1 = __fmul_rn(x[9 + i], c[i + 1]);
+          add2(x[i], x[i + 1], __fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1]), __fmul_rn(x[8 + i], -s[i]),
+               __fmul_rn(x[9 + i], -s[i + 1]));
+          add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
         }
       }
     }
@@ -328,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p
         widen_codes<DT>(lo, x);
         widen_codes<DT>(hi, x + 8);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = __fmul_rn(x[i], scale);
+        for (int i = 0; i < 16; i += 2) mul2(x[i], x[i + 1], x[i], x[i + 1], scale, scale);
       } else {
         widen(lo, x);
         widen(hi, x + 8);

@@ -30,7 +30,6 @@ the RoPE tables or a page outside the pool is skipped and reported by
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple
 
 import torch
@@ -114,7 +113,5 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
         if return_tau and tau_window is not None and int(tau_window) != win:
             raise ValueError("a local window exports its own τ row: tau_window must be the window")
     cos, sin = (rope[0], rope[1]) if rope is not None else (None, None)
-    if scale is None:
-        scale = math.sqrt(k_pages.shape[-1])
     return _capi.ext().paged_decode(q, k_pages, v_pages, page_table, lengths, mode, win, norm, scale,
                                     cos, sin, k, v, k_scale, v_scale, tw)
