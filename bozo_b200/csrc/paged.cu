@@ -248,76 +248,82 @@ __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int r
 constexpr int kMaxRows = kThreads / 2;  // rows of a block, at most
 // What hides the chain from a sequence's offset to its rows is other blocks, so the
 // kernels keep to the registers that let this many stay on an SM (36 rows · 2^10 of
-// 16 heads from bf16 to e4m3 and back: 113 µs; 118 with half as many blocks of twice
-// the threads, 128 where each group has two rows' loads in flight at the price of
-// a third of the blocks).
-constexpr int kWriteBlocks = 10, kReadBlocks = 16;
+// 16 heads from bf16 to e4m3 and back: 110 µs; 114 with eight writing blocks, 122
+// with as few as the registers they would take, 118 in blocks of twice the threads;
+// with two rows' loads of a group in flight 128).
+constexpr int kWriteBlocks = 9, kReadBlocks = 16;
+
+// A group's part of one row's keys (KEY) or values: heads h, h + per, … of p.Hk.
+// Returns the first head it did not take.
+template <int DT, typename I, bool KEY>
+__device__ __forceinline__ int write_heads(const PagedP& p, unsigned n, unsigned row0, int h, int per, int L, int l,
+                                           const float* c, const float* s) {
+  using T = typename PageT<DT>::type;
+  constexpr bool Q = sizeof(T) == 1;
+  const int half = L * 8, HD = half * 2;
+  const DevT4& src = KEY ? p.kn : p.vn;
+  const I* from = static_cast<const I*>(src.p) + n * src.sb + h * src.sh + 8 * l;
+  T* const pages = static_cast<T*>(KEY ? p.k : p.v) + 8 * l;
+  unsigned row = row0 + (unsigned)h * (unsigned)p.page;  // rows are numbered in 32 bits
+  const long long from_step = per * src.sh;
+  const unsigned row_step = (unsigned)(per * p.page);
+  const unsigned group = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+#pragma unroll 1
+  for (; h < p.Hk; h += per, from += from_step, row += row_step) {
+    float x[16];
+    const Eight<I> xl = ld8(from), xh = ld8(from + half);
+    widen(xl, x);
+    widen(xh, x + 8);
+    if (KEY && p.cos) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float d0 = __fmul_rn(x[i], s[i]), d1 = __fmul_rn(x[i + 1], s[i + 1]);
+        const float e0 = __fmul_rn(x[8 + i], c[i]), e1 = __fmul_rn(x[9 + i], c[i + 1]);
+        add2(x[i], x[i + 1], __fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1]), __fmul_rn(x[8 + i], -s[i]),
+             __fmul_rn(x[9 + i], -s[i + 1]));
+        add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
+      }
+    }
+    Eight<T> yl, yh;
+    if constexpr (Q) {
+      float a = x[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) a = max_abs(a, x[i]);
+      for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(group, a, o));
+      float scale, inv;
+      quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+      if (l == 0) (KEY ? p.ks : p.vs)[row] = scale;
+      narrow_codes<DT>(yl, x, inv);
+      narrow_codes<DT>(yh, x + 8, inv);
+    } else {
+      narrow(yl, x);
+      narrow(yh, x + 8);
+    }
+    T* to = pages + (size_t)row * HD;
+    st8(to, yl);
+    st8(to + half, yh);
+  }
+  return h;
+}
 
 template <int DT, typename I>
 __global__ void __launch_bounds__(kThreads, kWriteBlocks) paged_write_vec(PagedP p, int lanes, int rows) {
-  using T = typename PageT<DT>::type;
-  constexpr bool Q = sizeof(T) == 1;
   __shared__ unsigned srow[kMaxRows], spos[kMaxRows];
-  const int L = 1 << lanes, l = threadIdx.x & (L - 1), half = L * 8, HD = half * 2;
+  const int L = 1 << lanes, l = threadIdx.x & (L - 1);
   const int per = (kThreads >> lanes) / rows;  // groups of a row
   const int g = threadIdx.x >> lanes, r = g / per, sub = g - r * per;
   const unsigned n0 = blockIdx.x * rows, n = n0 + r;
   block_places<true>(p, n0, rows, srow, spos);
   const unsigned row0 = srow[r];
+  if (row0 == kNoRow) return;
   float c[8], s[8];
-  if (p.cos && row0 != kNoRow) {
-    const size_t at = (size_t)spos[r] * half + 8 * l;
+  if (p.cos && sub < p.Hk) {
+    const size_t at = (size_t)spos[r] * (L * 8) + 8 * l;
     widen(ld8(p.cos + at), c);
     widen(ld8(p.sin + at), s);
   }
-  // every lane goes through the loop (the maxima are shuffled in full warps)
-  for (int u = sub; u < 2 * p.Hk + sub; u += per) {
-    const bool on = u < 2 * p.Hk && row0 != kNoRow, key = u < p.Hk;
-    const int h = key ? u : u - p.Hk;
-    float x[16];
-    if (on) {
-      const DevT4& src = key ? p.kn : p.vn;
-      const I* at = static_cast<const I*>(src.p) + n * src.sb + h * src.sh;
-      const Eight<I> lo = ld8(at + 8 * l), hi = ld8(at + half + 8 * l);
-      widen(lo, x);
-      widen(hi, x + 8);
-      if (key && p.cos) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const float d0 = __fmul_rn(x[i], s[i]), d1 = __fmul_rn(x[i + 1], s[i + 1]);
-          const float e0 = __fmul_rn(x[8 + i], c[i]), e1 = __fmul_rn(x[9 + i], c[i + 1]);
-          add2(x[i], x[i + 1], __fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1]), __fmul_rn(x[8 + i], -s[i]),
-               __fmul_rn(x[9 + i], -s[i + 1]));
-          add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
-        }
-      }
-    }
-    const size_t row = (size_t)row0 + (size_t)h * p.page;
-    Eight<T> lo, hi;
-    if constexpr (Q) {
-      float a = 0.f;
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) a = max_abs(a, x[i]);
-      }
-      for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(0xffffffffu, a, o));
-      float scale, inv;
-      quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
-      if (on) {
-        if (l == 0) (key ? p.ks : p.vs)[row] = scale;
-        narrow_codes<DT>(lo, x, inv);
-        narrow_codes<DT>(hi, x + 8, inv);
-      }
-    } else if (on) {
-      narrow(lo, x);
-      narrow(hi, x + 8);
-    }
-    if (on) {
-      T* to = static_cast<T*>(key ? p.k : p.v) + row * HD + 8 * l;
-      st8(to, lo);
-      st8(to + half, hi);
-    }
-  }
+  const int h = write_heads<DT, I, true>(p, n, row0, sub, per, L, l, c, s);
+  write_heads<DT, I, false>(p, n, row0, h - p.Hk, per, L, l, c, s);
 }
 
 template <int DT, typename O>
@@ -373,8 +379,8 @@ bool vec_input(const DevT4& t, int dt) {
 }
 
 // Rows of a block: as many as leave each group at most 8 keys or values, fewer
-// where that gives less than six blocks an SM, down to one (the same prompts: 113.5 µs
-// at 8, 115.6 at 4, 115.2 at 12).
+// where that gives less than six blocks an SM, down to one (the same prompts: 110 µs
+// at 8, about 115 at 4 and at 12).
 constexpr int kGroupHeads = 8;
 int block_rows(const PagedP& p, int lanes, int sms) {
   const int groups = kThreads >> lanes;
