@@ -314,6 +314,7 @@ size_t paged_decode_bytes(const PagedP& p, int sms) {
 cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* launches) {
   const PagedPlan pl = plan(p, sms);
   cudaError_t e;
+  if ((long long)p.B * p.Hk * head_groups(p) * pl.S > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
   if (mma_path(p)) {
     switch (p.dt) {
       case BOZO_DT_BF16: e = launch_paged_mma_bf16(p, pl, st); break;

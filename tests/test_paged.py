@@ -350,6 +350,45 @@ def test_decode_long_rows_are_split_and_joined(dtype, HD):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,H,Hk,HD", [(BF16, 3, 3, 64), (I8, 6, 3, 32), (F16, 24, 3, 64), (F8, 3, 3, 128)])
+def test_decode_rows_in_two_pieces(dtype, H, Hk, HD):
+    """192 rows of a few hundred keys: two pieces, joined in a cluster, beside
+    rows of one piece and of none; new rows written by the piece that ends with them."""
+    io = dtype if dtype in ULP else BF16
+    lengths = [(37 * i) % 320 for i in range(62)] + [-1, 319]
+    tables = rope(HD, 330, "cuda")
+    pool = Pool(64, Hk, HD, 16, 20, dtype)
+    hist = fill(pool, lengths, Hk, HD, io, tables, HD)
+    q = torch.randn(64, H, HD, device="cuda").to(io)
+    k, v = (torch.randn(64, Hk, HD, device="cuda").to(io) for _ in "kv")
+    check_decode(pool, lengths, hist, q, window=None, tau_window=290, tables=tables, new=(k, v))
+    hist = history(pool, [t + 1 if t >= 0 else 0 for t in lengths], Hk, HD)
+    check_decode(pool, lengths, hist, q, window=250, normalize="count", tables=tables)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F8])
+def test_split_step_in_a_graph(dtype):
+    """The pieces and the kernel that joins them, captured and replayed with other
+    lengths than at the capture."""
+    io = dtype if dtype in ULP else BF16
+    pool = Pool(2, 1, 64, 16, 200, dtype)
+    fill(pool, [3200, 3000], 1, 64, io, None, 4)
+    q = torch.randn(2, 1, 64, device="cuda").to(io)
+    t = int32([5, 6])
+    run = lambda: paged.paged_tension(q, *pool.cache, t, window=None, **pool.scales)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for lens in ([3199, 17], [0, 2999], [130, -1], [1000, 2000]):
+        t.copy_(int32(lens))
+        q.normal_()
+        graph.replay()
+        assert torch.equal(out, run())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16, F8, I8])
 @pytest.mark.parametrize("shift", [-60.0, -25.0, 0.0, 40.0])
 def test_decode_scores_far_from_zero(dtype, shift):
