@@ -50,9 +50,13 @@ __device__ __forceinline__ Reach reach(const PagedP& p, int b, unsigned S) {
   r.lo = r.end - r.n;
   r.base = r.lo & ~15u;
   const unsigned len = r.end - r.base;
-  r.count = max(1u, min(S, (len + kMinPiece - 1) / kMinPiece));
-  r.size = max(16u, ((len + r.count - 1) / r.count + 15) & ~15u);
-  r.count = max(1u, (len + r.size - 1) / r.size);
+  r.count = 1;
+  r.size = max(16u, (len + 15) & ~15u);
+  if (S > 1) {
+    r.count = max(1u, min(S, (len + kMinPiece - 1) / kMinPiece));
+    r.size = max(16u, ((len + r.count - 1) / r.count + 15) & ~15u);
+    r.count = max(1u, (len + r.size - 1) / r.size);
+  }
   return r;
 }
 
@@ -72,13 +76,13 @@ __device__ __forceinline__ float* piece_mass(const PagedP& p, int S) {
 __device__ __forceinline__ bool writes_row(const PagedP& p, const Reach& r, unsigned piece, bool first) {
   return p.kn.p && r.active && (p.mode == BOZO_MODE_GLOBAL ? piece == r.count - 1 : piece == 0 && first);
 }
-__device__ __forceinline__ void append_row(const PagedP& p, int b, int hk, int t, int warp, int lane) {
-  if (warp > 1) return;
-  const bool key = warp == 0;
-  const NewRow x(p, key ? p.kn : p.vn, b, hk, (unsigned)t, key && p.cos, lane);
+__device__ __forceinline__ void append_row(const PagedP& p, int b, int hk, int t, int lane) {  // one warp
+  const NewRow k(p, p.kn, b, hk, (unsigned)t, p.cos != nullptr, lane), v(p, p.vn, b, hk, (unsigned)t, false, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
-  if (row0 != kNoRow)
-    x.put(p, key ? p.k : p.v, key ? p.ks : p.vs, (size_t)row0 + (size_t)hk * p.page, lane);
+  if (row0 == kNoRow) return;
+  const size_t row = (size_t)row0 + (size_t)hk * p.page;
+  k.put(p, p.k, p.ks, row, lane);
+  v.put(p, p.v, p.vs, row, lane);
 }
 
 // Rotated query element i of head h.

@@ -182,8 +182,15 @@ template <int SIZE, int R, bool V> __device__ __forceinline__ int ring_at(int r,
   }
 }
 
+// Block x: piece x mod S of key head hk's head group hg, (b·Hk + hk)·HG + hg = x / S.
+struct MmaGrid {
+  int S, G, HG;  // pieces, query heads of a key head, groups of them
+  FastDiv div_s, div_hg, div_hk;
+  bool clustered;
+};
+
 template <int DT, int HD, int GP, bool AL>
-__global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S, int HG, bool clustered) {
+__global__ void __launch_bounds__(kWarps * 32 + 32, 2) paged_decode_mma(PagedP p, MmaGrid grid) {
   using F = Fmt<DT>;
   using Z = Geo<DT, HD, GP>;
   constexpr bool BF = F::bf;
@@ -198,13 +205,11 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
   __shared__ float sq[kHeads][HD + 4];
   __shared__ float sback[kHeads];  // what undoes the power of two that q was multiplied by (halfs)
   __shared__ float smass[kWarps][kHeads];
-  const int G = p.H / p.Hk;
-  int x = blockIdx.x;
-  const int piece = x % S;
-  x /= S;
-  const int hg = x % HG;
-  x /= HG;
-  const int hk = x % p.Hk, b = x / p.Hk;
+  const int S = grid.S, G = grid.G;
+  const bool clustered = grid.clustered;
+  const unsigned row = fast_div(blockIdx.x, grid.div_s), head = fast_div(row, grid.div_hg);
+  const int piece = blockIdx.x - row * S, hg = row - head * grid.HG;
+  const int b = fast_div(head, grid.div_hk), hk = head - b * p.Hk;
   const int h0 = hk * G + hg * kHeads, Gh = min(kHeads, G - hg * kHeads);  // query heads h0 … h0+Gh−1
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const Reach rc = reach(p, b, S);
@@ -296,66 +301,71 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
       find(k + 1 + kBatch, nxt);
     }
   };
-  if (nk) {
-    find(0, cur);
-    find(AL ? kBatch : 1, nxt);
-  }
-  if (mine && rc.active)
-    for (int i = tid; i < GP * HD; i += kWarps * 32) {
-      const int h = i / HD, d = i - h * HD;
-      sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
-    }
+  // A warp beyond the others writes the new token's row.  Keys that end with it are
+  // read after a barrier: the one before the first tile is worked on, or if the
+  // row's tile is among those that are fetched before that, one of their own.
   const bool writes = writes_row(p, rc, piece, hg == 0);
-  if (writes && p.mode == BOZO_MODE_GLOBAL) {  // these keys end with the new one
-    append_row(p, b, hk, rc.t, warp, lane);
+  const bool early = writes && p.mode == BOZO_MODE_GLOBAL && nk <= (kStages - 1) * kWarps * KT;
+  if (warp == kWarps) {
+    if (writes) append_row(p, b, hk, rc.t, lane);
+    if (early) __syncthreads();
     __syncthreads();
-  }
-  if (nk)
-#pragma unroll
-    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
-  if (writes && p.mode == BOZO_MODE_LOCAL) append_row(p, b, hk, rc.t, warp, lane);
-  __syncthreads();
-  if (nk) {
+  } else {
     // columns of S: lane (g, c) holds k-pairs of column g, that is of head
     // (g/2) mod GQ (of each operand), its 16-bit part (g even) or the rest
     unsigned qb[NS][kSteps][2];
     float back[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int h = s * 4 + (g >> 1) % GQ;
-      float qs = 1.f;
-      if constexpr (!BF) {  // as halfs, brought near 1 by a power of two
-        float m = 0.f;
-        for (int d = c; d < HD; d += 4) m = fmaxf(m, fabsf(sq[h][d]));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const int e = m > 0.f ? min(126, max(-126, (int)(__float_as_uint(m) >> 23) - 127)) : 0;
-        qs = __uint_as_float((unsigned)(127 - e) << 23);
-        if (c == 0) sback[h] = __uint_as_float((unsigned)(127 + e) << 23);  // every warp the same
-      }
-      auto pair = [&](int d) {
-        const unsigned u = split<BF>(sq[h][d] * qs), v = split<BF>(sq[h][d + 1] * qs);
-        return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
-      };
-#pragma unroll
-      for (int k = 0; k < kSteps; ++k) {
-        if constexpr (SZ == 2) {
-          qb[s][k][0] = pair(16 * k + 2 * c);
-          qb[s][k][1] = pair(16 * k + 8 + 2 * c);
-        } else {
-          const int d = k / kKW * 4 * kKB + c * kKB + k % kKW * 4;
-          qb[s][k][0] = pair(d);
-          qb[s][k][1] = pair(d + 2);
-        }
-      }
-    }
-    __syncwarp();
-    // exponent of the sigmoid: −log2 e · score
-#pragma unroll
-    for (int s = 0; s < NS; ++s) back[s] = (BF ? 1.f : sback[s * 4 + c % GQ]) * p.inv_scale * -1.4426950408889634f;
     const int tsel = c / GQ % T;  // the tile (of T) whose τ this lane computes
     const int mrow = (lane & 7) + (lane & 8), mch = lane >> 4;  // row and piece of an 8×8 matrix's row
 
+    find(0, cur);
+    nxt[0] = kNoRow;
+    if (!AL || start(kBatch) < nk) find(AL ? kBatch : 1, nxt);
+    if (mine && rc.active)
+      for (int i = tid; i < GP * HD; i += kWarps * 32) {
+        const int h = i / HD, d = i - h * HD;
+        sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
+      }
+    if (early) __syncthreads();
+#pragma unroll 1
+    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
+    __syncthreads();
+    if (start(0) < nk) {
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int h = s * 4 + (g >> 1) % GQ;
+        float qs = 1.f;
+        if constexpr (!BF) {  // as halfs, brought near 1 by a power of two
+          float m = 0.f;
+          for (int d = c; d < HD; d += 4) m = fmaxf(m, fabsf(sq[h][d]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          const int e = m > 0.f ? min(126, max(-126, (int)(__float_as_uint(m) >> 23) - 127)) : 0;
+          qs = __uint_as_float((unsigned)(127 - e) << 23);
+          if (c == 0) sback[h] = __uint_as_float((unsigned)(127 + e) << 23);  // every warp the same
+        }
+        auto pair = [&](int d) {
+          const unsigned u = split<BF>(sq[h][d] * qs), v = split<BF>(sq[h][d + 1] * qs);
+          return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
+        };
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          if constexpr (SZ == 2) {
+            qb[s][i][0] = pair(16 * i + 2 * c);
+            qb[s][i][1] = pair(16 * i + 8 + 2 * c);
+          } else {
+            const int d = i / kKW * 4 * kKB + c * kKB + i % kKW * 4;
+            qb[s][i][0] = pair(d);
+            qb[s][i][1] = pair(d + 2);
+          }
+        }
+      }
+      __syncwarp();
+      // exponent of the sigmoid: −log2 e · score
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        back[s] = (BF ? 1.f : sback[s * 4 + c % GQ]) * p.inv_scale * -1.4426950408889634f;
+    }
     int slot = 0;
 #pragma unroll 1
     for (int k = 0; start(k) < nk; ++k) {
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
     float m = c / GQ < T ? mass[e] : 0.f;
 #pragma unroll
     for (int o = GQ; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-    if (lane < GQ) smass[warp][e * 4 + lane] = m;
+    if (lane < GQ && warp < kWarps) smass[warp][e * 4 + lane] = m;
   }
   float un = 1.f;  // of head g
   if constexpr (!BF) {
@@ -529,7 +539,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
       un = g < 4 ? un : u1;
     }
   }
-  if (g < Gh) {
+  if (g < Gh && warp < kWarps) {
     const float back = 1.f / un;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
@@ -541,7 +551,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
   }
   __syncthreads();
   float* sum = part + kWarps * Gh * HD;
-  for (int i = tid; i < Gh * HD; i += kWarps * 32) {
+  for (int i = tid; i < Gh * HD && warp < kWarps; i += kWarps * 32) {
     const int h = i / HD, d = i - h * HD;
     float o = 0.f, m = 0.f;
 #pragma unroll
@@ -561,12 +571,12 @@ __global__ void __launch_bounds__(kWarps * 32) paged_decode_mma(PagedP p, int S,
     }
   }
   if (p.tau && piece == 0)
-    for (int h = warp; h < Gh; h += kWarps) clear_tau(p, (size_t)b * p.H + h0 + h, rc.n, lane, 32);
+    for (int h = warp; h < Gh && warp < kWarps; h += kWarps) clear_tau(p, (size_t)b * p.H + h0 + h, rc.n, lane, 32);
   if (clustered) {
     // the pieces' sums through the cluster's shared memory, each block a part of
     // the elements, in the order of the pieces
     cluster_sync();
-    if (rc.count > 1)
+    if (rc.count > 1 && warp < kWarps)
       for (int i = tid + piece * kWarps * 32; i < Gh * HD; i += S * kWarps * 32) {
         const int h = i / HD, d = i - h * HD;
         float o = 0.f, m = 0.f;
@@ -600,7 +610,7 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hk * HG * pl.S));
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(kWarps * 32 + (p.kn.p ? 32 : 0));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -608,7 +618,7 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
   at.val.clusterDim = {(unsigned)pl.S, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = pl.clustered ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, p, pl.S, HG, pl.clustered);
+  return cudaLaunchKernelEx(&cfg, kern, p, MmaGrid{pl.S, G, HG, make_fastdiv(pl.S), make_fastdiv(HG), make_fastdiv(p.Hk), pl.clustered});
 }
 template <int DT, int HD, int GP>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
