@@ -31,9 +31,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
   const unsigned j0 = max(r.first(piece), r.lo), j1 = r.last(piece);
   if (r.active)
     for (int i = threadIdx.x; i < HD; i += kThreads) sq[i] = query(p, b, h, r.t, i);
-  if (writes_row(p, r, piece, h % (p.H / p.Hk) == 0)) {
-    if (warp == 0) append_row(p, b, hk, r.t, lane);
-  }
+  if (warp < 2 && writes_row(p, r, piece, h % (p.H / p.Hk) == 0)) append_part(p, b, hk, r.t, warp == 0, lane);
   __syncthreads();
   for (unsigned j = j0 + warp; j < j1; j += kThreads / 32) {
     const unsigned row0 = paged_row(p, b, j);
@@ -127,9 +125,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p,
       const int h = i / HD, d = i - h * HD;
       sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
     }
-  if (writes_row(p, rc, piece, hg == 0)) {
-    if (warp == 0) append_row(p, b, hk, rc.t, lane);
-  }
+  // the last two warps: the first ones fetch the query
+  if (warp >= kRowWarps - 2 && writes_row(p, rc, piece, hg == 0))
+    append_part(p, b, hk, rc.t, warp == kRowWarps - 1, lane);
   __syncthreads();
   const bool on[2] = {4 * l < HD, 4 * (l + L) < HD};
   const int own = NH == 1 ? 0 : l / (L / 4);  // the head whose τ this lane computes

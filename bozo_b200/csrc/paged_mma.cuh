@@ -160,6 +160,10 @@ template <int DT, int HD, int GP> struct Geo {
   static constexpr int scales = Fmt<DT>::scaled ? 2 * keys * 4 : 0;
   static constexpr int meta = scales + 16;                   // scales, and 16 bits a 16 keys: which are in reach
   static constexpr int pstride = keys + 8;                   // words of a head's τ
+  // Blocks an SM whose registers have to fit: two leave the compiler what it wants
+  // (e4m3 128 wide, 616 MB: 113 µs, with three 118; e4m3 32 wide 146 against 153),
+  // but 64 wide 8-bit rows are faster under the tighter bound (113 against 119).
+  static constexpr int blocks = Fmt<DT>::scaled && HD == 64 ? 3 : 2;
   static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * 4;
 };
 
@@ -190,7 +194,7 @@ struct MmaGrid {
 };
 
 template <int DT, int HD, int GP, bool AL>
-__global__ void __launch_bounds__(kWarps * 32 + 32, 2) paged_decode_mma(PagedP p, MmaGrid grid) {
+__global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) paged_decode_mma(PagedP p, MmaGrid grid) {
   using F = Fmt<DT>;
   using Z = Geo<DT, HD, GP>;
   constexpr bool BF = F::bf;
