@@ -233,22 +233,42 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p,
     for (int h = warp; h < Gh; h += kRowWarps) clear_tau(p, (size_t)b * p.H + h0 + h, rc.n, lane, 32);
 }
 
-// Rows cut into more than one piece: one block per (b, h).
+// Rows cut into more than one piece: one block per (b, h).  Groups of HD/4 threads
+// take every so many-th piece, so that all pieces' loads are in flight together,
+// and their sums are added in the groups' order.
 __global__ void __launch_bounds__(kThreads) paged_join(PagedP p, int S) {
+  __shared__ float part[kThreads * 4], smass[kThreads];
   const int bh = blockIdx.x, HD = p.HD;
-  grid_wait();
   const Reach r = reach(p, bh / p.H, S);
+  grid_wait();
   if (r.count < 2) return;
   const float* w = p.ws + (size_t)bh * S * HD;
   const float* wm = piece_mass(p, S) + (size_t)bh * S;
-  for (int d = threadIdx.x; d < HD; d += kThreads) {
-    float acc = 0.f, m = 0.f;
-#pragma unroll 8
-    for (unsigned i = 0; i < r.count; ++i) {
-      acc += w[i * HD + d];
+  const int each = HD % 4 ? 1 : 4, width = HD / each;  // elements of a thread, threads of a group
+  const int groups = kThreads / width, g = threadIdx.x / width, d = (threadIdx.x - g * width) * each;
+  if (g < groups) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, m = 0.f;
+#pragma unroll 4
+    for (unsigned i = g; i < r.count; i += groups) {
+      if (each == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(w + (size_t)i * HD + d);
+        acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+      } else {
+        acc[0] += w[(size_t)i * HD + d];
+      }
       m += wm[i];
     }
-    stf(p.out, (long long)bh * HD + d, p.out_dt, acc / norm_divisor(p, m, r.n));
+    for (int e = 0; e < each; ++e) part[g * HD + d + e] = acc[e];
+    if (d == 0) smass[g] = m;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < HD; i += kThreads) {
+    float acc = 0.f, m = 0.f;
+    for (int k = 0; k < groups; ++k) {
+      acc += part[k * HD + i];
+      m += smass[k];
+    }
+    stf(p.out, (long long)bh * HD + i, p.out_dt, acc / norm_divisor(p, m, r.n));
   }
 }
 
