@@ -8,6 +8,8 @@ Public API:
   install_as_triton_tension()
       registers this package under the module name ``triton_tension`` so the
       reference's model.py / train.py / generate.py import it unchanged.
+  paged.write_kv / read_kv / paged_tension, serving.PagedState / generate / ...
+      paged key/value caches and continuous batching (import the submodules).
 """
 from __future__ import annotations
 
