@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kThreads) paged_read_any(PagedP p) {
 // at once (one of B compares holds), each row's place by one thread; then groups of
 // HD/16 lanes go through the heads' keys and values of one row, sixteen elements a
 // lane: dimensions 8l … 8l+7 of either half of the row, so a lane has both halves of
-// its rotations, whose cosines and sines it loads once for all heads.
+// its rotations, whose cosines and sines it loads once for all heads.  A head's key
+// and value are in flight together.
 template <int DT> struct PageT;
 template <> struct PageT<BOZO_DT_F32> { using type = float; };
 template <> struct PageT<BOZO_DT_BF16> { using type = __nv_bfloat16; };
@@ -248,68 +249,54 @@ __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int r
 constexpr int kMaxRows = kThreads / 2;  // rows of a block, at most
 // What hides the chain from a sequence's offset to its rows is other blocks, so the
 // kernels keep to the registers that let this many stay on an SM (42136 rows of
-// 16 heads from bf16 to e4m3 and back: 110 µs; 114 with eight writing blocks, 122
-// with as few as the registers they would take, 118 in blocks of twice the threads;
-// with two rows' loads of a group in flight 128).
-constexpr int kWriteBlocks = 9, kReadBlocks = 16;
+// 16 heads from bf16 to e4m3 and back: 101 µs; with 16 reading blocks 104, with six
+// writing ones 110; a head's key and value one after the other 109).
+constexpr int kWriteBlocks = 9, kReadBlocks = 12;
 
-// A group's part of one row's keys (KEY) or values: heads h, h + per, … of p.Hk.
-// Returns the first head it did not take.
+// Sixteen elements a lane of one key (KEY) or value into its row.
 template <int DT, typename I, bool KEY>
-__device__ __forceinline__ int write_heads(const PagedP& p, unsigned n, unsigned row0, int h, int per, int L, int l,
-                                           const float* c, const float* s) {
+__device__ __forceinline__ void write_head(const PagedP& p, const Eight<I>& xl, const Eight<I>& xh, unsigned row, int L,
+                                           int l, unsigned group, const float* c, const float* s) {
   using T = typename PageT<DT>::type;
   constexpr bool Q = sizeof(T) == 1;
   const int half = L * 8, HD = half * 2;
-  const DevT4& src = KEY ? p.kn : p.vn;
-  const I* from = static_cast<const I*>(src.p) + n * src.sb + h * src.sh + 8 * l;
-  T* const pages = static_cast<T*>(KEY ? p.k : p.v) + 8 * l;
-  unsigned row = row0 + (unsigned)h * (unsigned)p.page;  // rows are numbered in 32 bits
-  const long long from_step = per * src.sh;
-  const unsigned row_step = (unsigned)(per * p.page);
-  const unsigned group = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
-#pragma unroll 1
-  for (; h < p.Hk; h += per, from += from_step, row += row_step) {
-    float x[16];
-    const Eight<I> xl = ld8(from), xh = ld8(from + half);
-    widen(xl, x);
-    widen(xh, x + 8);
-    if (KEY && p.cos) {
+  float x[16];
+  widen(xl, x);
+  widen(xh, x + 8);
+  if (KEY && p.cos) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float d0 = __fmul_rn(x[i], s[i]), d1 = __fmul_rn(x[i + 1], s[i + 1]);
-        const float e0 = __fmul_rn(x[8 + i], c[i]), e1 = __fmul_rn(x[9 + i], c[i + 1]);
-        add2(x[i], x[i + 1], __fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1]), __fmul_rn(x[8 + i], -s[i]),
-             __fmul_rn(x[9 + i], -s[i + 1]));
-        add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
-      }
+    for (int i = 0; i < 8; i += 2) {
+      const float d0 = __fmul_rn(x[i], s[i]), d1 = __fmul_rn(x[i + 1], s[i + 1]);
+      const float e0 = __fmul_rn(x[8 + i], c[i]), e1 = __fmul_rn(x[9 + i], c[i + 1]);
+      add2(x[i], x[i + 1], __fmul_rn(x[i], c[i]), __fmul_rn(x[i + 1], c[i + 1]), __fmul_rn(x[8 + i], -s[i]),
+           __fmul_rn(x[9 + i], -s[i + 1]));
+      add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
     }
-    Eight<T> yl, yh;
-    if constexpr (Q) {
-      float a = x[0];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) a = max_abs(a, x[i]);
-      for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(group, a, o));
-      float scale, inv;
-      quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
-      if (l == 0) (KEY ? p.ks : p.vs)[row] = scale;
-      narrow_codes<DT>(yl, x, inv);
-      narrow_codes<DT>(yh, x + 8, inv);
-    } else {
-      narrow(yl, x);
-      narrow(yh, x + 8);
-    }
-    T* to = pages + (size_t)row * HD;
-    st8(to, yl);
-    st8(to + half, yh);
   }
-  return h;
+  Eight<T> yl, yh;
+  if constexpr (Q) {
+    float a = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) a = max_abs(a, x[i]);
+    for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(group, a, o));
+    float scale, inv;
+    quant_scale(__float_as_uint(a) & 0x7fffffffu, DT == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+    if (l == 0) (KEY ? p.ks : p.vs)[row] = scale;
+    narrow_codes<DT>(yl, x, inv);
+    narrow_codes<DT>(yh, x + 8, inv);
+  } else {
+    narrow(yl, x);
+    narrow(yh, x + 8);
+  }
+  T* to = static_cast<T*>(KEY ? p.k : p.v) + (size_t)row * HD + 8 * l;
+  st8(to, yl);
+  st8(to + half, yh);
 }
 
 template <int DT, typename I>
 __global__ void __launch_bounds__(kThreads, kWriteBlocks) paged_write_vec(PagedP p, int lanes, int rows) {
   __shared__ unsigned srow[kMaxRows], spos[kMaxRows];
-  const int L = 1 << lanes, l = threadIdx.x & (L - 1);
+  const int L = 1 << lanes, l = threadIdx.x & (L - 1), half = L * 8;
   const int per = (kThreads >> lanes) / rows;  // groups of a row
   const int g = threadIdx.x >> lanes, r = g / per, sub = g - r * per;
   const unsigned n0 = blockIdx.x * rows, n = n0 + r;
@@ -318,12 +305,21 @@ __global__ void __launch_bounds__(kThreads, kWriteBlocks) paged_write_vec(PagedP
   if (row0 == kNoRow) return;
   float c[8], s[8];
   if (p.cos && sub < p.Hk) {
-    const size_t at = (size_t)spos[r] * (L * 8) + 8 * l;
+    const size_t at = (size_t)spos[r] * half + 8 * l;
     widen(ld8(p.cos + at), c);
     widen(ld8(p.sin + at), s);
   }
-  const int h = write_heads<DT, I, true>(p, n, row0, sub, per, L, l, c, s);
-  write_heads<DT, I, false>(p, n, row0, h - p.Hk, per, L, l, c, s);
+  const I* kf = static_cast<const I*>(p.kn.p) + n * p.kn.sb + sub * p.kn.sh + 8 * l;
+  const I* vf = static_cast<const I*>(p.vn.p) + n * p.vn.sb + sub * p.vn.sh + 8 * l;
+  unsigned row = row0 + (unsigned)sub * (unsigned)p.page;  // rows are numbered in 32 bits
+  const long long ks = per * p.kn.sh, vs = per * p.vn.sh;
+  const unsigned group = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
+#pragma unroll 1
+  for (int h = sub; h < p.Hk; h += per, kf += ks, vf += vs, row += (unsigned)(per * p.page)) {
+    const Eight<I> kl = ld8(kf), kh = ld8(kf + half), vl = ld8(vf), vh = ld8(vf + half);
+    write_head<DT, I, true>(p, kl, kh, row, L, l, group, c, s);
+    write_head<DT, I, false>(p, vl, vh, row, L, l, group, c, s);
+  }
 }
 
 template <int DT, typename O>
@@ -338,35 +334,46 @@ __global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p
   block_places<false>(p, n0, rows, srow, nullptr);
   const unsigned row0 = srow[r];
   if (n >= (unsigned)p.rows) return;
+  O* to[2] = {static_cast<O*>(p.k_out) + ((size_t)n * p.Hk + sub) * HD + 8 * l,
+              static_cast<O*>(p.v_out) + ((size_t)n * p.Hk + sub) * HD + 8 * l};
+  unsigned row = row0 + (unsigned)sub * (unsigned)p.page;
 #pragma unroll 1
-  for (int u = sub; u < 2 * p.Hk; u += per) {
-    const bool key = u < p.Hk;
-    const int h = key ? u : u - p.Hk;
-    float x[16];
+  for (int h = sub; h < p.Hk; h += per, row += (unsigned)(per * p.page)) {
+    Eight<T> lo[2], hi[2];
+    float scale[2] = {1.f, 1.f};
     if (row0 != kNoRow) {
-      const size_t row = (size_t)row0 + (size_t)h * p.page;
-      const T* at = static_cast<const T*>(key ? p.k : p.v) + row * HD + 8 * l;
-      const Eight<T> lo = ld8(at), hi = ld8(at + half);
-      if constexpr (Q) {
-        const float scale = __ldg((key ? p.ks : p.vs) + row);
-        widen_codes<DT>(lo, x);
-        widen_codes<DT>(hi, x + 8);
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) mul2(x[i], x[i + 1], x[i], x[i + 1], scale, scale);
-      } else {
-        widen(lo, x);
-        widen(hi, x + 8);
+      for (int j = 0; j < 2; ++j) {
+        const T* at = static_cast<const T*>(j ? p.v : p.k) + (size_t)row * HD + 8 * l;
+        lo[j] = ld8(at);
+        hi[j] = ld8(at + half);
+        if constexpr (Q) scale[j] = __ldg((j ? p.vs : p.ks) + row);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = 0.f;
     }
-    Eight<O> lo, hi;
-    narrow(lo, x);
-    narrow(hi, x + 8);
-    O* to = static_cast<O*>(key ? p.k_out : p.v_out) + ((size_t)n * p.Hk + h) * HD + 8 * l;
-    st8(to, lo);
-    st8(to + half, hi);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float x[16];
+      if (row0 != kNoRow) {
+        if constexpr (Q) {
+          widen_codes<DT>(lo[j], x);
+          widen_codes<DT>(hi[j], x + 8);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) mul2(x[i], x[i + 1], x[i], x[i + 1], scale[j], scale[j]);
+        } else {
+          widen(lo[j], x);
+          widen(hi[j], x + 8);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.f;
+      }
+      Eight<O> yl, yh;
+      narrow(yl, x);
+      narrow(yh, x + 8);
+      st8(to[j], yl);
+      st8(to[j] + half, yh);
+      to[j] += per * HD;
+    }
   }
 }
 
@@ -379,8 +386,8 @@ bool vec_input(const DevT4& t, int dt) {
 }
 
 // Rows of a block: as many as leave each group at most 8 keys or values, fewer
-// where that gives less than six blocks an SM, down to one (the same prompts: 110 µs
-// at 8, about 115 at 4 and at 12).
+// where that gives less than six blocks an SM, down to one (the same prompts: 101 µs
+// at 8, 105 at 4; reading 79868 rows out of e4m3 86 at 8 and 90 at 16).
 constexpr int kGroupHeads = 8;
 int block_rows(const PagedP& p, int lanes, int sms) {
   const int groups = kThreads >> lanes;
