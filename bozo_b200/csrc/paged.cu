@@ -385,7 +385,7 @@ bool vec_input(const DevT4& t, int dt) {
   return t.dt == dt && t.sd == 1 && !((reinterpret_cast<uintptr_t>(t.p) | (t.sb * e) | (t.sh * e)) & 15);
 }
 
-// Rows of a block: as many as leave each group at most 8 keys or values, fewer
+// Rows of a block: as many as leave each group at most 8 keys and values, fewer
 // where that gives less than six blocks an SM, down to one (the same prompts: 101 µs
 // at 8, 105 at 4; reading 79868 rows out of e4m3 86 at 8 and 90 at 16).
 constexpr int kGroupHeads = 8;
@@ -434,8 +434,9 @@ cudaError_t launch_paged_write(const PagedP& p, int sms, cudaStream_t st) {
       default: return write_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
-  const long long warps = p.rows * p.Hk;
-  paged_write_any<<<(unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(p);
+  const long long blocks = (p.rows * p.Hk + kThreads / 32 - 1) / (kThreads / 32);
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  paged_write_any<<<(unsigned)blocks, kThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 
@@ -450,8 +451,9 @@ cudaError_t launch_paged_read(const PagedP& p, int sms, cudaStream_t st) {
       default: return read_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
-  const long long warps = p.rows * p.Hk;
-  paged_read_any<<<(unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)), kThreads, 0, st>>>(p);
+  const long long blocks = (p.rows * p.Hk + kThreads / 32 - 1) / (kThreads / 32);
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
+  paged_read_any<<<(unsigned)blocks, kThreads, 0, st>>>(p);
   return cudaGetLastError();
 }
 

@@ -193,7 +193,8 @@ struct MmaGrid {
   bool clustered;
 };
 
-template <int DT, int HD, int GP, bool AL>
+// GR: positions from a multiple of GR on that lie in one page (16, 8 or 1).
+template <int DT, int HD, int GP, int GR>
 __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) paged_decode_mma(PagedP p, MmaGrid grid) {
   using F = Fmt<DT>;
   using Z = Geo<DT, HD, GP>;
@@ -233,16 +234,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * kStages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
   const char* kpages = static_cast<const char*>(p.k);
   const char* vpages = static_cast<const char*>(p.v);
-  // Row numbers: AL (16 positions from a multiple of 16 on lie in one page): lane
-  // L looks up 16 keys, those of tile (batch + L / NT), part L % NT; else one key
-  // each of the next tile.
-  constexpr int RR = AL ? 1 : (KT > 32 ? KT / 32 : 1), kBatch = 32 / NT;
+  // Row numbers.  GR > 1: a look-up for GR keys, 32 of them at once, kBatch tiles'
+  // worth; else one for each key of the next tile.
+  constexpr bool AL = GR > 1;
+  constexpr int RR = AL ? 1 : (KT > 32 ? KT / 32 : 1), kUnits = AL ? KT / GR : 1, kBatch = 32 / kUnits;
   unsigned cur[RR], nxt[RR];
   auto start = [&](int k) { return (unsigned)(warp + k * kWarps) * KT; };  // first key of the warp's tile k
   auto find = [&](int k, unsigned* rows) {
 #pragma unroll
     for (int r = 0; r < RR; ++r) {
-      const unsigned j = AL ? start(k + lane / NT) + lane % NT * 16 : start(k) + r * 32 + (KT < 32 ? lane % KT : lane);
+      const unsigned j =
+          AL ? start(k + lane / kUnits) + lane % kUnits * GR : start(k) + r * 32 + (KT < 32 ? lane % KT : lane);
       rows[r] = kNoRow;
       if (j < nk && (AL || p0 + j >= rc.lo)) {
         const unsigned row = paged_row(p, b, p0 + j);
@@ -255,25 +257,29 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     char* md = meta + slot * Z::meta;
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
-      const int src = AL ? k % kBatch * NT + u : 0;
-      const unsigned row = AL ? __shfl_sync(0xffffffffu, cur[0], src) : 0u;
+      // rows of these 16 keys: from r0 on, and with GR 8 from r1 on the last eight
+      const int src = AL ? k % kBatch * kUnits + u * 16 / GR : 0;
+      const unsigned r0 = AL ? __shfl_sync(0xffffffffu, cur[0], src) : 0u;
+      const unsigned r1 = GR == 8 ? __shfl_sync(0xffffffffu, cur[0], src + 1) : r0;
       const unsigned pos = p0 + start(k) + u * 16;
-      // the row of key r of these 16, or kNoRow
+      auto whole = [&](int r) { return GR == 8 && r >= 8 ? r1 + r - 8 : r0 + r; };
+      // the row of key r, or kNoRow
       auto row_of = [&](int r) {
-        if constexpr (AL) return row == kNoRow || pos + r < rc.lo || pos + r >= p1 ? kNoRow : row + r;
+        if constexpr (AL) return (r < 8 ? r0 : r1) == kNoRow || pos + r < rc.lo || pos + r >= p1 ? kNoRow : whole(r);
         else return __shfl_sync(0xffffffffu, cur[u / 2], (u * 16 + r) % 32);
       };
-      if (AL && row != kNoRow && pos >= rc.lo && pos + 16 <= p1) {
-        const size_t at = (size_t)row * R + lane * 16;
-        const char *ka = kpages + at, *va = vpages + at;
+      if (AL && r0 != kNoRow && r1 != kNoRow && pos >= rc.lo && pos + 16 <= p1) {
+        // rows that follow each other: from the first on 512 bytes a round
+        const size_t at = (size_t)r0 * R + lane * 16, at1 = (size_t)r1 * R + lane * 16;
 #pragma unroll
         for (int it = 0; it < (NCH + 1) / 2; ++it) {
-          const int r = u * 16 + (it * 32 + lane) / NCH, ch = lane % NCH;
-          copy16(kd + ring_at<SZ, R, false>(r, ch), ka + it * 512);
-          copy16(vd + ring_at<SZ, R, true>(r, ch), va + it * 512);
+          const int r = (it * 32 + lane) / NCH, ch = lane % NCH;
+          const size_t from = GR == 8 && r >= 8 ? at1 + it * 512 - 8 * R : at + it * 512;
+          copy16(kd + ring_at<SZ, R, false>(u * 16 + r, ch), kpages + from);
+          copy16(vd + ring_at<SZ, R, true>(u * 16 + r, ch), vpages + from);
         }
         if (F::scaled) copy4(smem_u32(md) + (((lane >> 4) * KT + u * 16 + (lane & 15)) << 2),
-                             (lane < 16 ? p.ks : p.vs) + row + (lane & 15), 4);
+                             (lane < 16 ? p.ks : p.vs) + whole(lane & 15), 4);
         if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = 0xffffu;
       } else {
 #pragma unroll
@@ -595,13 +601,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   }
 }
 
-template <int DT, int HD, int GP, bool AL>
+template <int DT, int HD, int GP, int GR>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
   const int G = p.H / p.Hk, HG = (G + kHeads - 1) / kHeads;
   const size_t ring = (size_t)kWarps * Geo<DT, HD, GP>::warp;
   const size_t part = (size_t)(kWarps + 1) * std::min(G, kHeads) * HD * sizeof(float);
   const size_t smem = std::max(ring, part);
-  auto kern = paged_decode_mma<DT, HD, GP, AL>;
+  auto kern = paged_decode_mma<DT, HD, GP, GR>;
   static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -626,8 +632,8 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
 }
 template <int DT, int HD, int GP>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
-  return p.page % 16 == 0 ? launch_paged_mma<DT, HD, GP, true>(p, pl, st)
-                          : launch_paged_mma<DT, HD, GP, false>(p, pl, st);
+  if (p.page % 16 == 0) return launch_paged_mma<DT, HD, GP, 16>(p, pl, st);
+  return p.page % 8 == 0 ? launch_paged_mma<DT, HD, GP, 8>(p, pl, st) : launch_paged_mma<DT, HD, GP, 1>(p, pl, st);
 }
 template <int DT, int HD>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
