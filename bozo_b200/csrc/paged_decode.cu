@@ -285,26 +285,29 @@ int head_groups(const PagedP& p) {
 }
 
 // Pieces of a row.  About three blocks an SM keep the memory busy (16 rows of
-// 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37; 192 rows of
-// 1024 keys: 11.9 µs whole, 10.5 in two, 13.6 in four).  Sequences of different
-// lengths want smaller pieces to even out — twelve an SM, of 2048 keys at least
-// (1024 rows of up to 8192 keys: 165 µs in two to four; 512 rows of up to 16384
-// keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).
-// Two pieces are joined inside a cluster; a cluster of more waits longer for its
-// place than a second kernel takes (192 rows in three: 15.2 against 14.2 µs), and a
-// second kernel costs 3 µs of a call, which short rows do not earn back (48 rows of
-// 256 keys: 5.2 µs whole, 5.9 in two, 6.5 in more; of 512 keys: 6.8, 6.5, 6.6; of 1024
-// keys: 9.7, 8.0, 6.8).
+// 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37).  Sequences
+// of different lengths want smaller pieces to even out — twelve an SM, of 2048 keys
+// at least (1024 rows of up to 8192 keys: 165 µs in two to four; 512 rows of up to
+// 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).
+// Up to eight pieces are joined inside a cluster, which saves a second kernel's
+// 2-3 µs of a call, where the clusters all find their place at once (12 rows of 1024
+// keys in eight: 5.9 µs and 8.2 a call, 6.1 and 10.1 with a second kernel; 192 rows
+// in four: 14.5 against 13.6); so a few pieces more than eight become eight, and
+// whatever is asked for where that leaves 256 keys (12 rows of 2048 keys: 6.5
+// against 6.7 µs in sixteen; of 8192 keys 11.2 against 8.7).  Short rows stay whole
+// (48 rows of 256 keys: 5.2 µs, 5.9 in two).
 PagedPlan plan(const PagedP& p, int sms) {
+  constexpr int kCluster = 8;
   const bool mma = mma_path(p);
   const long long keys = p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap;
   const long long rows = (long long)p.B * p.Hk * head_groups(p);
-  long long s = (3LL * sms + rows / 2) / rows;
+  long long s = 3LL * sms / rows;
   if (p.B > 1) s = std::max(s, std::min((12LL * sms + rows - 1) / rows, keys / 2048));
-  s = std::min(s, keys <= 256 ? 1 : keys <= 512 ? (mma ? 2 : 1) : (keys + 15 + kMinPiece - 1) / kMinPiece);
+  s = std::min(s, keys <= (mma ? 256 : 512) ? 1 : (keys + 15 + kMinPiece - 1) / kMinPiece);
+  if (mma && s > kCluster && (s <= kCluster + 4 || keys <= 256 * kCluster)) s = kCluster;
   if (!mma && !rows_path(p)) s = std::max(s, (keys + 15 + kMaxPiece - 1) / kMaxPiece);
   s = std::max(s, 1LL);
-  return {(int)s, mma && s == 2};
+  return {(int)s, mma && (s == 2 || (s > 2 && s <= kCluster && rows * s <= 3LL * sms))};
 }
 
 template <int DT>

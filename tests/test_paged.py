@@ -367,6 +367,26 @@ def test_decode_rows_in_two_pieces(dtype, H, Hk, HD):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,H,Hk,HD", [(BF16, 2, 2, 64), (F16, 18, 2, 32), (F8, 8, 2, 128), (I8, 2, 2, 64)])
+@pytest.mark.parametrize("cap", [496, 1040, 2048])
+def test_decode_rows_joined_in_clusters(dtype, H, Hk, HD, cap):
+    """Few rows: four to eight pieces in a cluster, rows of fewer pieces, of one
+    and of none among them; the longest have wrapped their ring."""
+    io = dtype if dtype in ULP else BF16
+    lengths = [cap + 5, cap - 1, cap // 2, 130, 129, 1, 0, -1]
+    tables = rope(HD, cap + 8, "cuda")
+    pool = Pool(8, Hk, HD, 16, cap // 16, dtype)
+    hist = fill(pool, lengths, Hk, HD, io, tables, HD)
+    q = torch.randn(8, H, HD, device="cuda").to(io)
+    k, v = (torch.randn(8, Hk, HD, device="cuda").to(io) for _ in "kv")
+    out, row = check_decode(pool, lengths, hist, q, window=None, tau_window=cap, tables=tables, new=(k, v))
+    assert ops.last_launches() == 1
+    again = paged.paged_tension(q, *pool.cache, int32(lengths), window=None, rope=tables, return_tau=True,
+                                tau_window=cap, **pool.scales)
+    assert torch.equal(again[0], out) and torch.equal(again[1], row)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F8])
 def test_split_step_in_a_graph(dtype):
     """The pieces and the kernel that joins them, captured and replayed with other
