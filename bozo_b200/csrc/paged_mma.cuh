@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <utility>
 
 #include "paged_decode.cuh"
 
@@ -65,10 +66,8 @@ __device__ __forceinline__ unsigned split(float x) {
 template <int DT>
 __device__ __forceinline__ void widen4(unsigned x, unsigned& p01, unsigned& p23) {
   if constexpr (DT == BOZO_DT_F8E4M3) {
-    const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x & 0xffffu), __NV_E4M3);
-    const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(x >> 16), __NV_E4M3);
-    p01 = *reinterpret_cast<const unsigned*>(&a);
-    p23 = *reinterpret_cast<const unsigned*>(&b);
+    asm("{.reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h;}"
+        : "=r"(p01), "=r"(p23) : "r"(x));
   } else {
     // 1024 + (code + 128) is the half with those low bits; less 1152 it is the code
     const unsigned u = x ^ 0x80808080u;
@@ -91,27 +90,24 @@ __device__ __forceinline__ float sigmoid_exp2(float y) {
 }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ uint4 lds128(unsigned a) {
-  uint4 x;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a) : "memory");
-  return x;
-}
-__device__ __forceinline__ uint2 lds64(unsigned a) {
-  uint2 x;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x.x), "=r"(x.y) : "r"(a) : "memory");
-  return x;
-}
-template <int N>  // N 32-bit words
+template <int N, int OFF>  // N 32-bit words at a + OFF
 __device__ __forceinline__ void lds_words(unsigned a, unsigned* w) {
-  if constexpr (N == 4) {
-    const uint4 x = lds128(a);
-    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-  } else if constexpr (N == 2) {
-    const uint2 x = lds64(a);
-    w[0] = x.x; w[1] = x.y;
-  } else {
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
-  }
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a), "n"(OFF) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2 + %3];" : "=r"(w[0]), "=r"(w[1]) : "r"(a), "n"(OFF) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(w[0]) : "r"(a), "n"(OFF) : "memory");
+}
+// f(0), f(1), … f(N − 1) with the number as a constant
+template <int... I, typename F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each_of(std::make_integer_sequence<int, N>{}, f);
 }
 template <bool T>
 __device__ __forceinline__ void ldmatrix4(unsigned a, unsigned* w) {
@@ -124,8 +120,9 @@ __device__ __forceinline__ void ldmatrix4(unsigned a, unsigned* w) {
 }
 
 // Asynchronous copies to shared memory; `bytes` 0 fills with zeros.
+template <int DST, int SRC>
 __device__ __forceinline__ void copy16(unsigned dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
 }
 __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -203,6 +200,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   constexpr int GQ = GP < 4 ? GP : 4, NS = GP == 8 ? 2 : 1;        // heads of an 8-column operand, operands
   constexpr int T = GP == 8 ? 1 : (NT < 4 / GQ ? NT : 4 / GQ);     // 16-key tiles whose scores the lanes share out
   constexpr int kSteps = HD / 16, kTiles = HD / 8;
+  constexpr int NC = NS == 1 && kSteps >= 4 ? 2 : 1;  // sums that a score's products run in side by side
   // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
   constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
   constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB / 4;
@@ -271,14 +269,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       if (AL && r0 != kNoRow && r1 != kNoRow && pos >= rc.lo && pos + 16 <= p1) {
         // rows that follow each other: from the first on 512 bytes a round
         const size_t at = (size_t)r0 * R + lane * 16, at1 = (size_t)r1 * R + lane * 16;
-#pragma unroll
-        for (int it = 0; it < (NCH + 1) / 2; ++it) {
-          const int r = (it * 32 + lane) / NCH, ch = lane % NCH;
-          const size_t from = GR == 8 && r >= 8 ? at1 + it * 512 - 8 * R : at + it * 512;
-          copy16(kd + ring_at<SZ, R, false>(u * 16 + r, ch), kpages + from);
-          copy16(vd + ring_at<SZ, R, true>(u * 16 + r, ch), vpages + from);
-        }
-        if (F::scaled) copy4(smem_u32(md) + (((lane >> 4) * KT + u * 16 + (lane & 15)) << 2),
+        // a round's place in the ring: the permutation repeats every 8 rows
+        constexpr int kSame = 8 * NCH / 32 < 1 ? 1 : 8 * NCH / 32;  // rounds of 8 rows
+        const char *ka = kpages + at, *va = vpages + at, *kb = kpages + at1, *vb = vpages + at1;
+        each<(NCH + 1) / 2>([&](auto i) {
+          constexpr int it = i, first = it % kSame, back = (it - first) * 512;
+          const int r = (first * 32 + lane) / NCH, ch = lane % NCH;
+          const bool second = GR == 8 && (it * 32 + lane) / NCH >= 8;
+          copy16<back, it * 512>(kd + u * 16 * R + ring_at<SZ, R, false>(r, ch), second ? kb - 8 * R : ka);
+          copy16<back, it * 512>(vd + u * 16 * R + ring_at<SZ, R, true>(r, ch), second ? vb - 8 * R : va);
+        });
+        if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
                              (lane < 16 ? p.ks : p.vs) + whole(lane & 15), 4);
         if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = 0xffffu;
       } else {
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           copy16(vd + ring_at<SZ, R, true>(u * 16 + r, ch), vpages + at, rr == kNoRow ? 0 : 16);
         }
         const unsigned rr = row_of(lane & 15);
-        if (F::scaled) copy4(smem_u32(md) + (((lane >> 4) * KT + u * 16 + (lane & 15)) << 2),
+        if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
                              (lane < 16 ? p.ks : p.vs) + (rr == kNoRow ? 0u : rr), rr == kNoRow ? 0 : 4);
         const unsigned m = __ballot_sync(0xffffffffu, rr != kNoRow);
         if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = (unsigned short)m;
@@ -384,15 +385,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       feed(slot == 0 ? kStages - 1 : slot - 1, k + kStages - 1);
       const unsigned kt = ring + slot * 2 * Z::kv, vt = kt + Z::kv;
       const char* md = meta + slot * Z::meta;
-      const float* sc = reinterpret_cast<const float*>(md);
+      const float2* sc = reinterpret_cast<const float2*>(md);
       slot = slot == kStages - 1 ? 0 : slot + 1;
 #pragma unroll
       for (int q = 0; q < NT / T; ++q) {
-        float s[T][NS][4];
+        float s[T][NS][NC][4];
 #pragma unroll
         for (int u = 0; u < T; ++u) {
 #pragma unroll
-          for (int e = 0; e < NS; ++e) s[u][e][0] = s[u][e][1] = s[u][e][2] = s[u][e][3] = 0.f;
+          for (int e = 0; e < NS; ++e)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[u][e][i][0] = s[u][e][i][1] = s[u][e][i][2] = s[u][e][i][3] = 0.f;
           const int r0 = (q * T + u) * 16;
           if constexpr (SZ == 2) {
             const unsigned a = kt + ring_at<SZ, R, false>(r0 + mrow, mch);
@@ -401,15 +404,20 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               unsigned w[4];
               ldmatrix4<false>(a ^ (st << 5), w);
 #pragma unroll
-              for (int e = 0; e < NS; ++e) mma16816<BF>(s[u][e], w[0], w[1], w[2], w[3], qb[e][st][0], qb[e][st][1]);
+              for (int e = 0; e < NS; ++e)
+                mma16816<BF>(s[u][e][st % NC], w[0], w[1], w[2], w[3], qb[e][st][0], qb[e][st][1]);
             }
           } else {
+            // 8 rows on the permutation is the same, and where a row is longer than a
+            // line two 16-byte pieces on it is that with another bit turned over
+            const int byte0 = c * kKB;
+            const unsigned a0_ = kt + r0 * R + ring_at<SZ, R, false>(g, byte0 >> 4) + (byte0 & 15);
 #pragma unroll
             for (int l = 0; l < kKL; ++l) {
               unsigned ka[kKW], kb[kKW];
-              const int byte = l * 4 * kKB + c * kKB;
-              lds_words<kKW>(kt + ring_at<SZ, R, false>(r0 + g, byte >> 4) + (byte & 15), ka);
-              lds_words<kKW>(kt + ring_at<SZ, R, false>(r0 + g + 8, byte >> 4) + (byte & 15), kb);
+              const unsigned at = a0_ ^ (l * 4 * kKB);
+              lds_words<kKW, 0>(at, ka);
+              lds_words<kKW, 8 * R>(at, kb);
 #pragma unroll
               for (int w = 0; w < kKW; ++w) {
                 unsigned a0, a1, a2, a3;
@@ -417,7 +425,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
                 widen4<DT>(kb[w], a1, a3);
 #pragma unroll
                 for (int e = 0; e < NS; ++e)
-                  mma16816<BF>(s[u][e], a0, a1, a2, a3, qb[e][l * kKW + w][0], qb[e][l * kKW + w][1]);
+                  mma16816<BF>(s[u][e][(l * kKW + w) % NC], a0, a1, a2, a3, qb[e][l * kKW + w][0],
+                               qb[e][l * kKW + w][1]);
               }
             }
           }
@@ -427,19 +436,22 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
         const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::scales)[tile] >> g;
         float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
         if constexpr (F::scaled) {
-          ks[0] = sc[tile * 16 + g];
-          ks[1] = sc[tile * 16 + g + 8];
-          vs[0] = sc[KT + tile * 16 + g];
-          vs[1] = sc[KT + tile * 16 + g + 8];
+          const float2 a = sc[tile * 16 + g], c2 = sc[tile * 16 + g + 8];  // a key's and a value's
+          ks[0] = a.x, vs[0] = a.y, ks[1] = c2.x, vs[1] = c2.y;
         }
 #pragma unroll
         for (int e = 0; e < NS; ++e) {
           float pr[2];
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
-            float z = s[0][e][2 * o] + s[0][e][2 * o + 1];
+            float z = 0.f;
 #pragma unroll
-            for (int u = 1; u < T; ++u) z = tsel == u ? s[u][e][2 * o] + s[u][e][2 * o + 1] : z;
+            for (int u = 0; u < T; ++u) {
+              float y = s[u][e][0][2 * o] + s[u][e][0][2 * o + 1];
+#pragma unroll
+              for (int i = 1; i < NC; ++i) y += s[u][e][i][2 * o] + s[u][e][i][2 * o + 1];
+              z = u == 0 || tsel == u ? y : z;
+            }
             z *= back[e];
             if constexpr (F::scaled) z *= ks[o];
             const bool on = (live >> (8 * o)) & 1;
@@ -487,11 +499,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
         unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0;
         if (g < GP) {
           const unsigned at = smem_u32(ps + g * Z::pstride + u * 16 + 2 * c);
-          const uint2 x = lds64(at), y = lds64(at + 32);
-          a0 = __byte_perm(x.x, x.y, 0x7632);
-          a1 = __byte_perm(x.x, x.y, 0x5410);
-          a2 = __byte_perm(y.x, y.y, 0x7632);
-          a3 = __byte_perm(y.x, y.y, 0x5410);
+          unsigned x[2], y[2];
+          lds_words<2, 0>(at, x);
+          lds_words<2, 32>(at, y);
+          a0 = __byte_perm(x[0], x[1], 0x7632);
+          a1 = __byte_perm(x[0], x[1], 0x5410);
+          a2 = __byte_perm(y[0], y[1], 0x7632);
+          a3 = __byte_perm(y[0], y[1], 0x5410);
         }
         if constexpr (SZ == 2) {
           const unsigned a = vt + ring_at<SZ, R, true>(u * 16 + mrow, mch);
@@ -507,10 +521,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           for (int l = 0; l < kVL; ++l) {
             unsigned vw[4][kVW];
             const int byte = l * 8 * kVB + g * kVB;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              lds_words<kVW>(vt + ring_at<SZ, R, true>(u * 16 + 8 * (i >> 1) + 2 * c + (i & 1), byte >> 4) + (byte & 15),
-                             vw[i]);
+            // rows 2c and 2c + 1 of each eight
+            const unsigned v0 = vt + u * 16 * R + ring_at<SZ, R, true>(2 * c, byte >> 4) + (byte & 15);
+            const unsigned v1 = vt + u * 16 * R + ring_at<SZ, R, true>(2 * c + 1, byte >> 4) + (byte & 15);
+            lds_words<kVW, 0>(v0, vw[0]);
+            lds_words<kVW, 0>(v1, vw[1]);
+            lds_words<kVW, 8 * R>(v0, vw[2]);
+            lds_words<kVW, 8 * R>(v1, vw[3]);
 #pragma unroll
             for (int w = 0; w < kVW; ++w)
 #pragma unroll
