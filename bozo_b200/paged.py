@@ -94,7 +94,9 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
                t − (W − w) (local); ``[B, H, tau_window]``, column c is key t − c
                (global); zero where there is no key.
 
-    Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.
+    Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.  A NaN or an infinity
+    in a query, or in a row that it reaches, makes that query's output NaN; rows
+    out of reach may hold anything.
     """
     norm = ops._NORM.get(normalize, -1)
     if norm < 0:
