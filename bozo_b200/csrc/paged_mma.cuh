@@ -5,17 +5,25 @@
 // tiles of its own through a ring in shared memory that 16-byte asynchronous
 // copies fill a few tiles ahead (rows out of reach are filled with zeros), and
 // feeds mma.m16n8k16 from it; nothing is shared between warps before the end.
-//   Sᵀ = K·Qᵀ  16 keys by 8 columns: a column is a query head's q rounded to 16
-//              bits or what that rounding left of it, side by side, so the sum
-//              of two neighbouring accumulators (in one lane) has q to 16 bits
-//              and more.  Up to 4 heads fit; where there are fewer, the columns
+//   Sᵀ = K·Qᵀ  16 keys by 8 columns: a column is a query head's q in 16 bits or
+//              what that left of it, side by side, so the sum of neighbouring
+//              accumulators has both.  Where there are few heads, the columns
 //              repeat them and each group of lanes takes its scores from a tile
 //              of its own, so that every lane computes different τ.
 //   O  = P·V   rows 0-7 the heads' τ (· the value row's scale) in 16 bits, rows
 //              8-15 what that left; τ goes from lanes to operands through a few
 //              words of shared memory.
-// Scores, τ, both sums and what is joined are fp32; the 16-bit parts keep q and τ to
-// 2^-17 (halfs: 2^-22 of the largest, which a power of two brings near one).
+// Scores, τ, both sums and what is joined are fp32.  Two halfs keep q and τ to 2^-22
+// of the largest, which a power of two brings near one.  A bf16 has 8 of fp32's 24
+// bits: q and τ go in as three, cut off one after the other, and are exact (two parts
+// keep 2^-17 of each, which an fp32 output showed as twenty times fp32's error).  The
+// three parts of q are
+//   up to 2 heads: four columns (one empty); two lanes share a sum and take a key each,
+//   4 heads:       two columns and, in a product of its own, the first one again,
+//   8 heads:       a column for each head, three products;
+// those of τ rows of their own with up to 4 heads, a second product with 8.  That costs
+// nothing measurable with a head or two of 64 or 128 elements, 2-8 % at 32, 3 % with four
+// heads and 9-17 % with eight (309 MB, 128 wide: 80 µs, with two parts 68).
 //
 // What bounds it: 1 flop a byte for 16-bit rows of a head of their own (memory),
 // instructions for 8-bit rows of shared heads.  4 warps with 3 tiles of 4 KB each and
@@ -55,19 +63,17 @@ __device__ __forceinline__ void mma16816(float* d, unsigned a0, unsigned a1, uns
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// x as a 16-bit number (high half) and what that left of it (low half)
-template <bool BF>
+// x as a half (high half) and what that left of it (low half)
 __device__ __forceinline__ unsigned split(float x) {
   unsigned w;
-  if constexpr (BF) {
-    unsigned h;  // bf16(x) in the high half is that number in fp32
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(x), "f"(0.f));
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x), "f"(x - __uint_as_float(h)));
-  } else {
-    const float h = __half2float(__float2half_rn(x));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x), "f"(x - h));
-  }
+  const float h = __half2float(__float2half_rn(x));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(x), "f"(x - h));
   return w;
+}
+// x = its first bf16 + the rest, exactly; the first bf16 of x and of y
+__device__ __forceinline__ float less_top(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ unsigned tops(float x, float y) {
+  return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
 }
 
 // Four 8-bit codes as two pairs of halfs (exact).
@@ -168,9 +174,10 @@ template <int DT, int HD, int GP> struct Geo {
   // Blocks an SM whose registers have to fit: two leave the compiler what it wants
   // (e4m3 128 wide, 616 MB: 113 µs, with three 118; e4m3 32 wide 146 against 153),
   // but 64 wide 8-bit rows are faster under the tighter bound (e4m3, 634 MB: 113
-  // against 119).
-  static constexpr int blocks = Fmt<DT>::scaled && HD == 64 ? 3 : 2;
-  static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * 4;
+  // against 119), and so are 64 wide bf16 rows of up to four heads, which else take
+  // a few registers too many for a third block (617 MB: 96.7 against 99.7).
+  static constexpr int blocks = HD == 64 && (Fmt<DT>::scaled || (Fmt<DT>::bf && GP <= 4)) ? 3 : 2;
+  static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
 };
 
 // Byte offset of 16-byte piece ch of row r of a K or V tile with R-byte rows.  The
@@ -206,10 +213,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   using Z = Geo<DT, HD, GP>;
   constexpr bool BF = F::bf;
   constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size;
-  constexpr int GQ = GP < 4 ? GP : 4, NS = GP == 8 ? 2 : 1;        // heads of an 8-column operand, operands
-  constexpr int T = GP == 8 ? 1 : (NT < 4 / GQ ? NT : 4 / GQ);     // 16-key tiles whose scores the lanes share out
+  constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns a head, one
+  constexpr int GQ = GP < 4 ? GP : 4;                              // heads whose columns repeat
+  constexpr int NS = GP == 8 ? 2 : 1;                              // heads of a lane
+  constexpr int NA = WIDE ? 1 : NS, NB = QUAD ? 1 : WIDE ? 3 : BF ? 2 : NS;  // accumulators, operands
+  constexpr int kCopies = (QUAD ? 2 : 4) / GQ;                     // groups of lanes with the same columns
+  constexpr int T = NT < kCopies ? NT : kCopies;                   // 16-key tiles whose scores they share out
   constexpr int kSteps = HD / 16, kTiles = HD / 8;
-  constexpr int NC = NS == 1 && kSteps >= 4 ? 2 : 1;  // sums that a score's products run in side by side
+  // sums that a score's products run in side by side
+  constexpr int NC = NA == 1 && kSteps * (BF ? NB : 1) >= 4 ? 2 : 1;
+  constexpr int NK = QUAD ? 1 : 2;      // keys of a lane, of a tile's 16
+  constexpr bool FOLD = BF && GP <= 4;  // τ's second parts have rows 4-7 of P
   // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
   constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
   constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB / 4;
@@ -239,6 +253,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   const unsigned ring = smem_u32(smb) + warp * kStages * 2 * Z::kv;
   char* meta = smb + kWarps * kStages * 2 * Z::kv + warp * kStages * Z::meta;
   unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * kStages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
+  char* lo = smb + kWarps * (kStages * (2 * Z::kv + Z::meta) + GP * Z::pstride * 4) + warp * GP * Z::pstride * 2;  // τ's third parts
   const char* kpages = static_cast<const char*>(p.k);
   const char* vpages = static_cast<const char*>(p.v);
   // Row numbers.  GR > 1: a look-up for GR keys, 32 of them at once, kBatch tiles'
@@ -331,11 +346,16 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     if (early) __syncthreads();
     __syncthreads();
   } else {
-    // columns of S: lane (g, c) holds k-pairs of column g, that is of head
-    // (g/2) mod GQ (of each operand), its 16-bit part (g even) or the rest
-    unsigned qb[NS][kSteps][2];
+    // columns of S: lane (g, c) holds k-pairs of column g.  Of halfs that is head
+    // (g/2) mod GQ of each operand, its 16-bit part (g even) or the rest.
+    unsigned qb[NB][kSteps][2];
     float back[NS];
-    const int tsel = c / GQ % T;  // the tile (of T) whose τ this lane computes
+    // the heads, the tile (of T) and the keys whose τ this lane computes; one of the
+    // lanes with the same
+    auto head_of = [&](int e) { return QUAD ? (c >> 1) % GQ : WIDE ? 2 * c + e : e * 4 + c % GQ; };
+    auto key_of = [&](int o) { return g + (QUAD ? 8 * (c & 1) : 8 * o); };
+    const int copy = WIDE ? 0 : (QUAD ? c >> 1 : c) / GQ, tsel = copy % T;
+    const bool once = copy < T;
     const int mrow = (lane & 7) + (lane & 8), mch = lane >> 4;  // row and piece of an 8×8 matrix's row
 
     find(0, cur);
@@ -351,32 +371,50 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     for (int k = 0; k < kStages - 1; ++k) feed(k, k);
     __syncthreads();
     if (start(0) < nk) {
+      if constexpr (BF) {
+        const int h = QUAD ? (g >> 2) % GQ : WIDE ? g : g >> 1;
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int h = s * 4 + (g >> 1) % GQ;
-        float qs = 1.f;
-        if constexpr (!BF) {  // as halfs, brought near 1 by a power of two
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = 16 * i + 8 * j + 2 * c;
+            const float x = sq[h][d], y = sq[h][d + 1], x1 = less_top(x), y1 = less_top(y);
+            const unsigned hi = tops(x, y), mid = tops(x1, y1), low = tops(less_top(x1), less_top(y1));
+            if constexpr (QUAD) {
+              qb[0][i][j] = g & 2 ? (g & 1 ? 0u : low) : g & 1 ? mid : hi;
+            } else if constexpr (WIDE) {
+              qb[0][i][j] = hi, qb[1][i][j] = mid, qb[2][i][j] = low;
+            } else {
+              qb[0][i][j] = g & 1 ? mid : hi;
+              qb[1][i][j] = g & 1 ? 0u : low;
+            }
+          }
+      } else {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          const int h = s * 4 + (g >> 1) % GQ;
+          // as halfs, brought near 1 by a power of two
           float m = 0.f;
           for (int d = c; d < HD; d += 4) m = fmaxf(m, fabsf(sq[h][d]));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
           const int e = m > 0.f ? min(126, max(-126, (int)(__float_as_uint(m) >> 23) - 127)) : 0;
-          qs = __uint_as_float((unsigned)(127 - e) << 23);
+          const float qs = __uint_as_float((unsigned)(127 - e) << 23);
           if (c == 0) sback[h] = __uint_as_float((unsigned)(127 + e) << 23);  // every warp the same
-        }
-        auto pair = [&](int d) {
-          const unsigned u = split<BF>(sq[h][d] * qs), v = split<BF>(sq[h][d + 1] * qs);
-          return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
-        };
+          auto pair = [&](int d) {
+            const unsigned u = split(sq[h][d] * qs), v = split(sq[h][d + 1] * qs);
+            return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
+          };
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          if constexpr (SZ == 2) {
-            qb[s][i][0] = pair(16 * i + 2 * c);
-            qb[s][i][1] = pair(16 * i + 8 + 2 * c);
-          } else {
-            const int d = i / kKW * 4 * kKB + c * kKB + i % kKW * 4;
-            qb[s][i][0] = pair(d);
-            qb[s][i][1] = pair(d + 2);
+          for (int i = 0; i < kSteps; ++i) {
+            if constexpr (SZ == 2) {
+              qb[s][i][0] = pair(16 * i + 2 * c);
+              qb[s][i][1] = pair(16 * i + 8 + 2 * c);
+            } else {
+              const int d = i / kKW * 4 * kKB + c * kKB + i % kKW * 4;
+              qb[s][i][0] = pair(d);
+              qb[s][i][1] = pair(d + 2);
+            }
           }
         }
       }
@@ -398,11 +436,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       slot = slot == kStages - 1 ? 0 : slot + 1;
 #pragma unroll
       for (int q = 0; q < NT / T; ++q) {
-        float s[T][NS][NC][4];
+        float s[T][NA][NC][4];
 #pragma unroll
         for (int u = 0; u < T; ++u) {
 #pragma unroll
-          for (int e = 0; e < NS; ++e)
+          for (int e = 0; e < NA; ++e)
 #pragma unroll
             for (int i = 0; i < NC; ++i) s[u][e][i][0] = s[u][e][i][1] = s[u][e][i][2] = s[u][e][i][3] = 0.f;
           const int r0 = (q * T + u) * 16;
@@ -413,8 +451,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               unsigned w[4];
               ldmatrix4<false>(a ^ (st << 5), w);
 #pragma unroll
-              for (int e = 0; e < NS; ++e)
-                mma16816<BF>(s[u][e][st % NC], w[0], w[1], w[2], w[3], qb[e][st][0], qb[e][st][1]);
+              for (int e = 0; e < NB; ++e)
+                mma16816<BF>(s[u][BF ? 0 : e][(BF ? st * NB + e : st) % NC], w[0], w[1], w[2], w[3], qb[e][st][0],
+                             qb[e][st][1]);
             }
           } else {
             // 8 rows on the permutation is the same, and where a row is longer than a
@@ -440,34 +479,49 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             }
           }
         }
-        // τ of the keys g, g + 8 of tile tsel and head c mod GQ of each operand
         const int tile = q * T + tsel;
-        const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::scales)[tile] >> g;
+        const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::scales)[tile];
         float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
         if constexpr (F::scaled) {
           const float2 a = sc[tile * 16 + g], c2 = sc[tile * 16 + g + 8];  // a key's and a value's
           ks[0] = a.x, vs[0] = a.y, ks[1] = c2.x, vs[1] = c2.y;
         }
+        // the score of key g + 8·o: a column's sums, or two columns'
+        auto score = [&](int e, int o) {
+          float z = 0.f;
+#pragma unroll
+          for (int u = 0; u < T; ++u) {
+            float y = 0.f;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+              const float x = WIDE ? s[u][0][i][2 * o + e] : s[u][e][i][2 * o] + s[u][e][i][2 * o + 1];
+              y = i == 0 ? x : y + x;
+            }
+            z = u == 0 || tsel == u ? y : z;
+          }
+          return z;
+        };
 #pragma unroll
         for (int e = 0; e < NS; ++e) {
-          float pr[2];
+          float pr[NK];
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            float z = 0.f;
-#pragma unroll
-            for (int u = 0; u < T; ++u) {
-              float y = s[u][e][0][2 * o] + s[u][e][0][2 * o + 1];
-#pragma unroll
-              for (int i = 1; i < NC; ++i) y += s[u][e][i][2 * o] + s[u][e][i][2 * o + 1];
-              z = u == 0 || tsel == u ? y : z;
+          for (int o = 0; o < NK; ++o) {
+            float z;
+            if constexpr (QUAD) {  // two lanes have two columns each: they swap halves of the keys
+              const float z0 = score(e, 0), z1 = score(e, 1);
+              const bool odd = c & 1;
+              z = (odd ? z1 : z0) + __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
+            } else {
+              z = score(e, o);
             }
             z *= back[e];
             if constexpr (F::scaled) z *= ks[o];
-            const bool on = (live >> (8 * o)) & 1;
+            const int key = key_of(o);
+            const bool on = (live >> key) & 1;
             const float tau = on ? sigmoid_exp2(z) : 0.f;
             mass[e] += tau;
-            if (p.tau && on && c / GQ < T && e * 4 + c % GQ < Gh)
-              put_tau(p, (size_t)b * p.H + h0 + e * 4 + c % GQ, rc.t, p0 + start(k) + tile * 16 + g + 8 * o, tau);
+            if (p.tau && on && once && head_of(e) < Gh)
+              put_tau(p, (size_t)b * p.H + h0 + head_of(e), rc.t, p0 + start(k) + tile * 16 + key, tau);
             pr[o] = F::scaled ? tau * vs[o] : tau;
           }
           if constexpr (!BF) {
@@ -497,24 +551,44 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             pr[0] *= unit[e];
             pr[1] *= unit[e];
           }
-          unsigned* pw = ps + (e * 4 + c % GQ) * Z::pstride + tile * 16 + g;
-          pw[0] = split<BF>(pr[0]);
-          pw[8] = split<BF>(pr[1]);
+#pragma unroll
+          for (int o = 0; o < NK; ++o) {
+            const int at = head_of(e) * Z::pstride + tile * 16 + key_of(o);
+            if constexpr (BF) {
+              const float rest = less_top(pr[o]);
+              ps[at] = tops(rest, pr[o]);
+              reinterpret_cast<unsigned short*>(lo)[at] = (unsigned short)(__float_as_uint(less_top(rest)) >> 16);
+            } else {
+              ps[at] = split(pr[o]);
+            }
+          }
         }
       }
       __syncwarp();
 #pragma unroll
       for (int u = 0; u < NT; ++u) {
-        unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0;
-        if (g < GP) {
-          const unsigned at = smem_u32(ps + g * Z::pstride + u * 16 + 2 * c);
+        unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0, l0 = 0, l2 = 0;
+        const int h = FOLD ? g & 3 : g;  // the head of rows g and g + 8
+        if (h < GP) {
+          const int i = h * Z::pstride + u * 16 + 2 * c;
           unsigned x[2], y[2];
-          lds_words<2, 0>(at, x);
-          lds_words<2, 32>(at, y);
-          a0 = __byte_perm(x[0], x[1], 0x7632);
-          a1 = __byte_perm(x[0], x[1], 0x5410);
-          a2 = __byte_perm(y[0], y[1], 0x7632);
-          a3 = __byte_perm(y[0], y[1], 0x5410);
+          lds_words<2, 0>(smem_u32(ps + i), x);
+          lds_words<2, 32>(smem_u32(ps + i), y);
+          if constexpr (BF) {
+            lds_words<1, 0>(smem_u32(lo) + 2 * i, &l0);
+            lds_words<1, 16>(smem_u32(lo) + 2 * i, &l2);
+          }
+          if constexpr (FOLD) {  // rows 0-3 and 8-11: first and third parts, rows 4-7: second parts
+            a0 = __byte_perm(x[0], x[1], g < 4 ? 0x7632 : 0x5410);
+            a2 = __byte_perm(y[0], y[1], g < 4 ? 0x7632 : 0x5410);
+            a1 = g < 4 ? l0 : 0u;
+            a3 = g < 4 ? l2 : 0u;
+          } else {
+            a0 = __byte_perm(x[0], x[1], 0x7632);
+            a1 = __byte_perm(x[0], x[1], 0x5410);
+            a2 = __byte_perm(y[0], y[1], 0x7632);
+            a3 = __byte_perm(y[0], y[1], 0x5410);
+          }
         }
         if constexpr (SZ == 2) {
           const unsigned a = vt + ring_at<SZ, R, true>(u * 16 + mrow, mch);
@@ -524,6 +598,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             ldmatrix4<true>(a ^ (j << 4), w);
             mma16816<BF>(acc[j], a0, a1, a2, a3, w[0], w[1]);
             mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
+            if constexpr (BF && !FOLD) {
+              mma16816<BF>(acc[j], l0, 0u, l2, 0u, w[0], w[1]);
+              mma16816<BF>(acc[j + 1], l0, 0u, l2, 0u, w[2], w[3]);
+            }
           }
         } else {
 #pragma unroll
@@ -562,10 +640,21 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   float* part = reinterpret_cast<float*>(smb);  // [warps][Gh][HD], then the block's [Gh][HD]
 #pragma unroll
   for (int e = 0; e < NS; ++e) {
-    float m = c / GQ < T ? mass[e] : 0.f;
+    // over all lanes but those of other heads
+    float m = mass[e];
+    if constexpr (QUAD) {
+      m = (c >> 1) / GQ < T ? m : 0.f;
+      m += __shfl_xor_sync(0xffffffffu, m, 1);
+      if (GQ == 1) m += __shfl_xor_sync(0xffffffffu, m, 2);
 #pragma unroll
-    for (int o = GQ; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
-    if (lane < GQ && warp < kWarps) smass[warp][e * 4 + lane] = m;
+      for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (lane < 2 * GQ && warp < kWarps) smass[warp][lane >> 1] = m;
+    } else {
+      m = c / GQ < T ? m : 0.f;
+#pragma unroll
+      for (int o = GQ; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
+      if (lane < GQ && warp < kWarps) smass[warp][WIDE ? 2 * lane + e : e * 4 + lane] = m;
+    }
   }
   float un = 1.f;  // of head g
   if constexpr (!BF) {
@@ -574,6 +663,12 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       const float u1 = __shfl_sync(0xffffffffu, unit[1], g % 4);
       un = g < 4 ? un : u1;
     }
+  }
+  if constexpr (FOLD) {
+#pragma unroll
+    for (int j = 0; j < kTiles; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[j][e] += __shfl_down_sync(0xffffffffu, acc[j][e], 16);
   }
   if (g < Gh && warp < kWarps) {
     const float back = 1.f / un;

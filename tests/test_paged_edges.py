@@ -1,0 +1,55 @@
+"""Paged caches (``bozo_b200.paged``) where calls go wrong first: precision of
+mixed types, pages that are not there, offsets that do not start at zero,
+elements that are not finite."""
+import math
+
+import pytest
+import torch
+
+from bozo_b200 import ops, paged
+from oracle import paged_oracle as orc
+from test_paged import (BF16, F8, F16, F32, I8, ULP, Pool, check_decode, fill, history, int32, offsets, plain_write,
+                        rope, same_bits)
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(0)
+
+
+# ── precision ──
+
+@gpu
+@pytest.mark.parametrize("H,Hk", [(2, 2), (4, 2), (3, 1), (8, 2), (5, 1), (16, 2), (11, 1)])
+@pytest.mark.parametrize("HD", [32, 64, 128])
+@pytest.mark.parametrize("window", [64, None])
+def test_fp32_queries_over_bf16_pages_keep_fp32(HD, H, Hk, window):
+    """A key's or value's bf16 elements are exact in fp32, so an fp32 step over them
+    is as near the float64 result as the same step in plain fp32 operations: its
+    score is a sum of three times as many terms (each part of q with each element,
+    √3 of the rounding) that the matrix instruction may truncate instead of round
+    (twice), hence at most 4 times; an exponential and a reciprocal add 2^-22."""
+    B, n = 6, 150
+    pool = Pool(B, Hk, HD, 16, 10, BF16)
+    hist = fill(pool, [n] * B, Hk, HD, BF16, None, HD + H)
+    q = torch.randn(B, H, HD, device="cuda") * 4
+    lengths = [n - 1 - i for i in range(B)]
+    out, tau = paged.paged_tension(q, *pool.cache, int32(lengths), window=window, return_tau=True,
+                                   tau_window=window or n)
+    ref = orc.decode(q.cpu().double(), hist, lengths, window=window, capacity=pool.cap, scale=math.sqrt(HD),
+                     normalize="mass", tau_width=window or n)
+    # the same in fp32, key by key
+    want = [torch.zeros_like(x, dtype=F32) for x in ref]
+    for b, t in enumerate(lengths):
+        hi = t if window else t + 1
+        lo = max(0, hi - (window or pool.cap))
+        k, v = (x[lo:hi].float().repeat_interleave(H // Hk, dim=1) for x in hist[b])
+        row = 1 / (1 + torch.exp(-(q[b].cpu() * k).sum(-1) / math.sqrt(HD)))        # [keys, H]
+        want[0][b] = (row[..., None] * v).sum(0) / row.sum(0)[:, None]
+        want[1][b, :, :hi - lo] = (row if window else row.flip(0)).T
+    for got, plain, exact, name in zip((out, tau), want, ref, ("out", "tau")):
+        norm = float(exact.norm())
+        err, base = (float((x.cpu().double() - exact).norm()) / norm for x in (got, plain))
+        assert err <= 4 * base + 2.0 ** -22, f"{name}: {err:.2e}, plain fp32 {base:.2e}"
