@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p,
       for (; o; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
       const float tau = live[u] ? sigmoid_exact(y * ks[u] * p.inv_scale) : 0.f;
       mass += tau;
-      if (p.tau && live[u] && (l & (L / NH - 1)) == 0 && own < Gh)
+      if (p.tau && j + u * step < j1 && (l & (L / NH - 1)) == 0 && own < Gh)  // zero where a key has no page
         put_tau(p, (size_t)b * p.H + h0 + own, rc.t, j + u * step, tau);
       const float w = tau * vs[u];
 #pragma unroll

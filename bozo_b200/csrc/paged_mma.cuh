@@ -520,8 +520,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             const bool on = (live >> key) & 1;
             const float tau = on ? sigmoid_exp2(z) : 0.f;
             mass[e] += tau;
-            if (p.tau && on && once && head_of(e) < Gh)
-              put_tau(p, (size_t)b * p.H + h0 + head_of(e), rc.t, p0 + start(k) + tile * 16 + key, tau);
+            // zero where a key in reach has no page
+            const unsigned pos = p0 + start(k) + tile * 16 + key;
+            if (p.tau && once && pos >= rc.lo && pos < p1 && head_of(e) < Gh)
+              put_tau(p, (size_t)b * p.H + h0 + head_of(e), rc.t, pos, tau);
             pr[o] = F::scaled ? tau * vs[o] : tau;
           }
           if constexpr (!BF) {

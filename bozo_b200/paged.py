@@ -92,7 +92,7 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
                cache already.
     return_tau : also return the token's τ row ``[B, H, W]``: slot w is key
                t − (W − w) (local); ``[B, H, tau_window]``, column c is key t − c
-               (global); zero where there is no key.
+               (global); zero where there is no key, or its page is outside the pool.
 
     Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.  A NaN or an infinity
     in a query, or in a row that it reaches, makes that query's output NaN; rows

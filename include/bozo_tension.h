@@ -225,7 +225,7 @@ int bozo_tension_decode(const bozo_tension_decode_args* args, void* stream);
  * lengths[b] < 0 marks an inactive sequence: its rows are not written, and its
  * outputs are zeros.  A position outside the RoPE tables or a needed page
  * outside [0, pages) is skipped (rows unwritten, values read as zeros, keys
- * left out) and sets the device error word (BOZO_ERR_DEVICE_INDEX from
+ * left out, their τ exported as zero) and sets the device error word (BOZO_ERR_DEVICE_INDEX from
  * bozo_tension_poll_error).  No counterpart in the reference, whose
  * generate_cached (model.py:718-768) keeps no keys. */
 typedef struct {

@@ -53,3 +53,38 @@ def test_fp32_queries_over_bf16_pages_keep_fp32(HD, H, Hk, window):
         norm = float(exact.norm())
         err, base = (float((x.cpu().double() - exact).norm()) / norm for x in (got, plain))
         assert err <= 4 * base + 2.0 ** -22, f"{name}: {err:.2e}, plain fp32 {base:.2e}"
+
+
+# ── pages that are not there ──
+
+@gpu
+@pytest.mark.parametrize("dtype,HD", [(BF16, 64), (F16, 32), (F8, 128), (I8, 64), (F32, 64), (BF16, 48), (BF16, 21)])
+@pytest.mark.parametrize("page", [16, 8, 5])
+@pytest.mark.parametrize("window", [30, None])
+def test_exported_tau_of_missing_pages_is_zero(dtype, HD, page, window):
+    """Keys whose page is outside the pool are left out: their τ is zero, not what
+    the allocator's memory held; the others' τ does not change."""
+    io = dtype if dtype in ULP else BF16
+    for H, lengths, width in ((2, [47, 40, 45], 48 // page + 1), (6, [47, 40, 45], 48 // page + 1),
+                              (2, [600], 620 // page + 1)):   # in one piece; shared heads; in several
+        pool = Pool(len(lengths), 2, HD, page, width, dtype)
+        hist = fill(pool, [t + 1 for t in lengths], 2, HD, io, None, page)
+        q = torch.randn(len(lengths), H, HD, device="cuda").to(io)
+        tw = window or max(lengths) + 5
+        _, whole = check_decode(pool, lengths, hist, q, window=window, tau_window=tw)
+        gone = (lengths[0] - 20) // page                    # in reach of the first sequence
+        pool.table[0, gone] = -1
+        ops.poll_device_error("cuda")
+        keep = torch.full((len(lengths), H, tw), math.nan, device="cuda", dtype=io)
+        del keep                                            # the next τ row of this size is that memory
+        _, tau = paged.paged_tension(q, *pool.cache, int32(lengths), window=window, return_tau=True,
+                                     tau_window=tw, **pool.scales)
+        with pytest.raises(RuntimeError, match="outside"):
+            ops.poll_device_error("cuda")
+        want = whole.clone()
+        for pos in range(gone * page, (gone + 1) * page):
+            back = lengths[0] - pos
+            slot = window - back if window else back
+            if 0 <= slot < tw:
+                want[0, :, slot] = 0
+        assert torch.equal(tau, want)
