@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       const unsigned j =
           AL ? start(k + lane / kUnits) + lane % kUnits * GR : start(k) + r * 32 + (KT < 32 ? lane % KT : lane);
       rows[r] = kNoRow;
-      if (j < nk && (AL || p0 + j >= rc.lo)) {
+      // none for positions wholly before the reach: their pages may be gone
+      if (j < nk && p0 + j + GR > rc.lo) {
         const unsigned row = paged_row(p, b, p0 + j);
         if (row != kNoRow) rows[r] = row + (unsigned)hk * p.page;
       }

@@ -88,3 +88,31 @@ def test_exported_tau_of_missing_pages_is_zero(dtype, HD, page, window):
             if 0 <= slot < tw:
                 want[0, :, slot] = 0
         assert torch.equal(tau, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,HD", [(BF16, 64), (BF16, 32), (F8, 64), (I8, 32), (F32, 64)])
+@pytest.mark.parametrize("page", [8, 24, 40, 16, 32, 7, 1])
+def test_pages_behind_the_window_may_be_gone(dtype, HD, page):
+    """A wide table whose pages wholly before the window have been given back: a
+    valid call, wherever the window begins, and no error is reported."""
+    io, W = dtype if dtype in ULP else BF16, 20
+    lengths = [130 + i for i in range(16)] + [3, W, W + 8]
+    pool = Pool(len(lengths), 1, HD, page, 160 // page + 1, dtype)
+    hist = fill(pool, lengths, 1, HD, io, None, page)
+    for b, t in enumerate(lengths):
+        pool.table[b, :max(0, t - W) // page] = -1
+    q = torch.randn(len(lengths), 1, HD, device="cuda").to(io)
+    ops.poll_device_error("cuda")
+    check_decode_of(pool, lengths, hist, q, W)
+    ops.poll_device_error("cuda")
+
+
+def check_decode_of(pool, lengths, hist, q, W):
+    out, row = paged.paged_tension(q, *pool.cache, int32(lengths), window=W, return_tau=True, **pool.scales)
+    ref = orc.decode(q.cpu().double(), hist, lengths, window=W, capacity=pool.cap, scale=math.sqrt(q.shape[-1]),
+                     normalize="mass", tau_width=W)
+    big = max([1.0] + [float(v.abs().max()) for _, v in hist])
+    for got, want, unit in zip((out, row), ref, (big, 1.0)):
+        err = (got.cpu().double() - want).abs()
+        assert bool((err <= ULP[q.dtype] * want.abs() + 1e-5 * unit).all())
