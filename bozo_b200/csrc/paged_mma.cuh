@@ -23,7 +23,7 @@
 //   8 heads:       a column for each head, three products;
 // those of τ rows of their own with up to 4 heads, a second product with 8.  That costs
 // nothing measurable with a head or two of 64 or 128 elements, 2-8 % at 32, 3 % with four
-// heads and 9-17 % with eight (309 MB, 128 wide: 80 µs, with two parts 68).
+// heads and 9-20 % with eight (309 MB, 128 wide: 82 µs, with two parts 68.5).
 //
 // What bounds it: 1 flop a byte for 16-bit rows of a head of their own (memory),
 // instructions for 8-bit rows of shared heads.  4 warps with 3 tiles of 4 KB each and
@@ -177,6 +177,8 @@ template <int DT, int HD, int GP> struct Geo {
   // against 119), and so are 64 wide bf16 rows of up to four heads, which else take
   // a few registers too many for a third block (617 MB: 96.7 against 99.7).
   static constexpr int blocks = HD == 64 && (Fmt<DT>::scaled || (Fmt<DT>::bf && GP <= 4)) ? 3 : 2;
+  static constexpr bool fold = Fmt<DT>::bf && GP <= 4;  // τ's second parts have rows 4-7 of P
+  static constexpr int parts = (fold ? 2 : 1) * kWarps;  // sums that are added at the end
   static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
 };
 
@@ -223,12 +225,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   // sums that a score's products run in side by side
   constexpr int NC = NA == 1 && kSteps * (BF ? NB : 1) >= 4 ? 2 : 1;
   constexpr int NK = QUAD ? 1 : 2;      // keys of a lane, of a tile's 16
-  constexpr bool FOLD = BF && GP <= 4;  // τ's second parts have rows 4-7 of P
+  constexpr bool FOLD = Z::fold;
   // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
   constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
   constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB / 4;
   extern __shared__ __align__(256) char smb[];
-  __shared__ float sq[kHeads][HD + 4];
+  __shared__ float sq[BF ? 1 : kHeads][HD + 4];
+  __shared__ __align__(4) unsigned short scut[BF ? GP : 1][3][HD + 8];  // the three bf16 of each q element
   __shared__ float sback[kHeads];  // what undoes the power of two that q was multiplied by (halfs)
   __shared__ float smass[kWarps][kHeads];
   const int S = grid.S, G = grid.G;
@@ -365,7 +368,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     if (mine && rc.active)
       for (int i = tid; i < GP * HD; i += kWarps * 32) {
         const int h = i / HD, d = i - h * HD;
-        sq[h][d] = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
+        const float x = h < Gh ? query(p, b, h0 + h, rc.t, d) : 0.f;
+        if constexpr (BF) {
+          const float x1 = less_top(x), x2 = less_top(x1);
+          scut[h][0][d] = (unsigned short)(__float_as_uint(x) >> 16);
+          scut[h][1][d] = (unsigned short)(__float_as_uint(x1) >> 16);
+          scut[h][2][d] = (unsigned short)(__float_as_uint(x2) >> 16);
+        } else {
+          sq[h][d] = x;
+        }
       }
     if (early) __syncthreads();
 #pragma unroll 1
@@ -374,20 +385,20 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     if (start(0) < nk) {
       if constexpr (BF) {
         const int h = QUAD ? (g >> 2) % GQ : WIDE ? g : g >> 1;
+        auto pair = [&](int part, int d) { return *reinterpret_cast<const unsigned*>(&scut[h][part][d]); };
 #pragma unroll
         for (int i = 0; i < kSteps; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int d = 16 * i + 8 * j + 2 * c;
-            const float x = sq[h][d], y = sq[h][d + 1], x1 = less_top(x), y1 = less_top(y);
-            const unsigned hi = tops(x, y), mid = tops(x1, y1), low = tops(less_top(x1), less_top(y1));
             if constexpr (QUAD) {
-              qb[0][i][j] = g & 2 ? (g & 1 ? 0u : low) : g & 1 ? mid : hi;
+              qb[0][i][j] = (g & 3) == 3 ? 0u : pair(g & 3, d);
             } else if constexpr (WIDE) {
-              qb[0][i][j] = hi, qb[1][i][j] = mid, qb[2][i][j] = low;
+#pragma unroll
+              for (int e = 0; e < 3; ++e) qb[e][i][j] = pair(e, d);
             } else {
-              qb[0][i][j] = g & 1 ? mid : hi;
-              qb[1][i][j] = g & 1 ? 0u : low;
+              qb[0][i][j] = pair(g & 1, d);
+              qb[1][i][j] = g & 1 ? 0u : pair(2, d);
             }
           }
       } else {
@@ -640,7 +651,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   // the warps' sums, added in order
   grid_release();
   __syncthreads();  // the rings and the queries are done with
-  float* part = reinterpret_cast<float*>(smb);  // [warps][Gh][HD], then the block's [Gh][HD]
+  float* part = reinterpret_cast<float*>(smb);  // [parts][Gh][HD], then the block's [Gh][HD]
 #pragma unroll
   for (int e = 0; e < NS; ++e) {
     // over all lanes but those of other heads
@@ -667,32 +678,27 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       un = g < 4 ? un : u1;
     }
   }
-  if constexpr (FOLD) {
-#pragma unroll
-    for (int j = 0; j < kTiles; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) acc[j][e] += __shfl_down_sync(0xffffffffu, acc[j][e], 16);
-  }
-  if (g < Gh && warp < kWarps) {
+  // rows of O: head g, or with FOLD head g mod 4 in two parts
+  const int hrow = FOLD ? g & 3 : g;
+  if (hrow < Gh && warp < kWarps) {
     const float back = 1.f / un;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int d = SZ == 2 ? 8 * j + 2 * c + e : j / kVB * 8 * kVB + (2 * c + e) * kVB + j % kVB;
-        part[(warp * Gh + g) * HD + d] = (acc[j][e] + acc[j][2 + e]) * back;
+        part[((FOLD ? 2 * warp + (g >> 2) : warp) * Gh + hrow) * HD + d] = (acc[j][e] + acc[j][2 + e]) * back;
       }
   }
   __syncthreads();
-  float* sum = part + kWarps * Gh * HD;
+  float* sum = part + Z::parts * Gh * HD;
   for (int i = tid; i < Gh * HD && warp < kWarps; i += kWarps * 32) {
     const int h = i / HD, d = i - h * HD;
     float o = 0.f, m = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      o += part[w * Gh * HD + i];
-      m += smass[w][h];
-    }
+    for (int w = 0; w < Z::parts; ++w) o += part[w * Gh * HD + i];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m += smass[w][h];
     const size_t bh = (size_t)b * p.H + h0 + h;
     if (rc.count == 1) {
       if (piece == 0) stf(p.out, (long long)(bh * HD + d), p.out_dt, o / norm_divisor(p, m, rc.n));
@@ -728,8 +734,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
 template <int DT, int HD, int GP, int GR>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
   const int G = p.H / p.Hk, HG = (G + kHeads - 1) / kHeads;
-  const size_t ring = (size_t)kWarps * Geo<DT, HD, GP>::warp;
-  const size_t part = (size_t)(kWarps + 1) * std::min(G, kHeads) * HD * sizeof(float);
+  using Z = Geo<DT, HD, GP>;
+  const size_t ring = (size_t)kWarps * Z::warp;
+  const size_t part = (size_t)(Z::parts + 1) * std::min(G, kHeads) * HD * sizeof(float);
   const size_t smem = std::max(ring, part);
   auto kern = paged_decode_mma<DT, HD, GP, GR>;
   static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
@@ -737,7 +744,7 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
-    const int most = (int)std::max(ring, (size_t)(kWarps + 1) * kHeads * HD * sizeof(float));
+    const int most = (int)std::max(ring, (size_t)(Z::parts + 1) * kHeads * HD * sizeof(float));
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
