@@ -145,10 +145,9 @@ class PagedState:
     def table(self, li: int) -> Tensor:
         return self.global_table if self.model.blocks[li].global_layer else self.local_table
 
-    def _write(self, li: int, slots: Tensor, start: Tensor, cu: Tensor, k: Tensor, v: Tensor) -> None:
+    def _write(self, li: int, table: Tensor, start: Tensor, cu: Tensor, k: Tensor, v: Tensor) -> None:
         lay = self.layers[li]
-        paged.write_kv(k, v, lay.k, lay.v, self.table(li)[slots], start, cu_rows=cu, rope=self.rope,
-                       **lay.scales)
+        paged.write_kv(k, v, lay.k, lay.v, table, start, cu_rows=cu, rope=self.rope, **lay.scales)
 
 
 @torch.no_grad()
@@ -182,7 +181,7 @@ def admit(state: PagedState, prompts: Sequence[Sequence[int]]):
         h = blk.pre_norm(x)
         _, k, v = blk.tension.project(h)
         k, v = (y.flatten(0, 1) if packed else y.flatten(0, 1)[rows] for y in (k, v))
-        state._write(li, at, start, cu, k, v)
+        state._write(li, state.table(li)[at], start, cu, k, v)
         x = blk.ffn(blk._osc(blk.tension(h)))
     last = x[torch.arange(len(lens), device=dev), n.long() - 1]
     logits = model.lm_head(model.final_norm(last))
@@ -196,7 +195,8 @@ def admit(state: PagedState, prompts: Sequence[Sequence[int]]):
 def extend(state: PagedState, slot: int, ids: Sequence[int]) -> Tensor:
     """Add ``ids`` to a held sequence in one forward over them; returns the logits
     ``[V]`` after the last.  The earlier keys and values that the new tokens
-    reach are read back from the pages."""
+    reach are read back from the pages.  Tokens past a global layer's reach attend
+    its last keys as they would in a step, one after another in those layers."""
     model, cfg = state.model, state.model.cfg
     t, T = state.length(slot), len(ids)
     if T < 1:
@@ -205,36 +205,52 @@ def extend(state: PagedState, slot: int, ids: Sequence[int]) -> Tensor:
     state._grow({slot: t + T})
     dev = state.lengths.device
     at = torch.tensor([slot], device=dev)
-    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
-    start = torch.tensor([t], dtype=torch.int32, device=dev)
     x = model.embedding(torch.tensor([list(ids)], device=dev))
     pos = torch.arange(t, t + T, device=dev)
+    at32 = pos.int()
+    start = at32[:1]
     if model.pos_embedding is not None:
         x = x + model.pos_embedding(pos)
     for li, blk in enumerate(model.blocks):
         layer, lay, table = blk.tension, state.layers[li], state.table(li)[at]
         h = blk.pre_norm(x)
         q, k, v = layer.project(h)
-        # the held rows that the first new query reaches come first, then the new
-        # ones, written only now: a ring may put them in the old ones' place
-        back = t if layer.global_layer else min(t, cfg.window)
-        back = min(back, table.shape[1] * state.page_size)
-        kk, vv = paged.read_kv(lay.k, lay.v, table, start - back, torch.tensor([0, back], dtype=torch.int32, device=dev),
-                               back, dtype=k.dtype, **lay.scales)
-        state._write(li, at, start, cu, k[0], v[0])
-        if state.rope is not None:
-            q, k = (decode._rotate(y, state.rope[0], state.rope[1], t).to(y.dtype) for y in (q, k))
-        kk = torch.cat([kk[None], k], dim=1)
-        vv = torch.cat([vv[None], v], dim=1)
-        qq = torch.cat([q.new_zeros(1, back, *q.shape[2:]), q], dim=1)
-        msg = ops.tension(qq, kk, vv, window=None if layer.global_layer else cfg.window,
-                          scale=layer.scale, rope_base=None,
-                          normalize="mass" if layer.global_layer else "count")[:, back:]
+        # tokens that reach all before them go together; past a global layer's last
+        # pages each new row takes the place of the oldest that the one before reaches
+        cap = table.shape[1] * state.page_size
+        m = min(T, max(0, cap - t)) if layer.global_layer else T
+        msg = [_chunk(state, li, table, start, t, q[:, :m], k[:, :m], v[:, :m])] if m else []
+        for i in range(m, T):
+            msg.append(paged.paged_tension(
+                q[:, i], lay.k, lay.v, table, at32[i:i + 1], window=None, scale=layer.scale, rope=state.rope,
+                k=k[:, i], v=v[:, i], **lay.scales).unsqueeze(1))
+        msg = msg[0] if len(msg) == 1 else torch.cat(msg, dim=1)
         hh = layer.norm.wo_add_forward(h, msg.reshape(1, T, -1), layer.wo, layer.dropout)
         x = blk.ffn(_oscillate(blk, hh, pos[None, :, None]))
     state.lengths[slot] = t + T
     state._len[slot] = t + T
     return model.lm_head(model.final_norm(x[0, -1]))
+
+
+def _chunk(state: PagedState, li: int, table: Tensor, start: Tensor, t: int, q: Tensor, k: Tensor,
+           v: Tensor) -> Tensor:
+    """One layer's tension ``[1, T, H, HD]`` of T new tokens from position t on that
+    reach every key before them (of a local layer, in their window)."""
+    cfg, layer, lay = state.model.cfg, state.model.blocks[li].tension, state.layers[li]
+    T, dev = q.shape[1], q.device
+    # the held rows that the first new query reaches come first, then the new
+    # ones, written only now: a ring may put them in the old ones' place
+    back = t if layer.global_layer else min(t, cfg.window)
+    kk, vv = paged.read_kv(lay.k, lay.v, table, start - back, torch.tensor([0, back], dtype=torch.int32, device=dev),
+                           back, dtype=k.dtype, **lay.scales)
+    state._write(li, table, start, torch.tensor([0, T], dtype=torch.int32, device=dev), k[0], v[0])
+    if state.rope is not None:
+        q, k = (decode._rotate(y, state.rope[0], state.rope[1], t).to(y.dtype) for y in (q, k))
+    kk = torch.cat([kk[None], k], dim=1)
+    vv = torch.cat([vv[None], v], dim=1)
+    qq = torch.cat([q.new_zeros(1, back, *q.shape[2:]), q], dim=1)
+    return ops.tension(qq, kk, vv, window=None if layer.global_layer else cfg.window, scale=layer.scale,
+                       rope_base=None, normalize="mass" if layer.global_layer else "count")[:, back:]
 
 
 def _oscillate(blk, x: Tensor, pos: Tensor) -> Tensor:

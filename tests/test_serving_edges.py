@@ -1,0 +1,60 @@
+"""Serving over paged caches (``bozo_b200.serving``) at its limits: sequences longer
+than a global layer's reach, and calls that are refused."""
+import pytest
+import torch
+
+from bozo_b200 import ops, serving
+from test_serving import close, ids, make
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def plain_matmuls():
+    torch.backends.cuda.matmul.allow_tf32 = False
+    torch.manual_seed(5)
+
+
+@gpu
+@pytest.mark.parametrize("chunks", [(1, 1, 1, 7), (3, 9, 1, 20), (40, 1, 5), (64, 2), (2, 31, 33)])
+def test_a_sequence_extended_past_the_reach(chunks):
+    """A global layer attends the last C keys, however the ids came: the same logits
+    as the same ids fed one by one, in chunks that end before, cross and begin past C,
+    and the same steps after them."""
+    model = make("rope_global")
+    model.cfg.max_seq_len = 32
+    one = serving.PagedState(model, 2, 120, page_size=16)
+    many = serving.PagedState(model, 2, 120, page_size=16)
+    first = ids(30, 8)
+    (a,), _ = serving.admit(one, [first])
+    (b,), _ = serving.admit(many, [first])
+    for i, n in enumerate(chunks):
+        new = ids(n, 40 + i)
+        for x in new:
+            want = serving.step(one, torch.full((2,), x, dtype=torch.long, device="cuda:0"))[a]
+        close(serving.extend(many, b, new), want, f"{n} ids from {one.length(a) - n} on")
+    assert one.length(a) == many.length(b)
+    for i in range(3):
+        tok = torch.tensor(ids(2, 90 + i), device="cuda:0")
+        close(serving.step(many, tok)[b], serving.step(one, tok)[a], f"step {i} after")
+    ops.poll_device_error("cuda:0")
+
+
+@gpu
+@pytest.mark.parametrize("cache", [torch.float8_e4m3fn, torch.int8])
+def test_extended_past_the_reach_of_an_8_bit_cache(cache):
+    """As above; the keys of a chunk that lies past C are attended as the cache holds
+    them, so a chunk of any length gives what the same ids give one by one."""
+    model = make("rope_global")
+    model.cfg.max_seq_len = 32
+    one, many = (serving.PagedState(model, 1, 100, page_size=16, cache_dtype=cache) for _ in range(2))
+    first = ids(32, 8)
+    for s in (one, many):
+        serving.admit(s, [first])
+    new = ids(9, 3)
+    for x in new:
+        want = serving.step(one, torch.tensor([x], device="cuda:0"))[0]
+    got = serving.extend(many, 0, new)
+    # local layers attend a chunk's own keys before they are rounded to 8 bits
+    tol = {torch.float8_e4m3fn: 2.0 ** -4, torch.int8: 2.0 ** -6}[cache]
+    assert float((got - want).norm() / want.norm()) <= tol
