@@ -211,10 +211,11 @@ template <bool WRITE>
 __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int rows, unsigned* srow, unsigned* spos) {
   __shared__ int found;
   if (p.cu) {
+    // the sequence of the block's first row, or the first one if that row comes before it
     if (threadIdx.x == 0) found = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < p.B; i += kThreads)
-      if (__ldg(p.cu + i) <= (int)n0 && (int)n0 < __ldg(p.cu + i + 1)) found = i;
+      if ((i == 0 || __ldg(p.cu + i) <= (int)n0) && (int)n0 < __ldg(p.cu + i + 1)) found = i;
     __syncthreads();
   }
   for (int r = threadIdx.x; r < rows; r += kThreads) {
@@ -227,7 +228,7 @@ __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int r
         if (b >= 0) {
           while (b < p.B && (next = __ldg(p.cu + b + 1)) <= (int)n) ++b;
           if (b < p.B) first = __ldg(p.cu + b);
-          else b = -1;
+          if (b == p.B || first > (int)n) b = -1;
         }
       }
       const int t = b < 0 ? -1 : __ldg(p.len + b);

@@ -48,7 +48,8 @@ def write_kv(k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, page_table:
     k, v    : ``[N, Hk, HD]`` pre-RoPE projections (any strides).
     cu_rows : ``[B + 1]`` int32 row offsets: sequence b's tokens are the rows
               ``cu_rows[b]:cu_rows[b+1]``, at positions ``lengths[b]``, …; rows
-              from ``cu_rows[B]`` on are padding.  ``None``: one row a sequence.
+              before ``cu_rows[0]`` and from ``cu_rows[B]`` on are padding.
+              ``None``: one row a sequence.
     rope    : ``(cos, sin, ...)`` tables ``[length, HD/2]`` (``ops.rope_tables``)
               for the keys, or ``None``.
 

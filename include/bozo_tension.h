@@ -246,13 +246,13 @@ typedef struct {
 
 /* Write new tokens' keys (rotated) and values.  Rows n with
  * cu_rows[b] ≤ n < cu_rows[b+1] are sequence b's tokens at positions
- * lengths[b] + n − cu_rows[b]; rows from cu_rows[B] on are padding.  Of more
- * than C tokens of one sequence the last C are written.  cu_rows NULL: one row
+ * lengths[b] + n − cu_rows[b]; rows before cu_rows[0] and from cu_rows[B] on are
+ * padding.  Of more than C tokens of one sequence the last C are written.  cu_rows NULL: one row
  * a sequence (rows = B).  `lengths` is not advanced. */
 typedef struct {
   bozo_paged_cache cache;
   int64_t rows;
-  const int32_t* cu_rows; /* [B+1] device, non-decreasing from 0, or NULL */
+  const int32_t* cu_rows; /* [B+1] device, non-decreasing, or NULL */
   int32_t rope_len;       /* rows of the RoPE tables or 0 for no RoPE */
   int32_t _pad;
   const float* rope_cos;  /* [rope_len, HD/2] fp32 contiguous, or NULL */

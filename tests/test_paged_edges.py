@@ -116,3 +116,30 @@ def check_decode_of(pool, lengths, hist, q, W):
     for got, want, unit in zip((out, row), ref, (big, 1.0)):
         err = (got.cpu().double() - want).abs()
         assert bool((err <= ULP[q.dtype] * want.abs() + 1e-5 * unit).all())
+
+
+# ── offsets ──
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F8, F32])
+@pytest.mark.parametrize("HD", [64, 32, 20])
+@pytest.mark.parametrize("first", [1, 5, 40, 300])
+def test_rows_before_the_first_offset_are_padding(dtype, HD, first):
+    """Offsets into a longer packed batch: rows before ``cu_rows[0]`` are padding as
+    those from ``cu_rows[B]`` on are, whichever kernel takes the call."""
+    counts, start = [9, 0, 1, 30], [0, 3, 11, 5]
+    cu = [first + x for x in offsets(counts)]
+    rows = cu[-1] + 3
+    tables = rope(HD, 64, "cuda")
+    pool = Pool(4, 3, HD, 16, 4, dtype)
+    k, v = (torch.randn(rows, 3, HD, device="cuda", dtype=BF16) for _ in "kv")
+    want = plain_write(pool, k[first:], v[first:], start, counts, tables)
+    paged.write_kv(k, v, *pool.cache, int32(start), cu_rows=int32(cu), rope=tables, **pool.scales)
+    for got, ref, name in zip((pool.k, pool.v, pool.ks, pool.vs), want, ("k_pages", "v_pages", "k_scale", "v_scale")):
+        if got is not None:
+            same_bits(got.cpu(), ref, name)
+    shifted = paged.read_kv(*pool.cache, int32(start), int32(cu), rows, **pool.scales)
+    plain = paged.read_kv(*pool.cache, int32(start), int32(offsets(counts)), rows - first, **pool.scales)
+    for x, y in zip(shifted, plain):
+        assert (x[:first] == 0).all()
+        same_bits(x[first:], y, "read")
