@@ -95,9 +95,13 @@ def paged_tension(q: Tensor, k_pages: Tensor, v_pages: Tensor, page_table: Tenso
                t − (W − w) (local); ``[B, H, tau_window]``, column c is key t − c
                (global); zero where there is no key, or its page is outside the pool.
 
-    Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.  A NaN or an infinity
-    in a query, or in a row that it reaches, makes that query's output NaN; rows
-    out of reach may hold anything.
+    Returns ``out [B, H, HD]`` in q's dtype, or ``(out, tau)``.  A NaN in a query or in
+    a key that it reaches makes that query's output NaN, a NaN in a value that column
+    of it; 8-bit rows with a NaN or an infinity are NaN as a whole.  An infinity in a
+    16- or 32-bit value makes its column an infinity or NaN; one in a query or a key
+    gives τ 0 or 1, or NaN, depending on the pages' type.  Neither reaches another
+    sequence, another key head or, from a query, another query, and rows out of reach
+    may hold anything.
     """
     norm = ops._NORM.get(normalize, -1)
     if norm < 0:

@@ -143,3 +143,47 @@ def test_rows_before_the_first_offset_are_padding(dtype, HD, first):
     for x, y in zip(shifted, plain):
         assert (x[:first] == 0).all()
         same_bits(x[first:], y, "read")
+
+
+# ── elements that are not finite ──
+
+@gpu
+@pytest.mark.parametrize("dtype,HD", [(BF16, 64), (F16, 64), (F32, 64), (F8, 64), (I8, 64), (BF16, 48), (F16, 21)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("where", ["key", "value", "query"])
+def test_one_element_that_is_not_finite(dtype, HD, bad, where):
+    """In one key, one value or one query: a NaN spoils the outputs that reach it (a
+    16- or 32-bit value's only in its own column), and nothing else changes: not
+    other sequences, other key heads or, for a query, other heads.  An infinite key
+    or query gives τ 0 or 1, or NaN, an infinite value no finite number."""
+    io = dtype if dtype in ULP else BF16
+    n, H, Hk = 40, 4, 2
+    q = torch.randn(3, H, HD, device="cuda").to(io)
+    k, v = (torch.randn(3 * n, Hk, HD, device="cuda").to(io) for _ in "kv")
+    outs = []
+    for spoil in (False, True):
+        pool, qq, kk, vv = Pool(3, Hk, HD, 16, 3, dtype), q.clone(), k.clone(), v.clone()
+        if spoil:
+            if where == "query":
+                qq[1, 2, 5] = bad
+            else:
+                (kk if where == "key" else vv)[n + 17, 1, 5] = bad
+        paged.write_kv(kk, vv, *pool.cache, int32([0] * 3), cu_rows=int32([0, n, 2 * n, 3 * n]), **pool.scales)
+        outs.append(paged.paged_tension(qq, *pool.cache, int32([n - 1] * 3), window=None, return_tau=True,
+                                        tau_window=n, **pool.scales))
+    (good, _), (got, tau) = outs
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    if where == "query":
+        hit[1, 2] = True
+    elif where == "value" and dtype in ULP:
+        hit[1, 2:, 5] = True
+    else:
+        hit[1, 2:] = True
+    assert torch.equal(got[~hit], good[~hit])
+    if math.isnan(bad) or (dtype not in ULP and where != "query"):   # an 8-bit row with either is all NaN
+        assert torch.isnan(got[hit]).all()
+    elif where == "value":
+        assert not torch.isfinite(got[hit]).any()
+    else:
+        tau = tau[1, 2] if where == "query" else tau[1, 2:, n - 1 - 17]
+        assert ((tau == 0) | (tau == 1) | torch.isnan(tau)).all()
