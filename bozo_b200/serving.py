@@ -196,7 +196,9 @@ def extend(state: PagedState, slot: int, ids: Sequence[int]) -> Tensor:
     """Add ``ids`` to a held sequence in one forward over them; returns the logits
     ``[V]`` after the last.  The earlier keys and values that the new tokens
     reach are read back from the pages.  Tokens past a global layer's reach attend
-    its last keys as they would in a step, one after another in those layers."""
+    its last keys as they would in a step, one after another in those layers.
+    Where it fails midway (out of memory), rings may hold some of the new rows:
+    release the slot."""
     model, cfg = state.model, state.model.cfg
     t, T = state.length(slot), len(ids)
     if T < 1:
@@ -261,14 +263,27 @@ def _oscillate(blk, x: Tensor, pos: Tensor) -> Tensor:
     return x * (1.0 + osc.amp * torch.sin(pos.float() * osc.freqs + osc.phases))
 
 
-def _advance(state: PagedState) -> None:
-    """Host side of a step: pages for the new tokens, lengths."""
+def _check_tokens(state: PagedState, tokens: Tensor) -> None:
+    if tokens.shape != (state.slots,):
+        raise ValueError(f"step: tokens must be [{state.slots}], got {tuple(tokens.shape)}")
+    if tokens.dtype == torch.bool or tokens.is_floating_point() or tokens.is_complex():
+        raise TypeError(f"step: tokens must be integers, got {tokens.dtype}")
+
+
+def _reserve(state: PagedState) -> dict:
+    """Pages for a step's new tokens; the lengths after it, by slot."""
     held = {s: n + 1 for s, n in enumerate(state._len) if n is not None}
-    for s, n in held.items():
+    for n in held.values():
         state._check(n)
     state._grow(held)
+    return held
+
+
+def _advance(state: PagedState, held: dict) -> None:
+    """The step is under way: the host's lengths follow the device's."""
     for s, n in held.items():
         state._len[s] = n
+    ops.check_device_error(state.lengths.device)
 
 
 @torch.no_grad()
@@ -297,7 +312,6 @@ def _step(state: PagedState, tokens: Tensor, export: bool):
         rows.append(tau)
     logits = model.lm_head(model.final_norm(x))[:, 0]
     state.lengths += (state.lengths >= 0).int()
-    ops.check_device_error(tokens.device)
     return (logits, rows) if export else logits
 
 
@@ -305,10 +319,13 @@ def step(state: PagedState, tokens: Tensor, export: bool = False):
     """Feed one token to every active slot (``tokens [slots]``; idle slots' entries
     are ignored); returns the logits ``[slots, V]`` and with ``export`` each
     layer's τ rows ``[slots, H, W]`` (as ``decode.step``, zeros in idle slots)."""
-    if tokens.shape != (state.slots,):
-        raise ValueError(f"step: tokens must be [{state.slots}], got {tuple(tokens.shape)}")
-    _advance(state)
-    return _step(state, tokens, export)
+    _check_tokens(state, tokens)
+    if tokens.device != state.lengths.device:
+        raise ValueError(f"step: tokens must be on {state.lengths.device}, got {tokens.device}")
+    held = _reserve(state)
+    res = _step(state, tokens.long(), export)
+    _advance(state, held)
+    return res
 
 
 class PagedStepGraph:
@@ -334,10 +351,11 @@ class PagedStepGraph:
         state.lengths.copy_(held)
 
     def __call__(self, tokens: Tensor):
-        _advance(self.state)
+        _check_tokens(self.state, tokens)
         self.tokens.copy_(tokens)
+        held = _reserve(self.state)
         self.graph.replay()
-        ops.check_device_error(self.tokens.device)
+        _advance(self.state, held)
         return self.out
 
 

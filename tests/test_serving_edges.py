@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from bozo_b200 import ops, serving
-from test_serving import close, ids, make
+from test_serving import close, full, ids, make
 
 gpu = pytest.mark.gpu
 
@@ -58,3 +58,51 @@ def test_extended_past_the_reach_of_an_8_bit_cache(cache):
     # local layers attend a chunk's own keys before they are rounded to 8 bits
     tol = {torch.float8_e4m3fn: 2.0 ** -4, torch.int8: 2.0 ** -6}[cache]
     assert float((got - want).norm() / want.norm()) <= tol
+
+
+@gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_refused_step_changes_nothing(graph):
+    """Tokens of a wrong shape, type or device: refused before any page is taken or
+    a length advanced."""
+    model = make("rope_global")
+    state = serving.PagedState(model, 2, 64, page_size=16)
+    (s,), _ = serving.admit(state, [ids(16, 1)])           # the next token takes a page
+    run = serving.PagedStepGraph(state) if graph else (lambda tok: serving.step(state, tok))
+    free, held = state.free_pages, state.length(s)
+    for bad in (torch.zeros(1, dtype=torch.long, device="cuda:0"), torch.zeros((), dtype=torch.long, device="cuda:0"),
+                torch.zeros(3, dtype=torch.long, device="cuda:0"), torch.zeros(2, 1, dtype=torch.long, device="cuda:0"),
+                torch.zeros(2, dtype=torch.float32, device="cuda:0"), torch.zeros(2, dtype=torch.bool, device="cuda:0"),
+                *([] if graph else [torch.zeros(2, dtype=torch.long)])):  # a replay copies tokens from any device
+        with pytest.raises((ValueError, TypeError), match="tokens"):
+            run(bad)
+        assert (state.free_pages, state.length(s)) == (free, held)
+        assert state.lengths.tolist()[s] == held
+    seq = ids(16, 1) + [7]
+    got = run(torch.full((2,), 7, dtype=torch.long, device="cuda:0"))
+    close(got[s], full(model, seq), "after the refusals")
+    seq.append(9)
+    got = run(torch.full((2,), 9, dtype=torch.int16, device="cuda:0"))
+    close(got[s], full(model, seq), "tokens of another integer type")
+
+
+@gpu
+def test_a_failed_step_advances_no_length(monkeypatch):
+    """A step that ends in an exception leaves the host's and the device's lengths
+    alike, and the next one gives what it would have given."""
+    model = make("rope_global")
+    state = serving.PagedState(model, 2, 64, page_size=16)
+    (s,), _ = serving.admit(state, [ids(16, 1)])
+    tok = torch.full((2,), 7, dtype=torch.long, device="cuda:0")
+
+    def fail(*a, **kw):
+        raise torch.OutOfMemoryError("out of memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(model.final_norm, "forward", fail)
+        with pytest.raises(torch.OutOfMemoryError):
+            serving.step(state, tok)
+    assert state.length(s) == state.lengths.tolist()[s] == 16
+    close(serving.step(state, tok)[s], full(model, ids(16, 1) + [7]), "the next step")
+    state.release(s)
+    assert state.free_pages == 8
