@@ -18,7 +18,9 @@ tables are read on the device, so admitting, releasing and growing between
 replays need no new capture.  ``generate`` is continuous batching on top: a
 queue of prompts over the slots, ``decode.generate``'s sampling for each.
 
-A step's logits equal those of ``decode.step`` for each sequence on its own.
+A step's logits equal those of ``decode.step`` for each sequence on its own, past
+``max_seq_len`` tokens where the page size divides it: global layers reach whole
+pages, so up to ``page_size − 1`` keys more otherwise.
 The caches may be held in 8 bits (``cache_dtype`` e4m3 or int8), a quarter of
 fp32 and half of bf16 plus 4 bytes a row.
 """
@@ -370,7 +372,8 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new: int = 200, temp: 
     model.eval()
     out = [list(p) for p in prompts]
     limit = model.cfg.max_seq_len
-    # the last max_seq_len ids are the context; without RoPE a sequence ends there
+    # the last max_seq_len ids are the context; without RoPE PagedState refuses what
+    # would pass them
     ctx = [p[-limit:] for p in out]
     queue = list(range(len(ctx))) if max_new > 0 else []
     if not queue:

@@ -3,7 +3,7 @@ than a global layer's reach, and calls that are refused."""
 import pytest
 import torch
 
-from bozo_b200 import ops, serving
+from bozo_b200 import decode, ops, serving
 from test_serving import close, full, ids, make
 
 gpu = pytest.mark.gpu
@@ -106,3 +106,21 @@ def test_a_failed_step_advances_no_length(monkeypatch):
     close(serving.step(state, tok)[s], full(model, ids(16, 1) + [7]), "the next step")
     state.release(s)
     assert state.free_pages == 8
+
+
+@gpu
+@pytest.mark.parametrize("page", [5, 7, 24])
+def test_past_max_seq_len_global_layers_reach_whole_pages(page):
+    """A page size that does not divide max_seq_len: the reach is that of a ring of
+    so many whole pages."""
+    model = make("rope_global")
+    model.cfg.max_seq_len = 32
+    state = serving.PagedState(model, 2, 100, page_size=page)
+    model.cfg.max_seq_len = state.global_table.shape[1] * page
+    ring = decode.DecodeState(model, 1, 100)
+    seq = ids(30, 3)
+    (slot,), a = serving.admit(state, [seq])
+    close(a[0], decode.prefill(ring, torch.tensor([seq], device="cuda:0"))[0], "prompt")
+    for i in range(25):
+        tok = torch.tensor(ids(2, 700 + i), device="cuda:0")
+        close(serving.step(state, tok)[slot], decode.step(ring, tok[slot:slot + 1])[0], f"step {i}")
