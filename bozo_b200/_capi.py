@@ -24,6 +24,7 @@ DT_F8E4M3, DT_I8 = 3, 4  # paged-cache rows only
 MODE_LOCAL, MODE_GLOBAL = 0, 1
 NORM_NONE, NORM_MASS, NORM_COUNT = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05 = 0, 1, 2
+PATH_MMA = 3  # reported by bozo_tension_last_path only
 
 EXPORTED = (
     "bozo_tension_fwd", "bozo_tension_bwd", "bozo_tension_bwd_workspace",

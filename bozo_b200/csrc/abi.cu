@@ -632,10 +632,10 @@ int bozo_paged_decode(const bozo_paged_decode_args* a, void* stream) {
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return BOZO_ERR_ALIGNMENT;
   p.ws = static_cast<float*>(a->workspace);
   if (!(p.err = error_word(&e))) return cuda_fail(e);
-  int launches = 0;
-  e = launch_paged_decode(p, sms, static_cast<cudaStream_t>(stream), &launches);
+  int launches = 0, path = BOZO_PATH_SIMT;
+  e = launch_paged_decode(p, sms, static_cast<cudaStream_t>(stream), &launches, &path);
   if (e != cudaSuccess) return cuda_fail(e);
-  t_last_path = BOZO_PATH_SIMT;
+  t_last_path = path;
   t_last_launches = launches;
   return BOZO_OK;
 }

@@ -57,7 +57,7 @@ inline PagedP paged_params(const bozo_paged_cache& c) {
 cudaError_t launch_paged_write(const PagedP& p, int sms, cudaStream_t st);
 cudaError_t launch_paged_read(const PagedP& p, int sms, cudaStream_t st);
 size_t paged_decode_bytes(const PagedP& p, int sms);
-cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* launches);
+cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* launches, int* path);
 
 constexpr unsigned kNoRow = 0xffffffffu;
 

@@ -340,7 +340,7 @@ size_t paged_decode_bytes(const PagedP& p, int sms) {
   return ((size_t)p.B * p.H * pl.S * (p.HD + 1) * sizeof(float) + 255) & ~(size_t)255;
 }
 
-cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* launches) {
+cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* launches, int* path) {
   const PagedPlan pl = plan(p, sms);
   cudaError_t e;
   if ((long long)p.B * p.Hk * head_groups(p) * pl.S > 0x7fffffffLL) return cudaErrorInvalidConfiguration;
@@ -366,6 +366,7 @@ cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* 
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;
+  *path = mma_path(p) ? BOZO_PATH_MMA : BOZO_PATH_SIMT;
   *launches = 1;
   if (pl.S > 1 && !pl.clustered) {
     e = launch_join(p, pl, st);

@@ -421,8 +421,8 @@ def tension(q: Tensor, k: Tensor, v: Tensor, *, window: Optional[int],
 
 
 def last_path() -> str:
-    """Kernel family of the last call on this thread ("simt"/"tcgen05")."""
-    return {0: "none", 1: "simt", 2: "tcgen05"}[_capi.lib().bozo_tension_last_path()]
+    """Kernel family of the last call on this thread ("simt"/"tcgen05"/"mma")."""
+    return {0: "none", 1: "simt", 2: "tcgen05", 3: "mma"}[_capi.lib().bozo_tension_last_path()]
 
 
 def last_launches() -> int:

@@ -77,7 +77,9 @@ typedef enum { BOZO_NORM_NONE = 0, BOZO_NORM_MASS = 1, BOZO_NORM_COUNT = 2 } boz
 enum {
   BOZO_PATH_AUTO = 0,
   BOZO_PATH_SIMT = 1,     /* force the fp32 CUDA-core path */
-  BOZO_PATH_TCGEN05 = 2   /* force the tensor-core path; error if ineligible */
+  BOZO_PATH_TCGEN05 = 2,  /* force the tensor-core path; error if ineligible */
+  BOZO_PATH_MMA = 3       /* not selected, only reported (bozo_tension_last_path): the
+                             warp-level matrix instructions of bozo_paged_decode */
 };
 
 /* A strided 4-D view [B,T,H,HD] (element strides). */
@@ -377,7 +379,7 @@ int bozo_tension_error_async(int32_t* host_dst, void* stream);
 int bozo_tension_wait_selftest(uint64_t limit_ns, int32_t* result, void* stream);
 
 /* Which kernel path the last successful call in this process ran:
- * BOZO_PATH_SIMT or BOZO_PATH_TCGEN05 (0 before any call). */
+ * BOZO_PATH_SIMT, BOZO_PATH_TCGEN05 or BOZO_PATH_MMA (0 before any call). */
 int bozo_tension_last_path(void);
 
 /* Number of kernels the last successful call in this process launched. */

@@ -187,3 +187,17 @@ def test_one_element_that_is_not_finite(dtype, HD, bad, where):
     else:
         tau = tau[1, 2] if where == "query" else tau[1, 2:, n - 1 - 17]
         assert ((tau == 0) | (tau == 1) | torch.isnan(tau)).all()
+
+
+# ── what a call says of itself ──
+
+@gpu
+@pytest.mark.parametrize("dtype,HD,path", [(BF16, 64, "mma"), (F16, 128, "mma"), (F8, 32, "mma"), (I8, 64, "mma"),
+                                           (F32, 64, "simt"), (BF16, 48, "simt"), (I8, 21, "simt")])
+def test_last_path_names_the_kernel(dtype, HD, path):
+    pool = Pool(1, 1, HD, 16, 2, dtype)
+    x = torch.randn(1, 1, HD, device="cuda").to(dtype if dtype in ULP else BF16)
+    paged.write_kv(x, x, *pool.cache, int32([0]), **pool.scales)
+    assert ops.last_path() == "simt"
+    paged.paged_tension(x, *pool.cache, int32([0]), window=None, **pool.scales)
+    assert ops.last_path() == path and ops.last_launches() == 1
