@@ -166,7 +166,7 @@ const char* bozo_status_string(int s) {
     case BOZO_ERR_BAD_SHAPE: return "bad shape or size argument";
     case BOZO_ERR_BAD_DTYPE: return "unsupported dtype code";
     case BOZO_ERR_UNSUPPORTED: return "unsupported configuration";
-    case BOZO_ERR_ALIGNMENT: return "tensor-core path needs 16-byte aligned rows with unit HD stride";
+    case BOZO_ERR_ALIGNMENT: return "tensor-core path needs 16-byte aligned rows with unit HD stride, a paged cache 16-byte aligned pages and workspace";
     case BOZO_ERR_NULL: return "required pointer is NULL";
     case BOZO_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait timed out";
     case BOZO_ERR_CUDA: return "CUDA runtime error";

@@ -430,8 +430,9 @@ def last_launches() -> int:
 
 
 def poll_device_error(device=None) -> None:
-    """Synchronise and raise if a bounded device-side wait timed out (the
-    error word is cleared by the read)."""
+    """Synchronise and raise if a bounded device-side wait timed out or a
+    paged-cache kernel skipped an index out of range (the error word is cleared
+    by the read)."""
     dev = torch.device(device) if device is not None else torch.device("cuda")
     with torch.cuda.device(dev):
         code = _capi.lib().bozo_tension_poll_error(_stream(dev))
@@ -455,9 +456,9 @@ def check_device_error(device=None) -> None:
 
     Reads the word copied by the previous call if that copy has completed
     (no synchronisation), raises through ``poll_device_error`` when a bounded
-    wait gave up in some earlier launch, then enqueues the next asynchronous
-    copy on the current stream.  A timeout is thus reported at most one step
-    late instead of never; nothing is enqueued while the stream is capturing
+    wait gave up or a paged-cache kernel skipped an index in some earlier launch,
+    then enqueues the next asynchronous copy on the current stream.  An error is
+    thus reported at most one step late instead of never; nothing is enqueued while the stream is capturing
     a CUDA graph."""
     if torch.cuda.is_current_stream_capturing():
         return  # no event query or copy may join a graph capture
@@ -470,7 +471,7 @@ def check_device_error(device=None) -> None:
     if w.event is not None and w.event.query() and int(w.host[0]) != 0:
         w.host.zero_()
         w.event = None
-        poll_device_error(dev)  # raises BOZO_ERR_DEVICE_TIMEOUT and clears the word
+        poll_device_error(dev)  # raises and clears the word
     with torch.cuda.device(dev):
         code = _capi.lib().bozo_tension_error_async(w.host.data_ptr(), _stream(dev))
     _capi.check(code, "device error copy")

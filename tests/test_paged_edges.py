@@ -201,3 +201,11 @@ def test_last_path_names_the_kernel(dtype, HD, path):
     assert ops.last_path() == "simt"
     paged.paged_tension(x, *pool.cache, int32([0]), window=None, **pool.scales)
     assert ops.last_path() == path and ops.last_launches() == 1
+
+
+@gpu
+def test_misaligned_pages_are_refused_by_name():
+    pages = torch.zeros(1 + 2 * 2 * 16 * 64, device="cuda", dtype=BF16)[1:].view(2, 2, 16, 64)
+    x, table = torch.randn(1, 2, 64, device="cuda", dtype=BF16), int32([[0]])
+    with pytest.raises(RuntimeError, match="aligned pages"):
+        paged.write_kv(x, x, pages, pages, table, int32([0]))
