@@ -291,8 +291,10 @@ int head_groups(const PagedP& p) {
 // 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).
 // Up to eight pieces are joined inside a cluster, which saves a second kernel's
 // 2-3 µs of a call, where the clusters all find their place at once (12 rows of 1024
-// keys in eight: 5.9 µs and 8.2 a call, 6.1 and 10.1 with a second kernel; 192 rows
-// in four: 14.5 against 13.6); so a few pieces more than eight become eight, and
+// keys in eight: 5.9 µs and 8.2 a call, 6.1 and 10.1 with a second kernel; 192 rows of up
+// to 1000 keys in two 9.7 against 10.4, in four 14.5 against 13.6; 300 rows of 4192 keys
+// in two 60.1 against 58.9, 1600 such rows 266 against 255, 1024 rows of up to 8191
+// keys 163.0 against 163.9); so a few pieces more than eight become eight, and
 // whatever is asked for where that leaves 256 keys (12 rows of 2048 keys: 6.5
 // against 6.7 µs in sixteen; of 8192 keys 11.2 against 8.7).  Short rows stay whole
 // (48 rows of 256 keys: 5.2 µs, 5.9 in two).
@@ -307,7 +309,7 @@ PagedPlan plan(const PagedP& p, int sms) {
   if (mma && s > kCluster && (s <= kCluster + 4 || keys <= 256 * kCluster)) s = kCluster;
   if (!mma && !rows_path(p)) s = std::max(s, (keys + 15 + kMaxPiece - 1) / kMaxPiece);
   s = std::max(s, 1LL);
-  return {(int)s, mma && (s == 2 || (s > 2 && s <= kCluster && rows * s <= 3LL * sms))};
+  return {(int)s, mma && s > 1 && s <= kCluster && rows * s <= 3LL * sms};
 }
 
 template <int DT>

@@ -209,3 +209,26 @@ def test_misaligned_pages_are_refused_by_name():
     x, table = torch.randn(1, 2, 64, device="cuda", dtype=BF16), int32([[0]])
     with pytest.raises(RuntimeError, match="aligned pages"):
         paged.write_kv(x, x, pages, pages, table, int32([0]))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F8])
+@pytest.mark.parametrize("B,launches", [(192, 1), (1024, 2)])
+def test_two_pieces_joined_in_a_cluster_or_by_a_kernel(dtype, B, launches):
+    """Pieces are joined in clusters where these all find their place at once, else by
+    a second kernel: with the same result as a few rows, cut up further, give."""
+    n = 640 if B == 192 else 4200
+    pool = Pool(1, 1, 32, 16, -(-n // 16), dtype)
+    fill(pool, [n], 1, 32, BF16, None, B)
+    lengths = [(i * 131) % n for i in range(B)]
+    q = torch.randn(B, 1, 32, device="cuda", dtype=BF16)
+
+    def run(rows):
+        table = pool.table.expand(len(rows), -1).contiguous()
+        return paged.paged_tension(q[rows], pool.k, pool.v, table, int32([lengths[i] for i in rows]), window=None,
+                                   **pool.scales).float()
+
+    out = run(list(range(B)))
+    assert ops.last_launches() == launches
+    some = list(range(0, B, B // 8))
+    torch.testing.assert_close(out[some], run(some), rtol=2.0 ** -7, atol=1e-5)
