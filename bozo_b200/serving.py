@@ -341,16 +341,19 @@ class PagedStepGraph:
         self.tokens = torch.zeros(state.slots, dtype=torch.long, device=dev)
         held = state.lengths.clone()
         side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):  # warm up with every slot idle: nothing is written
-            state.lengths.fill_(-1)
-            for _ in range(warmup):
-                _step(state, self.tokens, export)
-        torch.cuda.current_stream(dev).wait_stream(side)
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
-            self.out = _step(state, self.tokens, export)
-        state.lengths.copy_(held)
+        try:
+            state.lengths.fill_(-1)  # every slot idle: nothing is written
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                for _ in range(warmup):
+                    _step(state, self.tokens, export)
+            torch.cuda.current_stream(dev).wait_stream(side)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self.out = _step(state, self.tokens, export)
+        finally:
+            torch.cuda.current_stream(dev).wait_stream(side)
+            state.lengths.copy_(held)
 
     def __call__(self, tokens: Tensor):
         _check_tokens(self.state, tokens)

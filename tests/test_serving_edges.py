@@ -124,3 +124,21 @@ def test_past_max_seq_len_global_layers_reach_whole_pages(page):
     for i in range(25):
         tok = torch.tensor(ids(2, 700 + i), device="cuda:0")
         close(serving.step(state, tok)[slot], decode.step(ring, tok[slot:slot + 1])[0], f"step {i}")
+
+
+@gpu
+def test_a_failed_capture_leaves_the_sequences(monkeypatch):
+    model = make("rope_global")
+    state = serving.PagedState(model, 2, 64, page_size=16)
+    (s,), _ = serving.admit(state, [ids(16, 1)])
+
+    def fail(*a, **kw):
+        raise torch.OutOfMemoryError("out of memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(model.final_norm, "forward", fail)
+        with pytest.raises(torch.OutOfMemoryError):
+            serving.PagedStepGraph(state)
+    assert state.lengths.tolist()[s] == 16
+    run = serving.PagedStepGraph(state)
+    close(run(torch.full((2,), 7, dtype=torch.long, device="cuda:0"))[s], full(model, ids(16, 1) + [7]), "a step")
