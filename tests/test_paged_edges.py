@@ -232,3 +232,30 @@ def test_two_pieces_joined_in_a_cluster_or_by_a_kernel(dtype, B, launches):
     assert ops.last_launches() == launches
     some = list(range(0, B, B // 8))
     torch.testing.assert_close(out[some], run(some), rtol=2.0 ** -7, atol=1e-5)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,HD", [(BF16, 64), (F8, 32), (F32, 64), (F16, 48), (I8, 21)])
+@pytest.mark.parametrize("page", [16, 8, 3])
+def test_positions_up_to_the_largest(dtype, HD, page):
+    """The last positions that 32 bits hold give what the same rows give at the start
+    of their ring."""
+    cap, top = 48, 2 ** 31 - 1
+    io = dtype if dtype in ULP else BF16
+    for t in (top, top - 1, top - 20):
+        low = t % cap + cap                           # the same rows of the ring
+        k, v = (torch.randn(cap, 2, HD, device="cuda").to(io) for _ in "kv")
+        q, nk, nv = (torch.randn(1, 2, HD, device="cuda").to(io) for _ in range(3))
+        got = []
+        for at in (t, low):
+            pool = Pool(1, 2, HD, page, cap // page, dtype)
+            cu = int32([0, cap])
+            paged.write_kv(k, v, *pool.cache, int32([at - cap]), cu_rows=cu, **pool.scales)
+            got.append([*paged.read_kv(*pool.cache, int32([at - cap]), cu, cap, **pool.scales),
+                        *paged.paged_tension(q, *pool.cache, int32([at]), window=30, k=nk, v=nv, return_tau=True,
+                                             **pool.scales),
+                        *paged.paged_tension(q, *pool.cache, int32([at]), window=None, return_tau=True,
+                                             tau_window=cap, **pool.scales), pool.k, pool.v])
+        for x, y in zip(*got):
+            same_bits(x, y, f"position {t}")
+    ops.poll_device_error("cuda")
