@@ -55,6 +55,32 @@ def test_fp32_queries_over_bf16_pages_keep_fp32(HD, H, Hk, window):
         assert err <= 4 * base + 2.0 ** -22, f"{name}: {err:.2e}, plain fp32 {base:.2e}"
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16, F8, I8])
+@pytest.mark.parametrize("H", [1, 4, 8])
+@pytest.mark.parametrize("shift", [-60.0, -25.0])
+def test_tiny_tau_keep_their_precision(dtype, H, shift):
+    """Scores s of up to 80 in size, summed and multiplied by 1/scale and log2 e in
+    fp32: at most four roundings of 80 at 2^-23, and as large a relative error of
+    τ = e^s, however small."""
+    n, tol = 150, 80 * 2.0 ** -23 * 4
+    pool = Pool(2, 1, 64, 16, 10, dtype)
+    k = torch.randn(2 * n, 1, 64, device="cuda") * 0.1
+    k[..., 0] = shift / 8
+    v = torch.randn(2 * n, 1, 64, device="cuda")
+    paged.write_kv(k, v, *pool.cache, int32([0, 0]), cu_rows=int32([0, n, 2 * n]), **pool.scales)
+    hist = history(pool, [n, n], 1, 64)
+    q = torch.randn(2, H, 64, device="cuda")
+    q[..., 0] = 64.0
+    out, tau = paged.paged_tension(q, *pool.cache, int32([n - 1] * 2), window=140, normalize="count",
+                                   return_tau=True, **pool.scales)
+    ref = orc.decode(q.cpu().double(), hist, [n - 1] * 2, window=140, capacity=160, scale=8.0, normalize="count",
+                     tau_width=140)
+    assert float(((tau.cpu().double() - ref[1]).abs() / ref[1].clamp(min=1e-300)).max()) <= tol
+    size = (ref[1].sum(-1) / 140 * float(v.abs().max()))[..., None]    # of the sum of magnitudes
+    assert float(((out.cpu().double() - ref[0]).abs() / size).max()) <= tol
+
+
 # ── pages that are not there ──
 
 @gpu
