@@ -214,8 +214,10 @@ __device__ __forceinline__ void block_places(const PagedP& p, unsigned n0, int r
     // the sequence of the block's first row, or the first one if that row comes before it
     if (threadIdx.x == 0) found = -1;
     __syncthreads();
-    for (int i = threadIdx.x; i < p.B; i += kThreads)
-      if ((i == 0 || __ldg(p.cu + i) <= (int)n0) && (int)n0 < __ldg(p.cu + i + 1)) found = i;
+    for (int i = threadIdx.x; i < p.B; i += kThreads) {
+      const int lo = __ldg(p.cu + i), hi = __ldg(p.cu + i + 1);
+      if (((i == 0) | (lo <= (int)n0)) & ((int)n0 < hi)) found = i;
+    }
     __syncthreads();
   }
   for (int r = threadIdx.x; r < rows; r += kThreads) {
