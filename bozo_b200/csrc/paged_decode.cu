@@ -287,7 +287,7 @@ int head_groups(const PagedP& p) {
 // Pieces of a row.  About three blocks an SM keep the memory busy (16 rows of
 // 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37).  Sequences
 // of different lengths want smaller pieces to even out — twelve an SM, of 2048 keys
-// at least (1024 rows of up to 8192 keys: 165 µs in two to four; 512 rows of up to
+// at least (1024 rows of up to 8192 keys: 164 µs in two to four; 512 rows of up to
 // 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).
 // Up to eight pieces are joined inside a cluster, which saves a second kernel's
 // 2-3 µs of a call, where the clusters all find their place at once (12 rows of 1024

@@ -22,15 +22,16 @@
 //   4 heads:       two columns and, in a product of its own, the first one again,
 //   8 heads:       a column for each head, three products;
 // those of τ rows of their own with up to 4 heads, a second product with 8.  That costs
-// nothing measurable with a head or two of 64 or 128 elements, 2-8 % at 32, 3 % with four
-// heads and 9-20 % with eight (309 MB, 128 wide: 82 µs, with two parts 68.5).
+// 0.05 µs in the shortest step, nothing measurable with a head or two of 64 or 128
+// elements (up to 6 % at 32), 3-4 % with four heads and 9-20 % with eight (309 MB, 128
+// wide: 82 µs, with two parts 68.5).
 //
 // What bounds it: 1 flop a byte for 16-bit rows of a head of their own (memory),
 // instructions for 8-bit rows of shared heads.  4 warps with 3 tiles of 4 KB each and
 // 3-4 blocks an SM keep 100-130 KB under way.  Measured: 64 sequences of up to 8192
-// keys × 16 heads, bf16: 165 µs for 1084 MB, the rate of a copy; one row set of 120002
-// keys 76 µs (0.99); e4m3, 128 wide, four heads a key head: 190-200 µs for 1106 MB
-// (0.85-0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.
+// keys × 16 heads, bf16: 164 µs for 1084 MB, the rate of a copy; one row set of 120002
+// keys 75.6 µs (0.99); e4m3, 128 wide, four heads a key head: 189 µs for 1106 MB
+// (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.
 #pragma once
 
 #include <algorithm>
