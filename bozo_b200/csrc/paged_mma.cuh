@@ -21,10 +21,11 @@
 //   up to 2 heads: four columns (one empty); two lanes share a sum and take a key each,
 //   4 heads:       two columns and, in a product of its own, the first one again,
 //   8 heads:       a column for each head, three products;
-// those of τ rows of their own with up to 4 heads, a second product with 8.  That costs
-// 0.05 µs in the shortest step, nothing measurable with a head or two of 64 or 128
-// elements (up to 6 % at 32), 3-4 % with four heads and 9-20 % with eight (309 MB, 128
-// wide: 82 µs, with two parts 68.5).
+// those of τ rows of their own with up to 4 heads; with 8, O is turned round, Oᵀ =
+// Vᵀ·Pᵀ, a column for each head and three products.  That costs 0.05 µs in the
+// shortest step, nothing measurable with a head or two of 64 or 128 elements (up to
+// 6 % at 32), 3-4 % with four heads and 3-12 % with eight (309 MB, 64 wide: 68.4 µs,
+// with two parts 66.2; 128 wide 73.6 and 67.7, with half-filled second products 82).
 //
 // What bounds it: 1 flop a byte for 16-bit rows of a head of their own (memory),
 // instructions for 8-bit rows of shared heads.  4 warps with 3 tiles of 4 KB each and
@@ -175,9 +176,10 @@ template <int DT, int HD, int GP> struct Geo {
   // Blocks an SM whose registers have to fit: two leave the compiler what it wants
   // (e4m3 128 wide, 616 MB: 113 µs, with three 118; e4m3 32 wide 146 against 153),
   // but 64 wide 8-bit rows are faster under the tighter bound (e4m3, 634 MB: 113
-  // against 119), and so are 64 wide bf16 rows of up to four heads, which else take
-  // a few registers too many for a third block (617 MB: 96.7 against 99.7).
-  static constexpr int blocks = HD == 64 && (Fmt<DT>::scaled || (Fmt<DT>::bf && GP <= 4)) ? 3 : 2;
+  // against 119), and so are 64 wide bf16 rows, which else take a few registers too
+  // many for a third block (a head each, 617 MB: 96.7 against 99.7; eight heads, 309 MB:
+  // 68.4 against 74).
+  static constexpr int blocks = HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
   static constexpr bool fold = Fmt<DT>::bf && GP <= 4;  // τ's second parts have rows 4-7 of P
   static constexpr int parts = (fold ? 2 : 1) * kWarps;  // sums that are added at the end
   static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   using Z = Geo<DT, HD, GP>;
   constexpr bool BF = F::bf;
   constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size;
-  constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns a head, one
+  constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns of S a head, one
   constexpr int GQ = GP < 4 ? GP : 4;                              // heads whose columns repeat
   constexpr int NS = GP == 8 ? 2 : 1;                              // heads of a lane
   constexpr int NA = WIDE ? 1 : NS, NB = QUAD ? 1 : WIDE ? 3 : BF ? 2 : NS;  // accumulators, operands
@@ -248,11 +250,12 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   const unsigned p0 = rc.first(piece), p1 = mine ? rc.last(piece) : p0;  // this block's positions
   const unsigned nk = p1 > p0 ? p1 - p0 : 0u;
   float mass[NS], unit[NS], lim[NS];  // P operand: p · unit, renewed where p passes lim (halfs)
-  float acc[kTiles][4];
+  constexpr int kAcc = WIDE ? HD / 16 : kTiles;
+  float acc[kAcc][4];
 #pragma unroll
   for (int s = 0; s < NS; ++s) mass[s] = lim[s] = 0.f, unit[s] = 1.f;
 #pragma unroll
-  for (int j = 0; j < kTiles; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  for (int j = 0; j < kAcc; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
   const unsigned ring = smem_u32(smb) + warp * kStages * 2 * Z::kv;
   char* meta = smb + kWarps * kStages * 2 * Z::kv + warp * kStages * Z::meta;
@@ -607,15 +610,27 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
         }
         if constexpr (SZ == 2) {
           const unsigned a = vt + ring_at<SZ, R, true>(u * 16 + mrow, mch);
+          if constexpr (WIDE) {  // Oᵀ = Vᵀ·Pᵀ: a product for each of the eight heads' parts
+            constexpr int N = kAcc < 4 ? kAcc : 4;  // side by side
 #pragma unroll
-          for (int j = 0; j < kTiles; j += 2) {
-            unsigned w[4];
-            ldmatrix4<true>(a ^ (j << 4), w);
-            mma16816<BF>(acc[j], a0, a1, a2, a3, w[0], w[1]);
-            mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
-            if constexpr (BF && !FOLD) {
-              mma16816<BF>(acc[j], l0, 0u, l2, 0u, w[0], w[1]);
-              mma16816<BF>(acc[j + 1], l0, 0u, l2, 0u, w[2], w[3]);
+            for (int j = 0; j < kAcc; j += N) {
+              unsigned w[N][4];
+#pragma unroll
+              for (int i = 0; i < N; ++i) ldmatrix4<true>(a ^ ((j + i) << 5), w[i]);
+#pragma unroll
+              for (int i = 0; i < N; ++i) mma16816<BF>(acc[j + i], w[i][0], w[i][2], w[i][1], w[i][3], a0, a2);
+#pragma unroll
+              for (int i = 0; i < N; ++i) mma16816<BF>(acc[j + i], w[i][0], w[i][2], w[i][1], w[i][3], a1, a3);
+#pragma unroll
+              for (int i = 0; i < N; ++i) mma16816<BF>(acc[j + i], w[i][0], w[i][2], w[i][1], w[i][3], l0, l2);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kTiles; j += 2) {
+              unsigned w[4];
+              ldmatrix4<true>(a ^ (j << 4), w);
+              mma16816<BF>(acc[j], a0, a1, a2, a3, w[0], w[1]);
+              mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
             }
           }
         } else {
@@ -681,7 +696,14 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   }
   // rows of O: head g, or with FOLD head g mod 4 in two parts
   const int hrow = FOLD ? g & 3 : g;
-  if (hrow < Gh && warp < kWarps) {
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int j = 0; j < kAcc; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)  // head 2c or 2c + 1, element g or g + 8
+        if (2 * c + (e & 1) < Gh && warp < kWarps)
+          part[(warp * Gh + 2 * c + (e & 1)) * HD + 16 * j + g + 8 * (e >> 1)] = acc[j][e];
+  } else if (hrow < Gh && warp < kWarps) {
     const float back = 1.f / un;
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
