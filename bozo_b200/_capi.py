@@ -20,7 +20,7 @@ ERR_SCRATCH_LIMIT = 9
 ERR_DEVICE_INDEX = 10
 NOALLOC_SCRATCH_BYTES = 8 << 20  # BOZO_NOALLOC_SCRATCH_BYTES
 DT_F32, DT_BF16, DT_F16 = 0, 1, 2
-DT_F8E4M3, DT_I8 = 3, 4  # paged-cache rows only
+DT_F8E4M3, DT_I8, DT_F4E2M1 = 3, 4, 6  # paged-cache rows only
 MODE_LOCAL, MODE_GLOBAL = 0, 1
 NORM_NONE, NORM_MASS, NORM_COUNT = 0, 1, 2
 PATH_AUTO, PATH_SIMT, PATH_TCGEN05 = 0, 1, 2
@@ -41,6 +41,8 @@ EXPORTED = (
     "bozo_wo_add_rmsnorm_fwd", "bozo_wo_add_rmsnorm_supported",
     "bozo_embedding_bwd",
     "bozo_paged_write", "bozo_paged_read", "bozo_paged_decode", "bozo_paged_decode_workspace",
+    "bozo_paged_reserve", "bozo_paged_fork", "bozo_paged_copy",
+    "bozo_beam_select", "bozo_beam_select_workspace",
 )
 TAU_AUX_MAX_LAYERS = 64  # BOZO_TAU_AUX_MAX_LAYERS
 
@@ -111,6 +113,7 @@ class PagedWriteArgs(C.Structure):
         ("cache", PagedCache), ("rows", C.c_int64), ("cu_rows", C.c_void_p),
         ("rope_len", C.c_int32), ("_pad", C.c_int32), ("rope_cos", C.c_void_p),
         ("rope_sin", C.c_void_p), ("k", Tensor4), ("v", Tensor4),
+        ("k_group", C.c_void_p), ("v_group", C.c_void_p),
     ]
 
 
@@ -118,7 +121,7 @@ class PagedReadArgs(C.Structure):
     _fields_ = [
         ("cache", PagedCache), ("rows", C.c_int64), ("cu_rows", C.c_void_p),
         ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("out_dtype", C.c_int32),
-        ("_pad", C.c_int32),
+        ("_pad", C.c_int32), ("k_group", C.c_void_p), ("v_group", C.c_void_p),
     ]
 
 
@@ -130,6 +133,44 @@ class PagedDecodeArgs(C.Structure):
         ("rope_sin", C.c_void_p), ("q", Tensor4), ("k", Tensor4), ("v", Tensor4),
         ("out", C.c_void_p), ("tau", C.c_void_p), ("out_dtype", C.c_int32),
         ("tau_dtype", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("k_group", C.c_void_p), ("v_group", C.c_void_p),
+    ]
+
+
+class PagedReserveArgs(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("table_stride", C.c_int64), ("batch", C.c_int32),
+        ("width", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
+        ("lengths", C.c_void_p), ("tokens", C.c_void_p), ("refs", C.c_void_p),
+        ("cu_rows", C.c_void_p), ("missing", C.c_void_p), ("rows", C.c_int64),
+        ("seq", C.c_void_p), ("pos", C.c_void_p), ("slot", C.c_void_p),
+    ]
+
+
+class PagedForkArgs(C.Structure):
+    _fields_ = [
+        ("table", C.c_void_p), ("table_stride", C.c_int64), ("batch", C.c_int32),
+        ("width", C.c_int32), ("page_size", C.c_int32), ("pages", C.c_int32),
+        ("lengths", C.c_void_p), ("parents", C.c_void_p), ("refs", C.c_void_p),
+        ("share", C.c_int32), ("_pad", C.c_int32), ("copies", C.c_void_p), ("missing", C.c_void_p),
+    ]
+
+
+class PagedCopyArgs(C.Structure):
+    _fields_ = [
+        ("pools", C.POINTER(C.c_void_p)), ("page_bytes", C.POINTER(C.c_int64)),
+        ("n_pools", C.c_int32), ("pages", C.c_int32), ("copies", C.c_void_p),
+        ("n_copies", C.c_int64),
+    ]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [
+        ("logits", C.c_void_p), ("row_stride", C.c_int64), ("dtype", C.c_int32),
+        ("prompts", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("eos", C.c_int32),
+        ("_pad", C.c_int32), ("scores", C.c_void_p), ("done", C.c_void_p),
+        ("out_scores", C.c_void_p), ("out_tokens", C.c_void_p), ("out_rows", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -254,6 +295,16 @@ def lib():
                 L.bozo_paged_decode.restype = C.c_int
                 L.bozo_paged_decode_workspace.argtypes = [C.POINTER(PagedDecodeArgs)]
                 L.bozo_paged_decode_workspace.restype = C.c_size_t
+                L.bozo_paged_reserve.argtypes = [C.POINTER(PagedReserveArgs), C.c_void_p]
+                L.bozo_paged_reserve.restype = C.c_int
+                L.bozo_paged_fork.argtypes = [C.POINTER(PagedForkArgs), C.c_void_p]
+                L.bozo_paged_fork.restype = C.c_int
+                L.bozo_paged_copy.argtypes = [C.POINTER(PagedCopyArgs), C.c_void_p]
+                L.bozo_paged_copy.restype = C.c_int
+                L.bozo_beam_select.argtypes = [C.POINTER(BeamSelectArgs), C.c_void_p]
+                L.bozo_beam_select.restype = C.c_int
+                L.bozo_beam_select_workspace.argtypes = [C.POINTER(BeamSelectArgs)]
+                L.bozo_beam_select_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_workspace.argtypes = [C.POINTER(TauAuxFwdArgs)]
                 L.bozo_tau_aux_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_fwd.argtypes = [C.POINTER(TauAuxFwdArgs), C.c_void_p]

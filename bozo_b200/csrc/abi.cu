@@ -7,7 +7,9 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "beam.cuh"
 #include "paged.cuh"
+#include "pool.cuh"
 #include "tc.cuh"
 #include "tc_host.cuh"
 
@@ -500,22 +502,25 @@ int bozo_tension_decode(const bozo_tension_decode_args* a, void* stream) {
   return BOZO_OK;
 }
 
-static int check_paged(const bozo_paged_cache& c) {
+static int check_paged(const bozo_paged_cache& c, const uint8_t* kg, const uint8_t* vg) {
   if (c.pages <= 0 || c.kv_heads <= 0 || c.page_size <= 0 || c.HD <= 0 || c.batch <= 0 ||
       c.width <= 0 || c.table_stride < 0)
     return BOZO_ERR_BAD_SHAPE;
-  const bool eight = c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
-  if (!eight && !dtype_ok(c.dtype)) return BOZO_ERR_BAD_DTYPE;
-  if (c.HD > 128) return BOZO_ERR_UNSUPPORTED;
+  const bool four = c.dtype == BOZO_DT_F4E2M1;
+  const bool scaled = four || c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
+  if (!scaled && !dtype_ok(c.dtype)) return BOZO_ERR_BAD_DTYPE;
+  if (c.HD > 128 || (four && c.HD % 16)) return BOZO_ERR_UNSUPPORTED;
   // rows are numbered in 32 bits, and so are a sequence's positions
   if ((double)c.pages * c.kv_heads * c.page_size >= 4294967295.0 ||
       (long long)c.width * c.page_size > 0x7fffffffLL)
     return BOZO_ERR_UNSUPPORTED;
   if (!c.k_pages || !c.v_pages || !c.table || !c.lengths) return BOZO_ERR_NULL;
-  if (eight && (!c.k_scale || !c.v_scale)) return BOZO_ERR_NULL;
-  if (!eight && (c.k_scale || c.v_scale)) return BOZO_ERR_BAD_SHAPE;
+  if (scaled && (!c.k_scale || !c.v_scale)) return BOZO_ERR_NULL;
+  if (four && (!kg || !vg)) return BOZO_ERR_NULL;
+  if (!scaled && (c.k_scale || c.v_scale)) return BOZO_ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages)) & 15)
     return BOZO_ERR_ALIGNMENT;
+  if (four && ((reinterpret_cast<uintptr_t>(kg) | reinterpret_cast<uintptr_t>(vg)) & 15)) return BOZO_ERR_ALIGNMENT;
   return BOZO_OK;
 }
 
@@ -529,7 +534,7 @@ static int check_rope(int len, const float* cos, const float* sin, int HD) {
 int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
   int st;
-  if ((st = check_paged(a->cache))) return st;
+  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
   if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
     return BOZO_ERR_BAD_SHAPE;
   if ((st = check_rope(a->rope_len, a->rope_cos, a->rope_sin, a->cache.HD))) return st;
@@ -538,7 +543,7 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   DeviceRestore restore;
   cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
-  PagedP p = paged_params(a->cache);
+  PagedP p = paged_params(a->cache, a->k_group, a->v_group);
   p.rows = a->rows; p.cu = a->cu_rows;
   p.rope_len = a->rope_len;
   p.cos = a->rope_len ? a->rope_cos : nullptr;
@@ -555,7 +560,7 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
 int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
   int st;
-  if ((st = check_paged(a->cache))) return st;
+  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
   if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
     return BOZO_ERR_BAD_SHAPE;
   if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
@@ -564,7 +569,7 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   DeviceRestore restore;
   cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
-  PagedP p = paged_params(a->cache);
+  PagedP p = paged_params(a->cache, a->k_group, a->v_group);
   p.rows = a->rows; p.cu = a->cu_rows;
   p.k_out = a->k_out; p.v_out = a->v_out; p.out_dt = a->out_dtype;
   if (!(p.err = error_word(&e))) return cuda_fail(e);
@@ -579,7 +584,7 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
 static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
   if (!a) return BOZO_ERR_NULL;
   int st;
-  if ((st = check_paged(a->cache))) return st;
+  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
   const bozo_paged_cache& c = a->cache;
   if (a->H <= 0 || a->H % c.kv_heads) return BOZO_ERR_BAD_SHAPE;
   if ((long long)c.batch * a->H > 0x7fffffffLL / 4096) return BOZO_ERR_UNSUPPORTED;
@@ -599,7 +604,7 @@ static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
   if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
   if (a->tau && (!dtype_ok(a->tau_dtype) || a->tau_width < 1)) return BOZO_ERR_BAD_SHAPE;
   if (a->mode == BOZO_MODE_LOCAL && a->tau && a->tau_width != a->window) return BOZO_ERR_BAD_SHAPE;
-  p = paged_params(c);
+  p = paged_params(c, a->k_group, a->v_group);
   p.rows = c.batch;
   p.rope_len = a->rope_len;
   p.cos = a->rope_len ? a->rope_cos : nullptr;
@@ -637,6 +642,127 @@ int bozo_paged_decode(const bozo_paged_decode_args* a, void* stream) {
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = path;
   t_last_launches = launches;
+  return BOZO_OK;
+}
+
+static int check_table(const int32_t* table, int64_t stride, int B, int M, int page, int P, const int32_t* lengths,
+                       const int32_t* refs) {
+  if (B <= 0 || M <= 0 || page <= 0 || P <= 0 || stride < 0) return BOZO_ERR_BAD_SHAPE;
+  // places, positions and table entries are numbered in 31 bits
+  if (B > kMaxTableRows || (long long)P * page > 0x7fffffffLL || (long long)M * page > 0x7fffffffLL ||
+      (long long)B * M > 0x7fffffffLL)
+    return BOZO_ERR_UNSUPPORTED;
+  return table && lengths && refs ? BOZO_OK : BOZO_ERR_NULL;
+}
+
+int bozo_paged_reserve(const bozo_paged_reserve_args* a, void* stream) {
+  if (!a) return BOZO_ERR_NULL;
+  int st;
+  if ((st = check_table(a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->lengths, a->refs)))
+    return st;
+  if (a->rows < 0 || a->rows > 0x7fffffffLL) return BOZO_ERR_BAD_SHAPE;
+  if (!a->cu_rows || !a->missing || (a->rows && (!a->seq || !a->pos || !a->slot))) return BOZO_ERR_NULL;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->table, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  ReserveP p{a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->lengths, a->tokens, a->refs,
+             a->cu_rows, a->missing, a->rows, a->seq, a->pos, a->slot, error_word(&e)};
+  if (!p.err) return cuda_fail(e);
+  e = launch_paged_reserve(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = 1;
+  return BOZO_OK;
+}
+
+int bozo_paged_fork(const bozo_paged_fork_args* a, void* stream) {
+  if (!a) return BOZO_ERR_NULL;
+  int st;
+  if ((st = check_table(a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->lengths, a->refs)))
+    return st;
+  if (!a->parents || !a->copies || !a->missing) return BOZO_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->copies) & 7) return BOZO_ERR_ALIGNMENT;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->table, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  ForkP p{a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->share ? 1 : 0, a->lengths,
+          a->parents, a->refs, a->copies, a->missing, error_word(&e)};
+  if (!p.err) return cuda_fail(e);
+  e = launch_paged_fork(p, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = 1;
+  return BOZO_OK;
+}
+
+int bozo_paged_copy(const bozo_paged_copy_args* a, void* stream) {
+  if (!a) return BOZO_ERR_NULL;
+  if (a->n_pools < 0 || a->pages <= 0 || a->n_copies < 0 || a->n_copies > 0x7fffffffLL) return BOZO_ERR_BAD_SHAPE;
+  if (a->n_pools == 0 || a->n_copies == 0) return BOZO_OK;
+  if (!a->pools || !a->page_bytes || !a->copies) return BOZO_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(a->copies) & 7) return BOZO_ERR_ALIGNMENT;
+  for (int i = 0; i < a->n_pools; ++i) {
+    if (!a->pools[i]) return BOZO_ERR_NULL;
+    if (a->page_bytes[i] <= 0) return BOZO_ERR_BAD_SHAPE;
+  }
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->copies, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  int launches = 0;
+  for (int i = 0; i < a->n_pools; i += kCopyPools) {
+    const int n = a->n_pools - i < kCopyPools ? a->n_pools - i : kCopyPools;
+    CopyP p{};
+    for (int j = 0; j < n; ++j) {
+      p.pool[j] = static_cast<char*>(a->pools[i + j]);
+      p.bytes[j] = a->page_bytes[i + j];
+    }
+    p.P = a->pages;
+    p.copies = a->copies;
+    e = launch_paged_copy(p, n, a->n_copies, static_cast<cudaStream_t>(stream));
+    if (e != cudaSuccess) return cuda_fail(e);
+    ++launches;
+  }
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = launches;
+  return BOZO_OK;
+}
+
+static int beam_params(const bozo_beam_select_args* a, BeamP& p) {
+  if (!a) return BOZO_ERR_NULL;
+  if (a->prompts <= 0 || a->beams <= 0 || a->vocab < a->beams || a->row_stride < 0 || a->eos < -1 ||
+      a->eos >= a->vocab || (a->done && a->eos < 0))
+    return BOZO_ERR_BAD_SHAPE;
+  if (!dtype_ok(a->dtype)) return BOZO_ERR_BAD_DTYPE;
+  if (a->beams > kMaxBeams || a->vocab > kMaxVocab || (long long)a->prompts * a->beams > 65535)
+    return BOZO_ERR_UNSUPPORTED;
+  if (!a->logits || !a->scores || !a->out_scores || !a->out_tokens || !a->out_rows) return BOZO_ERR_NULL;
+  p = BeamP{};
+  p.logits = a->logits; p.stride = a->row_stride; p.dt = a->dtype;
+  p.N = a->prompts; p.K = a->beams; p.V = a->vocab; p.eos = a->eos;
+  p.scores = a->scores; p.done = a->done;
+  p.out_scores = a->out_scores; p.out_tokens = reinterpret_cast<long long*>(a->out_tokens); p.out_rows = a->out_rows;
+  return BOZO_OK;
+}
+
+size_t bozo_beam_select_workspace(const bozo_beam_select_args* a) {
+  BeamP p;
+  return beam_params(a, p) == BOZO_OK ? beam_bytes(p) : 0;
+}
+
+int bozo_beam_select(const bozo_beam_select_args* a, void* stream) {
+  BeamP p;
+  const int st = beam_params(a, p);
+  if (st) return st;
+  const size_t need = beam_bytes(p);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return BOZO_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return BOZO_ERR_ALIGNMENT;
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->logits, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  e = launch_beam(p, a->workspace, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e);
+  t_last_path = BOZO_PATH_SIMT;
+  t_last_launches = 2;
   return BOZO_OK;
 }
 

@@ -286,6 +286,7 @@ bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const 
   switch (k_pages.scalar_type()) {
     case at::kFloat8_e4m3fn: c.dtype = BOZO_DT_F8E4M3; break;
     case at::kChar: c.dtype = BOZO_DT_I8; break;
+    case at::ScalarType::Float4_e2m1fn_x2: c.dtype = BOZO_DT_F4E2M1; break;
     default: c.dtype = dtype_code(k_pages.scalar_type());
   }
   if (k_pages.dim() != 4 || !k_pages.is_contiguous() || !v_pages.is_contiguous() ||
@@ -299,17 +300,18 @@ bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const 
       lengths.size(0) != table.size(0) || !lengths.is_contiguous())
     throw bad("lengths must be an int32 [B] tensor on the pages' device");
   const at::Tensor* sc[2] = {given(k_scale), given(v_scale)};
-  const bool eight = c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
+  const bool four = c.dtype == BOZO_DT_F4E2M1;
+  const bool scaled = four || c.dtype == BOZO_DT_F8E4M3 || c.dtype == BOZO_DT_I8;
   for (const at::Tensor* t : sc) {
-    if (eight != (t != nullptr))
-      throw bad("k_scale and v_scale go with 8-bit pages, and only with them");
+    if (scaled != (t != nullptr))
+      throw bad("k_scale and v_scale go with 8- and 4-bit pages, and only with them");
     if (t && (t->scalar_type() != at::kFloat || t->device() != dev || !t->is_contiguous() ||
               t->sizes() != k_pages.sizes().slice(0, 3)))
       throw bad("scales must be contiguous float32 [pages, kv_heads, page_size] tensors on the pages' device");
   }
   c.k_pages = k_pages.data_ptr();
   c.v_pages = v_pages.data_ptr();
-  if (eight) {
+  if (scaled) {
     c.k_scale = sc[0]->data_ptr<float>();
     c.v_scale = sc[1]->data_ptr<float>();
   }
@@ -317,7 +319,7 @@ bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const 
   c.pages = (int32_t)k_pages.size(0);
   c.kv_heads = (int32_t)k_pages.size(1);
   c.page_size = (int32_t)k_pages.size(2);
-  c.HD = (int32_t)k_pages.size(3);
+  c.HD = (int32_t)k_pages.size(3) * (four ? 2 : 1);
   c.batch = (int32_t)table.size(0);
   c.width = (int32_t)table.size(1);
   c.table = table.data_ptr<int32_t>();
@@ -325,6 +327,25 @@ bozo_paged_cache paged_cache(const char* what, const at::Tensor& k_pages, const 
   c.lengths = lengths.data_ptr<int32_t>();
   c.device_current = 1;  // every caller holds a guard of the pages' device
   return c;
+}
+
+// The group scales of 4-bit pages.
+template <typename A>
+void groups_of(const char* what, A& a, const c10::optional<at::Tensor>& k_group, const c10::optional<at::Tensor>& v_group,
+               const at::Tensor& k_pages) {
+  auto bad = [&](const char* msg) { return std::invalid_argument(std::string(what) + ": " + msg); };
+  const at::Tensor* g[2] = {given(k_group), given(v_group)};
+  const bool four = a.cache.dtype == BOZO_DT_F4E2M1;
+  if (four && a.cache.HD % 16) throw bad("4-bit pages hold rows of a multiple of 16 elements");
+  for (const at::Tensor* t : g) {
+    if (four != (t != nullptr)) throw bad("k_group and v_group go with 4-bit pages, and only with them");
+    if (t && (t->scalar_type() != at::kFloat8_e4m3fn || t->device() != k_pages.device() || !t->is_contiguous() ||
+              t->dim() != 4 || t->sizes().slice(0, 3) != k_pages.sizes().slice(0, 3) || t->size(3) * 16 != a.cache.HD))
+      throw bad("group scales must be contiguous float8_e4m3fn [pages, kv_heads, page_size, HD/16] tensors on the pages' device");
+  }
+  if (!four) return;
+  a.k_group = static_cast<uint8_t*>(g[0]->data_ptr());
+  a.v_group = static_cast<uint8_t*>(g[1]->data_ptr());
 }
 
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Device& dev) {
@@ -377,11 +398,13 @@ void paged_write(const at::Tensor& k, const at::Tensor& v, const at::Tensor& k_p
                  const at::Tensor& v_pages, const at::Tensor& table, const at::Tensor& lengths,
                  const c10::optional<at::Tensor>& cu_rows, const c10::optional<at::Tensor>& cos,
                  const c10::optional<at::Tensor>& sin, const c10::optional<at::Tensor>& k_scale,
-                 const c10::optional<at::Tensor>& v_scale) {
+                 const c10::optional<at::Tensor>& v_scale, const c10::optional<at::Tensor>& k_group,
+                 const c10::optional<at::Tensor>& v_group) {
   const char* what = "write_kv";
   no_grad(what, {&k, &v});
   bozo_paged_write_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  groups_of(what, a, k_group, v_group, k_pages);
   const auto dev = k_pages.device();
   const c10::cuda::CUDAGuard guard(dev);
   a.rows = k.size(0);
@@ -396,10 +419,11 @@ std::tuple<at::Tensor, at::Tensor> paged_read(
     const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
     const at::Tensor& lengths, const c10::optional<at::Tensor>& cu_rows, int64_t rows,
     const c10::optional<at::Tensor>& k_scale, const c10::optional<at::Tensor>& v_scale,
-    int64_t out_dtype) {
+    int64_t out_dtype, const c10::optional<at::Tensor>& k_group, const c10::optional<at::Tensor>& v_group) {
   const char* what = "read_kv";
   bozo_paged_read_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  groups_of(what, a, k_group, v_group, k_pages);
   const auto dev = k_pages.device();
   const c10::cuda::CUDAGuard guard(dev);
   if (rows < 0) throw std::invalid_argument("read_kv: rows must not be negative");
@@ -424,11 +448,14 @@ pybind11::object paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
                                      const c10::optional<at::Tensor>& k,
                                      const c10::optional<at::Tensor>& v,
                                      const c10::optional<at::Tensor>& k_scale,
-                                     const c10::optional<at::Tensor>& v_scale, int64_t tau_width) {
+                                     const c10::optional<at::Tensor>& v_scale, int64_t tau_width,
+                                     const c10::optional<at::Tensor>& k_group,
+                                     const c10::optional<at::Tensor>& v_group) {
   const char* what = "paged_tension";
   no_grad(what, {&q, given(k), given(v)});
   bozo_paged_decode_args a{};
   a.cache = paged_cache(what, k_pages, v_pages, table, lengths, k_scale, v_scale);
+  groups_of(what, a, k_group, v_group, k_pages);
   const auto dev = k_pages.device();
   const c10::cuda::CUDAGuard guard(dev);
   const int64_t B = a.cache.batch, H = q.dim() == 3 ? q.size(1) : 0;
@@ -469,6 +496,159 @@ pybind11::object paged_decode(const at::Tensor& q, const at::Tensor& k_pages,
   check(bozo_paged_decode(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_decode");
   if (tau_width > 0) return pybind11::make_tuple(std::move(out), std::move(tau));
   return pybind11::cast(std::move(out));
+}
+
+// ── page tables on the device ──
+
+// The page table, lengths and counts of a pool, checked; returns the table's device.
+template <typename A>
+c10::Device table_of(const char* what, A& a, const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& refs,
+                     int64_t page_size) {
+  auto bad = [&](const char* msg) { return std::invalid_argument(std::string(what) + ": " + msg); };
+  const auto dev = table.device();
+  if (!dev.is_cuda()) throw std::runtime_error(std::string(what) + ": page tables live on CUDA only (no CPU fallback)");
+  if (table.dim() != 2 || table.scalar_type() != at::kInt || (table.size(1) > 1 && table.stride(1) != 1) ||
+      (table.size(0) > 1 && table.stride(0) < table.size(1)))
+    throw bad("page_table must be an int32 [B, width] tensor of rows of its own");
+  if (lengths.dim() != 1 || lengths.scalar_type() != at::kInt || lengths.device() != dev ||
+      lengths.size(0) != table.size(0) || !lengths.is_contiguous())
+    throw bad("lengths must be an int32 [B] tensor on the table's device");
+  if (refs.dim() != 1 || refs.scalar_type() != at::kInt || refs.device() != dev || !refs.is_contiguous())
+    throw bad("refs must be an int32 [pages] tensor on the table's device");
+  if (page_size < 1 || page_size > INT32_MAX || table.size(0) > INT32_MAX || table.size(1) > INT32_MAX ||
+      refs.size(0) > INT32_MAX)
+    throw bad("page_size must be at least 1, and sizes within 32 bits");
+  a.table = table.data_ptr<int32_t>();
+  a.table_stride = table.stride(0);
+  a.batch = (int32_t)table.size(0);
+  a.width = (int32_t)table.size(1);
+  a.page_size = (int32_t)page_size;
+  a.pages = (int32_t)refs.size(0);
+  a.lengths = lengths.data_ptr<int32_t>();
+  a.refs = refs.data_ptr<int32_t>();
+  return dev;
+}
+
+const int32_t* per_row(const char* what, const char* name, const at::Tensor& t, const at::Tensor& lengths) {
+  if (t.dim() != 1 || t.scalar_type() != at::kInt || t.device() != lengths.device() || t.size(0) != lengths.size(0) ||
+      !t.is_contiguous())
+    throw std::invalid_argument(std::string(what) + ": " + name + " must be an int32 [B] tensor on the table's device");
+  return t.data_ptr<int32_t>();
+}
+
+// (cu_rows [B + 1], missing [1], places [3, rows]: sequence, position and slot)
+std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_reserve(const at::Tensor& table, const at::Tensor& lengths,
+                                                             const c10::optional<at::Tensor>& tokens,
+                                                             const at::Tensor& refs, int64_t page_size, int64_t rows) {
+  const char* what = "reserve";
+  bozo_paged_reserve_args a{};
+  const auto dev = table_of(what, a, table, lengths, refs, page_size);
+  const c10::cuda::CUDAGuard guard(dev);
+  if (given(tokens)) a.tokens = per_row(what, "tokens", *tokens, lengths);
+  if (rows < 0 || rows > INT32_MAX) throw std::invalid_argument("reserve: rows must not be negative, nor pass 2^31");
+  at::Tensor cu = empty({a.batch + 1}, at::kInt, dev), missing = empty({1}, at::kInt, dev), at_ = empty({3, rows}, at::kInt, dev);
+  a.cu_rows = cu.data_ptr<int32_t>();
+  a.missing = missing.data_ptr<int32_t>();
+  a.rows = rows;
+  if (rows) {
+    a.seq = at_.data_ptr<int32_t>();
+    a.pos = a.seq + rows;
+    a.slot = a.pos + rows;
+  }
+  check(bozo_paged_reserve(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_reserve");
+  return {std::move(cu), std::move(missing), std::move(at_)};
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_fork(const at::Tensor& table, const at::Tensor& lengths,
+                                              const at::Tensor& parents, const at::Tensor& refs, int64_t page_size,
+                                              bool share) {
+  const char* what = "fork";
+  bozo_paged_fork_args a{};
+  const auto dev = table_of(what, a, table, lengths, refs, page_size);
+  const c10::cuda::CUDAGuard guard(dev);
+  a.parents = per_row(what, "parents", parents, lengths);
+  a.share = share;
+  const int64_t n = share ? (int64_t)a.batch : (int64_t)a.batch * a.width;
+  at::Tensor copies = empty({n, 2}, at::kInt, dev), missing = empty({1}, at::kInt, dev);
+  a.copies = copies.data_ptr<int32_t>();
+  a.missing = missing.data_ptr<int32_t>();
+  check(bozo_paged_fork(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_fork");
+  return {std::move(copies), std::move(missing)};
+}
+
+void paged_copy(const std::vector<at::Tensor>& pools, const at::Tensor& copies) {
+  const char* what = "copy_pages";
+  auto bad = [&](const char* msg) { return std::invalid_argument(std::string(what) + ": " + msg); };
+  const auto dev = copies.device();
+  if (!dev.is_cuda()) throw std::runtime_error("copy_pages: paged caches live on CUDA only (no CPU fallback)");
+  if (copies.dim() != 2 || copies.size(1) != 2 || copies.scalar_type() != at::kInt || !copies.is_contiguous())
+    throw bad("copies must be a contiguous int32 [n, 2] tensor");
+  if (pools.empty()) return;
+  const c10::cuda::CUDAGuard guard(dev);
+  std::vector<void*> ptrs;
+  std::vector<int64_t> bytes;
+  const int64_t P = pools[0].dim() ? pools[0].size(0) : 0;
+  if (P < 1 || P > INT32_MAX) throw bad("pools hold at least one page, and at most 2^31");
+  for (const at::Tensor& t : pools) {
+    if (t.dim() < 1 || t.size(0) != P || !t.is_contiguous() || t.device() != dev)
+      throw bad("pools must be contiguous tensors of the same number of pages on the copies' device");
+    if (t.numel() == 0) continue;
+    ptrs.push_back(t.data_ptr());
+    bytes.push_back(t.numel() / P * (int64_t)t.element_size());
+  }
+  bozo_paged_copy_args a{};
+  a.pools = ptrs.data();
+  a.page_bytes = bytes.data();
+  a.n_pools = (int32_t)ptrs.size();
+  a.pages = (int32_t)P;
+  a.copies = copies.data_ptr<int32_t>();
+  a.n_copies = copies.size(0);
+  check(bozo_paged_copy(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_copy");
+}
+
+// ── beam search ──
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& logits, const at::Tensor& scores,
+                                                           const c10::optional<at::Tensor>& done, int64_t eos) {
+  const char* what = "beam.select";
+  auto bad = [&](const char* msg) { return std::invalid_argument(std::string(what) + ": " + msg); };
+  const auto dev = logits.device();
+  if (!dev.is_cuda()) throw std::runtime_error("beam.select runs on CUDA only (no CPU fallback)");
+  no_grad(what, {&logits, &scores});
+  if (scores.dim() != 2 || scores.scalar_type() != at::kFloat || scores.device() != dev || !scores.is_contiguous())
+    throw bad("scores must be a contiguous float32 [prompts, beams] tensor on the logits' device");
+  const int64_t N = scores.size(0), K = scores.size(1);
+  if (logits.dim() != 2 || logits.size(0) != N * K || (logits.size(1) > 1 && logits.stride(1) != 1))
+    throw bad("logits must be [prompts * beams, vocab] with their rows contiguous");
+  if (N < 1 || K < 1 || K > 32 || logits.size(1) < K || logits.size(1) > (1 << 20) || N * K > 65535)
+    throw bad("1 to 32 beams, a vocabulary of at least as many tokens and at most 2^20, and at most 65535 hypotheses are supported");
+  bozo_beam_select_args a{};
+  const at::Tensor* d = given(done);
+  if (d && (d->scalar_type() != at::kBool || d->sizes() != scores.sizes() || d->device() != dev || !d->is_contiguous()))
+    throw bad("done must be a contiguous bool [prompts, beams] tensor on the logits' device");
+  if (eos < -1 || eos >= logits.size(1) || (d && eos < 0)) throw bad("eos must be a token, and is wanted with done");
+  const c10::cuda::CUDAGuard guard(dev);
+  a.logits = logits.data_ptr();
+  a.row_stride = logits.stride(0);
+  a.dtype = dtype_code(logits.scalar_type());
+  a.prompts = (int32_t)N;
+  a.beams = (int32_t)K;
+  a.vocab = (int32_t)logits.size(1);
+  a.eos = (int32_t)eos;
+  a.scores = scores.data_ptr<float>();
+  a.done = d ? static_cast<const uint8_t*>(d->data_ptr()) : nullptr;
+  at::Tensor s = empty({N, K}, at::kFloat, dev), t = empty({N, K}, at::kLong, dev), r = empty({N, K}, at::kInt, dev), ws;
+  a.out_scores = s.data_ptr<float>();
+  a.out_tokens = t.data_ptr<int64_t>();
+  a.out_rows = r.data_ptr<int32_t>();
+  const int64_t need = (int64_t)bozo_beam_select_workspace(&a);
+  if (need) {
+    ws = empty(need, at::kByte, dev);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = (size_t)need;
+  }
+  check(bozo_beam_select(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_beam_select");
+  return {std::move(s), std::move(t), std::move(r)};
 }
 
 // Graph bias [T, W] (window > 0) or [T, T] (window 0) from the context's
@@ -801,6 +981,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("tension_decode", &tension_decode, "one decode step through bozo_tension_decode");
   m.def("paged_write", &paged_write, "rows into a paged cache through bozo_paged_write");
   m.def("paged_read", &paged_read, "rows of a paged cache through bozo_paged_read");
+  m.def("paged_reserve", &paged_reserve, "pages and places for new tokens through bozo_paged_reserve");
+  m.def("paged_fork", &paged_fork, "page-table rows reordered through bozo_paged_fork");
+  m.def("paged_copy", &paged_copy, "pages copied inside their pools through bozo_paged_copy");
+  m.def("beam_select", &beam_select, "best continuations through bozo_beam_select");
   m.def("paged_decode", &paged_decode, "one decode step over a paged cache through bozo_paged_decode");
   m.def("graph_bias", &graph_bias, "graph bias through bozo_graph_bias_build");
   m.def("add_rmsnorm_fwd", &add_rmsnorm_fwd, "residual add + RMSNorm through bozo_add_rmsnorm_fwd");

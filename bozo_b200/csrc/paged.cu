@@ -30,8 +30,8 @@ __global__ void __launch_bounds__(kThreads) paged_write_any(PagedP p) {
   const unsigned row0 = paged_row(p, b, pos);
   if (row0 == kNoRow) return;
   const size_t row = row0 + (size_t)h * p.page;
-  NewRow(p, p.kn, n, h, pos, p.cos != nullptr, lane).put(p, p.k, p.ks, row, lane);
-  NewRow(p, p.vn, n, h, pos, false, lane).put(p, p.v, p.vs, row, lane);
+  NewRow(p, p.kn, n, h, pos, p.cos != nullptr, lane).put(p, p.k, p.ks, p.kg, row, lane);
+  NewRow(p, p.vn, n, h, pos, false, lane).put(p, p.v, p.vs, p.vg, row, lane);
 }
 
 // One warp per (row, head).
@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(kThreads) paged_read_any(PagedP p) {
   for (int d = lane; d < p.HD; d += 32) {
     float k = 0.f, v = 0.f;
     if (row0 != kNoRow) {
-      k = ld_page(p.k, at + d, p.dt);
-      v = ld_page(p.v, at + d, p.dt);
+      k = ld_page(p.k, p.kg, at + d, p.dt);
+      v = ld_page(p.v, p.vg, at + d, p.dt);
       if (p.ks) {
         k = __fmul_rn(k, p.ks[row]);
         v = __fmul_rn(v, p.vs[row]);
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p
 }
 
 // log2 of the lanes a row takes, or −1 where the vector kernels do not apply
-int vec_lanes(const PagedP& p) { return p.HD == 32 ? 1 : p.HD == 64 ? 2 : p.HD == 128 ? 3 : -1; }
+int vec_lanes(const PagedP& p) { return p.dt == BOZO_DT_F4E2M1 ? -1 : p.HD == 32 ? 1 : p.HD == 64 ? 2 : p.HD == 128 ? 3 : -1; }
 
 bool vec_input(const DevT4& t, int dt) {
   const long long e = dt == BOZO_DT_F32 ? 4 : 2;

@@ -2,6 +2,7 @@
 // (paged.cu, paged_decode.cu) and the device helpers they share.
 #pragma once
 
+#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -16,6 +17,8 @@ struct PagedP {
   void* v;
   float* ks;
   float* vs;
+  unsigned char* kg;  // 4-bit rows: e4m3 scales of 16 elements
+  unsigned char* vg;
   int dt, P, Hk, page, HD, B, M;
   unsigned cap;             // C = M·page
   FastDiv div_cap, div_page;
@@ -42,8 +45,9 @@ struct PagedP {
   int* err;
 };
 
-inline PagedP paged_params(const bozo_paged_cache& c) {
+inline PagedP paged_params(const bozo_paged_cache& c, unsigned char* kg, unsigned char* vg) {
   PagedP p{};
+  if (c.dtype == BOZO_DT_F4E2M1) p.kg = kg, p.vg = vg;
   p.k = c.k_pages; p.v = c.v_pages; p.ks = c.k_scale; p.vs = c.v_scale;
   p.dt = c.dtype; p.P = c.pages; p.Hk = c.kv_heads; p.page = c.page_size; p.HD = c.HD;
   p.B = c.batch; p.M = c.width;
@@ -133,9 +137,67 @@ __device__ __forceinline__ float code_value(unsigned char c, int dt) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
 }
 
-// Element i of a page, without its scale.
-__device__ __forceinline__ float ld_page(const void* p, size_t i, int dt) {
+// 4-bit rows.  The row's scale is a power of two, so the group scale is a correctly
+// rounded sixth and the code a correctly rounded quotient by a few bits: both are a
+// product with the rounded reciprocal and one correction by its exact remainder, as
+// in div_top (checked for every significand by 6 and by 8 … 15, those of an e4m3).
+constexpr float kTinyRow4 = 0x1p-80f;  // below it the remainders would lose bits
+struct Row4 {
+  float scale, inv, most;  // the row's scale, its inverse, the largest group scale
+  bool bad;
+  __device__ __forceinline__ explicit Row4(unsigned abs_bits) {
+    bad = abs_bits >= 0x7f800000u;  // an infinity or a NaN in the row
+    scale = bad ? __uint_as_float(0x7fc00000u) : 0.f;
+    inv = 0.f;
+    most = 448.f;
+    if (!bad && __uint_as_float(abs_bits) >= kTinyRow4) {
+      // 2688 = 1.3125 · 2^11
+      const unsigned e = (abs_bits >> 23) - 11u + ((abs_bits & 0x7fffffu) > 0x280000u ? 1u : 0u);
+      scale = __uint_as_float(e << 23);
+      inv = __uint_as_float((254u - e) << 23);
+      if (e == 127u + 117u) most = 320.f;  // 6 · 352 · 2^117 is past the largest float
+    }
+  }
+  // Scale of 16 elements with the largest magnitude a, as e4m3; unit: what a code of 1 stands for.
+  __device__ __forceinline__ unsigned char group(float a, float& unit, float& recip) const {
+    unsigned char c = 0;
+    unit = recip = 0.f;
+    if (inv != 0.f) {
+      const float q = __fmul_rn(a, 0x1.555556p-3f);
+      const float sixth = __fmaf_rn(__fmaf_rn(-q, 6.f, a), 0x1.555556p-3f, q);
+      c = (unsigned char)__nv_cvt_float_to_fp8(fminf(__fmul_rn(sixth, inv), most), __NV_SATFINITE, __NV_E4M3);
+      if (c) {
+        unit = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3))) * scale;
+        recip = __frcp_rn(unit);
+      }
+    }
+    return c;
+  }
+  // x / unit
+  __device__ __forceinline__ float in_units(float x, float unit, float recip) const {
+    if (bad) return 0.f;
+    const float q = __fmul_rn(x, recip);
+    return __fmaf_rn(__fmaf_rn(q, unit, -x), -recip, q);  // in this order −0 stays −0
+  }
+};
+// Two elements as a byte, the first in the low bits; and back (exact).
+__device__ __forceinline__ unsigned pack4(float x, float y) {
+  return __nv_cvt_float2_to_fp4x2(make_float2(x, y), __NV_E2M1, cudaRoundNearest);
+}
+__device__ __forceinline__ float2 unpack4(unsigned char c) {
+  return __half22float2(__half2(__nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)c, __NV_E2M1)));
+}
+__device__ __forceinline__ float e4m3(unsigned char c) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
+}
+
+// Element i of a page, without its row's scale; `groups` for 4-bit pages.
+__device__ __forceinline__ float ld_page(const void* p, const unsigned char* groups, size_t i, int dt) {
   if (dt <= BOZO_DT_F16) return ldf(p, (long long)i, dt);
+  if (dt == BOZO_DT_F4E2M1) {
+    const float2 x = unpack4(static_cast<const unsigned char*>(p)[i >> 1]);
+    return (i & 1 ? x.y : x.x) * e4m3(groups[i >> 4]);
+  }
   return code_value(static_cast<const unsigned char*>(p)[i], dt);
 }
 
@@ -162,14 +224,36 @@ struct NewRow {
     }
   }
   // … into row `row` of the pages.
-  __device__ __forceinline__ void put(const PagedP& p, void* pages, float* scales, size_t row, int lane) const {
+  __device__ __forceinline__ void put(const PagedP& p, void* pages, float* scales, unsigned char* groups, size_t row,
+                                      int lane) const {
     float inv = 1.f;
+    unsigned a = 0;
     if (p.dt > BOZO_DT_F16) {
-      unsigned a = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
+      a = __reduce_max_sync(0xffffffffu, a);
+    }
+    if (p.dt == BOZO_DT_F4E2M1) {
+      const Row4 r(a);
+      if (lane == 0) scales[row] = r.scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (32 * i >= p.HD) break;  // the same for all lanes
+        const int d = lane + 32 * i;
+        float m = fabsf(x[i]), unit, recip;
+#pragma unroll
+        for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const unsigned char c = r.group(m, unit, recip);
+        const float y = r.in_units(x[i], unit, recip), z = __shfl_down_sync(0xffffffffu, y, 1);
+        if (d >= p.HD) continue;
+        if (lane % 16 == 0) groups[row * (p.HD / 16) + d / 16] = c;
+        if (lane % 2 == 0) static_cast<unsigned char*>(pages)[(row * p.HD + d) / 2] = (unsigned char)pack4(y, z);
+      }
+      return;
+    }
+    if (p.dt > BOZO_DT_F16) {
       float scale;
-      quant_scale(__reduce_max_sync(0xffffffffu, a), p.dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+      quant_scale(a, p.dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
       if (lane == 0) scales[row] = scale;
     }
 #pragma unroll

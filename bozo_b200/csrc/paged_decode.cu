@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
     const size_t row = row0 + (size_t)hk * p.page;
     float dot = 0.f;
     if (row0 != kNoRow)
-      for (int d = lane; d < HD; d += 32) dot = fmaf(sq[d], ld_page(p.k, row * HD + d, p.dt), dot);
+      for (int d = lane; d < HD; d += 32) dot = fmaf(sq[d], ld_page(p.k, p.kg, row * HD + d, p.dt), dot);
     dot = warp_sum(dot);
     if (lane == 0) {
       if (row0 != kNoRow && p.ks) dot *= p.ks[row];
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
       const unsigned row0 = paged_row(p, b, j);
       if (row0 == kNoRow) continue;
       const size_t row = row0 + (size_t)hk * p.page;
-      float x = ld_page(p.v, row * HD + d, p.dt);
+      float x = ld_page(p.v, p.vg, row * HD + d, p.dt);
       acc = fmaf(p.vs ? stau[j - j0] * p.vs[row] : stau[j - j0], x, acc);
     }
     if (r.count == 1)
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) paged_decode_any(PagedP p, int S) {
 
 // Four consecutive elements of a page (at a multiple of 4).
 template <int DT>
-__device__ __forceinline__ void ld4(const void* pages, size_t at, float* x) {
+__device__ __forceinline__ void ld4(const void* pages, const unsigned char* groups, size_t at, float* x) {
   if constexpr (DT == BOZO_DT_F32) {
     const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(pages) + at);
     x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
@@ -89,6 +89,11 @@ __device__ __forceinline__ void ld4(const void* pages, size_t at, float* x) {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
     const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
     x[0] = a.x; x[1] = a.y; x[2] = c.x; x[3] = c.y;
+  } else if constexpr (DT == BOZO_DT_F4E2M1) {
+    const unsigned v = *reinterpret_cast<const unsigned short*>(static_cast<const unsigned char*>(pages) + at / 2);
+    const float2 a = unpack4((unsigned char)v), c = unpack4((unsigned char)(v >> 8));
+    const float g = e4m3(groups[at / 16]);
+    x[0] = a.x * g; x[1] = a.y * g; x[2] = c.x * g; x[3] = c.y * g;
   } else {
     const unsigned v = *reinterpret_cast<const unsigned*>(static_cast<const unsigned char*>(pages) + at);
 #pragma unroll
@@ -156,8 +161,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p,
 #pragma unroll
       for (int i = 0; i < 2; ++i)
         if (live[u] && on[i]) {
-          ld4<DT>(p.k, row * HD + 4 * (l + i * L), k[u] + 4 * i);
-          ld4<DT>(p.v, row * HD + 4 * (l + i * L), v[u] + 4 * i);
+          ld4<DT>(p.k, p.kg, row * HD + 4 * (l + i * L), k[u] + 4 * i);
+          ld4<DT>(p.v, p.vg, row * HD + 4 * (l + i * L), v[u] + 4 * i);
         }
       if (live[u] && DT > BOZO_DT_F16) {
         ks[u] = p.ks[row];
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedP p, int S) {
 }
 
 bool mma_path(const PagedP& p) {
-  return p.dt != BOZO_DT_F32 && (p.HD == 32 || p.HD == 64 || p.HD == 128);
+  return p.dt != BOZO_DT_F32 && p.dt != BOZO_DT_F4E2M1 && (p.HD == 32 || p.HD == 64 || p.HD == 128);
 }
 
 bool rows_path(const PagedP& p) { return p.HD % 4 == 0; }
@@ -359,6 +364,7 @@ cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* 
       case BOZO_DT_BF16: e = launch_rows<BOZO_DT_BF16>(p, pl, st); break;
       case BOZO_DT_F16: e = launch_rows<BOZO_DT_F16>(p, pl, st); break;
       case BOZO_DT_F8E4M3: e = launch_rows<BOZO_DT_F8E4M3>(p, pl, st); break;
+      case BOZO_DT_F4E2M1: e = launch_rows<BOZO_DT_F4E2M1>(p, pl, st); break;
       default: e = launch_rows<BOZO_DT_I8>(p, pl, st);
     }
   } else {

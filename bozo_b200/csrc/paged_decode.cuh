@@ -80,15 +80,15 @@ __device__ __forceinline__ void append_part(const PagedP& p, int b, int hk, int 
   const NewRow x(p, key ? p.kn : p.vn, b, hk, (unsigned)t, key && p.cos, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
   if (row0 != kNoRow)
-    x.put(p, key ? p.k : p.v, key ? p.ks : p.vs, (size_t)row0 + (size_t)hk * p.page, lane);
+    x.put(p, key ? p.k : p.v, key ? p.ks : p.vs, key ? p.kg : p.vg, (size_t)row0 + (size_t)hk * p.page, lane);
 }
 __device__ __forceinline__ void append_row(const PagedP& p, int b, int hk, int t, int lane) {  // by one warp
   const NewRow k(p, p.kn, b, hk, (unsigned)t, p.cos != nullptr, lane), v(p, p.vn, b, hk, (unsigned)t, false, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
   if (row0 == kNoRow) return;
   const size_t row = (size_t)row0 + (size_t)hk * p.page;
-  k.put(p, p.k, p.ks, row, lane);
-  v.put(p, p.v, p.vs, row, lane);
+  k.put(p, p.k, p.ks, p.kg, row, lane);
+  v.put(p, p.v, p.vs, p.vg, row, lane);
 }
 
 // Rotated query element i of head h.

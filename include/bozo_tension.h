@@ -66,7 +66,7 @@ typedef enum {
 typedef enum { BOZO_DT_F32 = 0, BOZO_DT_BF16 = 1, BOZO_DT_F16 = 2 } bozo_dtype;
 /* Types of paged-cache rows beside the bozo_dtype ones: 8-bit codes with one
  * fp32 scale a row (the row stands for code · scale). */
-enum { BOZO_DT_F8E4M3 = 3, BOZO_DT_I8 = 4 };
+enum { BOZO_DT_F8E4M3 = 3, BOZO_DT_I8 = 4, BOZO_DT_F4E2M1 = 6 };
 typedef enum { BOZO_MODE_LOCAL = 0, BOZO_MODE_GLOBAL = 1 } bozo_mode;
 typedef enum { BOZO_NORM_NONE = 0, BOZO_NORM_MASS = 1, BOZO_NORM_COUNT = 2 } bozo_norm;
 
@@ -224,6 +224,17 @@ int bozo_tension_decode(const bozo_tension_decode_args* args, void* stream);
  * 0), a row with an infinity or a NaN as zeros with scale NaN, so that
  * everything read from it is NaN.
  *
+ * 4-bit rows (BOZO_DT_F4E2M1; HD a multiple of 16) are HD/2 bytes, element 2i in the
+ * low and 2i + 1 in the high four bits of byte i, as e2m1 codes (sign; 0, 1/2, 1, 1 1/2,
+ * 2, 3, 4, 6).  Each 16 elements have an e4m3 scale (k_group, v_group of the argument
+ * blocks, [pages, kv_heads, page_size, HD/16]) and each row an fp32 one, a power of
+ * two: an element stands for (code · group) · scale.  scale is the least power of
+ * two with max |x| ≤ 2688 · scale, group = e4m3(max |x| / 6 / scale) over its 16 (at
+ * most 320 where scale is 2^117, so that 6 · group · scale is finite), and
+ * code = e2m1(x / (group · scale)), all correctly rounded, ties to even; the code
+ * keeps x's sign.  A row with max |x| < 2^-80 has scale 0, one with an infinity or a
+ * NaN the scale NaN, both groups and magnitudes of 0.
+ *
  * lengths[b] < 0 marks an inactive sequence: its rows are not written, and its
  * outputs are zeros.  A position outside the RoPE tables or a needed page
  * outside [0, pages) is skipped (rows unwritten, values read as zeros, keys
@@ -233,9 +244,9 @@ int bozo_tension_decode(const bozo_tension_decode_args* args, void* stream);
 typedef struct {
   void* k_pages;          /* [pages, kv_heads, page_size, HD] contiguous, 16-byte aligned */
   void* v_pages;
-  float* k_scale;         /* [pages, kv_heads, page_size] for 8-bit rows, else NULL */
+  float* k_scale;         /* [pages, kv_heads, page_size] for 8- and 4-bit rows, else NULL */
   float* v_scale;
-  int32_t dtype;          /* bozo_dtype, BOZO_DT_F8E4M3 or BOZO_DT_I8 */
+  int32_t dtype;          /* bozo_dtype, BOZO_DT_F8E4M3, BOZO_DT_I8 or BOZO_DT_F4E2M1 */
   int32_t pages, kv_heads, page_size, HD;
   int32_t batch;          /* sequences B */
   int32_t width;          /* pages of a sequence in the table */
@@ -260,6 +271,8 @@ typedef struct {
   const float* rope_cos;  /* [rope_len, HD/2] fp32 contiguous, or NULL */
   const float* rope_sin;
   bozo_tensor4 k, v;      /* [rows, 1, kv_heads, HD] views */
+  uint8_t* k_group;       /* 4-bit rows only (not read otherwise): e4m3 scales of 16 elements, */
+  uint8_t* v_group;       /* [pages, kv_heads, page_size, HD/16], 16-byte aligned */
 } bozo_paged_write_args;
 int bozo_paged_write(const bozo_paged_write_args* args, void* stream);
 
@@ -274,6 +287,8 @@ typedef struct {
   void* v_out;
   int32_t out_dtype;
   int32_t _pad;
+  uint8_t* k_group;       /* as for writing */
+  uint8_t* v_group;
 } bozo_paged_read_args;
 int bozo_paged_read(const bozo_paged_read_args* args, void* stream);
 
@@ -302,11 +317,112 @@ typedef struct {
   int32_t out_dtype, tau_dtype;
   void* workspace;        /* bozo_paged_decode_workspace() bytes, 16-byte aligned */
   size_t workspace_bytes;
+  uint8_t* k_group;       /* as for writing */
+  uint8_t* v_group;
 } bozo_paged_decode_args;
 /* Bytes for the current device, which has to be the pages' (its count of SMs
  * decides how far a row is split); 0 is possible. */
 size_t bozo_paged_decode_workspace(const bozo_paged_decode_args* args);
 int bozo_paged_decode(const bozo_paged_decode_args* args, void* stream);
+
+/* ── page tables on the device ──
+ * refs[p] counts the table rows that hold page p; 0: the page is free. */
+
+/* Pages and places for new tokens.  Sequence b (lengths[b] tokens, none new where it
+ * is negative) gets pages for tokens[b] more: its columns from ceil(lengths[b] /
+ * page_size) on, up to ceil((lengths[b] + tokens[b]) / page_size) and `width`, from the
+ * first one without a page (outside [0, pages)) on.  Free pages are given in
+ * ascending order to the sequences in theirs, and their refs become 1.  Where there
+ * are too few, none is given and *missing says how many more were wanted.
+ * cu_rows[b] is the sum of the tokens before b.  Row n of the packed new tokens,
+ * cu_rows[b] ≤ n < cu_rows[b+1], is token pos[n] = lengths[b] + n − cu_rows[b] of
+ * sequence seq[n] = b, at slot[n] = page · page_size + pos mod page_size of its table's
+ * page, or −1 where there is none or a later token of the same call takes its place;
+ * all three are −1 for rows from cu_rows[batch] on. */
+typedef struct {
+  int32_t* table;         /* [batch, width], rows table_stride apart; updated */
+  int64_t table_stride;
+  int32_t batch, width, page_size, pages;
+  const int32_t* lengths; /* [batch] */
+  const int32_t* tokens;  /* [batch] (negative counts as 0, and so does more than
+                             2^31 / batch, with BOZO_ERR_DEVICE_INDEX), or NULL: one each */
+  int32_t* refs;          /* [pages]; updated */
+  int32_t* cu_rows;       /* [batch + 1] out */
+  int32_t* missing;       /* [1] out */
+  int64_t rows;           /* rows of seq, pos and slot; 0: none wanted */
+  int32_t* seq;
+  int32_t* pos;
+  int32_t* slot;
+} bozo_paged_reserve_args;
+int bozo_paged_reserve(const bozo_paged_reserve_args* args, void* stream);
+
+/* Table rows reordered: row r becomes the row of its parent, parents[r] (lengths are
+ * those of the old rows, and are not changed); −1: an empty row.  A page that no row
+ * holds any more is free.
+ *   share: full pages (columns below lengths / page_size) are held by all children of
+ *     a row; the page that is being filled stays with the first child, each further
+ *     one gets a free page and copies[r] = (page to copy, its own).  A row must not
+ *     hold more than width · page_size tokens (BOZO_ERR_DEVICE_INDEX otherwise: such a
+ *     row's pages are written again).
+ *   else: every page is written again (rings): all of a row's pages stay with its first
+ *     child, each further child gets one for every page in use, with copies[r·width + j].
+ * Columns behind those in use stay with the first child.  Free pages, those given up
+ * by this call among them, are given in ascending order to the rows in theirs.  Where
+ * they are too few the last rows get none (−1) and *missing says how many.  Unused
+ * entries of `copies` are (−1, −1). */
+typedef struct {
+  int32_t* table;         /* [batch, width], rows table_stride apart; updated */
+  int64_t table_stride;
+  int32_t batch, width, page_size, pages;
+  const int32_t* lengths; /* [batch] */
+  const int32_t* parents; /* [batch] */
+  int32_t* refs;          /* [pages]; updated */
+  int32_t share;
+  int32_t _pad;
+  int32_t* copies;        /* [batch or batch·width, 2] out */
+  int32_t* missing;       /* [1] out */
+} bozo_paged_fork_args;
+int bozo_paged_fork(const bozo_paged_fork_args* args, void* stream);
+
+/* Copies whole pages inside each of n_pools pools: copies[i] = (from, to), skipped where
+ * either is outside [0, pages).  No page is both read and written in one call.
+ * `pools` and `page_bytes` are host arrays. */
+typedef struct {
+  void* const* pools;     /* [n_pools] device pointers */
+  const int64_t* page_bytes; /* [n_pools] bytes of a page */
+  int32_t n_pools;
+  int32_t pages;
+  const int32_t* copies;  /* [n_copies, 2] device */
+  int64_t n_copies;
+} bozo_paged_copy_args;
+int bozo_paged_copy(const bozo_paged_copy_args* args, void* stream);
+
+/* ── beam search ──
+ * The `beams` best continuations of each prompt's hypotheses.  Hypothesis k of prompt n
+ * has row n·beams + k of `logits`; continuing it with token v is worth
+ * scores[n][k] + logits[v] − log Σ exp(logits) (compared in 64 bits).  A hypothesis
+ * that has ended (done) goes on as itself only: token eos, its score unchanged.
+ * Higher values come first; of equal ones the lower hypothesis, of one hypothesis the
+ * higher logit, then the lower token.  A row that holds a NaN or +infinity, or nothing
+ * but −infinity, or whose score is not finite, and a masked token (−infinity) are worth
+ * −infinity: they come last, lowest token first. */
+typedef struct {
+  const void* logits;     /* [prompts·beams, vocab], rows row_stride elements apart */
+  int64_t row_stride;
+  int32_t dtype;          /* bozo_dtype */
+  int32_t prompts, beams, vocab; /* beams ≤ 32 and ≤ vocab ≤ 2^20, prompts·beams ≤ 65535 */
+  int32_t eos;            /* −1: hypotheses do not end */
+  int32_t _pad;
+  const float* scores;    /* [prompts, beams] */
+  const uint8_t* done;    /* [prompts, beams] or NULL */
+  float* out_scores;      /* [prompts, beams], best first */
+  int64_t* out_tokens;    /* [prompts, beams] */
+  int32_t* out_rows;      /* [prompts, beams]: the row of logits that was continued */
+  void* workspace;        /* bozo_beam_select_workspace() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+} bozo_beam_select_args;
+size_t bozo_beam_select_workspace(const bozo_beam_select_args* args);
+int bozo_beam_select(const bozo_beam_select_args* args, void* stream);
 
 /* 1 when this forward, given q_lp / k_lp, runs on the tensor-core kernels
  * from bf16 copies of fp32 q and k: the reference's mixed-dtype call
