@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedP p, int S) {
 }
 
 bool mma_path(const PagedP& p) {
-  return p.dt != BOZO_DT_F32 && p.dt != BOZO_DT_F4E2M1 && (p.HD == 32 || p.HD == 64 || p.HD == 128);
+  return p.dt != BOZO_DT_F32 && (p.HD == 32 || p.HD == 64 || p.HD == 128);
 }
 
 bool rows_path(const PagedP& p) { return p.HD % 4 == 0; }
@@ -356,6 +356,7 @@ cudaError_t launch_paged_decode(const PagedP& p, int sms, cudaStream_t st, int* 
       case BOZO_DT_BF16: e = launch_paged_mma_bf16(p, pl, st); break;
       case BOZO_DT_F16: e = launch_paged_mma_f16(p, pl, st); break;
       case BOZO_DT_F8E4M3: e = launch_paged_mma_f8(p, pl, st); break;
+      case BOZO_DT_F4E2M1: e = launch_paged_mma_f4(p, pl, st); break;
       default: e = launch_paged_mma_i8(p, pl, st);
     }
   } else if (rows_path(p)) {

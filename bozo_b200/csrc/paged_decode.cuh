@@ -25,6 +25,7 @@ cudaError_t launch_paged_mma_bf16(const PagedP& p, const PagedPlan& pl, cudaStre
 cudaError_t launch_paged_mma_f16(const PagedP& p, const PagedPlan& pl, cudaStream_t st);
 cudaError_t launch_paged_mma_f8(const PagedP& p, const PagedPlan& pl, cudaStream_t st);
 cudaError_t launch_paged_mma_i8(const PagedP& p, const PagedPlan& pl, cudaStream_t st);
+cudaError_t launch_paged_mma_f4(const PagedP& p, const PagedPlan& pl, cudaStream_t st);
 
 // Keys that a sequence's query reaches: the n positions [lo, end); none where it
 // is inactive.  They are cut into `count` pieces of `size` positions counted from

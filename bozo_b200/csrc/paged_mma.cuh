@@ -44,11 +44,13 @@
 namespace bozo {
 namespace {
 
+// size: bytes of an element, 0: half a byte
 template <int DT> struct Fmt;
 template <> struct Fmt<BOZO_DT_BF16> { static constexpr int size = 2; static constexpr bool bf = true, scaled = false; };
 template <> struct Fmt<BOZO_DT_F16> { static constexpr int size = 2; static constexpr bool bf = false, scaled = false; };
 template <> struct Fmt<BOZO_DT_F8E4M3> { static constexpr int size = 1; static constexpr bool bf = false, scaled = true; };
 template <> struct Fmt<BOZO_DT_I8> { static constexpr int size = 1; static constexpr bool bf = false, scaled = true; };
+template <> struct Fmt<BOZO_DT_F4E2M1> { static constexpr int size = 0; static constexpr bool bf = false, scaled = true; };
 
 template <bool BF>
 __device__ __forceinline__ void mma16816(float* d, unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
@@ -94,6 +96,31 @@ __device__ __forceinline__ void widen4(unsigned x, unsigned& p01, unsigned& p23)
     p01 = *reinterpret_cast<const unsigned*>(&ha);
     p23 = *reinterpret_cast<const unsigned*>(&hb);
   }
+}
+
+// Eight 4-bit codes as pairs of halfs, times the scales s (two halfs): exact, since the
+// product has 6 significant bits and lies between 2^-10 and 2688.
+__device__ __forceinline__ void widen8(unsigned x, unsigned s, unsigned* w) {
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b;"
+      " cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(x));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), *reinterpret_cast<const __half2*>(&s));
+    w[i] = *reinterpret_cast<const unsigned*>(&y);
+  }
+}
+// The two e4m3 in the low half of x as halfs.
+__device__ __forceinline__ unsigned group_pair(unsigned x) {
+  unsigned w;
+  asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(w) : "r"(x));
+  return w;
+}
+template <int N> __device__ __forceinline__ unsigned lds_part(unsigned a) {  // 1 or 2 bytes
+  unsigned short x;
+  if constexpr (N == 1) asm volatile("ld.shared.u8 %0, [%1];" : "=h"(x) : "r"(a) : "memory");
+  else asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(a) : "memory");
+  return x;
 }
 
 // σ(z) from −z·log2 e: one exponential and one reciprocal, each with a relative
@@ -146,6 +173,9 @@ __device__ __forceinline__ void copy16(unsigned dst, const void* src, int bytes)
 __device__ __forceinline__ void copy4(unsigned dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy8(unsigned dst, const void* src, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -167,11 +197,14 @@ constexpr int kStages = 3;
 
 // Geometry of the kernel for one page type, head width and count of heads.
 template <int DT, int HD, int GP> struct Geo {
-  static constexpr int row = HD * Fmt<DT>::size;             // bytes of a row
-  static constexpr int keys = row >= 128 ? 16 : 2048 / row;  // keys of a tile of the ring
-  static constexpr int kv = keys * row;                      // bytes of its K (or V): 2 KB, 4 KB at 256-byte rows
+  static constexpr bool four = Fmt<DT>::size == 0;
+  static constexpr int row = four ? HD / 2 : HD * Fmt<DT>::size;  // bytes of a row
+  static constexpr int keys = row >= 128 ? 16 : row >= 32 ? 2048 / row : 64;  // keys of a tile of the ring
+  static constexpr int kv = keys * row;                      // bytes of its K (or V): 1 or 2 KB, 4 KB at 256-byte rows
   static constexpr int scales = Fmt<DT>::scaled ? 2 * keys * 4 : 0;
-  static constexpr int meta = scales + 16;                   // scales, and 16 bits a 16 keys: which are in reach
+  static constexpr int gr = four ? HD / 16 : 0;              // bytes of a row's group scales
+  static constexpr int live = scales + 2 * keys * gr;        // offset of the 16 bits a 16 keys: which are in reach
+  static constexpr int meta = live + 16;                     // scales, K's and V's group scales, those bits
   static constexpr int pstride = keys + 8;                   // words of a head's τ
   // Blocks an SM whose registers have to fit: two leave the compiler what it wants
   // (e4m3 128 wide, 616 MB: 113 µs, with three 118; e4m3 32 wide 146 against 153),
@@ -196,6 +229,7 @@ template <int SIZE, int R, bool V> __device__ __forceinline__ int ring_at(int r,
   } else if constexpr (R >= 128) {
     return r * R + ((ch ^ (V ? ((r >> 1) & 3) << 1 : (r & 1) << 2)) << 4);
   } else if constexpr (V) {
+    if constexpr (R < 32) return r * R + (ch << 4);
     constexpr int per = 128 / R;  // rows of a line
     const int line = r / per, c8 = (r % per) * (R / 16) + ch;
     return line * 128 + ((c8 ^ (R == 64 ? (line & 3) << 1 : (line & 1) << 1)) << 4);
@@ -217,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   using F = Fmt<DT>;
   using Z = Geo<DT, HD, GP>;
   constexpr bool BF = F::bf;
-  constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size;
+  constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size, RS = Z::four ? 1 : SZ, GB = Z::gr;
   constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns of S a head, one
   constexpr int GQ = GP < 4 ? GP : 4;                              // heads whose columns repeat
   constexpr int NS = GP == 8 ? 2 : 1;                              // heads of a lane
@@ -231,7 +265,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   constexpr bool FOLD = Z::fold;
   // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
   constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
-  constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB / 4;
+  constexpr int kVB = R / 8 < 16 ? R / 8 : 16, kVL = R / (8 * kVB), kVW = kVB < 4 ? 1 : kVB / 4;
   extern __shared__ __align__(256) char smb[];
   __shared__ float sq[BF ? 1 : kHeads][HD + 4];
   __shared__ __align__(4) unsigned short scut[BF ? GP : 1][3][HD + 8];  // the three bf16 of each q element
@@ -282,6 +316,19 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       }
     }
   };
+  // The group scales of key u·16 + lane mod 16 (K's by the first 16 lanes, V's by the others)
+  // from row rr; zeros without one, as its codes: a product with what a page holds there
+  // could be NaN.
+  auto put_groups = [&](char* md, int u, unsigned rr) {
+    const unsigned to = smem_u32(md) + Z::scales + (lane >> 4) * KT * GB + (u * 16 + (lane & 15)) * GB;
+    const unsigned char* from = (lane < 16 ? p.kg : p.vg) + (rr == kNoRow ? 0 : (size_t)rr * GB);
+    if constexpr (GB == 8) copy8(to, from, rr == kNoRow ? 0 : 8);
+    else if constexpr (GB == 4) copy4(to, from, rr == kNoRow ? 0 : 4);
+    else if constexpr (GB == 2) {  // too short for an asynchronous copy; only at the ends of the reach and of odd pages
+      const unsigned short x = rr == kNoRow ? 0 : *reinterpret_cast<const unsigned short*>(from);
+      asm volatile("st.shared.u16 [%0], %1;" ::"r"(to), "h"(x) : "memory");
+    }
+  };
   auto fill = [&](int slot, int k) {
     const unsigned kd = ring + slot * 2 * Z::kv, vd = kd + Z::kv;
     char* md = meta + slot * Z::meta;
@@ -304,30 +351,49 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
         // a round's place in the ring: the permutation repeats every 8 rows
         constexpr int kSame = 8 * NCH / 32 < 1 ? 1 : 8 * NCH / 32;  // rounds of 8 rows
         const char *ka = kpages + at, *va = vpages + at, *kb = kpages + at1, *vb = vpages + at1;
-        each<(NCH + 1) / 2>([&](auto i) {
+        if constexpr (NCH == 1) {  // a piece a row: 16 lanes for K, 16 for V
+          const int r = lane & 15;
+          copy16((lane < 16 ? kd : vd) + u * 16 * R + r * R, (lane < 16 ? kpages : vpages) + (size_t)whole(r) * R, 16);
+        } else each<(NCH + 1) / 2>([&](auto i) {
           constexpr int it = i, first = it % kSame, back = (it - first) * 512;
           const int r = (first * 32 + lane) / NCH, ch = lane % NCH;
           const bool second = GR == 8 && (it * 32 + lane) / NCH >= 8;
-          copy16<back, it * 512>(kd + u * 16 * R + ring_at<SZ, R, false>(r, ch), second ? kb - 8 * R : ka);
-          copy16<back, it * 512>(vd + u * 16 * R + ring_at<SZ, R, true>(r, ch), second ? vb - 8 * R : va);
+          copy16<back, it * 512>(kd + u * 16 * R + ring_at<RS, R, false>(r, ch), second ? kb - 8 * R : ka);
+          copy16<back, it * 512>(vd + u * 16 * R + ring_at<RS, R, true>(r, ch), second ? vb - 8 * R : va);
         });
         if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
                              (lane < 16 ? p.ks : p.vs) + whole(lane & 15), 4);
-        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = 0xffffu;
+        if constexpr (GB == 2) {  // two rows' at a time, which begin at an even one
+          const int r = 2 * (lane & 7);
+          if (lane < 16)
+            copy4(smem_u32(md) + Z::scales + (lane >> 3) * KT * GB + (u * 16 + r) * GB,
+                  (lane < 8 ? p.kg : p.vg) + (size_t)whole(r) * GB, 4);
+        } else if constexpr (GB > 0) {
+          put_groups(md, u, whole(lane & 15));
+        }
+        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::live)[u] = 0xffffu;
       } else {
-#pragma unroll
-        for (int it = 0; it < (NCH + 1) / 2; ++it) {
-          const int r = (it * 32 + lane) / NCH, ch = lane % NCH;
+        if constexpr (NCH == 1) {
+          const int r = lane & 15;
           const unsigned rr = row_of(r);
-          const size_t at = rr == kNoRow ? 0 : (size_t)rr * R + ch * 16;
-          copy16(kd + ring_at<SZ, R, false>(u * 16 + r, ch), kpages + at, rr == kNoRow ? 0 : 16);
-          copy16(vd + ring_at<SZ, R, true>(u * 16 + r, ch), vpages + at, rr == kNoRow ? 0 : 16);
+          copy16((lane < 16 ? kd : vd) + (u * 16 + r) * R,
+                 (lane < 16 ? kpages : vpages) + (rr == kNoRow ? 0 : (size_t)rr * R), rr == kNoRow ? 0 : 16);
+        } else {
+#pragma unroll
+          for (int it = 0; it < (NCH + 1) / 2; ++it) {
+            const int r = (it * 32 + lane) / NCH, ch = lane % NCH;
+            const unsigned rr = row_of(r);
+            const size_t at = rr == kNoRow ? 0 : (size_t)rr * R + ch * 16;
+            copy16(kd + ring_at<RS, R, false>(u * 16 + r, ch), kpages + at, rr == kNoRow ? 0 : 16);
+            copy16(vd + ring_at<RS, R, true>(u * 16 + r, ch), vpages + at, rr == kNoRow ? 0 : 16);
+          }
         }
         const unsigned rr = row_of(lane & 15);
         if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
                              (lane < 16 ? p.ks : p.vs) + (rr == kNoRow ? 0u : rr), rr == kNoRow ? 0 : 4);
+        if constexpr (GB > 0) put_groups(md, u, rr);
         const unsigned m = __ballot_sync(0xffffffffu, rr != kNoRow);
-        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::scales)[u] = (unsigned short)m;
+        if (lane == 0) reinterpret_cast<unsigned short*>(md + Z::live)[u] = (unsigned short)m;
       }
     }
   };
@@ -427,7 +493,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               qb[s][i][0] = pair(16 * i + 2 * c);
               qb[s][i][1] = pair(16 * i + 8 + 2 * c);
             } else {
-              const int d = i / kKW * 4 * kKB + c * kKB + i % kKW * 4;
+              const int d = SZ == 0 ? c * 2 * kKB + 4 * i : i / kKW * 4 * kKB + c * kKB + i % kKW * 4;
               qb[s][i][0] = pair(d);
               qb[s][i][1] = pair(d + 2);
             }
@@ -461,7 +527,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             for (int i = 0; i < NC; ++i) s[u][e][i][0] = s[u][e][i][1] = s[u][e][i][2] = s[u][e][i][3] = 0.f;
           const int r0 = (q * T + u) * 16;
           if constexpr (SZ == 2) {
-            const unsigned a = kt + ring_at<SZ, R, false>(r0 + mrow, mch);
+            const unsigned a = kt + ring_at<RS, R, false>(r0 + mrow, mch);
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
               unsigned w[4];
@@ -471,11 +537,33 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
                 mma16816<BF>(s[u][BF ? 0 : e][(BF ? st * NB + e : st) % NC], w[0], w[1], w[2], w[3], qb[e][st][0],
                              qb[e][st][1]);
             }
+          } else if constexpr (SZ == 0) {
+            // lane (g, c): a quarter of rows g and g + 8, 8, 16 or 32 elements from c·HD/4 on
+            const unsigned at = kt + (r0 + g) * R + c * kKB;
+            const unsigned gs = smem_u32(md) + Z::scales + (r0 + g) * GB + c * GB / 4;
+            unsigned ka[kKW], kb[kKW];
+            lds_words<kKW, 0>(at, ka);
+            lds_words<kKW, 8 * R>(at, kb);
+            constexpr int NG = GB == 8 ? 2 : 1;  // groups of a lane's elements
+            const unsigned ga = lds_part<NG>(gs), gb = lds_part<NG>(gs + 8 * GB);
+#pragma unroll
+            for (int w = 0; w < kKW; ++w) {
+              const unsigned sel = NG == 2 && w >= kKW / 2 ? 0x1111 : 0x0000;
+              unsigned x[4], y[4];
+              widen8(ka[w], group_pair(__byte_perm(ga, 0, sel)), x);
+              widen8(kb[w], group_pair(__byte_perm(gb, 0, sel)), y);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < NS; ++e)
+                  mma16816<BF>(s[u][e][(2 * w + h) % NC], x[2 * h], y[2 * h], x[2 * h + 1], y[2 * h + 1],
+                               qb[e][2 * w + h][0], qb[e][2 * w + h][1]);
+            }
           } else {
             // 8 rows on the permutation is the same, and where a row is longer than a
             // line two 16-byte pieces on it is that with another bit turned over
             const int byte0 = c * kKB;
-            const unsigned a0_ = kt + r0 * R + ring_at<SZ, R, false>(g, byte0 >> 4) + (byte0 & 15);
+            const unsigned a0_ = kt + r0 * R + ring_at<RS, R, false>(g, byte0 >> 4) + (byte0 & 15);
 #pragma unroll
             for (int l = 0; l < kKL; ++l) {
               unsigned ka[kKW], kb[kKW];
@@ -496,7 +584,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           }
         }
         const int tile = q * T + tsel;
-        const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::scales)[tile];
+        const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::live)[tile];
         float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
         if constexpr (F::scaled) {
           const float2 a = sc[tile * 16 + g], c2 = sc[tile * 16 + g + 8];  // a key's and a value's
@@ -609,7 +697,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           }
         }
         if constexpr (SZ == 2) {
-          const unsigned a = vt + ring_at<SZ, R, true>(u * 16 + mrow, mch);
+          const unsigned a = vt + ring_at<RS, R, true>(u * 16 + mrow, mch);
           if constexpr (WIDE) {  // Oᵀ = Vᵀ·Pᵀ: a product for each of the eight heads' parts
             constexpr int N = kAcc < 4 ? kAcc : 4;  // side by side
 #pragma unroll
@@ -633,14 +721,47 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
             }
           }
+        } else if constexpr (SZ == 0) {
+          // lane (g, c): an eighth of rows 2c, 2c + 1, 2c + 8, 2c + 9: HD/8 elements from g·HD/8 on
+          const int byte = g * kVB;
+          const unsigned v0 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c, byte >> 4) + (byte & 15);
+          const unsigned v1 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c + 1, byte >> 4) + (byte & 15);
+          unsigned vw[4][kVB < 4 ? 1 : kVB / 4];
+          if constexpr (kVB < 4) {
+            vw[0][0] = lds_part<2>(v0);
+            vw[1][0] = lds_part<2>(v1);
+            vw[2][0] = lds_part<2>(v0 + 8 * R);
+            vw[3][0] = lds_part<2>(v1 + 8 * R);
+          } else {
+            lds_words<kVW, 0>(v0, vw[0]);
+            lds_words<kVW, 0>(v1, vw[1]);
+            lds_words<kVW, 8 * R>(v0, vw[2]);
+            lds_words<kVW, 8 * R>(v1, vw[3]);
+          }
+          // the two rows' scales of that group, side by side
+          const unsigned gs = smem_u32(md) + Z::scales + KT * GB + (u * 16 + 2 * c) * GB + g * GB / 8;
+          const unsigned s01 = group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8);
+          const unsigned s89 = group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8);
+#pragma unroll
+          for (int w = 0; w < (kVB < 4 ? 1 : kVB / 4); ++w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // even, odd elements: two keys' codes in a byte
+              const unsigned a = vw[0][w], b2 = vw[1][w], d = vw[2][w], f = vw[3][w];
+              unsigned x[4], y[4];
+              widen8(i ? (a >> 4 & 0x0f0f0f0fu) | (b2 & 0xf0f0f0f0u) : (a & 0x0f0f0f0fu) | (b2 << 4 & 0xf0f0f0f0u), s01, x);
+              widen8(i ? (d >> 4 & 0x0f0f0f0fu) | (f & 0xf0f0f0f0u) : (d & 0x0f0f0f0fu) | (f << 4 & 0xf0f0f0f0u), s89, y);
+#pragma unroll
+              for (int h = 0; h < (kVB < 4 ? kVB : 4); ++h)
+                mma16816<BF>(acc[8 * w + 2 * h + i], a0, a1, a2, a3, x[h], y[h]);
+            }
         } else {
 #pragma unroll
           for (int l = 0; l < kVL; ++l) {
             unsigned vw[4][kVW];
             const int byte = l * 8 * kVB + g * kVB;
             // rows 2c and 2c + 1 of each eight
-            const unsigned v0 = vt + u * 16 * R + ring_at<SZ, R, true>(2 * c, byte >> 4) + (byte & 15);
-            const unsigned v1 = vt + u * 16 * R + ring_at<SZ, R, true>(2 * c + 1, byte >> 4) + (byte & 15);
+            const unsigned v0 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c, byte >> 4) + (byte & 15);
+            const unsigned v1 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c + 1, byte >> 4) + (byte & 15);
             lds_words<kVW, 0>(v0, vw[0]);
             lds_words<kVW, 0>(v1, vw[1]);
             lds_words<kVW, 8 * R>(v0, vw[2]);
@@ -709,7 +830,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     for (int j = 0; j < kTiles; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int d = SZ == 2 ? 8 * j + 2 * c + e : j / kVB * 8 * kVB + (2 * c + e) * kVB + j % kVB;
+        const int d = SZ == 2 ? 8 * j + 2 * c + e : SZ == 0 ? (2 * c + e) * (HD / 8) + j : j / kVB * 8 * kVB + (2 * c + e) * kVB + j % kVB;
         part[((FOLD ? 2 * warp + (g >> 2) : warp) * Gh + hrow) * HD + d] = (acc[j][e] + acc[j][2 + e]) * back;
       }
   }
