@@ -72,6 +72,7 @@ template <> struct PageT<BOZO_DT_BF16> { using type = __nv_bfloat16; };
 template <> struct PageT<BOZO_DT_F16> { using type = __half; };
 template <> struct PageT<BOZO_DT_F8E4M3> { using type = unsigned char; };
 template <> struct PageT<BOZO_DT_I8> { using type = unsigned char; };
+template <> struct PageT<BOZO_DT_F4E2M1> { using type = unsigned char; };  // two elements
 
 // Eight elements of type T: 8, 16 or 32 bytes, moved in pieces of up to 16.
 template <typename T> struct Eight {
@@ -205,6 +206,32 @@ __device__ __forceinline__ float max_abs(float a, float b) {  // ± max(|a|, |b|
   return r;
 }
 
+// Eight elements in units of their group, as 4-bit codes.
+__device__ __forceinline__ unsigned narrow4(const Row4& r, const float* x, float unit, float recip) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = r.in_units(x[i], unit, recip);
+  unsigned w;
+  asm("{.reg .b8 a, b, c, d; cvt.rn.satfinite.e2m1x2.f32 a, %2, %1; cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5; cvt.rn.satfinite.e2m1x2.f32 d, %8, %7; mov.b32 %0, {a, b, c, d};}"
+      : "=r"(w)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  return w;
+}
+// Eight codes times their group's scale.
+__device__ __forceinline__ void widen4(unsigned x, float group, float* y) {
+  unsigned w[4];
+  asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b;"
+      " cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(x));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    y[2 * i] = f.x * group;
+    y[2 * i + 1] = f.y * group;
+  }
+}
+
 // The places of a block's rows n0 … n0 + rows − 1: row numbers (head 0) and
 // positions in shared memory.
 template <bool WRITE>
@@ -276,6 +303,33 @@ __device__ __forceinline__ void write_head(const PagedP& p, const Eight<I>& xl, 
       add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
     }
   }
+  if constexpr (DT == BOZO_DT_F4E2M1) {
+    // sixteen consecutive elements: eight of this lane's and eight of its neighbour's, in either half
+    float lo = x[0], hi = x[8];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) {
+      lo = max_abs(lo, x[i]);
+      hi = max_abs(hi, x[8 + i]);
+    }
+    lo = max_abs(lo, __shfl_xor_sync(group, lo, 1));
+    hi = max_abs(hi, __shfl_xor_sync(group, hi, 1));
+    float a = max_abs(lo, hi);
+    for (int o = L / 2; o > 1; o >>= 1) a = max_abs(a, __shfl_xor_sync(group, a, o));
+    const Row4 r(__float_as_uint(a) & 0x7fffffffu);
+    unsigned* to = reinterpret_cast<unsigned*>(static_cast<unsigned char*>(KEY ? p.k : p.v) + (size_t)row * half) + l;
+    unsigned char* gto = (KEY ? p.kg : p.vg) + (size_t)row * L;
+    float unit, recip;
+    const unsigned char cl = r.group(fabsf(lo), unit, recip);
+    to[0] = narrow4(r, x, unit, recip);
+    const unsigned char ch = r.group(fabsf(hi), unit, recip);
+    to[L] = narrow4(r, x + 8, unit, recip);
+    if ((l & 1) == 0) {
+      gto[l / 2] = cl;
+      gto[(L + l) / 2] = ch;
+    }
+    if (l == 0) (KEY ? p.ks : p.vs)[row] = r.scale;
+    return;
+  }
   Eight<T> yl, yh;
   if constexpr (Q) {
     float a = x[0];
@@ -340,6 +394,39 @@ __global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p
   O* to[2] = {static_cast<O*>(p.k_out) + ((size_t)n * p.Hk + sub) * HD + 8 * l,
               static_cast<O*>(p.v_out) + ((size_t)n * p.Hk + sub) * HD + 8 * l};
   unsigned row = row0 + (unsigned)sub * (unsigned)p.page;
+  if constexpr (DT == BOZO_DT_F4E2M1) {
+    // sixteen consecutive elements a lane: one group
+    to[0] += 8 * l;
+    to[1] += 8 * l;
+#pragma unroll 1
+    for (int h = sub; h < p.Hk; h += per, row += (unsigned)(per * p.page)) {
+      uint2 codes[2] = {};
+      float scale[2] = {}, grp[2] = {};
+      if (row0 != kNoRow) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          codes[j] = __ldg(reinterpret_cast<const uint2*>(static_cast<const unsigned char*>(j ? p.v : p.k) + (size_t)row * half) + l);
+          grp[j] = e4m3(__ldg((j ? p.vg : p.kg) + (size_t)row * L + l));
+          scale[j] = __ldg((j ? p.vs : p.ks) + row);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x[16];
+        widen4(codes[j].x, grp[j], x);
+        widen4(codes[j].y, grp[j], x + 8);
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) mul2(x[i], x[i + 1], x[i], x[i + 1], scale[j], scale[j]);
+        Eight<O> yl, yh;
+        narrow(yl, x);
+        narrow(yh, x + 8);
+        st8(to[j], yl);
+        st8(to[j] + 8, yh);
+        to[j] += per * HD;
+      }
+    }
+    return;
+  }
 #pragma unroll 1
   for (int h = sub; h < p.Hk; h += per, row += (unsigned)(per * p.page)) {
     Eight<T> lo[2], hi[2];
@@ -381,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, kReadBlocks) paged_read_vec(PagedP p
 }
 
 // log2 of the lanes a row takes, or −1 where the vector kernels do not apply
-int vec_lanes(const PagedP& p) { return p.dt == BOZO_DT_F4E2M1 ? -1 : p.HD == 32 ? 1 : p.HD == 64 ? 2 : p.HD == 128 ? 3 : -1; }
+int vec_lanes(const PagedP& p) { return p.HD == 32 ? 1 : p.HD == 64 ? 2 : p.HD == 128 ? 3 : -1; }
 
 bool vec_input(const DevT4& t, int dt) {
   const long long e = dt == BOZO_DT_F32 ? 4 : 2;
@@ -434,6 +521,7 @@ cudaError_t launch_paged_write(const PagedP& p, int sms, cudaStream_t st) {
       case BOZO_DT_BF16: return write_vec<BOZO_DT_BF16>(p, lanes, sms, st);
       case BOZO_DT_F16: return write_vec<BOZO_DT_F16>(p, lanes, sms, st);
       case BOZO_DT_F8E4M3: return write_vec<BOZO_DT_F8E4M3>(p, lanes, sms, st);
+      case BOZO_DT_F4E2M1: return write_vec<BOZO_DT_F4E2M1>(p, lanes, sms, st);
       default: return write_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
@@ -451,6 +539,7 @@ cudaError_t launch_paged_read(const PagedP& p, int sms, cudaStream_t st) {
       case BOZO_DT_BF16: return read_vec<BOZO_DT_BF16>(p, lanes, sms, st);
       case BOZO_DT_F16: return read_vec<BOZO_DT_F16>(p, lanes, sms, st);
       case BOZO_DT_F8E4M3: return read_vec<BOZO_DT_F8E4M3>(p, lanes, sms, st);
+      case BOZO_DT_F4E2M1: return read_vec<BOZO_DT_F4E2M1>(p, lanes, sms, st);
       default: return read_vec<BOZO_DT_I8>(p, lanes, sms, st);
     }
   }
