@@ -42,7 +42,7 @@ EXPORTED = (
     "bozo_embedding_bwd",
     "bozo_paged_write", "bozo_paged_read", "bozo_paged_decode", "bozo_paged_decode_workspace",
     "bozo_paged_reserve", "bozo_paged_fork", "bozo_paged_copy",
-    "bozo_beam_select", "bozo_beam_select_workspace",
+    "bozo_beam_select",
 )
 TAU_AUX_MAX_LAYERS = 64  # BOZO_TAU_AUX_MAX_LAYERS
 
@@ -170,7 +170,6 @@ class BeamSelectArgs(C.Structure):
         ("prompts", C.c_int32), ("beams", C.c_int32), ("vocab", C.c_int32), ("eos", C.c_int32),
         ("_pad", C.c_int32), ("scores", C.c_void_p), ("done", C.c_void_p),
         ("out_scores", C.c_void_p), ("out_tokens", C.c_void_p), ("out_rows", C.c_void_p),
-        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -303,8 +302,6 @@ def lib():
                 L.bozo_paged_copy.restype = C.c_int
                 L.bozo_beam_select.argtypes = [C.POINTER(BeamSelectArgs), C.c_void_p]
                 L.bozo_beam_select.restype = C.c_int
-                L.bozo_beam_select_workspace.argtypes = [C.POINTER(BeamSelectArgs)]
-                L.bozo_beam_select_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_workspace.argtypes = [C.POINTER(TauAuxFwdArgs)]
                 L.bozo_tau_aux_workspace.restype = C.c_size_t
                 L.bozo_tau_aux_fwd.argtypes = [C.POINTER(TauAuxFwdArgs), C.c_void_p]

@@ -727,7 +727,7 @@ int bozo_paged_copy(const bozo_paged_copy_args* a, void* stream) {
   return BOZO_OK;
 }
 
-static int beam_params(const bozo_beam_select_args* a, BeamP& p) {
+int bozo_beam_select(const bozo_beam_select_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
   if (a->prompts <= 0 || a->beams <= 0 || a->vocab < a->beams || a->row_stride < 0 || a->eos < -1 ||
       a->eos >= a->vocab || (a->done && a->eos < 0))
@@ -736,33 +736,18 @@ static int beam_params(const bozo_beam_select_args* a, BeamP& p) {
   if (a->beams > kMaxBeams || a->vocab > kMaxVocab || (long long)a->prompts * a->beams > 65535)
     return BOZO_ERR_UNSUPPORTED;
   if (!a->logits || !a->scores || !a->out_scores || !a->out_tokens || !a->out_rows) return BOZO_ERR_NULL;
-  p = BeamP{};
+  DeviceRestore restore;
+  cudaError_t e = bind_device(a->logits, restore);
+  if (e != cudaSuccess) return cuda_fail(e);
+  BeamP p{};
   p.logits = a->logits; p.stride = a->row_stride; p.dt = a->dtype;
   p.N = a->prompts; p.K = a->beams; p.V = a->vocab; p.eos = a->eos;
   p.scores = a->scores; p.done = a->done;
   p.out_scores = a->out_scores; p.out_tokens = reinterpret_cast<long long*>(a->out_tokens); p.out_rows = a->out_rows;
-  return BOZO_OK;
-}
-
-size_t bozo_beam_select_workspace(const bozo_beam_select_args* a) {
-  BeamP p;
-  return beam_params(a, p) == BOZO_OK ? beam_bytes(p) : 0;
-}
-
-int bozo_beam_select(const bozo_beam_select_args* a, void* stream) {
-  BeamP p;
-  const int st = beam_params(a, p);
-  if (st) return st;
-  const size_t need = beam_bytes(p);
-  if (need && (!a->workspace || a->workspace_bytes < need)) return BOZO_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return BOZO_ERR_ALIGNMENT;
-  DeviceRestore restore;
-  cudaError_t e = bind_device(a->logits, restore);
-  if (e != cudaSuccess) return cuda_fail(e);
-  e = launch_beam(p, a->workspace, static_cast<cudaStream_t>(stream));
+  e = launch_beam(p, num_sms(), static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = BOZO_PATH_SIMT;
-  t_last_launches = 2;
+  t_last_launches = 1;
   return BOZO_OK;
 }
 

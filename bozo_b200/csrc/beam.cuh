@@ -17,10 +17,7 @@ struct BeamP {
   float* out_scores;
   long long* out_tokens;
   int* out_rows;
-  unsigned long long* keys;  // each chunk's best, sorted [N·K][chunks][K]
-  float2* sums;              // its largest logit and Σ exp(logit − largest)
 };
-size_t beam_bytes(const BeamP& p);
-cudaError_t launch_beam(BeamP p, void* ws, cudaStream_t st);
+cudaError_t launch_beam(const BeamP& p, int sms, cudaStream_t st);
 
 }  // namespace bozo

@@ -637,16 +637,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& log
   a.eos = (int32_t)eos;
   a.scores = scores.data_ptr<float>();
   a.done = d ? static_cast<const uint8_t*>(d->data_ptr()) : nullptr;
-  at::Tensor s = empty({N, K}, at::kFloat, dev), t = empty({N, K}, at::kLong, dev), r = empty({N, K}, at::kInt, dev), ws;
+  at::Tensor s = empty({N, K}, at::kFloat, dev), t = empty({N, K}, at::kLong, dev), r = empty({N, K}, at::kInt, dev);
   a.out_scores = s.data_ptr<float>();
   a.out_tokens = t.data_ptr<int64_t>();
   a.out_rows = r.data_ptr<int32_t>();
-  const int64_t need = (int64_t)bozo_beam_select_workspace(&a);
-  if (need) {
-    ws = empty(need, at::kByte, dev);
-    a.workspace = ws.data_ptr();
-    a.workspace_bytes = (size_t)need;
-  }
   check(bozo_beam_select(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_beam_select");
   return {std::move(s), std::move(t), std::move(r)};
 }

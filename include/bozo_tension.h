@@ -418,10 +418,7 @@ typedef struct {
   float* out_scores;      /* [prompts, beams], best first */
   int64_t* out_tokens;    /* [prompts, beams] */
   int32_t* out_rows;      /* [prompts, beams]: the row of logits that was continued */
-  void* workspace;        /* bozo_beam_select_workspace() bytes, 16-byte aligned */
-  size_t workspace_bytes;
 } bozo_beam_select_args;
-size_t bozo_beam_select_workspace(const bozo_beam_select_args* args);
 int bozo_beam_select(const bozo_beam_select_args* args, void* stream);
 
 /* 1 when this forward, given q_lp / k_lp, runs on the tensor-core kernels
