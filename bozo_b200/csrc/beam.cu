@@ -3,10 +3,12 @@
 // A continuation is worth score + logit − log Σ exp(logits); within one row the logits
 // alone order them.  One cluster a prompt, each block a row, a part of one, or (more
 // than kCluster hypotheses) a few rows, and one pass over the logits:
-//   * a tile of a row in registers: its largest value and Σ exp(x − largest);
-//   * its K best: the K-th largest of 64 groups' maxima is a bound that at least K
-//     elements reach, and for unequal logits few more, so that only those are compared
-//     with one another (many equal ones: the best are taken out one after the other);
+//   * the row's largest value and Σ exp(x − largest), 32 logits a thread at a time;
+//   * its K best: the K-th largest of 64 groups of threads' maxima is a bound that at least
+//     K elements reach, and for unequal logits few more.  The threads that hold them read
+//     theirs once more, and only those elements are compared with one another (many equal
+//     ones: the best are taken out one after the other).  Keeping a row in registers
+//     instead left one block an SM (64 prompts' eight hypotheses: 43 µs);
 //   * every block's K best keys and sum go to the first block's shared memory, which
 //     finds the prompt's best among them in 64 bits.
 // Bound by the logits' bytes where rows are many, by the chain of these steps where
@@ -23,7 +25,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 using Key = unsigned long long;
-constexpr int kThreads = 512, kWarps = kThreads / 32, kGroups = 64, kCluster = 8;
+constexpr int kGroups = 64, kCluster = 16;
+constexpr int kParts = 8;  // blocks that share a prompt's rows out in parts, at most
 constexpr int kList = 512;  // elements that reach the bound, at most, before equal ones get a way of their own
 
 // Larger keys come first: the logit, then the lower token.
@@ -134,10 +137,17 @@ struct Best {  // one list in the first block's shared memory: K keys, then
   float m, s;  // its part's largest logit and Σ exp(logit − largest)
 };
 
-// Items in order: value, then the lower hypothesis, then the key.
+// Items in order: value, then the lower hypothesis, then the key.  The value is a double
+// as an integer in its order; 0 is no item.
+__device__ __forceinline__ Key ordered(double x) {
+  const Key u = (Key)__double_as_longlong(x + 0.);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double value_of(Key o) {
+  return __longlong_as_double((long long)(o >> 63 ? o & ~(1ull << 63) : ~o));
+}
 struct Item {
-  double value;
-  Key key;
+  Key value, key;
   int beam;
 };
 __device__ __forceinline__ bool ahead(const Item& a, const Item& b) {
@@ -146,227 +156,299 @@ __device__ __forceinline__ bool ahead(const Item& a, const Item& b) {
   return a.key > b.key;
 }
 
-struct Scratch {
-  float top[kGroups], wm[kWarps], ws[kWarps];
-  Key list[kList + 32], cur[32], wbest[kWarps];
-  float bound;
-  int n;
+template <int kThreads> struct Scratch {
+  float top[kGroups], wm[32], ws[32];
+  Key list[kList], cur[32], wbest[32];
+  float bound, m, s;
+  unsigned short holds[kThreads];
+  int n, held;
 };
 
-// The K best of pieces [q0, q1) of a row, sorted, into sc.cur, and its largest logit and sum.
-template <int DT, int NV>
-__device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, Scratch& sc, float& M, float& S) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int N = Vec<DT>::N;
-  float m = -INFINITY, s = 0.f;  // this thread's, over all tiles
-  for (int base = q0; base < q1; base += NV * kThreads) {
-    Vec<DT> v[NV];
+// Two exponentials relative to m, added to (a, b).
+__device__ __forceinline__ void add_pow2(float& a, float& b, float x, float y, float m) {
+  asm("{.reg .b64 p, q; .reg .f32 x, y; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %4}; add.rn.f32x2 p, p, q;"
+      " mov.b64 q, {%5, %5}; mul.rn.f32x2 p, p, q; mov.b64 {x, y}, p; ex2.approx.ftz.f32 x, x;"
+      " ex2.approx.ftz.f32 y, y; mov.b64 p, {x, y}; mov.b64 q, {%0, %1}; add.rn.f32x2 p, p, q; mov.b64 {%0, %1}, p;}"
+      : "+f"(a), "+f"(b) : "f"(x), "f"(y), "f"(-m), "f"(kLog2e));
+}
+
+// put(i, how many of the n items come before item i), eight threads an item.
+template <int kThreads, typename B, typename P>
+__device__ __forceinline__ void for_ranks(int n, B is_before, P put) {
+  const int sub = threadIdx.x & 7;
+  for (int i0 = 0; i0 < n; i0 += kThreads / 8) {  // the same for all threads
+    const int i = i0 + (threadIdx.x >> 3), me = min(i, n - 1);
+    int r = 0;
+#pragma unroll 4
+    for (int j = sub; j < n; j += 8) r += is_before(me, j);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) v[j] = row.load(base + j * kThreads + tid, q1);
-    float t = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) t = fmaxf(t, v[j].most());
-    const float to = fmaxf(m, t), ref = finite_or_0(to);
-    s *= rescale(m, to);
-    m = to;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float e[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) e[i] = pow2((v[j].at(i) - ref) * kLog2e);
-#pragma unroll
-      for (int o = N / 2; o; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < o; ++i) e[i] += e[i + o];
-      s += e[0];
-    }
-    float g = t;
-#pragma unroll
-    for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if (tid % (kThreads / kGroups) == 0) sc.top[tid / (kThreads / kGroups)] = g;
-    const bool more = base != q0;  // the best of the tiles before are in cur
-    if (tid == 0) sc.n = more ? K : 0;
-    if (more && tid < K) sc.list[tid] = sc.cur[tid];
-    __syncthreads();
-    // the K-th largest group: each warp ranks its share of them
-    const float a = sc.top[lane], b = sc.top[lane + 32];
-#pragma unroll
-    for (int i = 0; i < kGroups / kWarps; ++i) {
-      const int me = warp * (kGroups / kWarps) + i;
-      const float x = __shfl_sync(0xffffffffu, me < 32 ? a : b, me & 31);
-      const int r = __popc(__ballot_sync(0xffffffffu, a > x || (a == x && lane < me))) +
-                    __popc(__ballot_sync(0xffffffffu, b > x || (b == x && lane + 32 < me)));
-      if (r == K - 1 && lane == 0) sc.bound = x;
-    }
-    __syncthreads();
-    const float bound = sc.bound;
-    // tokens before this tile's were lower: an equal key of theirs comes first by itself
-    if (t >= bound) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int q = base + j * kThreads + tid, f = q * N;
-        if (v[j].most() < bound || q >= q1) continue;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float x = v[j].at(i);
-          if (x >= bound && f + i < row.V) {
-            const int at = atomicAdd(&sc.n, 1);
-            if (at < kList + 32) sc.list[at] = key_of(x, f + i);
-          }
-        }
-      }
-    }
-    __syncthreads();
-    const int n = sc.n;
-    if (n <= kList + 32) {
-      // each warp ranks its share of what reached the bound
-      for (int i = warp; i < n; i += kWarps) {
-        const Key x = sc.list[i];
-        int r = 0;
-        for (int j = lane; j - lane < n; j += 32) r += __popc(__ballot_sync(0xffffffffu, j < n && sc.list[j] > x));
-        if (lane == 0 && r < K) sc.cur[r] = x;
-      }
-      if (n < K && tid >= n && tid < K) sc.cur[tid] = 0;  // a row with fewer tokens so far
-      __syncthreads();
-    } else {
-      // many equal logits: the largest key below the last, K times
-      Key last = ~0ull, mine = more && tid < K ? sc.cur[tid] : 0;
-      __syncthreads();
-      for (int k = 0; k < K; ++k) {
-        Key best = mine < last ? mine : 0;
-#pragma unroll 1
-        for (int q = base + tid; q < min(q1, base + NV * kThreads); q += kThreads) {
-          const Vec<DT> u = row.load(q, q1);
-          const int f = q * N;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const Key x = key_of(u.at(i), f + i);
-            if (f + i < row.V && x < last && x > best) best = x;
-          }
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        if (lane == 0) sc.wbest[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < kWarps; ++w) best = max(best, sc.wbest[w]);
-        if (tid == 0) sc.cur[k] = best;
-        last = best;
-        __syncthreads();
-      }
-    }
+    for (int o = 1; o < 8; o <<= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (sub == 0 && i < n) put(i, r);
   }
-  float wm = m;
+}
+
+// A thread's pieces into its largest logit and sum.
+template <int DT, int U>
+__device__ __forceinline__ void take(const Vec<DT>* v, float& m, float& s) {
+  constexpr int N = Vec<DT>::N;
+  float to = m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+  for (int j = 0; j < U; ++j) to = fmaxf(to, v[j].most());
+  const float ref = finite_or_0(to);
+  float a[2] = {s * rescale(m, to), 0.f}, b[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < U; ++j)
+#pragma unroll
+    for (int i = 0; i < N; i += 2) add_pow2(a[i / 2 % 2], b[i / 2 % 2], v[j].at(i), v[j].at(i + 1), ref);
+  s = (a[0] + a[1]) + (b[0] + b[1]);
+  m = to;
+}
+
+// The K best of pieces [q0, q1) of a row, sorted, into sc.cur, its largest logit and sum (to all
+// threads), and the two's logarithm (to the first of the last warp).
+template <int DT, int kThreads>
+__device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, Scratch<kThreads>& sc, float& M, float& S,
+                                     double& lse) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kWarps = kThreads / 32, N = Vec<DT>::N, U = 8;  // pieces in flight
+  float m = -INFINITY, s = 0.f;
+  int q = q0 + tid;
+  // whole pieces first, in the same order wherever the row lies
+  for (const int whole = min(q1, row.V / N); q + (U - 1) * kThreads < whole; q += U * kThreads) {
+    Vec<DT> v[U];
+    if (row.off == 0) {
+      const uint4* from = reinterpret_cast<const uint4*>(row.at) + q;
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const uint4 x = __ldg(from + j * kThreads);
+        v[j].w[0] = x.x; v[j].w[1] = x.y; v[j].w[2] = x.z; v[j].w[3] = x.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < U; ++j) v[j] = row.load(q + j * kThreads, q1);
+    }
+    take<DT, U>(v, m, s);
+  }
+  for (; q < q1; q += 2 * kThreads) {
+    Vec<DT> v[2] = {row.load(q, q1), row.load(q + kThreads, q1)};
+    take<DT, 2>(v, m, s);
+  }
+  float g = m, wm = m;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+    if (2 * o == kThreads / kGroups) g = wm;
+  }
+  if (tid % (kThreads / kGroups) == 0) sc.top[tid / (kThreads / kGroups)] = g;
   s = warp_sum(s * rescale(m, wm));
   if (lane == 0) {
     sc.wm[warp] = wm;
     sc.ws[warp] = s;
   }
+  if (tid == 0) sc.n = sc.held = 0;
   __syncthreads();
-  M = -INFINITY;
+  // the K-th largest group: each has kThreads / kGroups threads that compare it with a share
+  constexpr int kEach = kThreads / kGroups;
+  {
+    const int me = tid / kEach;
+    const float x = sc.top[me];
+    int r = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sc.wm[w]);
-  S = 0.f;
+    for (int i = 0; i < kGroups / kEach; ++i) {
+      const int j = i * kEach + tid % kEach;
+      const float y = sc.top[j];
+      r += y > x || (y == x && j < me);
+    }
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) S += sc.ws[w] * rescale(sc.wm[w], M);
+    for (int o = 1; o < kEach; o <<= 1) r += __shfl_xor_sync(0xffffffffu, r, o);
+    if (r == K - 1 && tid % kEach == 0) sc.bound = x;
+  }
+  if (warp == kWarps - 1) {
+    const float y = lane < kWarps ? sc.wm[lane] : -INFINITY;
+    M = y;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    S = warp_sum(lane < kWarps ? sc.ws[lane] * rescale(y, M) : 0.f);
+    if (lane == 0) {
+      sc.m = M;
+      sc.s = S;
+    }
+  }
+  __syncthreads();
+  M = sc.m;
+  S = sc.s;
+  const float bound = sc.bound;
+  // the few threads that hold such logits have theirs read again, by all threads at once
+  if (m >= bound) sc.holds[atomicAdd(&sc.held, 1)] = (unsigned short)tid;
+  __syncthreads();
+  const int held = sc.held, each = (q1 - q0 + kThreads - 1) / kThreads;
+  for (int i = tid; i < held * each; i += kThreads) {
+    const int q = q0 + sc.holds[i / each] + i % each * kThreads, f = q * N;
+    if (q >= q1) continue;
+    const Vec<DT> v = row.load(q, q1);
+    if (v.most() < bound) continue;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float x = v.at(j);
+      if (x >= bound && f + j < row.V) {
+        const int at = atomicAdd(&sc.n, 1);
+        if (at < kList) sc.list[at] = key_of(x, f + j);
+      }
+    }
+  }
+  if (tid == kThreads - 32) lse = (double)M + log((double)S);
+  __syncthreads();
+  const int n = sc.n;
+  if (n <= kList) {
+    for_ranks<kThreads>(n, [&](int i, int j) { return sc.list[j] > sc.list[i]; },
+                        [&](int i, int r) { if (r < K) sc.cur[r] = sc.list[i]; });
+    if (tid >= n && tid < K) sc.cur[tid] = 0;  // a part with fewer tokens
+    __syncthreads();
+  } else {
+    // many equal logits: the largest key below the last, K times
+    Key last = ~0ull;
+    for (int k = 0; k < K; ++k) {
+      Key best = 0;
+#pragma unroll 1
+      for (int q = q0 + tid; q < q1; q += kThreads) {
+        const Vec<DT> u = row.load(q, q1);
+        const int f = q * N;
+        if (u.most() < bound) continue;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const Key x = key_of(u.at(i), f + i);
+          if (f + i < row.V && x < last && x > best) best = x;
+        }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+      if (lane == 0) sc.wbest[warp] = best;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w) best = max(best, sc.wbest[w]);
+      if (tid == 0) sc.cur[k] = best;
+      last = best;
+      __syncthreads();
+    }
+  }
 }
 
 // Parts of a row and blocks of a cluster: parts · K blocks, or (K > kCluster) blocks that
 // take every so many-th row.
-template <int DT, int NV>
-__global__ void __launch_bounds__(kThreads) beam_select(BeamP p, int parts) {
-  __shared__ Scratch sc;
+template <int DT, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) beam_select(BeamP p, int log_parts) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ Scratch<kThreads> sc;
   // of the first block: every list, and what is left of them
   __shared__ Key keys[32 * 32];
   __shared__ Best sums[32];
   __shared__ Item kept[32 * 32];
   __shared__ Item heads[32], limit;
   __shared__ double lse[32];
+  __shared__ float score[32];
   __shared__ int kind[32], n;  // 0: scanned, 1: ended, 2: nothing but −infinity
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
-  const int prompt = blockIdx.x / blocks, K = p.K, L = K * parts;
+  const int prompt = blockIdx.x / blocks, K = p.K, parts = 1 << log_parts, L = K << log_parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (blocks > 1) cl.sync();  // the first block is there
+  if (blocks > 1) cl.barrier_arrive();
+  if (tid < K) {
+    score[tid] = p.scores[prompt * K + tid];
+    const bool ended = p.done && p.done[prompt * K + tid];
+    kind[tid] = !isfinite(score[tid]) ? 2 : ended ? 1 : 0;
+  }
+  if (tid == 0) n = 0;
+  __syncthreads();
+  bool there = blocks == 1;  // the first block is
   for (int list = rank; list < L; list += blocks) {
-    const int r = prompt * K + list / parts;
-    if (!isfinite(p.scores[r]) || (p.done && p.done[r])) continue;
+    const int r = prompt * K + (list >> log_parts);
+    if (kind[list >> log_parts]) continue;
     const Row<DT> row(p, r);
-    const int each = (row.pieces + parts - 1) / parts, q0 = min(row.pieces, each * (list % parts));
+    const int each = (row.pieces + parts - 1) >> log_parts, q0 = min(row.pieces, each * ((list & (parts - 1))));
     float M, S;
-    if (tid < K) sc.cur[tid] = 0;  // a part without a piece
-    __syncthreads();
-    scan<DT, NV>(row, q0, min(row.pieces, q0 + each), K, sc, M, S);
+    double one;
+    scan<DT, kThreads>(row, q0, min(row.pieces, q0 + each), K, sc, M, S, one);
+    if (!there) cl.barrier_wait();
+    there = true;
     Key* to = cl.map_shared_rank(keys, 0) + list * K;
     if (tid < K) to[tid] = sc.cur[tid];
-    if (tid == 0) *(cl.map_shared_rank(sums, 0) + list) = Best{M, S};
+    if (tid == kThreads - 32) {
+      *(cl.map_shared_rank(sums, 0) + list) = Best{M, S};
+      if (parts == 1) *(cl.map_shared_rank(lse, 0) + list) = one;
+    }
     __syncthreads();
   }
+  if (!there) cl.barrier_wait();
   if (blocks > 1) cl.sync();
   if (rank != 0) return;
-  __syncthreads();
 
-  if (tid == 0) n = 0;
   if (tid < K) {
-    const float score = p.scores[prompt * K + tid];
-    int k = !isfinite(score) ? 2 : p.done && p.done[prompt * K + tid] ? 1 : 0;
-    if (k == 0) {
-      float m = -INFINITY, s = 0.f;
-      for (int i = 0; i < parts; ++i) m = fmaxf(m, sums[tid * parts + i].m);
-      for (int i = 0; i < parts; ++i)
-        s += sums[tid * parts + i].s * rescale(sums[tid * parts + i].m, m);
-      lse[tid] = (double)m + log((double)s);
-      if (!isfinite(lse[tid])) k = 2;
+    if (kind[tid] == 0) {
+      if (parts > 1) {
+        float m = -INFINITY, s = 0.f;
+        for (int i = 0; i < parts; ++i) m = fmaxf(m, sums[tid * parts + i].m);
+        for (int i = 0; i < parts; ++i) s += sums[tid * parts + i].s * rescale(sums[tid * parts + i].m, m);
+        lse[tid] = (double)m + log((double)s);
+      }
+      if (!isfinite(lse[tid])) kind[tid] = 2;
     }
-    kind[tid] = k;
   }
   __syncthreads();
   // item i of a list
   auto item = [&](int list, int i) {
-    const int k = list / parts;
-    Item it{-INFINITY, 0ull, k};
+    const int k = list >> log_parts;
+    Item it{0ull, 0ull, k};
     if (kind[k] == 0) {
       it.key = keys[list * K + i];
-      if (it.key) it.value = (double)p.scores[prompt * K + k] + ((double)logit_of(it.key) - lse[k]);
-    } else if (list % parts == 0) {  // one list: eos first, then the other tokens
+      if (it.key) it.value = ordered((double)score[k] + ((double)logit_of(it.key) - lse[k]));
+    } else if ((list & (parts - 1)) == 0) {  // one list: eos first, then the other tokens
       int token = i;
       if (kind[k] == 1) {
         token = i == 0 ? p.eos : i - 1 + (i - 1 >= p.eos);
-        if (i == 0) it.value = p.scores[prompt * K + k];
       }
-      if (token < p.V) it.key = (unsigned)~(unsigned)token | (Key)(i == 0 && kind[k] == 1) << 32;
+      it.value = ordered(i == 0 && kind[k] == 1 ? score[k] : -INFINITY);
+      it.key = (unsigned)~(unsigned)token | (Key)(i == 0 && kind[k] == 1) << 32;
     }
     return it;
   };
-  // the K-th of the lists' first items bounds what can be among the K best
-  if (tid < L) heads[tid] = item(tid, 0);
-  __syncthreads();
-  for (int i = warp; i < L; i += kWarps) {
-    const bool is = lane < L && lane != i && (ahead(heads[lane], heads[i]) || (lane < i && !ahead(heads[i], heads[lane])));
-    if (__popc(__ballot_sync(0xffffffffu, is)) == K - 1 && lane == 0) limit = heads[i];
-  }
-  __syncthreads();
-  for (int i = tid; i < L * K; i += kThreads) {
-    const Item it = item(i / K, i % K);
-    if (it.key && !ahead(limit, it)) kept[atomicAdd(&n, 1)] = it;
-  }
-  __syncthreads();
-  for (int i = warp; i < n; i += kWarps) {
-    const Item mine = kept[i];
-    int r = 0;
-    for (int j = lane; j - lane < n; j += 32) r += __popc(__ballot_sync(0xffffffffu, j < n && ahead(kept[j], mine)));
-    if (lane == 0 && r < K) {
-      const int o = prompt * K + r;
-      p.out_scores[o] = (float)mine.value;
-      p.out_tokens[o] = token_of(mine.key);
-      p.out_rows[o] = prompt * K + mine.beam;
+  // few items: all; of many those that the K-th of the lists' first ones does not come before
+  if (L * K <= 256) {
+    for (int i = tid; i < L * K; i += kThreads) kept[i] = item(i / K, i % K);
+    if (tid == 0) n = L * K;
+  } else {
+    if (tid < L) heads[tid] = item(tid, 0);
+    __syncthreads();
+    for_ranks<kThreads>(L, [&](int i, int j) { return ahead(heads[j], heads[i]) || (j < i && !ahead(heads[i], heads[j])); },
+                        [&](int i, int r) { if (r == K - 1) limit = heads[i]; });
+    __syncthreads();
+    for (int i = tid; i < L * K; i += kThreads) {
+      const Item it = item(i / K, i % K);
+      if (it.key && !ahead(limit, it)) kept[atomicAdd(&n, 1)] = it;
     }
   }
+  __syncthreads();
+  for_ranks<kThreads>(n, [&](int i, int j) { return ahead(kept[j], kept[i]); },
+                      [&](int i, int r) {
+                        if (r >= K || !kept[i].key) return;
+                        const int o = prompt * K + r;
+                        p.out_scores[o] = (float)value_of(kept[i].value);
+                        p.out_tokens[o] = token_of(kept[i].key);
+                        p.out_rows[o] = prompt * K + kept[i].beam;
+                      });
 }
 
-template <int DT, int NV>
-cudaError_t launch(const BeamP& p, int parts, int blocks, cudaStream_t st) {
+template <int DT, int kThreads>
+cudaError_t launch(const BeamP& p, int log_parts, int blocks, cudaStream_t st) {
+  if (blocks > 8) {
+    static std::atomic<unsigned long long> allowed{0};  // devices where clusters of more than 8 are
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+      e = cudaFuncSetAttribute(beam_select<DT, kThreads>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+      if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.N * blocks));
   cfg.blockDim = dim3(kThreads);
@@ -376,17 +458,18 @@ cudaError_t launch(const BeamP& p, int parts, int blocks, cudaStream_t st) {
   at.val.clusterDim = {(unsigned)blocks, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, beam_select<DT, NV>, p, parts);
+  return cudaLaunchKernelEx(&cfg, beam_select<DT, kThreads>, p, log_parts);
 }
 
 template <int DT>
 cudaError_t launch(const BeamP& p, int sms, cudaStream_t st) {
-  constexpr int tile = kThreads * Vec<DT>::N;  // a piece a thread
-  // a row is shared out where there are fewer rows than SMs, while every thread has a piece
-  int parts = 1;
-  while (parts * 2 * p.K <= kCluster && p.N * p.K * parts * 2 <= sms && p.V > parts * tile) parts *= 2;
+  // a row is shared out where there are fewer rows than SMs, while 256 threads have a piece each
+  int parts = 1, log_parts = 0;
+  while (parts * 2 * p.K <= kParts && p.N * p.K * parts * 2 <= sms && p.V > parts * 256 * Vec<DT>::N) parts *= 2, ++log_parts;
   const int blocks = std::min(p.K * parts, kCluster);
-  return p.V / parts <= 2 * tile ? launch<DT, 2>(p, parts, blocks, st) : launch<DT, 8>(p, parts, blocks, st);
+  // long rows in few blocks: more threads
+  if (2 * p.N * blocks <= sms && p.V / parts >= 4096 * Vec<DT>::N) return launch<DT, 1024>(p, log_parts, blocks, st);
+  return launch<DT, 256>(p, log_parts, blocks, st);
 }
 
 }  // namespace
