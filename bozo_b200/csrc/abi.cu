@@ -666,12 +666,15 @@ int bozo_paged_reserve(const bozo_paged_reserve_args* a, void* stream) {
   cudaError_t e = bind_device(a->table, restore);
   if (e != cudaSuccess) return cuda_fail(e);
   ReserveP p{a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->lengths, a->tokens, a->refs,
-             a->cu_rows, a->missing, a->rows, a->seq, a->pos, a->slot, error_word(&e)};
+             a->cu_rows, a->missing, a->rows, a->seq, a->pos, a->slot, error_word(&e),
+             (unsigned)a->width * (unsigned)a->page_size, make_fastdiv((unsigned)a->width * (unsigned)a->page_size),
+             make_fastdiv((unsigned)a->page_size)};
   if (!p.err) return cuda_fail(e);
-  e = launch_paged_reserve(p, static_cast<cudaStream_t>(stream));
+  int launches = 0;
+  e = launch_paged_reserve(p, static_cast<cudaStream_t>(stream), &launches);
   if (e != cudaSuccess) return cuda_fail(e);
   t_last_path = BOZO_PATH_SIMT;
-  t_last_launches = 1;
+  t_last_launches = launches;
   return BOZO_OK;
 }
 
@@ -686,7 +689,7 @@ int bozo_paged_fork(const bozo_paged_fork_args* a, void* stream) {
   cudaError_t e = bind_device(a->table, restore);
   if (e != cudaSuccess) return cuda_fail(e);
   ForkP p{a->table, a->table_stride, a->batch, a->width, a->page_size, a->pages, a->share ? 1 : 0, a->lengths,
-          a->parents, a->refs, a->copies, a->missing, error_word(&e)};
+          a->parents, a->refs, a->copies, a->missing, error_word(&e), make_fastdiv((unsigned)a->page_size)};
   if (!p.err) return cuda_fail(e);
   e = launch_paged_fork(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e);

@@ -536,27 +536,30 @@ const int32_t* per_row(const char* what, const char* name, const at::Tensor& t, 
   return t.data_ptr<int32_t>();
 }
 
-// (cu_rows [B + 1], missing [1], places [3, rows]: sequence, position and slot)
-std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_reserve(const at::Tensor& table, const at::Tensor& lengths,
-                                                             const c10::optional<at::Tensor>& tokens,
-                                                             const at::Tensor& refs, int64_t page_size, int64_t rows) {
+// (cu_rows [B + 1], missing [1], and with rows ≥ 0: sequence, position and slot, [rows] each)
+pybind11::tuple paged_reserve(const at::Tensor& table, const at::Tensor& lengths,
+                              const c10::optional<at::Tensor>& tokens, const at::Tensor& refs, int64_t page_size,
+                              int64_t rows) {
   const char* what = "reserve";
   bozo_paged_reserve_args a{};
   const auto dev = table_of(what, a, table, lengths, refs, page_size);
   const c10::cuda::CUDAGuard guard(dev);
   if (given(tokens)) a.tokens = per_row(what, "tokens", *tokens, lengths);
-  if (rows < 0 || rows > INT32_MAX) throw std::invalid_argument("reserve: rows must not be negative, nor pass 2^31");
-  at::Tensor cu = empty({a.batch + 1}, at::kInt, dev), missing = empty({1}, at::kInt, dev), at_ = empty({3, rows}, at::kInt, dev);
+  if (rows < -1 || rows > INT32_MAX) throw std::invalid_argument("reserve: rows must not be negative, nor pass 2^31");
+  at::Tensor cu = empty({a.batch + 1}, at::kInt, dev), missing = empty({1}, at::kInt, dev), at_[3];
   a.cu_rows = cu.data_ptr<int32_t>();
   a.missing = missing.data_ptr<int32_t>();
-  a.rows = rows;
-  if (rows) {
-    a.seq = at_.data_ptr<int32_t>();
-    a.pos = a.seq + rows;
-    a.slot = a.pos + rows;
+  if (rows >= 0)
+    for (at::Tensor& t : at_) t = empty({rows}, at::kInt, dev);
+  if (rows > 0) {
+    a.rows = rows;
+    a.seq = at_[0].data_ptr<int32_t>();
+    a.pos = at_[1].data_ptr<int32_t>();
+    a.slot = at_[2].data_ptr<int32_t>();
   }
   check(bozo_paged_reserve(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_reserve");
-  return {std::move(cu), std::move(missing), std::move(at_)};
+  if (rows < 0) return pybind11::make_tuple(cu, missing, pybind11::none(), pybind11::none(), pybind11::none());
+  return pybind11::make_tuple(cu, missing, at_[0], at_[1], at_[2]);
 }
 
 std::tuple<at::Tensor, at::Tensor> paged_fork(const at::Tensor& table, const at::Tensor& lengths,

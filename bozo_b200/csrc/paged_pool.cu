@@ -17,6 +17,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
+constexpr int kSmallPool = 16384;  // pages that one block counts
 
 // Inclusive scan of v over the block; `total`: the sum.  `tmp`: 32 words.
 __device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* tmp,
@@ -55,50 +56,71 @@ __device__ __forceinline__ int find(const int* sums, int n, int x) {
   return lo;
 }
 
-__device__ __forceinline__ bool free_page(const int* refs, int p) { return __ldcg(refs + p) == 0; }
-
-// The part of the pool that this block of the cluster looks after.
-struct Part {
+// A thread's run of consecutive pages, of a block's part of the pool.
+struct Run {
   int lo, hi;
-  __device__ Part(int pages, unsigned rank, unsigned blocks) {
-    const int each = (int)(((long long)pages + blocks - 1) / blocks);
-    lo = min(pages, each * (int)rank);
+  __device__ Run(int pages, unsigned rank, unsigned blocks) {
+    const int each = (int)(((long long)pages + (long long)blocks * kThreads - 1) / ((long long)blocks * kThreads));
+    lo = (int)min((long long)pages, (long long)each * (rank * kThreads + threadIdx.x));
     hi = min(pages, lo + each);
+  }
+  __device__ int count(const int* refs) const {
+    int n = 0;
+#pragma unroll 8
+    for (int p = lo; p < hi; ++p) n += refs[p] == 0;
+    return n;
   }
 };
 
-// Free pages before this block's part and in all; `count`: one word of shared memory.
-__device__ __forceinline__ void count_free(const int* refs, Part part, int* count, unsigned long long* tmp, int& before,
-                                           int& all) {
+// From each thread's free pages, those before its own and in all; `count`: one word of
+// shared memory.  With more than one block the cluster is synchronised in between.
+__device__ __forceinline__ void scan_free(int mine, int* count, unsigned long long* tmp, int& before, int& all) {
   cg::cluster_group cl = cg::this_cluster();
-  int n = 0;
-  for (int p = part.lo + threadIdx.x; p < part.hi; p += kThreads) n += free_page(refs, p);
   unsigned long long total;
-  block_scan(n, tmp, total);
-  if (threadIdx.x == 0) *count = (int)total;
-  cl.sync();
-  before = all = 0;
-  for (unsigned r = 0; r < cl.num_blocks(); ++r) {
-    const int c = *cl.map_shared_rank(count, r);
-    if (r < cl.block_rank()) before += c;
-    all += c;
+  before = (int)block_scan(mine, tmp, total) - mine;
+  all = (int)total;
+  if (cl.num_blocks() > 1) {
+    if (threadIdx.x == 0) *count = all;
+    cl.sync();
+    all = 0;
+    for (unsigned r = 0; r < cl.num_blocks(); ++r) {
+      const int c = *cl.map_shared_rank(count, r);
+      if (r < cl.block_rank()) before += c;
+      all += c;
+    }
   }
 }
+__device__ __forceinline__ void sync_all() {
+  cg::cluster_group cl = cg::this_cluster();
+  if (cl.num_blocks() > 1) cl.sync();
+  else __syncthreads();
+}
 
-// f(rank, page) for this block's free pages of rank < want, in ascending order.
+// f(rank, page) for this thread's free pages of rank < want, in ascending order.
 template <typename F>
-__device__ __forceinline__ void give(const int* refs, Part part, int before, int want, unsigned long long* tmp, F f) {
-  for (int base = part.lo; base < part.hi && before < want; base += kThreads) {
-    const int p = base + threadIdx.x;
-    const bool is = p < part.hi && free_page(refs, p);
-    unsigned long long total;
-    const int rank = before + (int)block_scan(is, tmp, total) - 1;
-    if (is && rank < want) f(rank, p);
-    before += (int)total;
-  }
+__device__ __forceinline__ void give(const int* refs, Run run, int rank, int want, F f) {
+  for (int p = run.lo; p < run.hi && rank < want; ++p)
+    if (refs[p] == 0) f(rank++, p);
 }
 
-__global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p) {
+// Where row i of the packed new tokens goes: sequence b, which has the rows [first, next).
+__device__ __forceinline__ void place(const ReserveP& p, int i, int b, int first, int next, int& at, int& slot) {
+  const long long t = p.lengths[b], pos = t + (i - first);
+  at = (int)pos;
+  slot = -1;
+  if (pos < t + (next - first) - (long long)p.cap || pos > 0x7fffffffLL) return;
+  const unsigned s = (unsigned)pos - fast_div((unsigned)pos, p.div_cap) * p.cap, j = fast_div(s, p.div_page);
+  const int page = __ldcg(p.table + b * p.ts + j);
+  if ((unsigned)page < (unsigned)p.P) slot = page * p.page + (int)(s - j * p.page);
+}
+
+// Columns that t < 2^32 tokens fill.
+__device__ __forceinline__ int pages_of(const ReserveP& p, unsigned t) {
+  const unsigned whole = fast_div(t, p.div_page);
+  return (int)min((unsigned)p.M, whole + (whole * (unsigned)p.page < t));
+}
+
+__global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool places) {
   extern __shared__ int sm[];
   int* off = sm;               // wanted pages before each sequence [B + 1]
   int* cu = off + p.B + 1;     // new tokens before it [B + 1]
@@ -107,21 +129,23 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p) {
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned rank = cl.block_rank();
-  const long long cap = (long long)p.M * p.page;
+  const Run run(p.P, rank, cl.num_blocks());
+  const int mine = run.count(p.refs);
   unsigned long long carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
     int want = 0, n = 0, have = 0;
     if (b < p.B) {
       const int t = p.lengths[b];
-      if (t >= 0) {
-        n = p.tokens ? max(0, p.tokens[b]) : 1;
-        if (n > 0x7fffffff / p.B) {  // the sums are held in 31 bits
-          atomicCAS(p.err, 0, kErrPaged | 1);
-          n = 0;
-        }
-        have = (int)min((long long)p.M, ((long long)t + p.page - 1) / p.page);
-        const int need = n ? (int)min((long long)p.M, ((long long)t + n + p.page - 1) / p.page) : have;
+      n = p.tokens ? max(0, p.tokens[b]) : 1;
+      if (t < 0) n = 0;
+      if (n > 0x7fffffff / p.B) {  // the sums are held in 31 bits
+        atomicCAS(p.err, 0, kErrPaged | 1);
+        n = 0;
+      }
+      if (n) {
+        have = pages_of(p, t);
+        const int need = pages_of(p, (unsigned)t + (unsigned)n);
         while (have < need && (unsigned)__ldcg(p.table + b * p.ts + have) < (unsigned)p.P) ++have;
         want = need - have;
       }
@@ -146,27 +170,22 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p) {
     for (int b = threadIdx.x; b <= p.B; b += kThreads) p.cu[b] = cu[b];
   int before = 0, all = 0;
   if (want) {
-    const Part part(p.P, rank, cl.num_blocks());
-    count_free(p.refs, part, &count, tmp, before, all);  // every block has read the table by now
+    scan_free(mine, &count, tmp, before, all);  // every block has read the table by now
     if (want <= all)
-      give(p.refs, part, before, want, tmp, [&](int i, int page) {
+      give(p.refs, run, before, want, [&](int i, int page) {
         const int b = find(off, p.B, i);
         p.table[b * p.ts + col[b] + i - off[b]] = page;
         p.refs[page] = 1;
       });
-    cl.sync();  // the table is whole, and no block's count is read any more
+    sync_all();  // the table is whole, and no block's count is read any more
   }
   if (rank == 0 && threadIdx.x == 0) *p.missing = max(0, want - all);
+  if (!places) return;
   for (long long i = (long long)rank * kThreads + threadIdx.x; i < p.rows; i += (long long)cl.num_blocks() * kThreads) {
     int b = -1, at = -1, slot = -1;
     if (i < rows) {
       b = find(cu, p.B, (int)i);
-      const long long t = (long long)p.lengths[b] + (i - cu[b]), end = (long long)p.lengths[b] + (cu[b + 1] - cu[b]);
-      at = (int)t;
-      if (t >= end - cap) {
-        const int s = (int)(t % cap), j = s / p.page, page = __ldcg(p.table + b * p.ts + j);
-        if ((unsigned)page < (unsigned)p.P) slot = page * p.page + (s - j * p.page);
-      }
+      place(p, (int)i, b, cu[b], cu[b + 1], at, slot);
     }
     p.seq[i] = b;
     p.pos[i] = at;
@@ -174,54 +193,95 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p) {
   }
 }
 
-// A row's full and used columns.
-struct Used {
-  int full, held;
-  __device__ Used(const ForkP& p, int t) {
-    full = p.share && t > 0 ? (int)min((long long)p.M, (long long)t / p.page) : 0;
-    held = t > 0 ? (int)min((long long)p.M, ((long long)t + p.page - 1) / p.page) : 0;
+// The places of many rows, four a thread.
+constexpr int kPlaceThreads = 256;
+__global__ void __launch_bounds__(kPlaceThreads) paged_places(ReserveP p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long i0 = ((long long)blockIdx.x * kPlaceThreads + threadIdx.x) * 4;
+  if (i0 >= p.rows) return;
+  const int rows = __ldcg(p.cu + p.B);
+  int lo = 0, hi = p.B;  // the last b with cu[b] ≤ i0
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu[mid] <= i0) lo = mid; else hi = mid;
   }
-};
-__device__ __forceinline__ int parent_of(const ForkP& p, int r) {
-  const int x = p.parents[r];
-  return (unsigned)x < (unsigned)p.B ? x : -1;
+  int b = lo, first = p.cu[b], next = p.cu[b + 1];
+  int seq[4], at[4], slot[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const long long i = i0 + k;
+    seq[k] = at[k] = slot[k] = -1;
+    if (i >= rows) continue;
+    while (i >= next) {
+      ++b;
+      first = next;
+      next = p.cu[b + 1];
+    }
+    seq[k] = b;
+    place(p, (int)i, b, first, next, at[k], slot[k]);
+  }
+  if (i0 + 4 <= p.rows && !((reinterpret_cast<uintptr_t>(p.seq) | reinterpret_cast<uintptr_t>(p.pos) | reinterpret_cast<uintptr_t>(p.slot)) & 15)) {
+    reinterpret_cast<int4*>(p.seq + i0)[0] = make_int4(seq[0], seq[1], seq[2], seq[3]);
+    reinterpret_cast<int4*>(p.pos + i0)[0] = make_int4(at[0], at[1], at[2], at[3]);
+    reinterpret_cast<int4*>(p.slot + i0)[0] = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    return;
+  }
+  for (int k = 0; k < 4 && i0 + k < p.rows; ++k) {
+    p.seq[i0 + k] = seq[k];
+    p.pos[i0 + k] = at[k];
+    p.slot[i0 + k] = slot[k];
+  }
 }
 
-__global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile) {
+__global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDiv div_tile) {
   extern __shared__ int sm[];
-  int* children = sm;             // of each row [B]
+  int* parent = sm;               // of each new row, −1 for none [B]
+  int* children = parent + p.B;   // of each old row [B]
   int* eldest = children + p.B;   // the first of them [B]
-  int* off = eldest + p.B;        // pages wanted before each new row [B + 1]
+  int* full = eldest + p.B;       // its columns that its children share [B]
+  int* off = full + p.B;          // pages wanted before each new row [B + 1]
   int* old = off + p.B + 1;       // `tile` columns of the table [B][tile]
   __shared__ unsigned long long tmp[32];
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
+  // the old entries of columns c0 …: thread i has every kThreads-th of a tile's B · tile
+  auto load = [&](int c0) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < p.B * tile; i += kThreads) {
+      const int r = (int)fast_div((unsigned)i, div_tile), c = c0 + i - r * tile;
+      old[i] = c < p.M ? __ldcg(p.table + r * p.ts + c) : -1;
+    }
+  };
+  load(rank * tile);
   for (int r = threadIdx.x; r < p.B; r += kThreads) {
+    const int x = p.parents[r], t = p.lengths[r];
+    parent[r] = (unsigned)x < (unsigned)p.B ? x : -1;
     children[r] = 0;
     eldest[r] = p.B;
+    full[r] = p.share && t > 0 ? min(p.M, (int)fast_div((unsigned)t, p.div_page)) : 0;
+    if (x >= p.B || (p.share && t > (long long)p.M * p.page)) atomicCAS(p.err, 0, kErrPaged | 1);
   }
   __syncthreads();
   for (int r = threadIdx.x; r < p.B; r += kThreads) {
-    const int x = parent_of(p, r);
-    if (x >= 0) {
-      atomicAdd(children + x, 1);
-      atomicMin(eldest + x, r);
-    } else if (p.parents[r] >= 0) {
-      atomicCAS(p.err, 0, kErrPaged | 1);
-    }
-    if (p.share && p.lengths[r] > (long long)p.M * p.page) atomicCAS(p.err, 0, kErrPaged | 1);
+    const int x = parent[r];
+    if (x < 0) continue;
+    atomicAdd(children + x, 1);
+    atomicMin(eldest + x, r);
   }
+  const long long n_copies = (long long)p.B * (p.share ? 1 : p.M);
+  for (long long i = (long long)rank * kThreads + threadIdx.x; i < n_copies; i += (long long)blocks * kThreads)
+    reinterpret_cast<int2*>(p.copies)[i] = make_int2(-1, -1);
   __syncthreads();
   unsigned long long carry = 0;
   for (int r0 = 0; r0 < p.B; r0 += kThreads) {
     const int r = r0 + threadIdx.x;
     unsigned need = 0;
     if (r < p.B) {
-      const int x = parent_of(p, r);
+      const int x = parent[r];
       if (x >= 0 && eldest[x] != r) {
-        const Used u(p, p.lengths[x]);
-        need = u.held - u.full;
+        const int t = max(0, p.lengths[x]), whole = (int)fast_div((unsigned)t, p.div_page);
+        need = min(p.M, whole + (t > whole * p.page)) - full[x];
       }
     }
     unsigned long long total;
@@ -231,66 +291,64 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile) {
   }
   const int want = (int)carry;
   if (threadIdx.x == 0) off[p.B] = want;
-  const long long n_copies = (long long)p.B * (p.share ? 1 : p.M);
-  for (long long i = (long long)rank * kThreads + threadIdx.x; i < n_copies; i += (long long)blocks * kThreads)
-    reinterpret_cast<int2*>(p.copies)[i] = make_int2(-1, -1);
   // whole columns at a time: their old entries are read before any is written
   for (int c0 = rank * tile; c0 < p.M; c0 += blocks * tile) {
-    __syncthreads();
-    const int w = min(tile, p.M - c0);
-    for (int i = threadIdx.x; i < p.B * w; i += kThreads) {
-      const int r = i / w, j = i - r * w;
-      old[r * tile + j] = __ldcg(p.table + r * p.ts + c0 + j);
+    if (c0 != rank * tile) {
+      __syncthreads();
+      load(c0);
+      __syncthreads();
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.B * w; i += kThreads) {
-      const int r = i / w, j = i - r * w, c = c0 + j, x = parent_of(p, r);
-      int page = -1;
-      if (x >= 0 && (eldest[x] == r || c < Used(p, p.lengths[x]).full)) page = old[x * tile + j];
-      p.table[r * p.ts + c] = page;
+    for (int i = threadIdx.x; i < p.B * tile; i += kThreads) {
+      const int r = (int)fast_div((unsigned)i, div_tile), j = i - r * tile, c = c0 + j, x = parent[r];
+      if (c >= p.M) continue;
+      p.table[r * p.ts + c] = x >= 0 && (eldest[x] == r || c < full[x]) ? old[x * tile + j] : -1;
       // what the old row gives up, or its further children take
-      const int was = old[r * tile + j], n = children[r];
-      if ((unsigned)was < (unsigned)p.P) {
-        const int d = (c < Used(p, p.lengths[r]).full ? n : min(n, 1)) - 1;
-        if (d) atomicAdd(p.refs + was, d);
-      }
+      const int was = old[i], n = children[r], d = (c < full[r] ? n : min(n, 1)) - 1;
+      if (d && (unsigned)was < (unsigned)p.P) atomicAdd(p.refs + was, d);
     }
   }
-  cl.sync();
+  sync_all();
   int before = 0, all = 0;
   if (want) {
-    const Part part(p.P, rank, blocks);
-    count_free(p.refs, part, &count, tmp, before, all);
-    give(p.refs, part, before, want, tmp, [&](int i, int page) {
-      const int r = find(off, p.B, i), x = p.parents[r], k = i - off[r];
-      const int c = Used(p, p.lengths[x]).full + k;
+    const Run run(p.P, rank, blocks);
+    scan_free(run.count(p.refs), &count, tmp, before, all);
+    give(p.refs, run, before, want, [&](int i, int page) {
+      const int r = find(off, p.B, i), x = parent[r], c = full[x] + i - off[r];
       const int from = __ldcg(p.table + eldest[x] * p.ts + c);
       p.table[r * p.ts + c] = page;
       p.refs[page] = 1;
       if ((unsigned)from < (unsigned)p.P)
         reinterpret_cast<int2*>(p.copies)[p.share ? r : (long long)r * p.M + c] = make_int2(from, page);
     });
-    cl.sync();  // no block's count is read any more
+    if (blocks > 1) cl.sync();  // no block's count is read any more
   }
   if (rank == 0 && threadIdx.x == 0) *p.missing = max(0, want - all);
 }
 
 constexpr int kCopyThreads = 256;
-template <typename T>
-__device__ __forceinline__ void copy_page(const char* from, char* to, long long bytes) {
-  const T* a = reinterpret_cast<const T*>(from);
-  T* b = reinterpret_cast<T*>(to);
-  for (long long i = threadIdx.x; i < bytes / (long long)sizeof(T); i += kCopyThreads) b[i] = a[i];
-}
+constexpr int kCopyBytes = kCopyThreads * 16 * 4;  // of a page, by one block
 __global__ void __launch_bounds__(kCopyThreads) paged_copy(const __grid_constant__ CopyP p) {
-  const int2 c = __ldg(reinterpret_cast<const int2*>(p.copies) + blockIdx.x);
+  const long long bytes = p.bytes[blockIdx.y], lo = (long long)blockIdx.z * kCopyBytes;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (lo >= bytes) return;
+  const int2 c = __ldcg(reinterpret_cast<const int2*>(p.copies) + blockIdx.x);
   if ((unsigned)c.x >= (unsigned)p.P || (unsigned)c.y >= (unsigned)p.P || c.x == c.y) return;
-  char* pool = p.pool[blockIdx.y];
-  const long long bytes = p.bytes[blockIdx.y];
-  const char* from = pool + (long long)c.x * bytes;
-  char* to = pool + (long long)c.y * bytes;
-  if (!((reinterpret_cast<uintptr_t>(pool) | bytes) & 15)) copy_page<uint4>(from, to, bytes);
-  else copy_page<char>(from, to, bytes);
+  const char* from = p.pool[blockIdx.y] + (long long)c.x * bytes;
+  char* to = p.pool[blockIdx.y] + (long long)c.y * bytes;
+  const long long hi = blockIdx.z + 1 == gridDim.z ? bytes : min(bytes, lo + kCopyBytes);
+  if ((reinterpret_cast<uintptr_t>(p.pool[blockIdx.y]) | bytes) & 15) {
+    for (long long i = lo + threadIdx.x; i < hi; i += kCopyThreads) to[i] = from[i];
+    return;
+  }
+  for (long long i0 = lo + threadIdx.x * 16; i0 < hi; i0 += kCopyBytes) {
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * kCopyThreads * 16 < hi) x[j] = *reinterpret_cast<const uint4*>(from + i0 + j * kCopyThreads * 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * kCopyThreads * 16 < hi) *reinterpret_cast<uint4*>(to + i0 + j * kCopyThreads * 16) = x[j];
+  }
 }
 
 template <typename K, typename P, typename... A>
@@ -312,21 +370,47 @@ cudaError_t launch_cluster(K kern, int blocks, size_t smem, cudaStream_t st, con
   return cudaLaunchKernelEx(&cfg, kern, p, a...);
 }
 
+// A kernel that may be launched before the one ahead of it is done, which it waits for.
+template <typename P>
+cudaError_t launch_after(void (*kern)(P), dim3 grid, int threads, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
+}
+
 }  // namespace
 
-cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st) {
-  return launch_cluster(paged_reserve, 8, (size_t)(3 * p.B + 2) * sizeof(int), st, p);
+cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launches) {
+  const int blocks = p.P <= kSmallPool ? 1 : 8;
+  const bool here = p.rows <= 4096;
+  cudaError_t e = launch_cluster(paged_reserve, blocks, (size_t)(3 * p.B + 2) * sizeof(int), st, p, here);
+  *launches = here ? 1 : 2;
+  if (e != cudaSuccess || here) return e;
+  return launch_after(paged_places, dim3((unsigned)((p.rows + 4 * kPlaceThreads - 1) / (4 * kPlaceThreads))),
+                      kPlaceThreads, st, p);
 }
 
 cudaError_t launch_paged_fork(const ForkP& p, cudaStream_t st) {
-  // a sector's worth of columns, fewer where the rows are many
-  const int tile = p.B <= 2048 ? 8 : 2;
-  return launch_cluster(paged_fork, 8, ((size_t)3 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile);
+  // small tables: one block, whole; else a sector's worth of columns, fewer where the rows are many
+  const bool small = p.P <= kSmallPool && (long long)p.B * p.M <= 8192;
+  const int tile = small ? p.M : p.B <= 2048 ? 8 : 2;
+  return launch_cluster(paged_fork, small ? 1 : 8, ((size_t)5 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
+                        make_fastdiv((unsigned)tile));
 }
 
 cudaError_t launch_paged_copy(const CopyP& p, int pools, long long n, cudaStream_t st) {
-  paged_copy<<<dim3((unsigned)n, (unsigned)pools), kCopyThreads, 0, st>>>(p);
-  return cudaGetLastError();
+  long long most = 0;
+  for (int i = 0; i < pools; ++i) most = p.bytes[i] > most ? p.bytes[i] : most;
+  const long long parts = (most + kCopyBytes - 1) / kCopyBytes;
+  return launch_after(paged_copy, dim3((unsigned)n, (unsigned)pools, (unsigned)(parts < 65535 ? parts : 65535)),
+                      kCopyThreads, st, p);
 }
 
 }  // namespace bozo

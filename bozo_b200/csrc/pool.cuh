@@ -22,8 +22,10 @@ struct ReserveP {
   int* pos;
   int* slot;
   int* err;
+  unsigned cap;  // M·page
+  FastDiv div_cap, div_page;
 };
-cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st);
+cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launches);
 
 struct ForkP {
   int* table;
@@ -35,6 +37,7 @@ struct ForkP {
   int* copies;
   int* missing;
   int* err;
+  FastDiv div_page;
 };
 cudaError_t launch_paged_fork(const ForkP& p, cudaStream_t st);
 

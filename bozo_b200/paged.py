@@ -165,8 +165,10 @@ def reserve(page_table: Tensor, lengths: Tensor, tokens: Optional[Tensor], refs:
     ⌈(lengths + tokens) / page_size⌉ and M, so pages reserved before are kept.  Free
     pages are given in ascending order, to the sequences in theirs; where there are too
     few, no table row changes.  ``lengths`` is not advanced.  Up to 8192 sequences."""
-    cu, missing, at = _capi.ext().paged_reserve(page_table, lengths, tokens, refs, page_size, rows or 0)
-    return Plan(cu, missing, *(at.unbind(0) if rows is not None else (None,) * 3))
+    if rows is not None and rows < 0:
+        raise ValueError("reserve: rows must not be negative")
+    return Plan._make(_capi.ext().paged_reserve(page_table, lengths, tokens, refs, page_size,
+                                                -1 if rows is None else rows))
 
 
 def fork(page_table: Tensor, lengths: Tensor, parents: Tensor, refs: Tensor, page_size: int, *,
