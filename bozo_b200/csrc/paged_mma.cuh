@@ -98,12 +98,16 @@ __device__ __forceinline__ void widen4(unsigned x, unsigned& p01, unsigned& p23)
   }
 }
 
-// Eight 4-bit codes as pairs of halfs, times the scales s (two halfs): exact, since the
-// product has 6 significant bits and lies between 2^-10 and 2688.
-__device__ __forceinline__ void widen8(unsigned x, unsigned s, unsigned* w) {
+// Eight 4-bit codes as pairs of halfs.
+__device__ __forceinline__ void codes8(unsigned x, unsigned* w) {
   asm("{.reg .b8 a, b, c, d; mov.b32 {a, b, c, d}, %4; cvt.rn.f16x2.e2m1x2 %0, a; cvt.rn.f16x2.e2m1x2 %1, b;"
       " cvt.rn.f16x2.e2m1x2 %2, c; cvt.rn.f16x2.e2m1x2 %3, d;}"
       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(x));
+}
+// … times the scales s (two halfs): exact, since the product has 6 significant bits and
+// lies between 2^-10 and 2688.
+__device__ __forceinline__ void widen8(unsigned x, unsigned s, unsigned* w) {
+  codes8(x, w);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&w[i]), *reinterpret_cast<const __half2*>(&s));
@@ -114,6 +118,19 @@ __device__ __forceinline__ void widen8(unsigned x, unsigned s, unsigned* w) {
 __device__ __forceinline__ unsigned group_pair(unsigned x) {
   unsigned w;
   asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; cvt.rn.f16x2.e4m3x2 %0, l;}" : "=r"(w) : "r"(x));
+  return w;
+}
+__device__ __forceinline__ float2 halves(unsigned x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// τ · unit · kGroupUnit times a group's scale (≤ 448) stays under 65504, and keeps 2^-24
+// of it where the scale is 2^-6 of the row's largest.
+constexpr float kGroupUnit = 0x1p-6f;
+// x and y as halfs, or (rest 1) what that left of them.
+__device__ __forceinline__ unsigned half_or_rest(float x, float y, float rest) {
+  unsigned w;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
+  const float2 h = halves(w);
+  // the half itself where rest is 0: x − 0 · h rounds to it again
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(fmaf(-rest, h.y, y)), "f"(fmaf(-rest, h.x, x)));
   return w;
 }
 template <int N> __device__ __forceinline__ unsigned lds_part(unsigned a) {  // 1 or 2 bytes
@@ -193,7 +210,7 @@ __device__ __forceinline__ float ld_peer(unsigned addr, unsigned rank) {
 }
 
 constexpr int kWarps = 4;
-constexpr int kStages = 3;
+
 
 // Geometry of the kernel for one page type, head width and count of heads.
 template <int DT, int HD, int GP> struct Geo {
@@ -212,10 +229,12 @@ template <int DT, int HD, int GP> struct Geo {
   // against 119), and so are 64 wide bf16 rows, which else take a few registers too
   // many for a third block (a head each, 617 MB: 96.7 against 99.7; eight heads, 309 MB:
   // 68.4 against 74).
-  static constexpr int blocks = HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
+  static constexpr bool lone = four && GP == 1;  // a head each: group scales go to the scores and to τ
+  static constexpr int blocks = four ? (HD == 128 ? (GP == 8 ? 2 : 3) : 4) : HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
   static constexpr bool fold = Fmt<DT>::bf && GP <= 4;  // τ's second parts have rows 4-7 of P
   static constexpr int parts = (fold ? 2 : 1) * kWarps;  // sums that are added at the end
-  static constexpr int warp = kStages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
+  static constexpr int stages = four ? 2 : 3;                // tiles of the ring
+  static constexpr int warp = stages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
 };
 
 // Byte offset of 16-byte piece ch of row r of a K or V tile with R-byte rows.  The
@@ -253,6 +272,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   constexpr bool BF = F::bf;
   constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size, RS = Z::four ? 1 : SZ, GB = Z::gr;
   constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns of S a head, one
+  constexpr bool LONE = Z::lone;
   constexpr int GQ = GP < 4 ? GP : 4;                              // heads whose columns repeat
   constexpr int NS = GP == 8 ? 2 : 1;                              // heads of a lane
   constexpr int NA = WIDE ? 1 : NS, NB = QUAD ? 1 : WIDE ? 3 : BF ? 2 : NS;  // accumulators, operands
@@ -261,7 +281,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   constexpr int kSteps = HD / 16, kTiles = HD / 8;
   // sums that a score's products run in side by side
   constexpr int NC = NA == 1 && kSteps * (BF ? NB : 1) >= 4 ? 2 : 1;
-  constexpr int NK = QUAD ? 1 : 2;      // keys of a lane, of a tile's 16
+  constexpr bool ONE = QUAD || (LONE && T == 2);
+  constexpr int NK = ONE ? 1 : 2;       // keys of a lane, of a tile's 16
   constexpr bool FOLD = Z::fold;
   // 8-bit rows: lane (g, c) reads a quarter of key rows g, g + 8 and an eighth of four value rows
   constexpr int kKB = R / 4 < 16 ? R / 4 : 16, kKL = R / (4 * kKB), kKW = kKB / 4;
@@ -284,17 +305,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   const unsigned p0 = rc.first(piece), p1 = mine ? rc.last(piece) : p0;  // this block's positions
   const unsigned nk = p1 > p0 ? p1 - p0 : 0u;
   float mass[NS], unit[NS], lim[NS];  // P operand: p · unit, renewed where p passes lim (halfs)
-  constexpr int kAcc = WIDE ? HD / 16 : kTiles;
+  constexpr int kAcc = WIDE || LONE ? HD / 16 : kTiles;
   float acc[kAcc][4];
 #pragma unroll
   for (int s = 0; s < NS; ++s) mass[s] = lim[s] = 0.f, unit[s] = 1.f;
 #pragma unroll
   for (int j = 0; j < kAcc; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 
-  const unsigned ring = smem_u32(smb) + warp * kStages * 2 * Z::kv;
-  char* meta = smb + kWarps * kStages * 2 * Z::kv + warp * kStages * Z::meta;
-  unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * kStages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
-  char* lo = smb + kWarps * (kStages * (2 * Z::kv + Z::meta) + GP * Z::pstride * 4) + warp * GP * Z::pstride * 2;  // τ's third parts
+  const unsigned ring = smem_u32(smb) + warp * Z::stages * 2 * Z::kv;
+  char* meta = smb + kWarps * Z::stages * 2 * Z::kv + warp * Z::stages * Z::meta;
+  unsigned* ps = reinterpret_cast<unsigned*>(smb + kWarps * Z::stages * (2 * Z::kv + Z::meta)) + warp * GP * Z::pstride;
+  char* lo = smb + kWarps * (Z::stages * (2 * Z::kv + Z::meta) + GP * Z::pstride * 4) + warp * GP * Z::pstride * 2;  // τ's third parts
   const char* kpages = static_cast<const char*>(p.k);
   const char* vpages = static_cast<const char*>(p.v);
   // Row numbers.  GR > 1: a look-up for GR keys, 32 of them at once, kBatch tiles'
@@ -414,7 +435,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   // read after a barrier: the one before the first tile is worked on, or if the
   // row's tile is among those that are fetched before that, one of their own.
   const bool writes = writes_row(p, rc, piece, hg == 0);
-  const bool early = writes && p.mode == BOZO_MODE_GLOBAL && nk <= (kStages - 1) * kWarps * KT;
+  const bool early = writes && p.mode == BOZO_MODE_GLOBAL && nk <= (Z::stages - 1) * kWarps * KT;
   if (warp == kWarps) {
     if (writes) append_row(p, b, hk, rc.t, lane);
     if (early) __syncthreads();
@@ -426,10 +447,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     float back[NS];
     // the heads, the tile (of T) and the keys whose τ this lane computes; one of the
     // lanes with the same
-    auto head_of = [&](int e) { return QUAD ? (c >> 1) % GQ : WIDE ? 2 * c + e : e * 4 + c % GQ; };
-    auto key_of = [&](int o) { return g + (QUAD ? 8 * (c & 1) : 8 * o); };
+    auto head_of = [&](int e) { return LONE ? 0 : QUAD ? (c >> 1) % GQ : WIDE ? 2 * c + e : e * 4 + c % GQ; };
+    auto key_of = [&](int o) { return g + (QUAD ? 8 * (c & 1) : ONE ? 8 * (c >> 1) : 8 * o); };
     const int copy = WIDE ? 0 : (QUAD ? c >> 1 : c) / GQ, tsel = copy % T;
-    const bool once = copy < T;
+    const bool once = LONE || copy < T;
     const int mrow = (lane & 7) + (lane & 8), mch = lane >> 4;  // row and piece of an 8×8 matrix's row
 
     find(0, cur);
@@ -450,7 +471,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       }
     if (early) __syncthreads();
 #pragma unroll 1
-    for (int k = 0; k < kStages - 1; ++k) feed(k, k);
+    for (int k = 0; k < Z::stages - 1; ++k) feed(k, k);
     __syncthreads();
     if (start(0) < nk) {
       if constexpr (BF) {
@@ -474,7 +495,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       } else {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-          const int h = s * 4 + (g >> 1) % GQ;
+          const int h = LONE ? 0 : s * 4 + (g >> 1) % GQ;
           // as halfs, brought near 1 by a power of two
           float m = 0.f;
           for (int d = c; d < HD; d += 4) m = fmaxf(m, fabsf(sq[h][d]));
@@ -485,7 +506,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           if (c == 0) sback[h] = __uint_as_float((unsigned)(127 + e) << 23);  // every warp the same
           auto pair = [&](int d) {
             const unsigned u = split(sq[h][d] * qs), v = split(sq[h][d + 1] * qs);
-            return __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
+            // a head each: two columns for each quarter of the elements, which have scales of their own
+            return LONE && c != g >> 1 ? 0u : __byte_perm(u, v, g & 1 ? 0x5410 : 0x7632);
           };
 #pragma unroll
           for (int i = 0; i < kSteps; ++i) {
@@ -509,16 +531,16 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
     int slot = 0;
 #pragma unroll 1
     for (int k = 0; start(k) < nk; ++k) {
-      copy_wait<kStages - 2>();
+      copy_wait<Z::stages - 2>();
       __syncwarp();
-      feed(slot == 0 ? kStages - 1 : slot - 1, k + kStages - 1);
+      feed(slot == 0 ? Z::stages - 1 : slot - 1, k + Z::stages - 1);
       const unsigned kt = ring + slot * 2 * Z::kv, vt = kt + Z::kv;
       const char* md = meta + slot * Z::meta;
       const float2* sc = reinterpret_cast<const float2*>(md);
-      slot = slot == kStages - 1 ? 0 : slot + 1;
+      slot = slot == Z::stages - 1 ? 0 : slot + 1;
 #pragma unroll
       for (int q = 0; q < NT / T; ++q) {
-        float s[T][NA][NC][4];
+        float s[T][NA][NC][4], y[LONE ? T : 1][2];
 #pragma unroll
         for (int u = 0; u < T; ++u) {
 #pragma unroll
@@ -546,6 +568,30 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             lds_words<kKW, 8 * R>(at, kb);
             constexpr int NG = GB == 8 ? 2 : 1;  // groups of a lane's elements
             const unsigned ga = lds_part<NG>(gs), gb = lds_part<NG>(gs + 8 * GB);
+            if constexpr (LONE) {
+              // the codes as they are; this lane's two columns are those of its quarter, so
+              // its sums take the quarter's scales (128 wide: two sums, of a group each)
+              static_assert(NC >= NG, "a sum for each group");
+#pragma unroll
+              for (int w = 0; w < kKW; ++w) {
+                const int i = NG == 2 ? w / (kKW / 2) : 0;
+                unsigned x[4], z[4];
+                codes8(ka[w], x);
+                codes8(kb[w], z);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  mma16816<BF>(s[u][0][i], x[2 * h], z[2 * h], x[2 * h + 1], z[2 * h + 1], qb[0][2 * w + h][0],
+                               qb[0][2 * w + h][1]);
+              }
+              const float2 fa = halves(group_pair(ga)), fb = halves(group_pair(gb));
+              y[u][0] = (s[u][0][0][0] + s[u][0][0][1]) * fa.x;
+              y[u][1] = (s[u][0][0][2] + s[u][0][0][3]) * fb.x;
+              if constexpr (NG == 2) {
+                y[u][0] = fmaf(s[u][0][NG - 1][0] + s[u][0][NG - 1][1], fa.y, y[u][0]);
+                y[u][1] = fmaf(s[u][0][NG - 1][2] + s[u][0][NG - 1][3], fb.y, y[u][1]);
+              }
+              continue;
+            }
 #pragma unroll
             for (int w = 0; w < kKW; ++w) {
               const unsigned sel = NG == 2 && w >= kKW / 2 ? 0x1111 : 0x0000;
@@ -583,6 +629,29 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             }
           }
         }
+        float z4[2];
+        if constexpr (LONE) {
+          // the four quarters' sums: each lane is left with its tile's keys
+          if constexpr (T == 4) {
+            const bool up = c & 2, odd = c & 1;
+            float h[2][2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int o = 0; o < 2; ++o)
+                h[i][o] = (up ? y[i + 2][o] : y[i][o]) + __shfl_xor_sync(0xffffffffu, up ? y[i][o] : y[i + 2][o], 2);
+#pragma unroll
+            for (int o = 0; o < 2; ++o)
+              z4[o] = (odd ? h[1][o] : h[0][o]) + __shfl_xor_sync(0xffffffffu, odd ? h[0][o] : h[1][o], 1);
+          } else {  // two tiles: one key each
+            const bool up = c & 2, odd = c & 1;
+            float h[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              h[i] = (up ? y[i][1] : y[i][0]) + __shfl_xor_sync(0xffffffffu, up ? y[i][0] : y[i][1], 2);
+            z4[0] = (odd ? h[1] : h[0]) + __shfl_xor_sync(0xffffffffu, odd ? h[0] : h[1], 1);
+          }
+        }
         const int tile = q * T + tsel;
         const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::live)[tile];
         float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
@@ -611,7 +680,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
 #pragma unroll
           for (int o = 0; o < NK; ++o) {
             float z;
-            if constexpr (QUAD) {  // two lanes have two columns each: they swap halves of the keys
+            if constexpr (LONE) {
+              z = z4[o];
+            } else if constexpr (QUAD) {  // two lanes have two columns each: they swap halves of the keys
               const float z0 = score(e, 0), z1 = score(e, 1);
               const bool odd = c & 1;
               z = (odd ? z1 : z0) + __shfl_xor_sync(0xffffffffu, odd ? z0 : z1, 1);
@@ -619,7 +690,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               z = score(e, o);
             }
             z *= back[e];
-            if constexpr (F::scaled) z *= ks[o];
+            if constexpr (F::scaled) z *= ONE ? (c & 2 ? ks[1] : ks[0]) : ks[o];
             const int key = key_of(o);
             const bool on = (live >> key) & 1;
             const float tau = on ? sigmoid_exp2(z) : 0.f;
@@ -628,12 +699,12 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             const unsigned pos = p0 + start(k) + tile * 16 + key;
             if (p.tau && once && pos >= rc.lo && pos < p1 && head_of(e) < Gh)
               put_tau(p, (size_t)b * p.H + h0 + head_of(e), rc.t, pos, tau);
-            pr[o] = F::scaled ? tau * vs[o] : tau;
+            pr[o] = F::scaled ? tau * (ONE ? (c & 2 ? vs[1] : vs[0]) : vs[o]) : tau;
           }
           if constexpr (!BF) {
             // halfs reach from 2^-24 to 65504: keep the largest p of a head between 1
             // and 4096 by a power of two, what was summed before following it
-            const float pm = fmaxf(pr[0], pr[1]);
+            const float pm = fmaxf(pr[0], pr[NK - 1]);
             if (__any_sync(0xffffffffu, pm > lim[e])) {
               float m = pm;
 #pragma unroll
@@ -649,13 +720,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               f = __shfl_sync(0xffffffffu, f, g % 4 % GQ);  // of this lane's row of O
               if (g / 4 == e || GP <= 4) {
 #pragma unroll
-                for (int j = 0; j < kTiles; ++j)
+                for (int j = 0; j < kAcc; ++j)
 #pragma unroll
                   for (int i = 0; i < 4; ++i) acc[j][i] *= f;
               }
             }
-            pr[0] *= unit[e];
-            pr[1] *= unit[e];
+#pragma unroll
+            for (int o = 0; o < NK; ++o) pr[o] *= LONE ? unit[e] * kGroupUnit : unit[e];
           }
 #pragma unroll
           for (int o = 0; o < NK; ++o) {
@@ -665,7 +736,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               ps[at] = tops(rest, pr[o]);
               reinterpret_cast<unsigned short*>(lo)[at] = (unsigned short)(__float_as_uint(less_top(rest)) >> 16);
             } else {
-              ps[at] = split(pr[o]);
+              ps[at] = LONE ? __float_as_uint(pr[o]) : split(pr[o]);
             }
           }
         }
@@ -675,7 +746,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       for (int u = 0; u < NT; ++u) {
         unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0, l0 = 0, l2 = 0;
         const int h = FOLD ? g & 3 : g;  // the head of rows g and g + 8
-        if (h < GP) {
+        if (!LONE && h < GP) {
           const int i = h * Z::pstride + u * 16 + 2 * c;
           unsigned x[2], y[2];
           lds_words<2, 0>(smem_u32(ps + i), x);
@@ -720,6 +791,43 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               mma16816<BF>(acc[j], a0, a1, a2, a3, w[0], w[1]);
               mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
             }
+          }
+        } else if constexpr (LONE) {
+          // Oᵀ = Vᵀ·Pᵀ: a column pair for each group, τ times the group's scale as a half and the
+          // rest of it; of the products the ones of an element's own group count.  Lane (g, c):
+          // elements 8g … 8g + 7 (32 wide: 4g …) of rows 2c, 2c + 1, 2c + 8, 2c + 9, and columns g
+          float pk[4];
+          lds_words<2, 0>(smem_u32(ps + u * 16 + 2 * c), reinterpret_cast<unsigned*>(pk));
+          lds_words<2, 32>(smem_u32(ps + u * 16 + 2 * c), reinterpret_cast<unsigned*>(pk + 2));
+          const float rest = g & 1 ? 1.f : 0.f;
+          constexpr int kHalves = GB == 8 ? 2 : 1;  // of four groups
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) {
+            const int grp = GB == 2 ? (g >> 1) & 1 : hf * 4 + (g >> 1);
+            const unsigned gs = smem_u32(md) + Z::scales + KT * GB + (u * 16 + 2 * c) * GB + grp;
+            const float2 s01 = halves(group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8));
+            const float2 s89 = halves(group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8));
+            const unsigned b0 = half_or_rest(pk[0] * s01.x, pk[1] * s01.y, rest);
+            const unsigned b1 = half_or_rest(pk[2] * s89.x, pk[3] * s89.y, rest);
+            constexpr int kBytes = GB == 2 ? 2 : 4;  // of a row: two elements each
+            const int byte = hf * (R / 2) + g * kBytes;
+            const unsigned v0 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c, byte >> 4) + (byte & 15);
+            const unsigned v1 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c + 1, byte >> 4) + (byte & 15);
+            unsigned w[4];
+            if constexpr (kBytes == 2) {
+              w[0] = lds_part<2>(v0), w[1] = lds_part<2>(v1), w[2] = lds_part<2>(v0 + 8 * R), w[3] = lds_part<2>(v1 + 8 * R);
+            } else {
+              lds_words<1, 0>(v0, w), lds_words<1, 0>(v1, w + 1), lds_words<1, 8 * R>(v0, w + 2), lds_words<1, 8 * R>(v1, w + 3);
+            }
+            unsigned a[4][4];  // even and odd elements of the first two rows, and of the others
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              codes8((w[2 * i] & 0x0f0f0f0fu) | (w[2 * i + 1] << 4 & 0xf0f0f0f0u), a[2 * i]);
+              codes8((w[2 * i] >> 4 & 0x0f0f0f0fu) | (w[2 * i + 1] & 0xf0f0f0f0u), a[2 * i + 1]);
+            }
+#pragma unroll
+            for (int m = 0; m < kBytes; ++m)
+              mma16816<BF>(acc[hf * 4 + m], a[0][m], a[1][m], a[2][m], a[3][m], b0, b1);
           }
         } else if constexpr (SZ == 0) {
           // lane (g, c): an eighth of rows 2c, 2c + 1, 2c + 8, 2c + 9: HD/8 elements from g·HD/8 on
@@ -801,7 +909,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       for (int o = 4; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
       if (lane < 2 * GQ && warp < kWarps) smass[warp][lane >> 1] = m;
     } else {
-      m = c / GQ < T ? m : 0.f;
+      m = LONE || c / GQ < T ? m : 0.f;
 #pragma unroll
       for (int o = GQ; o < 32; o <<= 1) m += __shfl_xor_sync(0xffffffffu, m, o);
       if (lane < GQ && warp < kWarps) smass[warp][WIDE ? 2 * lane + e : e * 4 + lane] = m;
@@ -824,6 +932,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       for (int e = 0; e < 4; ++e)  // head 2c or 2c + 1, element g or g + 8
         if (2 * c + (e & 1) < Gh && warp < kWarps)
           part[(warp * Gh + 2 * c + (e & 1)) * HD + 16 * j + g + 8 * (e >> 1)] = acc[j][e];
+  } else if constexpr (LONE) {
+    if (c == (GB == 2 ? g >> 2 : g >> 1) && warp < kWarps) {  // the columns of these elements' group
+      const float back = 1.f / (un * kGroupUnit);
+      constexpr int kBytes = GB == 2 ? 2 : 4;
+#pragma unroll
+      for (int j = 0; j < kAcc; ++j) {
+        const int d = j / kBytes * 64 + 2 * kBytes * g + 2 * (j % kBytes);
+        part[warp * HD + d] = (acc[j][0] + acc[j][1]) * back;
+        part[warp * HD + d + 1] = (acc[j][2] + acc[j][3]) * back;
+      }
+    }
   } else if (hrow < Gh && warp < kWarps) {
     const float back = 1.f / un;
 #pragma unroll
