@@ -520,7 +520,9 @@ static int check_paged(const bozo_paged_cache& c, const uint8_t* kg, const uint8
   if (!scaled && (c.k_scale || c.v_scale)) return BOZO_ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages)) & 15)
     return BOZO_ERR_ALIGNMENT;
-  if (four && ((reinterpret_cast<uintptr_t>(kg) | reinterpret_cast<uintptr_t>(vg)) & 15)) return BOZO_ERR_ALIGNMENT;
+  if (four && ((reinterpret_cast<uintptr_t>(kg) | reinterpret_cast<uintptr_t>(vg) |
+                reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale)) & 15))
+    return BOZO_ERR_ALIGNMENT;
   return BOZO_OK;
 }
 

@@ -293,7 +293,10 @@ int head_groups(const PagedP& p) {
 // 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37).  Sequences
 // of different lengths want smaller pieces to even out — twelve an SM, of 2048 keys
 // at least (1024 rows of up to 8192 keys: 164 µs in two to four; 512 rows of up to
-// 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).
+// 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).  4-bit
+// pages' blocks take the longest sequences first, which evens them out by itself: six an
+// SM (1024 rows of up to 8192 keys 80 µs in one piece, 88 in two; 512 rows of up to 16384
+// with four heads 135 in two, 141 in four, 228 in one).
 // Up to eight pieces are joined inside a cluster, which saves a second kernel's
 // 2-3 µs of a call, where the clusters all find their place at once (12 rows of 1024
 // keys in eight: 5.9 µs and 8.2 a call, 6.1 and 10.1 with a second kernel; 192 rows of up
@@ -309,7 +312,8 @@ PagedPlan plan(const PagedP& p, int sms) {
   const long long keys = p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap;
   const long long rows = (long long)p.B * p.Hk * head_groups(p);
   long long s = 3LL * sms / rows;
-  if (p.B > 1) s = std::max(s, std::min((12LL * sms + rows - 1) / rows, keys / 2048));
+  const long long per_sm = mma && p.dt == BOZO_DT_F4E2M1 && p.B <= kSorted && p.mode == BOZO_MODE_GLOBAL ? 6 : 12;
+  if (p.B > 1) s = std::max(s, std::min((per_sm * sms + rows - 1) / rows, keys / 2048));
   s = std::min(s, keys <= (mma ? 256 : 512) ? 1 : (keys + 15 + kMinPiece - 1) / kMinPiece);
   if (mma && s > kCluster && (s <= kCluster + 4 || keys <= 256 * kCluster)) s = kCluster;
   if (!mma && !rows_path(p)) s = std::max(s, (keys + 15 + kMaxPiece - 1) / kMaxPiece);

@@ -9,6 +9,7 @@ namespace bozo {
 
 constexpr int kMinPiece = 128;  // positions of a piece, at least (where there are two)
 constexpr int kHeads = 8;       // query heads of a block in the tensor-core kernel, at most
+constexpr int kSorted = 128;    // sequences that its blocks put in the order of their lengths, at most
 
 // A join that is launched before its pieces are done waits for them here; a block
 // that has no more to start lets it be launched.

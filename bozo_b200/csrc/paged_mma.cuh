@@ -35,6 +35,8 @@
 // (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.
 #pragma once
 
+#include <limits.h>
+
 #include <algorithm>
 #include <atomic>
 #include <utility>
@@ -230,10 +232,14 @@ template <int DT, int HD, int GP> struct Geo {
   // many for a third block (a head each, 617 MB: 96.7 against 99.7; eight heads, 309 MB:
   // 68.4 against 74).
   static constexpr bool lone = four && GP == 1;  // a head each: group scales go to the scores and to τ
-  static constexpr int blocks = four ? (HD == 128 ? (GP == 8 ? 2 : 3) : 4) : HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
+  static constexpr bool turned = four && GP <= 4;  // O turned round: a column for each head's two halfs
+  // 4-bit rows (64 ragged sequences): 64 wide four (a head each 87 µs, with three 91, two 98),
+  // 128 wide three (four heads 141, with four 150, two 152); eight heads one less (157 to 139).
+  static constexpr int blocks = four ? (HD == 128 ? 3 : 4) - (GP == 8) : HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
   static constexpr bool fold = Fmt<DT>::bf && GP <= 4;  // τ's second parts have rows 4-7 of P
   static constexpr int parts = (fold ? 2 : 1) * kWarps;  // sums that are added at the end
-  static constexpr int stages = four ? 2 : 3;                // tiles of the ring
+  static constexpr int stages = four ? 2 : 3;                // tiles of the ring; 4-bit rows' take so long that
+                                                             // two do (64 ragged sequences 104 µs, with three 114)
   static constexpr int warp = stages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
 };
 
@@ -262,7 +268,32 @@ struct MmaGrid {
   int S, G, HG;  // pieces, query heads of a key head, groups of them
   FastDiv div_s, div_hg, div_hk;
   bool clustered;
+  bool sorted;   // the longest sequences' blocks first
 };
+
+// The sequence with `rank` longer ones, of up to kSorted.  With the longest first the
+// blocks that start last are short (64 sequences of up to 8192 keys, 4-bit pages: 94 µs,
+// in their own order 105).
+constexpr int kSortedBlocks = 600;  // more than one wave
+__device__ __forceinline__ int by_length(const PagedP& p, int rank) {
+  __shared__ __align__(16) int len[kSorted];
+  __shared__ int found;
+  const int t = threadIdx.x;
+  if (t < kSorted) len[t] = t < p.B ? __ldg(p.len + t) : INT_MIN;
+  __syncthreads();
+  if (t < p.B) {
+    const int mine = len[t];
+    int before = 0;
+    for (int i = 0; i < p.B; i += 4) {
+      const int4 x = *reinterpret_cast<const int4*>(len + i);
+      before += (x.x > mine) + (x.y > mine) + (x.z > mine) + (x.w > mine);
+      before += (x.x == mine && i < t) + (x.y == mine && i + 1 < t) + (x.z == mine && i + 2 < t) + (x.w == mine && i + 3 < t);
+    }
+    if (before == rank) found = t;
+  }
+  __syncthreads();
+  return found;
+}
 
 // GR: positions from a multiple of GR on that lie in one page (16, 8 or 1).
 template <int DT, int HD, int GP, int GR>
@@ -272,7 +303,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   constexpr bool BF = F::bf;
   constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size, RS = Z::four ? 1 : SZ, GB = Z::gr;
   constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns of S a head, one
-  constexpr bool LONE = Z::lone;
+  constexpr bool LONE = Z::lone, TURN = Z::turned;
   constexpr int GQ = GP < 4 ? GP : 4;                              // heads whose columns repeat
   constexpr int NS = GP == 8 ? 2 : 1;                              // heads of a lane
   constexpr int NA = WIDE ? 1 : NS, NB = QUAD ? 1 : WIDE ? 3 : BF ? 2 : NS;  // accumulators, operands
@@ -296,7 +327,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   const bool clustered = grid.clustered;
   const unsigned row = fast_div(blockIdx.x, grid.div_s), head = fast_div(row, grid.div_hg);
   const int piece = blockIdx.x - row * S, hg = row - head * grid.HG;
-  const int b = fast_div(head, grid.div_hk), hk = head - b * p.Hk;
+  int b = fast_div(head, grid.div_hk);
+  const int hk = head - b * p.Hk;
+  if constexpr (Z::four) {
+    if (grid.sorted) b = by_length(p, b);
+  }
   const int h0 = hk * G + hg * kHeads, Gh = min(kHeads, G - hg * kHeads);  // query heads h0 … h0+Gh−1
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const Reach rc = reach(p, b, S);
@@ -305,7 +340,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   const unsigned p0 = rc.first(piece), p1 = mine ? rc.last(piece) : p0;  // this block's positions
   const unsigned nk = p1 > p0 ? p1 - p0 : 0u;
   float mass[NS], unit[NS], lim[NS];  // P operand: p · unit, renewed where p passes lim (halfs)
-  constexpr int kAcc = WIDE || LONE ? HD / 16 : kTiles;
+  constexpr int kAcc = WIDE || TURN ? HD / 16 : kTiles;
   float acc[kAcc][4];
 #pragma unroll
   for (int s = 0; s < NS; ++s) mass[s] = lim[s] = 0.f, unit[s] = 1.f;
@@ -340,6 +375,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   // The group scales of key u·16 + lane mod 16 (K's by the first 16 lanes, V's by the others)
   // from row rr; zeros without one, as its codes: a product with what a page holds there
   // could be NaN.
+  // (offset of a key's scale, of K and of V: side by side, or for 4 bits all of K's first)
+  auto scale_at = [](int key, int v) { return Z::four ? (v * KT + key) * 4 : key * 8 + v * 4; };
   auto put_groups = [&](char* md, int u, unsigned rr) {
     const unsigned to = smem_u32(md) + Z::scales + (lane >> 4) * KT * GB + (u * 16 + (lane & 15)) * GB;
     const unsigned char* from = (lane < 16 ? p.kg : p.vg) + (rr == kNoRow ? 0 : (size_t)rr * GB);
@@ -353,6 +390,35 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   auto fill = [&](int slot, int k) {
     const unsigned kd = ring + slot * 2 * Z::kv, vd = kd + Z::kv;
     char* md = meta + slot * Z::meta;
+    if constexpr (Z::four && GR == 16) {
+      // a tile of whole pages' parts: rows and both kinds of scales 16 bytes at a time
+      const int at = k % kBatch * kUnits;
+      const unsigned pos = p0 + start(k), have = __ballot_sync(0xffffffffu, cur[0] != kNoRow) >> at;
+      if (pos >= rc.lo && pos + KT <= p1 && (have & ((1u << NT) - 1u)) == (1u << NT) - 1u) {
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const size_t r0 = (size_t)__shfl_sync(0xffffffffu, cur[0], at + u) * R;
+          if constexpr (NCH == 1) {
+            copy16((lane < 16 ? kd : vd) + u * 16 * R + (lane & 15) * R, (lane < 16 ? kpages : vpages) + r0 + (lane & 15) * R, 16);
+          } else {
+            const char *ka = kpages + r0 + lane * 16, *va = vpages + r0 + lane * 16;
+            each<NCH / 2>([&](auto i) {
+              constexpr int it = i;  // the permutation repeats every 8 rows: the places of all rounds are alike
+              copy16<0, it * 512>(kd + (u * 16 + it * 32 / NCH) * R + ring_at<RS, R, false>(lane / NCH, lane % NCH), ka);
+              copy16<0, it * 512>(vd + (u * 16 + it * 32 / NCH) * R + ring_at<RS, R, true>(lane / NCH, lane % NCH), va);
+            });
+          }
+        }
+        constexpr int NS4 = NT * 4, NG4 = NT * GB;  // 16-byte pieces of a tile's scales, group scales
+        const unsigned to = smem_u32(md) + lane * 16;
+        const unsigned rs = __shfl_sync(0xffffffffu, cur[0], at + lane % NS4 / 4);
+        if (lane < 2 * NS4) copy16(to, (lane < NS4 ? p.ks : p.vs) + rs + lane % 4 * 4, 16);
+        const unsigned rg = __shfl_sync(0xffffffffu, cur[0], at + lane % NG4 / GB);
+        if (lane < 2 * NG4) copy16(to + Z::scales, (lane < NG4 ? p.kg : p.vg) + (size_t)rg * GB + lane % GB * 16, 16);
+        if (lane < NT) reinterpret_cast<unsigned short*>(md + Z::live)[lane] = 0xffffu;
+        return;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       // rows of these 16 keys: from r0 on, and with GR 8 from r1 on the last eight
@@ -382,7 +448,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           copy16<back, it * 512>(kd + u * 16 * R + ring_at<RS, R, false>(r, ch), second ? kb - 8 * R : ka);
           copy16<back, it * 512>(vd + u * 16 * R + ring_at<RS, R, true>(r, ch), second ? vb - 8 * R : va);
         });
-        if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
+        if (F::scaled) copy4(smem_u32(md) + scale_at(u * 16 + (lane & 15), lane >> 4),
                              (lane < 16 ? p.ks : p.vs) + whole(lane & 15), 4);
         if constexpr (GB == 2) {  // two rows' at a time, which begin at an even one
           const int r = 2 * (lane & 7);
@@ -410,7 +476,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           }
         }
         const unsigned rr = row_of(lane & 15);
-        if (F::scaled) copy4(smem_u32(md) + ((u * 16 + (lane & 15)) << 3) + (lane >> 4) * 4,
+        if (F::scaled) copy4(smem_u32(md) + scale_at(u * 16 + (lane & 15), lane >> 4),
                              (lane < 16 ? p.ks : p.vs) + (rr == kNoRow ? 0u : rr), rr == kNoRow ? 0 : 4);
         if constexpr (GB > 0) put_groups(md, u, rr);
         const unsigned m = __ballot_sync(0xffffffffu, rr != kNoRow);
@@ -656,8 +722,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
         const unsigned live = reinterpret_cast<const unsigned short*>(md + Z::live)[tile];
         float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
         if constexpr (F::scaled) {
-          const float2 a = sc[tile * 16 + g], c2 = sc[tile * 16 + g + 8];  // a key's and a value's
-          ks[0] = a.x, vs[0] = a.y, ks[1] = c2.x, vs[1] = c2.y;
+          if constexpr (Z::four) {
+            const float* f = reinterpret_cast<const float*>(md) + tile * 16 + g;
+            ks[0] = f[0], ks[1] = f[8], vs[0] = f[KT], vs[1] = f[KT + 8];
+          } else {
+            const float2 a = sc[tile * 16 + g], c2 = sc[tile * 16 + g + 8];  // a key's and a value's
+            ks[0] = a.x, vs[0] = a.y, ks[1] = c2.x, vs[1] = c2.y;
+          }
         }
         // the score of key g + 8·o: a column's sums, or two columns'
         auto score = [&](int e, int o) {
@@ -717,7 +788,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
                 unit[e] = nu;
                 lim[e] = __uint_as_float((unsigned)(127 + ex + 12) << 23);
               }
-              f = __shfl_sync(0xffffffffu, f, g % 4 % GQ);  // of this lane's row of O
+              if (!TURN) f = __shfl_sync(0xffffffffu, f, g % 4 % GQ);  // of this lane's row of O; else its columns' own
               if (g / 4 == e || GP <= 4) {
 #pragma unroll
                 for (int j = 0; j < kAcc; ++j)
@@ -746,7 +817,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       for (int u = 0; u < NT; ++u) {
         unsigned a0 = 0, a1 = 0, a2 = 0, a3 = 0, l0 = 0, l2 = 0;
         const int h = FOLD ? g & 3 : g;  // the head of rows g and g + 8
-        if (!LONE && h < GP) {
+        if (!TURN && h < GP) {
           const int i = h * Z::pstride + u * 16 + 2 * c;
           unsigned x[2], y[2];
           lds_words<2, 0>(smem_u32(ps + i), x);
@@ -792,23 +863,32 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
               mma16816<BF>(acc[j + 1], a0, a1, a2, a3, w[2], w[3]);
             }
           }
-        } else if constexpr (LONE) {
-          // Oᵀ = Vᵀ·Pᵀ: a column pair for each group, τ times the group's scale as a half and the
-          // rest of it; of the products the ones of an element's own group count.  Lane (g, c):
-          // elements 8g … 8g + 7 (32 wide: 4g …) of rows 2c, 2c + 1, 2c + 8, 2c + 9, and columns g
-          float pk[4];
-          lds_words<2, 0>(smem_u32(ps + u * 16 + 2 * c), reinterpret_cast<unsigned*>(pk));
-          lds_words<2, 32>(smem_u32(ps + u * 16 + 2 * c), reinterpret_cast<unsigned*>(pk + 2));
+        } else if constexpr (TURN) {
+          // Oᵀ = Vᵀ·Pᵀ.  Lane (g, c): elements 8g … 8g + 7 (32 wide: 4g …) of rows 2c, 2c + 1,
+          // 2c + 8, 2c + 9, and column g: of a head the half of τ or the rest of it.  With a head
+          // each there is a column pair for each group, τ times the group's scale, and of the
+          // products the ones of an element's own group count; else the values are scaled.
+          unsigned pk[4];
+          const unsigned pa = smem_u32(ps + (LONE ? 0 : (g >> 1) % GP * Z::pstride) + u * 16 + 2 * c);
+          lds_words<2, 0>(pa, pk);
+          lds_words<2, 32>(pa, pk + 2);
           const float rest = g & 1 ? 1.f : 0.f;
           constexpr int kHalves = GB == 8 ? 2 : 1;  // of four groups
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf) {
-            const int grp = GB == 2 ? (g >> 1) & 1 : hf * 4 + (g >> 1);
+            const int grp = LONE ? (GB == 2 ? (g >> 1) & 1 : hf * 4 + (g >> 1)) : GB == 2 ? g >> 2 : hf * 4 + (g >> 1);
             const unsigned gs = smem_u32(md) + Z::scales + KT * GB + (u * 16 + 2 * c) * GB + grp;
-            const float2 s01 = halves(group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8));
-            const float2 s89 = halves(group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8));
-            const unsigned b0 = half_or_rest(pk[0] * s01.x, pk[1] * s01.y, rest);
-            const unsigned b1 = half_or_rest(pk[2] * s89.x, pk[3] * s89.y, rest);
+            const unsigned s01 = group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8);
+            const unsigned s89 = group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8);
+            unsigned b0, b1;
+            if constexpr (LONE) {
+              const float2 f01 = halves(s01), f89 = halves(s89);
+              b0 = half_or_rest(__uint_as_float(pk[0]) * f01.x, __uint_as_float(pk[1]) * f01.y, rest);
+              b1 = half_or_rest(__uint_as_float(pk[2]) * f89.x, __uint_as_float(pk[3]) * f89.y, rest);
+            } else {
+              b0 = __byte_perm(pk[0], pk[1], g & 1 ? 0x5410 : 0x7632);
+              b1 = __byte_perm(pk[2], pk[3], g & 1 ? 0x5410 : 0x7632);
+            }
             constexpr int kBytes = GB == 2 ? 2 : 4;  // of a row: two elements each
             const int byte = hf * (R / 2) + g * kBytes;
             const unsigned v0 = vt + u * 16 * R + ring_at<RS, R, true>(2 * c, byte >> 4) + (byte & 15);
@@ -822,8 +902,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
             unsigned a[4][4];  // even and odd elements of the first two rows, and of the others
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              codes8((w[2 * i] & 0x0f0f0f0fu) | (w[2 * i + 1] << 4 & 0xf0f0f0f0u), a[2 * i]);
-              codes8((w[2 * i] >> 4 & 0x0f0f0f0fu) | (w[2 * i + 1] & 0xf0f0f0f0u), a[2 * i + 1]);
+              const unsigned even = (w[2 * i] & 0x0f0f0f0fu) | (w[2 * i + 1] << 4 & 0xf0f0f0f0u);
+              const unsigned odd = (w[2 * i] >> 4 & 0x0f0f0f0fu) | (w[2 * i + 1] & 0xf0f0f0f0u);
+              if constexpr (LONE) {
+                codes8(even, a[2 * i]);
+                codes8(odd, a[2 * i + 1]);
+              } else {
+                widen8(even, i ? s89 : s01, a[2 * i]);
+                widen8(odd, i ? s89 : s01, a[2 * i + 1]);
+              }
             }
 #pragma unroll
             for (int m = 0; m < kBytes; ++m)
@@ -932,15 +1019,17 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       for (int e = 0; e < 4; ++e)  // head 2c or 2c + 1, element g or g + 8
         if (2 * c + (e & 1) < Gh && warp < kWarps)
           part[(warp * Gh + 2 * c + (e & 1)) * HD + 16 * j + g + 8 * (e >> 1)] = acc[j][e];
-  } else if constexpr (LONE) {
-    if (c == (GB == 2 ? g >> 2 : g >> 1) && warp < kWarps) {  // the columns of these elements' group
-      const float back = 1.f / (un * kGroupUnit);
+  } else if constexpr (TURN) {
+    // this lane's columns: of these elements' group, or of head c
+    if ((LONE ? c == (GB == 2 ? g >> 2 : g >> 1) : c < Gh) && warp < kWarps) {
+      const float back = 1.f / (LONE ? unit[0] * kGroupUnit : unit[0]);
       constexpr int kBytes = GB == 2 ? 2 : 4;
 #pragma unroll
       for (int j = 0; j < kAcc; ++j) {
         const int d = j / kBytes * 64 + 2 * kBytes * g + 2 * (j % kBytes);
-        part[warp * HD + d] = (acc[j][0] + acc[j][1]) * back;
-        part[warp * HD + d + 1] = (acc[j][2] + acc[j][3]) * back;
+        float* to = part + (warp * Gh + (LONE ? 0 : c)) * HD + d;
+        to[0] = (acc[j][0] + acc[j][1]) * back;
+        to[1] = (acc[j][2] + acc[j][3]) * back;
       }
     }
   } else if (hrow < Gh && warp < kWarps) {
@@ -1012,6 +1101,8 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
     if (e != cudaSuccess) return e;
     if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
+  const bool sorted = Z::four && p.mode == BOZO_MODE_GLOBAL && p.B > 1 && p.B <= kSorted && !pl.clustered &&
+                      (long long)p.B * p.Hk * HG * pl.S > kSortedBlocks;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hk * HG * pl.S));
   cfg.blockDim = dim3(kWarps * 32 + (p.kn.p ? 32 : 0));
@@ -1022,7 +1113,7 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
   at.val.clusterDim = {(unsigned)pl.S, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = pl.clustered ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, p, MmaGrid{pl.S, G, HG, make_fastdiv(pl.S), make_fastdiv(HG), make_fastdiv(p.Hk), pl.clustered});
+  return cudaLaunchKernelEx(&cfg, kern, p, MmaGrid{pl.S, G, HG, make_fastdiv(pl.S), make_fastdiv(HG), make_fastdiv(p.Hk), pl.clustered, sorted});
 }
 template <int DT, int HD, int GP>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {

@@ -244,7 +244,7 @@ int bozo_tension_decode(const bozo_tension_decode_args* args, void* stream);
 typedef struct {
   void* k_pages;          /* [pages, kv_heads, page_size, HD] contiguous, 16-byte aligned */
   void* v_pages;
-  float* k_scale;         /* [pages, kv_heads, page_size] for 8- and 4-bit rows, else NULL */
+  float* k_scale;         /* [pages, kv_heads, page_size] for 8- and (16-byte aligned) 4-bit rows, else NULL */
   float* v_scale;
   int32_t dtype;          /* bozo_dtype, BOZO_DT_F8E4M3, BOZO_DT_I8 or BOZO_DT_F4E2M1 */
   int32_t pages, kv_heads, page_size, HD;
