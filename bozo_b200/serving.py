@@ -17,33 +17,48 @@ a slot.  ``PagedStepGraph`` replays the step as a CUDA graph: positions and page
 tables are read on the device, so admitting, releasing and growing between
 replays need no new capture.  ``generate`` is continuous batching on top: a
 queue of prompts over the slots, ``decode.generate``'s sampling for each.
+``beam_search`` keeps several hypotheses of each prompt (``BeamState``): a step
+takes their pages, feeds their tokens, chooses the best continuations and
+reorders tables and caches on the device, in one CUDA graph a token.
 
 A step's logits equal those of ``decode.step`` for each sequence on its own, past
 ``max_seq_len`` tokens where the page size divides it: global layers reach whole
 pages, so up to ``page_size − 1`` keys more otherwise.
 The caches may be held in 8 bits (``cache_dtype`` e4m3 or int8), a quarter of
-fp32 and half of bf16 plus 4 bytes a row.
+fp32 and half of bf16 plus 4 bytes a row, or in 4 (``torch.float4_e2m1fn_x2``), half
+of that plus a byte for 16 elements.
 """
 from __future__ import annotations
 
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
 
-from . import _capi, decode, ops, paged
+from . import _capi, beam, decode, ops, paged
 
-__all__ = ["PagedState", "PagedStepGraph", "admit", "extend", "step", "generate"]
+__all__ = ["PagedState", "PagedStepGraph", "BeamState", "admit", "extend", "step", "generate", "beam_search"]
 
 
 class _Layer:
     """One layer's pages (and scales)."""
 
     def __init__(self, pages: int, heads: int, page: int, width: int, dtype: torch.dtype, dev):
-        self.k, self.v = (torch.zeros(pages, heads, page, width, dtype=dtype, device=dev) for _ in "kv")
-        eight = dtype in (torch.float8_e4m3fn, torch.int8)
-        self.scales = {n: torch.zeros(pages, heads, page, device=dev) if eight else None
+        four = dtype == torch.float4_e2m1fn_x2
+        shape = (pages, heads, page, width // 2 if four else width)
+        self.k, self.v = (torch.zeros(shape, dtype=torch.uint8 if four else dtype, device=dev) for _ in "kv")
+        scaled = four or dtype in (torch.float8_e4m3fn, torch.int8)
+        self.scales = {n: torch.zeros(pages, heads, page, device=dev) if scaled else None
                        for n in ("k_scale", "v_scale")}
+        if four:
+            self.k, self.v = self.k.view(dtype), self.v.view(dtype)
+            self.scales.update({n: torch.zeros(pages, heads, page, width // 16, dtype=torch.float8_e4m3fn, device=dev)
+                                for n in ("k_group", "v_group")})
+
+    @property
+    def pools(self) -> List[Tensor]:
+        """Everything that is held by pages."""
+        return [self.k, self.v] + [s for s in self.scales.values() if s is not None]
 
 
 class PagedState:
@@ -75,6 +90,8 @@ class PagedState:
         self.model, self.slots, self.max_len, self.page_size = model, slots, max_len, page_size
         self.dtype = dtype or next(model.parameters()).dtype
         cache_dtype = cache_dtype or self.dtype
+        if cache_dtype == torch.float4_e2m1fn_x2 and cfg.head_dim % 16:
+            raise ValueError("4-bit caches hold heads of a multiple of 16 elements")
         ring = -(-(cfg.window + 1) // page_size)
         reach = -(-min(max_len, cfg.max_seq_len) // page_size)
         pages = slots * reach if pages is None else pages
@@ -144,8 +161,13 @@ class PagedState:
 
     # ── device side ──
 
+    @property
+    def tables(self) -> dict:
+        """The page tables: of the global layers (``True``) and of the local ones."""
+        return {True: self.global_table, False: self.local_table}
+
     def table(self, li: int) -> Tensor:
-        return self.global_table if self.model.blocks[li].global_layer else self.local_table
+        return self.tables[bool(self.model.blocks[li].global_layer)]
 
     def _write(self, li: int, table: Tensor, start: Tensor, cu: Tensor, k: Tensor, v: Tensor) -> None:
         lay = self.layers[li]
@@ -175,6 +197,19 @@ def admit(state: PagedState, prompts: Sequence[Sequence[int]]):
     start = torch.zeros_like(n)
     # the padded forward's rows that are tokens (its padding comes after them)
     rows = torch.cat([torch.arange(m) + i * T for i, m in enumerate(lens)]).to(dev)
+    logits = _prefill(state, ids, n.long(), rows, {g: t[at] for g, t in state.tables.items()}, start, cu)
+    state.lengths[at] = n
+    for s, m in zip(slots, lens):
+        state._len[s] = m
+    return slots, logits
+
+
+def _prefill(state: PagedState, ids: Tensor, n: Tensor, rows: Tensor, tables: dict, start: Tensor,
+             cu: Tensor) -> Tensor:
+    """The model over padded prompts ``ids [B, T]`` of ``n [B]`` tokens, whose packed rows
+    are ``rows`` of the flattened batch: their keys and values into the caches, the
+    logits ``[B, V]`` after each."""
+    model, T = state.model, ids.shape[1]
     packed = len(rows) == ids.numel()
     x = model.embedding(ids)
     if model.pos_embedding is not None:
@@ -183,14 +218,10 @@ def admit(state: PagedState, prompts: Sequence[Sequence[int]]):
         h = blk.pre_norm(x)
         _, k, v = blk.tension.project(h)
         k, v = (y.flatten(0, 1) if packed else y.flatten(0, 1)[rows] for y in (k, v))
-        state._write(li, state.table(li)[at], start, cu, k, v)
+        state._write(li, tables[bool(blk.global_layer)], start, cu, k, v)
         x = blk.ffn(blk._osc(blk.tension(h)))
-    last = x[torch.arange(len(lens), device=dev), n.long() - 1]
-    logits = model.lm_head(model.final_norm(last))
-    state.lengths[at] = n
-    for s, m in zip(slots, lens):
-        state._len[s] = m
-    return slots, logits
+    last = x[torch.arange(len(ids), device=ids.device), n - 1]
+    return model.lm_head(model.final_norm(last))
 
 
 @torch.no_grad()
@@ -415,4 +446,186 @@ def generate(model, prompts: Sequence[Sequence[int]], max_new: int = 200, temp: 
         logits = run(tok).clone()
         for slot in list(pending):
             take(slot, logits[slot])
+    return out
+
+
+class BeamState(PagedState):
+    """``beams`` hypotheses of each of up to ``prompts`` prompts, searched together on the
+    device: hypothesis k of prompt n has slot n · beams + k.
+
+    The pages of both kinds of layers are counted on the device (``paged.reserve``,
+    ``paged.fork``): hypotheses share the full pages of what they have in common, and
+    the rings of local layers move or are copied with them.  ``start`` takes the
+    prompts, ``advance`` adds a token to every hypothesis (a replayed CUDA graph unless
+    ``graph=False``), ``results`` reads what was found.
+
+    max_len : longest prompt with its new tokens; with global layers at most
+              ``max_seq_len``, since shared pages cannot be rings.
+    eos     : token that ends a hypothesis, or ``None``.
+    """
+
+    def __init__(self, model, prompts: int, beams: int, max_len: int, *, eos: Optional[int] = None,
+                 page_size: int = 16, dtype: Optional[torch.dtype] = None,
+                 cache_dtype: Optional[torch.dtype] = None, graph: bool = True, warmup: int = 2):
+        cfg = model.cfg
+        if prompts < 1 or not 1 <= beams <= 32 or beams > cfg.vocab_size:
+            raise ValueError("beam search takes at least one prompt and 1 to 32 beams, no more than tokens")
+        if eos is not None and not 0 <= eos < cfg.vocab_size:
+            raise ValueError(f"eos must be a token, got {eos}")
+        if any(b.global_layer for b in model.blocks) and max_len > cfg.max_seq_len:
+            raise ValueError(f"beam search holds whole sequences: {max_len} tokens pass max_seq_len {cfg.max_seq_len}")
+        super().__init__(model, prompts * beams, max_len, page_size=page_size, dtype=dtype, cache_dtype=cache_dtype)
+        dev = self.lengths.device
+        self.prompts, self.beams, self.eos = prompts, beams, eos
+        # by kind of layer (global or not): what its pages hold, and how many rows hold a page
+        self.pools = {g: [p for lay, b in zip(self.layers, model.blocks) if bool(b.global_layer) == g
+                          for p in lay.pools] for g in sorted({bool(b.global_layer) for b in model.blocks})}
+        self.refs = {g: torch.zeros(p[0].shape[0], dtype=torch.int32, device=dev) for g, p in self.pools.items()}
+        self.local_table.fill_(-1)  # pages of rings, too, go from hypothesis to hypothesis
+        self.tokens = torch.zeros(self.slots, dtype=torch.long, device=dev)
+        self.scores = torch.zeros(prompts, beams, device=dev)
+        self.done = None if eos is None else torch.zeros(prompts, beams, dtype=torch.bool, device=dev)
+        # what each step chose: tokens, and the slots that were continued
+        self.chosen = torch.zeros(max_len, 2, self.slots, dtype=torch.long, device=dev)
+        self.steps = torch.zeros(1, dtype=torch.long, device=dev)
+        self.taken = 0
+        self._graph = None
+        if graph:
+            # nothing is held yet: every slot is idle, and no page moves
+            side = torch.cuda.Stream(dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                for _ in range(warmup):
+                    self._advance()
+                    self.steps.zero_()
+            torch.cuda.current_stream(dev).wait_stream(side)
+            captured = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(captured):
+                self._advance()
+            self._graph = captured
+        self.taken = 0
+
+    def release(self, slot: int) -> None:
+        raise RuntimeError("a beam search's slots are given up together: start() takes new prompts")
+
+    @torch.no_grad()
+    def start(self, prompts: Sequence[Sequence[int]]) -> None:
+        """Take new prompts (lists of ids of 1 to ``max_seq_len``, as many as there is room
+        for); what was held before is given up."""
+        K, dev = self.beams, self.lengths.device
+        lens = [len(p) for p in prompts]
+        if len(prompts) != self.prompts or min(lens) < 1 or max(lens) > min(self.max_len, self.model.cfg.max_seq_len):
+            raise ValueError(f"start: {self.prompts} prompts of 1 to {min(self.max_len, self.model.cfg.max_seq_len)} "
+                             "ids are wanted")
+        T = max(lens)
+        ids = torch.tensor([list(p) + [0] * (T - m) for p, m in zip(prompts, lens)], device=dev)
+        n = torch.tensor(lens, device=dev)
+        for g in self.pools:
+            self.tables[g].fill_(-1)
+            self.refs[g].zero_()
+        self.lengths.fill_(-1)
+        self.lengths[::K] = 0
+        tokens = torch.zeros(self.slots, dtype=torch.int32, device=dev)
+        tokens[::K] = n.int()
+        for g in self.pools:
+            plan = self._reserve(g, tokens, rows=sum(lens))
+        rows = plan.seq.long() // K * T + plan.pos  # of the padded batch
+        logits = _prefill(self, ids, n, rows, self.tables, self.lengths, plan.cu_rows)
+        self.lengths[::K] = n.int()
+        self.scores.fill_(float("-inf"))
+        self.scores[:, 0] = 0
+        if self.done is not None:
+            self.done.zero_()
+        self.steps.zero_()
+        self.taken, self.longest = 0, T
+        self._choose(logits.repeat_interleave(K, 0))
+
+    def advance(self) -> None:
+        """Feed every hypothesis its token and choose the best continuations."""
+        if not self.taken:
+            raise RuntimeError("advance: start() takes the prompts first")
+        self._check(self.longest + self.taken)
+        if self._graph is not None:
+            self._graph.replay()
+            self.taken += 1
+        else:
+            self._advance()
+        ops.check_device_error(self.lengths.device)
+
+    def _reserve(self, glob: bool, tokens: Optional[Tensor], rows: Optional[int] = None) -> paged.Plan:
+        return paged.reserve(self.tables[glob], self.lengths, tokens, self.refs[glob], self.page_size, rows=rows)
+
+    @torch.no_grad()
+    def _advance(self) -> None:
+        for g in self.pools:
+            self._reserve(g, None)
+        self._choose(_step(self, self.tokens, False))
+
+    def _choose(self, logits: Tensor) -> None:
+        scores, tokens, rows = beam.select(logits, self.scores, done=self.done, eos=self.eos)
+        rows = rows.view(-1)
+        for g, pools in self.pools.items():
+            copies, _ = paged.fork(self.tables[g], self.lengths, rows, self.refs[g], self.page_size, share=g)
+            paged.copy_pages(pools, copies)
+        at = rows.long()
+        self.lengths.copy_(self.lengths[at])
+        self.scores.copy_(scores)
+        if self.done is not None:
+            self.done.copy_(self.done.view(-1)[at].view_as(scores) | (tokens == self.eos))
+        self.tokens.copy_(tokens.view(-1))
+        self.chosen.index_copy_(0, self.steps, torch.stack([self.tokens, at]).unsqueeze(0))
+        self.steps += 1
+        if not torch.cuda.is_current_stream_capturing():
+            self.taken += 1
+
+    def results(self, length_penalty: float = 0.0) -> List[List[Tuple[List[int], float]]]:
+        """For each prompt its hypotheses' new ids (up to and with ``eos``) and scores, each
+        the sum of log probabilities over (number of new ids) ^ ``length_penalty``, best
+        first."""
+        tokens, rows = self.chosen[:self.taken].cpu().unbind(1)
+        scores, out = self.scores.tolist(), []
+        for n in range(self.prompts):
+            found = []
+            for k in range(self.beams):
+                r, ids = n * self.beams + k, []
+                for t in range(self.taken - 1, -1, -1):
+                    ids.append(int(tokens[t, r]))
+                    r = int(rows[t, r])
+                ids.reverse()
+                if self.eos in ids:
+                    ids = ids[:ids.index(self.eos) + 1]
+                found.append((ids, scores[n][k] / len(ids) ** length_penalty))
+            out.append(sorted(found, key=lambda x: -x[1]))
+        return out
+
+
+def beam_search(model, prompts: Sequence[Sequence[int]], beams: int = 4, max_new: int = 64, *,
+                eos: Optional[int] = None, length_penalty: float = 0.0, batch: int = 16,
+                dtype: Optional[torch.dtype] = None, cache_dtype: Optional[torch.dtype] = None,
+                page_size: int = 16, graph: bool = True) -> List[List[Tuple[List[int], float]]]:
+    """The ``beams`` best continuations of each prompt by beam search, ``batch`` prompts at
+    a time: for each prompt ``(new ids, score)``, best first, as ``BeamState.results``
+    returns them.  Prompts longer than ``max_seq_len − max_new`` keep their last ids where
+    the model has global layers or learned positions."""
+    model.eval()
+    if max_new < 1:
+        raise ValueError("max_new must be at least 1")
+    cfg, out = model.cfg, []
+    bounded = not cfg.use_rope or any(b.global_layer for b in model.blocks)
+    limit = cfg.max_seq_len - max_new + 1 if bounded else cfg.max_seq_len
+    if limit < 1:
+        raise ValueError(f"{max_new} new tokens do not fit max_seq_len {cfg.max_seq_len}")
+    ctx = [list(p)[-limit:] for p in prompts]
+    for i in range(0, len(ctx), batch):
+        part = ctx[i:i + batch]
+        state = BeamState(model, len(part), beams, max(map(len, part)) + max_new - 1, eos=eos,
+                          page_size=page_size, dtype=dtype, cache_dtype=cache_dtype, graph=graph and max_new > 1)
+        state.start(part)
+        for step_ in range(1, max_new):
+            # the host looks at the ended hypotheses now and then
+            if eos is not None and step_ % 8 == 0 and bool(state.done.all()):
+                break
+            state.advance()
+        ops.poll_device_error(state.lengths.device)
+        out += state.results(length_penalty)
     return out

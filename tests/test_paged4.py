@@ -253,6 +253,18 @@ def test_decode_rows_in_two_pieces(H, Hk, HD):
 
 
 @gpu
+@pytest.mark.parametrize("B,H,Hk,HD", [(64, 10, 10, 64), (128, 5, 5, 32), (129, 5, 5, 32), (100, 28, 7, 128)])
+def test_decode_many_rows_of_uneven_lengths(B, H, Hk, HD):
+    """More blocks than run at a time, sequences of equal lengths and idle ones among them."""
+    lengths = [(7 * i * i) % 90 - (i % 11 == 3) * 200 for i in range(B)]
+    lengths = [max(t, -1) for t in lengths]
+    pool = Pool4(B, Hk, HD, 16, 6)
+    hist = fill(pool, [t + 1 for t in lengths], Hk, HD, BF16, None, B)
+    q = torch.randn(B, H, HD, device="cuda", dtype=BF16)
+    check_decode(pool, lengths, hist, q, window=None, tau_window=50)
+
+
+@gpu
 @pytest.mark.parametrize("shift", [-60.0, -25.0, 0.0, 40.0])
 def test_decode_scores_far_from_zero(shift):
     pool = Pool4(2, 1, 64, 16, 10)
