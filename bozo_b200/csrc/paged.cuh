@@ -139,8 +139,9 @@ __device__ __forceinline__ float code_value(unsigned char c, int dt) {
 
 // 4-bit rows.  The row's scale is a power of two, so the group scale is a correctly
 // rounded sixth and the code a correctly rounded quotient by a few bits: both are a
-// product with the rounded reciprocal and one correction by its exact remainder, as
-// in div_top (checked for every significand by 6 and by 8 … 15, those of an e4m3).
+// product with a reciprocal and one correction by its exact remainder, as in div_top
+// (checked for every significand by 6 and by 8 … 15, those of an e4m3, with reciprocals
+// up to two units off: the approximate one is at most one).
 constexpr float kTinyRow4 = 0x1p-80f;  // below it the remainders would lose bits
 struct Row4 {
   float scale, inv, most;  // the row's scale, its inverse, the largest group scale
@@ -168,14 +169,13 @@ struct Row4 {
       c = (unsigned char)__nv_cvt_float_to_fp8(fminf(__fmul_rn(sixth, inv), most), __NV_SATFINITE, __NV_E4M3);
       if (c) {
         unit = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3))) * scale;
-        recip = __frcp_rn(unit);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(recip) : "f"(unit));
       }
     }
     return c;
   }
-  // x / unit
+  // x / unit, anything in a bad row
   __device__ __forceinline__ float in_units(float x, float unit, float recip) const {
-    if (bad) return 0.f;
     const float q = __fmul_rn(x, recip);
     return __fmaf_rn(__fmaf_rn(q, unit, -x), -recip, q);  // in this order −0 stays −0
   }
@@ -244,7 +244,7 @@ struct NewRow {
 #pragma unroll
         for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         const unsigned char c = r.group(m, unit, recip);
-        const float y = r.in_units(x[i], unit, recip), z = __shfl_down_sync(0xffffffffu, y, 1);
+        const float y = r.bad ? 0.f : r.in_units(x[i], unit, recip), z = __shfl_down_sync(0xffffffffu, y, 1);
         if (d >= p.HD) continue;
         if (lane % 16 == 0) groups[row * (p.HD / 16) + d / 16] = c;
         if (lane % 2 == 0) static_cast<unsigned char*>(pages)[(row * p.HD + d) / 2] = (unsigned char)pack4(y, z);
