@@ -19,32 +19,32 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
 constexpr int kSmallPool = 16384;  // pages that one block counts
 
-// Inclusive scan of v over the block; `total`: the sum.  `tmp`: 32 words.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* tmp,
-                                                         unsigned long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Sums over the block's threads, one barrier each: every warp adds the warps' totals up
+// for itself, and two buffers take turns, so that none is written while it is read.
+struct Scan {
+  unsigned long long tmp[2][32];
+  // v's inclusive sum; `total`: of all threads.  `turn`: the same count in every thread.
+  __device__ __forceinline__ unsigned long long run(unsigned long long v, unsigned long long& total, int& turn) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned long long* t = tmp[turn++ & 1];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) tmp[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    unsigned long long w = tmp[lane];
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) t[warp] = v;
+    __syncthreads();
+    unsigned long long w = t[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned long long u = __shfl_up_sync(0xffffffffu, w, o);
       if (lane >= o) w += u;
     }
-    tmp[lane] = w;
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const unsigned long long before = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+    return warp ? v + before : v;
   }
-  __syncthreads();
-  total = tmp[31];
-  if (warp) v += tmp[warp - 1];
-  __syncthreads();
-  return v;
-}
+};
 
 // The last i in [0, n) with sums[i] ≤ x (sums[0] ≤ x, non-decreasing).
 __device__ __forceinline__ int find(const int* sums, int n, int x) {
@@ -56,28 +56,52 @@ __device__ __forceinline__ int find(const int* sums, int n, int x) {
   return lo;
 }
 
-// A thread's run of consecutive pages, of a block's part of the pool.
+// The pool is shared out in order: a run of consecutive pages a warp, in words of 32 that
+// all its lanes read together.
 struct Run {
-  int lo, hi;
+  int from, to, words;
   __device__ Run(int pages, unsigned rank, unsigned blocks) {
-    const int each = (int)(((long long)pages + (long long)blocks * kThreads - 1) / ((long long)blocks * kThreads));
-    lo = (int)min((long long)pages, (long long)each * (rank * kThreads + threadIdx.x));
-    hi = min(pages, lo + each);
+    const long long warps = (long long)blocks * (kThreads / 32), warp = (long long)rank * (kThreads / 32) + (threadIdx.x >> 5);
+    words = (int)((pages + warps * 32 - 1) / (warps * 32));
+    from = (int)min((long long)pages, warp * words * 32);
+    to = (int)min((long long)pages, from + (long long)words * 32);
   }
-  __device__ int count(const int* refs) const {
-    int n = 0;
+  __device__ unsigned word(const int* refs, int p) const {
+    const int lane = threadIdx.x & 31;
+    return __ballot_sync(0xffffffffu, p + lane < to && refs[p + lane] == 0);
+  }
+  // the warp's free pages; `mask`: which of word `lane` are
+  __device__ int count(const int* refs, unsigned& mask) const {
+    int n = 0, i = 0;
+    mask = 0;
 #pragma unroll 8
-    for (int p = lo; p < hi; ++p) n += refs[p] == 0;
+    for (int p = from; p < to; p += 32, ++i) {
+      const unsigned b = word(refs, p);
+      n += __popc(b);
+      if (i == (int)(threadIdx.x & 31)) mask = b;
+    }
     return n;
+  }
+  // f(rank, page) for its free pages of rank < want, the first of which has rank `before`
+  template <typename F>
+  __device__ void give(const int* refs, unsigned mask, int n, int before, int want, F f) const {
+    const int lane = threadIdx.x & 31;
+    if (n == 0) return;
+    for (int p = from, i = 0; p < to && before < want; p += 32, ++i) {
+      const unsigned b = i < 32 ? __shfl_sync(0xffffffffu, mask, i) : word(refs, p);
+      const int rank = before + __popc(b & ((1u << lane) - 1u));
+      if (b >> lane & 1 && rank < want) f(rank, p + lane);
+      before += __popc(b);
+    }
   }
 };
 
-// From each thread's free pages, those before its own and in all; `count`: one word of
+// From each warp's free pages, those before its own and in all; `count`: one word of
 // shared memory.  With more than one block the cluster is synchronised in between.
-__device__ __forceinline__ void scan_free(int mine, int* count, unsigned long long* tmp, int& before, int& all) {
+__device__ __forceinline__ void scan_free(int mine, int* count, Scan& scan, int& turn, int& before, int& all) {
   cg::cluster_group cl = cg::this_cluster();
   unsigned long long total;
-  before = (int)block_scan(mine, tmp, total) - mine;
+  before = (int)scan.run((threadIdx.x & 31) == 0 ? mine : 0, total, turn) - mine;
   all = (int)total;
   if (cl.num_blocks() > 1) {
     if (threadIdx.x == 0) *count = all;
@@ -96,16 +120,9 @@ __device__ __forceinline__ void sync_all() {
   else __syncthreads();
 }
 
-// f(rank, page) for this thread's free pages of rank < want, in ascending order.
-template <typename F>
-__device__ __forceinline__ void give(const int* refs, Run run, int rank, int want, F f) {
-  for (int p = run.lo; p < run.hi && rank < want; ++p)
-    if (refs[p] == 0) f(rank++, p);
-}
-
 // Where row i of the packed new tokens goes: sequence b, which has the rows [first, next).
-__device__ __forceinline__ void place(const ReserveP& p, int i, int b, int first, int next, int& at, int& slot) {
-  const long long t = p.lengths[b], pos = t + (i - first);
+__device__ __forceinline__ void place(const ReserveP& p, int i, int b, int len, int first, int next, int& at, int& slot) {
+  const long long t = len, pos = t + (i - first);
   at = (int)pos;
   slot = -1;
   if (pos < t + (next - first) - (long long)p.cap || pos > 0x7fffffffLL) return;
@@ -125,12 +142,15 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
   int* off = sm;               // wanted pages before each sequence [B + 1]
   int* cu = off + p.B + 1;     // new tokens before it [B + 1]
   int* col = cu + p.B + 1;     // its first new column [B]
-  __shared__ unsigned long long tmp[32];
+  int* len = col + p.B;        // the tokens it holds [B]
+  __shared__ Scan scan;
+  int turn = 0;
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned rank = cl.block_rank();
   const Run run(p.P, rank, cl.num_blocks());
-  const int mine = run.count(p.refs);
+  unsigned mask;
+  const int mine = run.count(p.refs, mask);
   unsigned long long carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
@@ -138,6 +158,7 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
     if (b < p.B) {
       const int t = p.lengths[b];
       n = p.tokens ? max(0, p.tokens[b]) : 1;
+      len[b] = t;
       if (t < 0) n = 0;
       if (n > 0x7fffffff / p.B) {  // the sums are held in 31 bits
         atomicCAS(p.err, 0, kErrPaged | 1);
@@ -152,7 +173,7 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
     }
     unsigned long long total;
     const unsigned long long v = (unsigned long long)(unsigned)want << 32 | (unsigned)n;
-    const unsigned long long before = carry + block_scan(v, tmp, total) - v;
+    const unsigned long long before = carry + scan.run(v, total, turn) - v;
     if (b < p.B) {
       off[b] = (int)(before >> 32);
       cu[b] = (int)(unsigned)before;
@@ -170,9 +191,9 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
     for (int b = threadIdx.x; b <= p.B; b += kThreads) p.cu[b] = cu[b];
   int before = 0, all = 0;
   if (want) {
-    scan_free(mine, &count, tmp, before, all);  // every block has read the table by now
+    scan_free(mine, &count, scan, turn, before, all);  // every block has read the table by now
     if (want <= all)
-      give(p.refs, run, before, want, [&](int i, int page) {
+      run.give(p.refs, mask, mine, before, want, [&](int i, int page) {
         const int b = find(off, p.B, i);
         p.table[b * p.ts + col[b] + i - off[b]] = page;
         p.refs[page] = 1;
@@ -185,7 +206,7 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
     int b = -1, at = -1, slot = -1;
     if (i < rows) {
       b = find(cu, p.B, (int)i);
-      place(p, (int)i, b, cu[b], cu[b + 1], at, slot);
+      place(p, (int)i, b, len[b], cu[b], cu[b + 1], at, slot);
     }
     p.seq[i] = b;
     p.pos[i] = at;
@@ -218,7 +239,7 @@ __global__ void __launch_bounds__(kPlaceThreads) paged_places(ReserveP p) {
       next = p.cu[b + 1];
     }
     seq[k] = b;
-    place(p, (int)i, b, first, next, at[k], slot[k]);
+    place(p, (int)i, b, p.lengths[b], first, next, at[k], slot[k]);
   }
   if (i0 + 4 <= p.rows && !((reinterpret_cast<uintptr_t>(p.seq) | reinterpret_cast<uintptr_t>(p.pos) | reinterpret_cast<uintptr_t>(p.slot)) & 15)) {
     reinterpret_cast<int4*>(p.seq + i0)[0] = make_int4(seq[0], seq[1], seq[2], seq[3]);
@@ -238,10 +259,12 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
   int* parent = sm;               // of each new row, −1 for none [B]
   int* children = parent + p.B;   // of each old row [B]
   int* eldest = children + p.B;   // the first of them [B]
-  int* full = eldest + p.B;       // its columns that its children share [B]
-  int* off = full + p.B;          // pages wanted before each new row [B + 1]
+  int* full = eldest + p.B;       // its columns that its children share [B],
+  int* held = full + p.B;         // and those in use [B]
+  int* off = held + p.B;          // pages wanted before each new row [B + 1]
   int* old = off + p.B + 1;       // `tile` columns of the table [B][tile]
-  __shared__ unsigned long long tmp[32];
+  __shared__ Scan scan;
+  int turn = 0;
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
@@ -253,13 +276,16 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
       old[i] = c < p.M ? __ldcg(p.table + r * p.ts + c) : -1;
     }
   };
+  const int x0 = (int)threadIdx.x < p.B ? p.parents[threadIdx.x] : 0, t0 = (int)threadIdx.x < p.B ? p.lengths[threadIdx.x] : 0;
   load(rank * tile);
   for (int r = threadIdx.x; r < p.B; r += kThreads) {
-    const int x = p.parents[r], t = p.lengths[r];
+    const int x = r < kThreads ? x0 : p.parents[r], t = r < kThreads ? t0 : p.lengths[r];
     parent[r] = (unsigned)x < (unsigned)p.B ? x : -1;
     children[r] = 0;
     eldest[r] = p.B;
-    full[r] = p.share && t > 0 ? min(p.M, (int)fast_div((unsigned)t, p.div_page)) : 0;
+    const int whole = t > 0 ? (int)fast_div((unsigned)t, p.div_page) : 0;
+    full[r] = p.share ? min(p.M, whole) : 0;
+    held[r] = min(p.M, whole + (t > whole * p.page));
     if (x >= p.B || (p.share && t > (long long)p.M * p.page)) atomicCAS(p.err, 0, kErrPaged | 1);
   }
   __syncthreads();
@@ -279,13 +305,10 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
     unsigned need = 0;
     if (r < p.B) {
       const int x = parent[r];
-      if (x >= 0 && eldest[x] != r) {
-        const int t = max(0, p.lengths[x]), whole = (int)fast_div((unsigned)t, p.div_page);
-        need = min(p.M, whole + (t > whole * p.page)) - full[x];
-      }
+      if (x >= 0 && eldest[x] != r) need = held[x] - full[x];
     }
     unsigned long long total;
-    const unsigned long long before = carry + block_scan(need, tmp, total) - need;
+    const unsigned long long before = carry + scan.run(need, total, turn) - need;
     if (r < p.B) off[r] = (int)before;
     carry += total;
   }
@@ -298,6 +321,7 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
       load(c0);
       __syncthreads();
     }
+#pragma unroll 4
     for (int i = threadIdx.x; i < p.B * tile; i += kThreads) {
       const int r = (int)fast_div((unsigned)i, div_tile), j = i - r * tile, c = c0 + j, x = parent[r];
       if (c >= p.M) continue;
@@ -311,10 +335,12 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
   int before = 0, all = 0;
   if (want) {
     const Run run(p.P, rank, blocks);
-    scan_free(run.count(p.refs), &count, tmp, before, all);
-    give(p.refs, run, before, want, [&](int i, int page) {
+    unsigned mask;
+    const int mine = run.count(p.refs, mask);
+    scan_free(mine, &count, scan, turn, before, all);
+    run.give(p.refs, mask, mine, before, want, [&](int i, int page) {
       const int r = find(off, p.B, i), x = parent[r], c = full[x] + i - off[r];
-      const int from = __ldcg(p.table + eldest[x] * p.ts + c);
+      const int from = blocks == 1 ? old[x * tile + c] : __ldcg(p.table + eldest[x] * p.ts + c);
       p.table[r * p.ts + c] = page;
       p.refs[page] = 1;
       if ((unsigned)from < (unsigned)p.P)
@@ -390,7 +416,7 @@ cudaError_t launch_after(void (*kern)(P), dim3 grid, int threads, cudaStream_t s
 cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launches) {
   const int blocks = p.P <= kSmallPool ? 1 : 8;
   const bool here = p.rows <= 4096;
-  cudaError_t e = launch_cluster(paged_reserve, blocks, (size_t)(3 * p.B + 2) * sizeof(int), st, p, here);
+  cudaError_t e = launch_cluster(paged_reserve, blocks, (size_t)(4 * p.B + 2) * sizeof(int), st, p, here);
   *launches = here ? 1 : 2;
   if (e != cudaSuccess || here) return e;
   return launch_after(paged_places, dim3((unsigned)((p.rows + 4 * kPlaceThreads - 1) / (4 * kPlaceThreads))),
@@ -400,8 +426,8 @@ cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launch
 cudaError_t launch_paged_fork(const ForkP& p, cudaStream_t st) {
   // small tables: one block, whole; else a sector's worth of columns, fewer where the rows are many
   const bool small = p.P <= kSmallPool && (long long)p.B * p.M <= 8192;
-  const int tile = small ? p.M : p.B <= 2048 ? 8 : 2;
-  return launch_cluster(paged_fork, small ? 1 : 8, ((size_t)5 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
+  const int tile = small ? p.M : p.B <= 2048 ? 8 : p.B <= 4096 ? 2 : 1;
+  return launch_cluster(paged_fork, small ? 1 : 8, ((size_t)6 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
                         make_fastdiv((unsigned)tile));
 }
 

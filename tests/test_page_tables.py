@@ -128,7 +128,7 @@ def check_fork(table, lengths, parents, refs, page, share):
 
 @gpu
 @pytest.mark.parametrize("share", [True, False])
-@pytest.mark.parametrize("B,M,page", [(1, 1, 1), (4, 9, 16), (60, 12, 5), (300, 40, 8), (2300, 5, 4), (5000, 3, 2)])
+@pytest.mark.parametrize("B,M,page", [(1, 1, 1), (4, 9, 16), (60, 12, 5), (300, 40, 8), (2000, 5, 4), (2300, 5, 4), (5000, 3, 2)])
 def test_fork_generations(share, B, M, page):
     """Rows that multiply, go and grow over several steps; pages come back."""
     rng = random.Random(B)
