@@ -126,13 +126,9 @@ __device__ __forceinline__ float2 halves(unsigned x) { return __half22float2(*re
 // τ · unit · kGroupUnit times a group's scale (≤ 448) stays under 65504, and keeps 2^-24
 // of it where the scale is 2^-6 of the row's largest.
 constexpr float kGroupUnit = 0x1p-6f;
-// x and y as halfs, or (rest 1) what that left of them.
-__device__ __forceinline__ unsigned half_or_rest(float x, float y, float rest) {
+__device__ __forceinline__ unsigned two_halves(float x, float y) {
   unsigned w;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
-  const float2 h = halves(w);
-  // the half itself where rest is 0: x − 0 · h rounds to it again
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(fmaf(-rest, h.y, y)), "f"(fmaf(-rest, h.x, x)));
   return w;
 }
 template <int N> __device__ __forceinline__ unsigned lds_part(unsigned a) {  // 1 or 2 bytes
@@ -334,6 +330,9 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   }
   const int h0 = hk * G + hg * kHeads, Gh = min(kHeads, G - hg * kHeads);  // query heads h0 … h0+Gh−1
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  // a short table's row (a window's ring) is fetched beside the length
+  const bool ring_row = Z::four && p.M <= 32;
+  const int my_page = ring_row && lane < p.M ? __ldg(p.table + b * p.ts + lane) : 0;
   const Reach rc = reach(p, b, S);
   const bool mine = (unsigned)piece < rc.count;
   if (!mine && !clustered) return;
@@ -365,6 +364,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
       const unsigned j =
           AL ? start(k + lane / kUnits) + lane % kUnits * GR : start(k) + r * 32 + (KT < 32 ? lane % KT : lane);
       rows[r] = kNoRow;
+      if (Z::four && ring_row) {
+        const unsigned pos = p0 + j, s = pos - fast_div(pos, p.div_cap) * p.cap, col = fast_div(s, p.div_page);
+        const unsigned pid = (unsigned)__shfl_sync(0xffffffffu, my_page, col & 31);
+        if (j < nk && pos + GR > rc.lo) {
+          if (pid < (unsigned)p.P) rows[r] = (pid * (unsigned)p.Hk + (unsigned)hk) * (unsigned)p.page + (s - col * (unsigned)p.page);
+          else atomicCAS(p.err, 0, kErrPaged | 2);
+        }
+        continue;
+      }
       // none for positions wholly before the reach: their pages may be gone
       if (j < nk && p0 + j + GR > rc.lo) {
         const unsigned row = paged_row(p, b, p0 + j);
@@ -868,26 +876,38 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
           // 2c + 8, 2c + 9, and column g: of a head the half of τ or the rest of it.  With a head
           // each there is a column pair for each group, τ times the group's scale, and of the
           // products the ones of an element's own group count; else the values are scaled.
-          unsigned pk[4];
+          const bool odd = g & 1;
           const unsigned pa = smem_u32(ps + (LONE ? 0 : (g >> 1) % GP * Z::pstride) + u * 16 + 2 * c);
-          lds_words<2, 0>(pa, pk);
-          lds_words<2, 32>(pa, pk + 2);
-          const float rest = g & 1 ? 1.f : 0.f;
+          unsigned pk[4];
+          if constexpr (LONE) {
+            lds_words<2, 0>(pa + (odd ? 32 : 0), pk);
+          } else {
+            lds_words<2, 0>(pa, pk);
+            lds_words<2, 32>(pa, pk + 2);
+          }
           constexpr int kHalves = GB == 8 ? 2 : 1;  // of four groups
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf) {
             const int grp = LONE ? (GB == 2 ? (g >> 1) & 1 : hf * 4 + (g >> 1)) : GB == 2 ? g >> 2 : hf * 4 + (g >> 1);
             const unsigned gs = smem_u32(md) + Z::scales + KT * GB + (u * 16 + 2 * c) * GB + grp;
-            const unsigned s01 = group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8);
-            const unsigned s89 = group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8);
-            unsigned b0, b1;
+            unsigned b0, b1, s01 = 0, s89 = 0;
             if constexpr (LONE) {
-              const float2 f01 = halves(s01), f89 = halves(s89);
-              b0 = half_or_rest(__uint_as_float(pk[0]) * f01.x, __uint_as_float(pk[1]) * f01.y, rest);
-              b1 = half_or_rest(__uint_as_float(pk[2]) * f89.x, __uint_as_float(pk[3]) * f89.y, rest);
+              // a column's halfs or rests of two of the four keys, and of the other two from the
+              // lane that has the column beside it, which has made both
+              const unsigned at = gs + (odd ? 8 * GB : 0);
+              const float2 f = halves(group_pair(lds_part<1>(at) | lds_part<1>(at + GB) << 8));
+              const float x = __uint_as_float(pk[0]) * f.x, y = __uint_as_float(pk[1]) * f.y;
+              const unsigned hi = two_halves(x, y);
+              const float2 h = halves(hi);
+              const unsigned lo = two_halves(x - h.x, y - h.y);
+              const unsigned got = __shfl_xor_sync(0xffffffffu, odd ? hi : lo, 4);
+              b0 = odd ? got : hi;
+              b1 = odd ? lo : got;
             } else {
-              b0 = __byte_perm(pk[0], pk[1], g & 1 ? 0x5410 : 0x7632);
-              b1 = __byte_perm(pk[2], pk[3], g & 1 ? 0x5410 : 0x7632);
+              s01 = group_pair(lds_part<1>(gs) | lds_part<1>(gs + GB) << 8);
+              s89 = group_pair(lds_part<1>(gs + 8 * GB) | lds_part<1>(gs + 9 * GB) << 8);
+              b0 = __byte_perm(pk[0], pk[1], odd ? 0x5410 : 0x7632);
+              b1 = __byte_perm(pk[2], pk[3], odd ? 0x5410 : 0x7632);
             }
             constexpr int kBytes = GB == 2 ? 2 : 4;  // of a row: two elements each
             const int byte = hf * (R / 2) + g * kBytes;
@@ -903,13 +923,13 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const unsigned even = (w[2 * i] & 0x0f0f0f0fu) | (w[2 * i + 1] << 4 & 0xf0f0f0f0u);
-              const unsigned odd = (w[2 * i] >> 4 & 0x0f0f0f0fu) | (w[2 * i + 1] & 0xf0f0f0f0u);
+              const unsigned odds = (w[2 * i] >> 4 & 0x0f0f0f0fu) | (w[2 * i + 1] & 0xf0f0f0f0u);
               if constexpr (LONE) {
                 codes8(even, a[2 * i]);
-                codes8(odd, a[2 * i + 1]);
+                codes8(odds, a[2 * i + 1]);
               } else {
                 widen8(even, i ? s89 : s01, a[2 * i]);
-                widen8(odd, i ? s89 : s01, a[2 * i + 1]);
+                widen8(odds, i ? s89 : s01, a[2 * i + 1]);
               }
             }
 #pragma unroll
