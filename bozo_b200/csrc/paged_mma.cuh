@@ -27,12 +27,25 @@
 // 6 % at 32), 3-4 % with four heads and 3-12 % with eight (309 MB, 64 wide: 68.4 µs,
 // with two parts 66.2; 128 wide 73.6 and 67.7, with half-filled second products 82).
 //
+// 4-bit rows: a code (e2m1) times its group's scale (e4m3) is a half exactly, so a product
+// goes as for 8 bits, and O is turned round up to four heads (half the products, and half
+// the accumulators).  With a head each the scales of groups are not multiplied into the
+// codes at all.  Of S's eight columns two belong to each quarter of the elements, which
+// are those of one lane of four, with scales of its own: its sums take them, and the four
+// lanes add up theirs.  Of O's, two belong to each group (128 wide: of either half): τ times
+// the key's scale of that group, as a half and the rest of it; of the products those of an
+// element's own group are kept.
+//
 // What bounds it: 1 flop a byte for 16-bit rows of a head of their own (memory),
 // instructions for 8-bit rows of shared heads.  4 warps with 3 tiles of 4 KB each and
 // 3-4 blocks an SM keep 100-130 KB under way.  Measured: 64 sequences of up to 8192
 // keys × 16 heads, bf16: 164 µs for 1084 MB, the rate of a copy; one row set of 120002
 // keys 75.6 µs (0.99); e4m3, 128 wide, four heads a key head: 189 µs for 1106 MB
-// (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.
+// (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.  4-bit rows: 180
+// instructions for 16 keys of 1.3 KB, most of them conversions and selections that run at
+// half rate (a head each, 64 ragged sequences × 16 heads: 78 µs for 337 MB, 0.66 of a copy;
+// scaled codes 103 µs; with the memory left out 78 → 60); 128 wide, four heads: 179 µs for
+// 658 MB.
 #pragma once
 
 #include <limits.h>
@@ -208,13 +221,17 @@ __device__ __forceinline__ float ld_peer(unsigned addr, unsigned rank) {
 }
 
 constexpr int kWarps = 4;
+// Windows up to here take tiles of 32 4-bit rows, for more of the warps (16 sequences × 12
+// heads, 64 keys: 4.6 µs a call, with 64 rows 5.3; 128 keys 5.5 and 5.3, 256 keys 6.4 and 7.0).
+constexpr int kShortWindow = 256;
 
 
 // Geometry of the kernel for one page type, head width and count of heads.
-template <int DT, int HD, int GP> struct Geo {
+// KEYS: of a tile, where it is not the usual count.
+template <int DT, int HD, int GP, int KEYS = 0> struct Geo {
   static constexpr bool four = Fmt<DT>::size == 0;
   static constexpr int row = four ? HD / 2 : HD * Fmt<DT>::size;  // bytes of a row
-  static constexpr int keys = row >= 128 ? 16 : row >= 32 ? 2048 / row : 64;  // keys of a tile of the ring
+  static constexpr int keys = KEYS ? KEYS : row >= 128 ? 16 : row >= 32 ? 2048 / row : 64;  // keys of a tile of the ring
   static constexpr int kv = keys * row;                      // bytes of its K (or V): 1 or 2 KB, 4 KB at 256-byte rows
   static constexpr int scales = Fmt<DT>::scaled ? 2 * keys * 4 : 0;
   static constexpr int gr = four ? HD / 16 : 0;              // bytes of a row's group scales
@@ -234,7 +251,7 @@ template <int DT, int HD, int GP> struct Geo {
   static constexpr int blocks = four ? (HD == 128 ? 3 : 4) - (GP == 8) : HD == 64 && (Fmt<DT>::scaled || Fmt<DT>::bf) ? 3 : 2;
   static constexpr bool fold = Fmt<DT>::bf && GP <= 4;  // τ's second parts have rows 4-7 of P
   static constexpr int parts = (fold ? 2 : 1) * kWarps;  // sums that are added at the end
-  static constexpr int stages = four ? 2 : 3;                // tiles of the ring; 4-bit rows' take so long that
+  static constexpr int stages = four && !KEYS ? 2 : 3;                // tiles of the ring; 4-bit rows' take so long that
                                                              // two do (64 ragged sequences 104 µs, with three 114)
   static constexpr int warp = stages * (2 * kv + meta) + GP * pstride * (Fmt<DT>::bf ? 6 : 4);
 };
@@ -292,10 +309,10 @@ __device__ __forceinline__ int by_length(const PagedP& p, int rank) {
 }
 
 // GR: positions from a multiple of GR on that lie in one page (16, 8 or 1).
-template <int DT, int HD, int GP, int GR>
-__global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) paged_decode_mma(PagedP p, MmaGrid grid) {
+template <int DT, int HD, int GP, int GR, int KEYS = 0>
+__global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP, KEYS>::blocks) paged_decode_mma(PagedP p, MmaGrid grid) {
   using F = Fmt<DT>;
-  using Z = Geo<DT, HD, GP>;
+  using Z = Geo<DT, HD, GP, KEYS>;
   constexpr bool BF = F::bf;
   constexpr int R = Z::row, KT = Z::keys, NT = KT / 16, NCH = R / 16, SZ = F::size, RS = Z::four ? 1 : SZ, GB = Z::gr;
   constexpr bool QUAD = BF && GP <= 2, WIDE = BF && GP == 8;       // four columns of S a head, one
@@ -1103,14 +1120,14 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP>::blocks) pag
   }
 }
 
-template <int DT, int HD, int GP, int GR>
+template <int DT, int HD, int GP, int GR, int KEYS = 0>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
   const int G = p.H / p.Hk, HG = (G + kHeads - 1) / kHeads;
-  using Z = Geo<DT, HD, GP>;
+  using Z = Geo<DT, HD, GP, KEYS>;
   const size_t ring = (size_t)kWarps * Z::warp;
   const size_t part = (size_t)(Z::parts + 1) * std::min(G, kHeads) * HD * sizeof(float);
   const size_t smem = std::max(ring, part);
-  auto kern = paged_decode_mma<DT, HD, GP, GR>;
+  auto kern = paged_decode_mma<DT, HD, GP, GR, KEYS>;
   static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1137,6 +1154,10 @@ cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t 
 }
 template <int DT, int HD, int GP>
 cudaError_t launch_paged_mma(const PagedP& p, const PagedPlan& pl, cudaStream_t st) {
+  // short windows: tiles of half the keys, for more of the warps
+  if constexpr (Geo<DT, HD, GP>::lone && Geo<DT, HD, GP>::keys == 64)
+    if (p.page % 16 == 0 && p.mode == BOZO_MODE_LOCAL && p.W <= kShortWindow)
+      return launch_paged_mma<DT, HD, GP, 16, 32>(p, pl, st);
   if (p.page % 16 == 0) return launch_paged_mma<DT, HD, GP, 16>(p, pl, st);
   return p.page % 8 == 0 ? launch_paged_mma<DT, HD, GP, 8>(p, pl, st) : launch_paged_mma<DT, HD, GP, 1>(p, pl, st);
 }

@@ -185,8 +185,8 @@ LENGTHS = [0, 1, 2, 15, 16, 17, 63, 64, 65, 130, -1, 200]
 
 @gpu
 @pytest.mark.parametrize("io", [F32, BF16, F16])
-@pytest.mark.parametrize("HD,page", [(32, 16), (32, 7), (64, 16), (64, 8), (128, 16), (128, 5), (48, 16)])
-@pytest.mark.parametrize("window,normalize", [(16, "mass"), (64, "count"), (1, "none"), (None, "mass")])
+@pytest.mark.parametrize("HD,page", [(32, 16), (32, 7), (64, 16), (64, 8), (128, 16), (128, 5), (48, 16), (16, 8)])
+@pytest.mark.parametrize("window,normalize", [(16, "mass"), (64, "count"), (1, "none"), (190, "mass"), (None, "mass")])
 def test_decode_matches_float64(io, HD, page, window, normalize):
     tables = rope(HD, 256, "cuda")
     pool = Pool4(len(LENGTHS), 2, HD, page, -(-201 // page))
