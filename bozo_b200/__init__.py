@@ -10,6 +10,8 @@ Public API:
       reference's model.py / train.py / generate.py import it unchanged.
   paged.write_kv / read_kv / paged_tension, serving.PagedState / generate / ...
       paged key/value caches and continuous batching (import the submodules).
+  paged.reserve / fork / copy_pages, beam.select, serving.beam_search
+      page tables kept on the device, and beam search on them.
 """
 from __future__ import annotations
 

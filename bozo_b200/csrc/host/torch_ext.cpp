@@ -546,11 +546,20 @@ pybind11::tuple paged_reserve(const at::Tensor& table, const at::Tensor& lengths
   const c10::cuda::CUDAGuard guard(dev);
   if (given(tokens)) a.tokens = per_row(what, "tokens", *tokens, lengths);
   if (rows < -1 || rows > INT32_MAX) throw std::invalid_argument("reserve: rows must not be negative, nor pass 2^31");
-  at::Tensor cu = empty({a.batch + 1}, at::kInt, dev), missing = empty({1}, at::kInt, dev), at_[3];
+  // one allocation: seq, pos and slot (16-byte aligned), cu_rows, missing
+  const int64_t n = rows > 0 ? (rows + 3) / 4 * 4 : 0, count = (int64_t)a.batch + 1;
+  const at::Tensor all = empty({3 * n + count + 1}, at::kInt, dev);
+  auto part = [&](int64_t at, int64_t size) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(at);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+    return t;
+  };
+  at::Tensor cu = part(3 * n, count), missing = part(3 * n + count, 1), at_[3];
   a.cu_rows = cu.data_ptr<int32_t>();
   a.missing = missing.data_ptr<int32_t>();
   if (rows >= 0)
-    for (at::Tensor& t : at_) t = empty({rows}, at::kInt, dev);
+    for (int i = 0; i < 3; ++i) at_[i] = part(i * n, rows);
   if (rows > 0) {
     a.rows = rows;
     a.seq = at_[0].data_ptr<int32_t>();

@@ -290,7 +290,8 @@ int head_groups(const PagedP& p) {
 }
 
 // Pieces of a row.  About three blocks an SM keep the memory busy (16 rows of
-// 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37).  Sequences
+// 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37; four of 4-bit
+// pages, 46.1 µs at 27, 43.9 at 37, 50 at 92).  Sequences
 // of different lengths want smaller pieces to even out — twelve an SM, of 2048 keys
 // at least (1024 rows of up to 8192 keys: 164 µs in two to four; 512 rows of up to
 // 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).  4-bit
@@ -311,8 +312,9 @@ PagedPlan plan(const PagedP& p, int sms) {
   const bool mma = mma_path(p);
   const long long keys = p.mode == BOZO_MODE_LOCAL ? p.W : (long long)p.cap;
   const long long rows = (long long)p.B * p.Hk * head_groups(p);
-  long long s = 3LL * sms / rows;
-  const long long per_sm = mma && p.dt == BOZO_DT_F4E2M1 && p.B <= kSorted && p.mode == BOZO_MODE_GLOBAL ? 6 : 12;
+  const bool four = mma && p.dt == BOZO_DT_F4E2M1;
+  long long s = (four ? 4LL : 3LL) * sms / rows;
+  const long long per_sm = four && p.B <= kSorted && p.mode == BOZO_MODE_GLOBAL ? 6 : 12;
   if (p.B > 1) s = std::max(s, std::min((per_sm * sms + rows - 1) / rows, keys / 2048));
   s = std::min(s, keys <= (mma ? 256 : 512) ? 1 : (keys + 15 + kMinPiece - 1) / kMinPiece);
   if (mma && s > kCluster && (s <= kCluster + 4 || keys <= 256 * kCluster)) s = kCluster;

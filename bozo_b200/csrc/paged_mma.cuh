@@ -42,10 +42,10 @@
 // keys × 16 heads, bf16: 164 µs for 1084 MB, the rate of a copy; one row set of 120002
 // keys 75.6 µs (0.99); e4m3, 128 wide, four heads a key head: 189 µs for 1106 MB
 // (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.  4-bit rows: 180
-// instructions for 16 keys of 1.3 KB, most of them conversions and selections that run at
-// half rate (a head each, 64 ragged sequences × 16 heads: 78 µs for 337 MB, 0.66 of a copy;
-// scaled codes 103 µs; with the memory left out 78 → 60); 128 wide, four heads: 179 µs for
-// 658 MB.
+// instructions for 16 keys of 1.3 KB, many of them conversions and selections that run at
+// half rate, bound them (a head each, 64 ragged sequences × 16 heads: 79 µs for 337 MB, 0.65
+// of a copy; 66 with no page read at all; with scaled codes 83).  128 wide, four heads: 179
+// µs for 658 MB.
 #pragma once
 
 #include <limits.h>

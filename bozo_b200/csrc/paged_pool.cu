@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const unsigned rank = cl.block_rank();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the places' kernel, which waits for this one
   const Run run(p.P, rank, cl.num_blocks());
   unsigned mask;
   const int mine = run.count(p.refs, mask);
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
   __shared__ int count;
   cg::cluster_group cl = cg::this_cluster();
   const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the copies' kernel, which waits for this one
   // the old entries of columns c0 …: thread i has every kThreads-th of a tile's B · tile
   auto load = [&](int c0) {
 #pragma unroll 4

@@ -215,3 +215,21 @@ def test_oracle_by_hand():
     s, t, r = orc.select(x, torch.log(torch.tensor([[0.4, 0.5]])), None, None)
     assert t.tolist() == [[1, 0]] and r.tolist() == [[1, 0]]
     assert torch.allclose(torch.exp(s), torch.tensor([[0.3, 0.2]], dtype=torch.float64), atol=1e-6)
+
+
+@gpu
+def test_logits_past_32_bits():
+    """More than 2^32 bytes of logits: the last prompts' rows."""
+    N, K, V = 9000, 4, 65536
+    try:
+        logits = torch.empty(N * K, V, device="cuda", dtype=BF16)
+    except torch.cuda.OutOfMemoryError:
+        pytest.skip("needs 5 GB of free device memory")
+    scores = torch.full((N, K), -math.inf, device="cuda")   # only the last ones are read
+    logits[-3 * K:] = torch.randn(3 * K, V, device="cuda").to(BF16)
+    scores[-3:] = -torch.rand(3, K, device="cuda")
+    s, t, r = beam.select(logits, scores)
+    want = beam.select(logits[-3 * K:].clone(), scores[-3:].clone())
+    assert torch.equal(s[-3:], want[0]) and torch.equal(t[-3:], want[1])
+    assert torch.equal(r[-3:], want[2] + (N - 3) * K)
+    assert (s[:-3] == -math.inf).all() and torch.equal(t[0], torch.arange(K, device="cuda"))

@@ -359,3 +359,47 @@ def test_struct_layout_matches_header(tmp_path):
         name, _, f = key.partition(".")
         got = getattr(structs[name], f).offset if f else C.sizeof(structs[name])
         assert got == int(val), key
+
+
+# ── the largest ──
+
+@gpu
+def test_as_many_rows_as_there_may_be():
+    rng = random.Random(11)
+    B, M, page = 8192, 2, 4
+    lengths = [rng.choice([-1, 0, 3, 4, 5, 8]) for _ in range(B)]
+    table, refs = random_tables(rng, B, M, page, lengths, spare=12000)
+    tokens = [rng.randint(0, max(0, min(4, 8 - t))) for t in lengths]
+    got = check_reserve(table, lengths, tokens, refs, page, sum(tokens))
+    lengths = [t + n if t >= 0 else t for t, n in zip(lengths, tokens)]
+    for share in (True, False):
+        parents = [rng.randrange(-1, B) for _ in range(B)]
+        check_fork(got[0], lengths, parents, got[1], page, share)
+
+
+@gpu
+def test_a_long_row_and_a_large_pool():
+    """A sequence of 2^20 tokens, and pages behind 300000 others."""
+    P, page, M = 370_000, 16, 65536
+    refs = [1] * 300_000 + [0, 1] * 35_000
+    plan_refs, table = int32(refs), torch.full((1, M), -1, dtype=torch.int32, device="cuda")
+    plan = paged.reserve(table, int32([0]), int32([35_000 * 16]), plan_refs, page, rows=1 << 20)
+    free = torch.arange(300_000, P, 2, device="cuda", dtype=torch.int32)
+    assert torch.equal(table[0, :35_000], free) and (table[0, 35_000:] == -1).all() and (plan_refs == 1).all()
+    n = torch.arange(35_000 * 16, device="cuda")
+    assert torch.equal(plan.pos[:len(n)].long(), n) and (plan.seq[:len(n)] == 0).all()
+    assert torch.equal(plan.slot[:len(n)].long(), free[n // 16].long() * 16 + n % 16)
+    assert (plan.seq[len(n):] == -1).all() and (plan.slot[len(n):] == -1).all() and plan.missing.item() == 0
+
+
+@gpu
+def test_copies_past_32_bits():
+    """Pages beyond the first 2^32 bytes of a pool."""
+    try:
+        pool = torch.empty(5000, 1 << 20, device="cuda", dtype=torch.uint8)
+    except torch.cuda.OutOfMemoryError:
+        pytest.skip("needs 5 GB of free device memory")
+    pool[[0, 4997]] = torch.randint(0, 256, (2, 1 << 20), device="cuda", dtype=torch.uint8)
+    keep = pool[4996].fill_(7).clone()
+    paged.copy_pages([pool], int32([[0, 4999], [4997, 1]]))
+    assert torch.equal(pool[4999], pool[0]) and torch.equal(pool[1], pool[4997]) and torch.equal(pool[4996], keep)
