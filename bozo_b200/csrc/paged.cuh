@@ -223,17 +223,19 @@ struct NewRow {
                       : __fadd_rn(__fmul_rn(y, s), __fmul_rn(x[i], c));
     }
   }
-  // … into row `row` of the pages.
+  // … into row `row` of the pages, whose type is DT where it is known.
+  template <int DT = -1>
   __device__ __forceinline__ void put(const PagedP& p, void* pages, float* scales, unsigned char* groups, size_t row,
                                       int lane) const {
+    const int dt = DT >= 0 ? DT : p.dt;
     float inv = 1.f;
     unsigned a = 0;
-    if (p.dt > BOZO_DT_F16) {
+    if (dt > BOZO_DT_F16) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
       a = __reduce_max_sync(0xffffffffu, a);
     }
-    if (p.dt == BOZO_DT_F4E2M1) {
+    if (dt == BOZO_DT_F4E2M1) {
       const Row4 r(a);
       if (lane == 0) scales[row] = r.scale;
 #pragma unroll
@@ -251,17 +253,17 @@ struct NewRow {
       }
       return;
     }
-    if (p.dt > BOZO_DT_F16) {
+    if (dt > BOZO_DT_F16) {
       float scale;
-      quant_scale(a, p.dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
+      quant_scale(a, dt == BOZO_DT_I8 ? 127.f : 448.f, scale, inv);
       if (lane == 0) scales[row] = scale;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int d = lane + 32 * i;
       if (d >= p.HD) continue;
-      if (p.dt <= BOZO_DT_F16) stf(pages, (long long)(row * p.HD + d), p.dt, x[i]);
-      else static_cast<unsigned char*>(pages)[row * p.HD + d] = quant_code(x[i], inv, p.dt);
+      if (dt <= BOZO_DT_F16) stf(pages, (long long)(row * p.HD + d), dt, x[i]);
+      else static_cast<unsigned char*>(pages)[row * p.HD + d] = quant_code(x[i], inv, dt);
     }
   }
 };

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_decode_rows(PagedP p,
     }
   // the last two warps: the first ones fetch the query
   if (warp >= kRowWarps - 2 && writes_row(p, rc, piece, hg == 0))
-    append_part(p, b, hk, rc.t, warp == kRowWarps - 1, lane);
+    append_part<DT>(p, b, hk, rc.t, warp == kRowWarps - 1, lane);
   __syncthreads();
   const bool on[2] = {4 * l < HD, 4 * (l + L) < HD};
   const int own = NH == 1 ? 0 : l / (L / 4);  // the head whose τ this lane computes

@@ -78,19 +78,21 @@ __device__ __forceinline__ float* piece_mass(const PagedP& p, int S) {
 __device__ __forceinline__ bool writes_row(const PagedP& p, const Reach& r, unsigned piece, bool first) {
   return p.kn.p && r.active && (p.mode == BOZO_MODE_GLOBAL ? piece == r.count - 1 : piece == 0 && first);
 }
+template <int DT = -1>
 __device__ __forceinline__ void append_part(const PagedP& p, int b, int hk, int t, bool key, int lane) {
   const NewRow x(p, key ? p.kn : p.vn, b, hk, (unsigned)t, key && p.cos, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
   if (row0 != kNoRow)
-    x.put(p, key ? p.k : p.v, key ? p.ks : p.vs, key ? p.kg : p.vg, (size_t)row0 + (size_t)hk * p.page, lane);
+    x.template put<DT>(p, key ? p.k : p.v, key ? p.ks : p.vs, key ? p.kg : p.vg, (size_t)row0 + (size_t)hk * p.page, lane);
 }
+template <int DT>
 __device__ __forceinline__ void append_row(const PagedP& p, int b, int hk, int t, int lane) {  // by one warp
   const NewRow k(p, p.kn, b, hk, (unsigned)t, p.cos != nullptr, lane), v(p, p.vn, b, hk, (unsigned)t, false, lane);
   const unsigned row0 = paged_row(p, b, (unsigned)t);
   if (row0 == kNoRow) return;
   const size_t row = (size_t)row0 + (size_t)hk * p.page;
-  k.put(p, p.k, p.ks, p.kg, row, lane);
-  v.put(p, p.v, p.vs, p.vg, row, lane);
+  k.template put<DT>(p, p.k, p.ks, p.kg, row, lane);
+  v.template put<DT>(p, p.v, p.vs, p.vg, row, lane);
 }
 
 // Rotated query element i of head h.

@@ -528,7 +528,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP, KEYS>::block
   const bool writes = writes_row(p, rc, piece, hg == 0);
   const bool early = writes && p.mode == BOZO_MODE_GLOBAL && nk <= (Z::stages - 1) * kWarps * KT;
   if (warp == kWarps) {
-    if (writes) append_row(p, b, hk, rc.t, lane);
+    if (writes) append_row<DT>(p, b, hk, rc.t, lane);
     if (early) __syncthreads();
     __syncthreads();
   } else {
