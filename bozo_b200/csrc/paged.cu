@@ -308,6 +308,21 @@ __device__ __forceinline__ void write_head(const PagedP& p, const Eight<I>& xl, 
       add2(x[8 + i], x[9 + i], d0, d1, e0, e1);
     }
   }
+  if constexpr (DT == BOZO_DT_F4E2M1 && !KEY) {  // the lane's elements are a group
+    float m = x[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) m = max_abs(m, x[i]);
+    float a = m;
+    for (int o = L / 2; o; o >>= 1) a = max_abs(a, __shfl_xor_sync(group, a, o));
+    const Row4 r(__float_as_uint(a) & 0x7fffffffu);
+    float unit, recip;
+    const unsigned char c4 = r.group(fabsf(m), unit, recip);
+    reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.v) + (size_t)row * half)[l] =
+        make_uint2(narrow4(r, x, unit, recip), narrow4(r, x + 8, unit, recip));
+    p.vg[(size_t)row * L + l] = c4;
+    if (l == 0) p.vs[row] = r.scale;
+    return;
+  }
   if constexpr (DT == BOZO_DT_F4E2M1) {
     // sixteen consecutive elements: eight of this lane's and eight of its neighbour's, in either half
     float lo = x[0], hi = x[8];
@@ -372,13 +387,15 @@ __global__ void __launch_bounds__(kThreads, DT == BOZO_DT_F4E2M1 ? kWriteBlocks4
     widen(ld8(p.sin + at), s);
   }
   const I* kf = static_cast<const I*>(p.kn.p) + n * p.kn.sb + sub * p.kn.sh + 8 * l;
-  const I* vf = static_cast<const I*>(p.vn.p) + n * p.vn.sb + sub * p.vn.sh + 8 * l;
+  // 4-bit values, which are not rotated, go as sixteen consecutive elements
+  constexpr bool FOUR = DT == BOZO_DT_F4E2M1;
+  const I* vf = static_cast<const I*>(p.vn.p) + n * p.vn.sb + sub * p.vn.sh + (FOUR ? 16 : 8) * l;
   unsigned row = row0 + (unsigned)sub * (unsigned)p.page;  // rows are numbered in 32 bits
   const long long ks = per * p.kn.sh, vs = per * p.vn.sh;
   const unsigned group = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
 #pragma unroll 1
   for (int h = sub; h < p.Hk; h += per, kf += ks, vf += vs, row += (unsigned)(per * p.page)) {
-    const Eight<I> kl = ld8(kf), kh = ld8(kf + half), vl = ld8(vf), vh = ld8(vf + half);
+    const Eight<I> kl = ld8(kf), kh = ld8(kf + half), vl = ld8(vf), vh = ld8(vf + (FOUR ? 8 : half));
     write_head<DT, I, true>(p, kl, kh, row, L, l, group, c, s);
     write_head<DT, I, false>(p, vl, vh, row, L, l, group, c, s);
   }
