@@ -164,6 +164,32 @@ template <int kThreads> struct Scratch {
   int n, held;
 };
 
+// The warp's largest; NaN are passed over.
+__device__ __forceinline__ float warp_most(float x) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// log s to about 1e-9 for a sum of exponentials of which the largest is 1: with s = 2^e · f,
+// f in [√½, √2), log f = 2·atanh z, z = (f − 1) / (f + 1); z in 64 bits, the series' further
+// terms, a hundredth of the first, in 32.  (The library's function takes a few times as long,
+// which every selection waits for.)
+__device__ __forceinline__ double log_sum(float s) {
+  if (!(s >= 0.5f && s < 3e38f)) return log((double)s);  // nothing, or not finite
+  int e = (int)(__float_as_uint(s) >> 23) - 127;
+  float f = __uint_as_float((__float_as_uint(s) & 0x7fffffu) | 0x3f800000u);
+  if (f > 1.41421356f) {
+    f *= 0.5f;
+    ++e;
+  }
+  const double n = (double)f - 1., d = (double)f + 1.;
+  const float r = __frcp_rn(f + 1.f), z0 = (f - 1.f) * r, w = z0 * z0;
+  const double z = fma(fma(-(double)z0, d, n), (double)r, (double)z0);
+  const float p = w * fmaf(w, fmaf(w, fmaf(w, fmaf(w, fmaf(w, 1.f / 13, 1.f / 11), 1.f / 9), 1.f / 7), 1.f / 5), 1.f / 3);
+  return fma((double)e, 0.69314718055994530942, fma(2. * z, (double)p, 2. * z));
+}
+
 // Two exponentials relative to m, added to (a, b).
 __device__ __forceinline__ void add_pow2(float& a, float& b, float x, float y, float m) {
   asm("{.reg .b64 p, q; .reg .f32 x, y; mov.b64 p, {%2, %3}; mov.b64 q, {%4, %4}; add.rn.f32x2 p, p, q;"
@@ -204,41 +230,52 @@ __device__ __forceinline__ void take(const Vec<DT>* v, float& m, float& s) {
   m = to;
 }
 
-// The K best of pieces [q0, q1) of a row, sorted, into sc.cur, its largest logit and sum (to all
-// threads), and the two's logarithm (to the first of the last warp).
-template <int DT, int kThreads>
-__device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, Scratch<kThreads>& sc, float& M, float& S,
-                                     double& lse) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int kWarps = kThreads / 32, N = Vec<DT>::N, U = 8;  // pieces in flight
-  float m = -INFINITY, s = 0.f;
-  int q = q0 + tid;
-  // whole pieces first, in the same order wherever the row lies
-  for (const int whole = min(q1, row.V / N); q + (U - 1) * kThreads < whole; q += U * kThreads) {
-    Vec<DT> v[U];
-    if (row.off == 0) {
-      const uint4* from = reinterpret_cast<const uint4*>(row.at) + q;
+// A thread's batch of pieces q, q + kThreads, … below q1: whole pieces of an aligned row are
+// nothing but loads.
+constexpr int kBatch = 8;
+template <int DT, int kThreads, int U = kBatch>
+__device__ __forceinline__ void batch(const Row<DT>& row, int q, int q1, Vec<DT>* v) {
+  if (row.off == 0 && q + (U - 1) * kThreads < min(q1, row.V / Vec<DT>::N)) {
+    const uint4* from = reinterpret_cast<const uint4*>(row.at) + q;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const uint4 x = __ldg(from + j * kThreads);
-        v[j].w[0] = x.x; v[j].w[1] = x.y; v[j].w[2] = x.z; v[j].w[3] = x.w;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < U; ++j) v[j] = row.load(q + j * kThreads, q1);
+    for (int j = 0; j < U; ++j) {
+      const uint4 x = __ldg(from + j * kThreads);
+      v[j].w[0] = x.x; v[j].w[1] = x.y; v[j].w[2] = x.z; v[j].w[3] = x.w;
     }
-    take<DT, U>(v, m, s);
-  }
-  for (; q < q1; q += 2 * kThreads) {
-    Vec<DT> v[2] = {row.load(q, q1), row.load(q + kThreads, q1)};
-    take<DT, 2>(v, m, s);
-  }
-  float g = m, wm = m;
+  } else {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    if (2 * o == kThreads / kGroups) g = wm;
+    for (int j = 0; j < U; ++j) v[j] = row.load(q + j * kThreads, q1);
   }
+}
+// The first one of pieces [q0, q1): half of one where that is all there is.
+template <int DT, int kThreads>
+__device__ __forceinline__ void first_batch(const Row<DT>& row, int q0, int q1, Vec<DT>* v) {
+  if (q1 - q0 <= kBatch / 2 * kThreads) batch<DT, kThreads, kBatch / 2>(row, q0 + threadIdx.x, q1, v);
+  else batch<DT, kThreads>(row, q0 + threadIdx.x, q1, v);
+}
+
+// The K best of pieces [q0, q1) of a row, sorted, into sc.cur, its largest logit and sum (to all
+// threads), and the two's logarithm (to the first of the last warp).  v: the first batch.
+template <int DT, int kThreads>
+__device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, Scratch<kThreads>& sc, Vec<DT>* v,
+                                     float& M, float& S, double& lse) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int kWarps = kThreads / 32, N = Vec<DT>::N;
+  float m = -INFINITY, s = 0.f;
+  if (q1 - q0 <= kBatch / 2 * kThreads) {
+    take<DT, kBatch / 2>(v, m, s);
+  } else {
+    for (int q = q0 + tid;;) {
+      take<DT, kBatch>(v, m, s);
+      q += kBatch * kThreads;
+      if (q >= q1) break;
+      batch<DT, kThreads>(row, q, q1, v);
+    }
+  }
+  float g = m;
+#pragma unroll
+  for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+  const float wm = warp_most(m);
   if (tid % (kThreads / kGroups) == 0) sc.top[tid / (kThreads / kGroups)] = g;
   s = warp_sum(s * rescale(m, wm));
   if (lane == 0) {
@@ -265,9 +302,7 @@ __device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, 
   }
   if (warp == kWarps - 1) {
     const float y = lane < kWarps ? sc.wm[lane] : -INFINITY;
-    M = y;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    M = warp_most(y);
     S = warp_sum(lane < kWarps ? sc.ws[lane] * rescale(y, M) : 0.f);
     if (lane == 0) {
       sc.m = M;
@@ -296,7 +331,7 @@ __device__ __forceinline__ void scan(const Row<DT>& row, int q0, int q1, int K, 
       }
     }
   }
-  if (tid == kThreads - 32) lse = (double)M + log((double)S);
+  if (tid == kThreads - 32) lse = (double)M + log_sum(S);
   __syncthreads();
   const int n = sc.n;
   if (n <= kList) {
@@ -351,22 +386,39 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) beam_select(BeamP p
   const int prompt = blockIdx.x / blocks, K = p.K, parts = 1 << log_parts, L = K << log_parts;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (blocks > 1) cl.barrier_arrive();
+  // this block's pieces of a list's row
+  auto part_of = [&](const Row<DT>& row, int list, int& q0, int& q1) {
+    const int each = (row.pieces + parts - 1) >> log_parts;
+    q0 = min(row.pieces, each * (list & (parts - 1)));
+    q1 = min(row.pieces, q0 + each);
+  };
+  // the first one's first logits are fetched beside the scores (L ≥ blocks)
+  Vec<DT> v[kBatch];
+  {
+    const Row<DT> row(p, prompt * K + (rank >> log_parts));
+    int q0, q1;
+    part_of(row, rank, q0, q1);
+    first_batch<DT, kThreads>(row, q0, q1, v);
+  }
   if (tid < K) {
     score[tid] = p.scores[prompt * K + tid];
     const bool ended = p.done && p.done[prompt * K + tid];
     kind[tid] = !isfinite(score[tid]) ? 2 : ended ? 1 : 0;
   }
   if (tid == 0) n = 0;
+  const int my_list = tid / K, my_item = tid - my_list * K;
   __syncthreads();
   bool there = blocks == 1;  // the first block is
   for (int list = rank; list < L; list += blocks) {
     const int r = prompt * K + (list >> log_parts);
     if (kind[list >> log_parts]) continue;
     const Row<DT> row(p, r);
-    const int each = (row.pieces + parts - 1) >> log_parts, q0 = min(row.pieces, each * ((list & (parts - 1))));
+    int q0, q1;
+    part_of(row, list, q0, q1);
+    if (list != rank) first_batch<DT, kThreads>(row, q0, q1, v);
     float M, S;
     double one;
-    scan<DT, kThreads>(row, q0, min(row.pieces, q0 + each), K, sc, M, S, one);
+    scan<DT, kThreads>(row, q0, q1, K, sc, v, M, S, one);
     if (!there) cl.barrier_wait();
     there = true;
     Key* to = cl.map_shared_rank(keys, 0) + list * K;
@@ -381,47 +433,44 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) beam_select(BeamP p
   if (blocks > 1) cl.sync();
   if (rank != 0) return;
 
-  if (tid < K) {
-    if (kind[tid] == 0) {
-      if (parts > 1) {
-        float m = -INFINITY, s = 0.f;
-        for (int i = 0; i < parts; ++i) m = fmaxf(m, sums[tid * parts + i].m);
-        for (int i = 0; i < parts; ++i) s += sums[tid * parts + i].s * rescale(sums[tid * parts + i].m, m);
-        lse[tid] = (double)m + log((double)s);
-      }
-      if (!isfinite(lse[tid])) kind[tid] = 2;
-    }
-  }
-  __syncthreads();
-  // item i of a list
-  auto item = [&](int list, int i) {
+  // log Σ exp of hypothesis k's logits, from its parts' sums
+  auto log_of = [&](int k) {
+    if (parts == 1) return lse[k];
+    float m = -INFINITY, s = 0.f;
+    for (int i = 0; i < parts; ++i) m = fmaxf(m, sums[k * parts + i].m);
+    for (int i = 0; i < parts; ++i) s += sums[k * parts + i].s * rescale(sums[k * parts + i].m, m);
+    return (double)m + log_sum(s);
+  };
+  // item i of a list, whose hypothesis' logarithm is `log`
+  auto item = [&](int list, int i, double log) {
     const int k = list >> log_parts;
     Item it{0ull, 0ull, k};
-    if (kind[k] == 0) {
+    if (kind[k] == 0 && isfinite(log)) {
       it.key = keys[list * K + i];
-      if (it.key) it.value = ordered((double)score[k] + ((double)logit_of(it.key) - lse[k]));
+      if (it.key) it.value = ordered((double)score[k] + ((double)logit_of(it.key) - log));
     } else if ((list & (parts - 1)) == 0) {  // one list: eos first, then the other tokens
-      int token = i;
-      if (kind[k] == 1) {
-        token = i == 0 ? p.eos : i - 1 + (i - 1 >= p.eos);
-      }
-      it.value = ordered(i == 0 && kind[k] == 1 ? score[k] : -INFINITY);
-      it.key = (unsigned)~(unsigned)token | (Key)(i == 0 && kind[k] == 1) << 32;
+      const bool ended = kind[k] == 1;
+      const int token = !ended ? i : i == 0 ? p.eos : i - 1 + (i - 1 >= p.eos);
+      it.value = ordered(ended && i == 0 ? score[k] : -INFINITY);
+      it.key = (unsigned)~(unsigned)token | (Key)(ended && i == 0) << 32;
     }
     return it;
   };
-  // few items: all; of many those that the K-th of the lists' first ones does not come before
-  if (L * K <= 256) {
-    for (int i = tid; i < L * K; i += kThreads) kept[i] = item(i / K, i % K);
+  if (L * K <= 256) {  // one a thread
+    if (tid < L * K) kept[tid] = item(my_list, my_item, kind[my_list >> log_parts] ? 0. : log_of(my_list >> log_parts));
     if (tid == 0) n = L * K;
   } else {
-    if (tid < L) heads[tid] = item(tid, 0);
+    // of many items those that the K-th of the lists' first ones does not come before
+    __syncthreads();
+    if (tid < K && parts > 1 && kind[tid] == 0) lse[tid] = log_of(tid);
+    __syncthreads();
+    if (tid < L) heads[tid] = item(tid, 0, lse[tid >> log_parts]);
     __syncthreads();
     for_ranks<kThreads>(L, [&](int i, int j) { return ahead(heads[j], heads[i]) || (j < i && !ahead(heads[i], heads[j])); },
                         [&](int i, int r) { if (r == K - 1) limit = heads[i]; });
     __syncthreads();
     for (int i = tid; i < L * K; i += kThreads) {
-      const Item it = item(i / K, i % K);
+      const Item it = item(i / K, i % K, lse[i / K >> log_parts]);
       if (it.key && !ahead(limit, it)) kept[atomicAdd(&n, 1)] = it;
     }
   }
