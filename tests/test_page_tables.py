@@ -259,6 +259,58 @@ def test_captured_and_on_another_stream():
         assert [tuple(x) for x in out[1].tolist()] == copies
 
 
+@gpu
+def test_copies_captured_behind_anything():
+    """``copy_pages`` (and ``reserve`` with many rows) as a graph's first node, behind a copy,
+    behind a kernel of another library, and where two streams meet."""
+    pool = torch.arange(10 * 64, device="cuda", dtype=torch.int32).view(10, 64)
+    first, pairs, other = int32([[0, 3], [1, 4]]), int32([[-1, -1], [-1, -1]]), torch.zeros(64, device="cuda")
+    table, refs, t, n = torch.full((2, 600), -1, dtype=torch.int32, device="cuda"), int32([0] * 1300), int32([0, 0]), int32([5000, 4000])
+    paged.copy_pages([pool], pairs), paged.reserve(table, t, n, refs, 16, rows=9000)
+    table.fill_(-1), refs.zero_()
+    side = torch.cuda.Stream()
+
+    def alone():
+        paged.copy_pages([pool], first)
+
+    def behind_a_copy():
+        pairs.copy_(first)
+        paged.copy_pages([pool], pairs)
+
+    def behind_a_kernel():
+        other.add_(1)
+        paged.copy_pages([pool], first)
+
+    def behind_two_streams():
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            other.mul_(2)
+        pairs.copy_(first)
+        here.wait_stream(side)
+        paged.copy_pages([pool], pairs)
+
+    def reserved():
+        table.fill_(-1)
+        refs.zero_()
+        return paged.reserve(table, t, n, refs, 16, rows=9000)
+
+    for run in (alone, behind_a_copy, behind_a_kernel, behind_two_streams, reserved):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        for i in range(3):
+            pool.copy_(torch.randint(0, 1000, pool.shape, device="cuda", dtype=torch.int32))
+            want = pool.clone()
+            if run is not reserved:
+                want[3], want[4] = want[0], want[1]
+            graph.replay()
+            assert torch.equal(pool, want), run.__name__
+        if run is reserved:
+            assert out.cu_rows.tolist() == [0, 5000, 9000] and int(refs.sum()) == 313 + 250
+            assert torch.equal(out.slot, table.view(-1)[out.seq.long() * 600 + out.pos // 16] * 16 + out.pos % 16)
+
+
 # ── refusals ──
 
 @gpu
