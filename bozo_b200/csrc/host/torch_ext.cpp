@@ -352,6 +352,16 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Device& d
   return at::detail::empty_cuda(shape, type, dev, c10::nullopt);
 }
 
+// A contiguous tensor of its own in `all`'s memory, from byte `at` on (a multiple of its
+// type's size): several results of a call from one allocation.
+at::Tensor part_of(const at::Tensor& all, int64_t at, at::ScalarType type, at::IntArrayRef shape) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                          c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_storage_offset(at / (int64_t)c10::elementSize(type));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+  return t;
+}
+
 // [rows, heads, HD] (any strides) as the ABI's [rows, 1, heads, HD] view
 bozo_tensor4 rows_view(const char* what, const char* name, const at::Tensor& t, const bozo_paged_cache& c,
                        int64_t rows, int64_t heads, const at::Device& dev) {
@@ -546,15 +556,10 @@ pybind11::tuple paged_reserve(const at::Tensor& table, const at::Tensor& lengths
   const c10::cuda::CUDAGuard guard(dev);
   if (given(tokens)) a.tokens = per_row(what, "tokens", *tokens, lengths);
   if (rows < -1 || rows > INT32_MAX) throw std::invalid_argument("reserve: rows must not be negative, nor pass 2^31");
-  // one allocation: seq, pos and slot (16-byte aligned), cu_rows, missing
+  // seq, pos and slot (16-byte aligned), cu_rows, missing
   const int64_t n = rows > 0 ? (rows + 3) / 4 * 4 : 0, count = (int64_t)a.batch + 1;
   const at::Tensor all = empty({3 * n + count + 1}, at::kInt, dev);
-  auto part = [&](int64_t at, int64_t size) {
-    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
-    t.unsafeGetTensorImpl()->set_storage_offset(at);
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
-    return t;
-  };
+  auto part = [&](int64_t at, int64_t size) { return part_of(all, 4 * at, at::kInt, {size}); };
   at::Tensor cu = part(3 * n, count), missing = part(3 * n + count, 1), at_[3];
   a.cu_rows = cu.data_ptr<int32_t>();
   a.missing = missing.data_ptr<int32_t>();
@@ -581,7 +586,8 @@ std::tuple<at::Tensor, at::Tensor> paged_fork(const at::Tensor& table, const at:
   a.parents = per_row(what, "parents", parents, lengths);
   a.share = share;
   const int64_t n = share ? (int64_t)a.batch : (int64_t)a.batch * a.width;
-  at::Tensor copies = empty({n, 2}, at::kInt, dev), missing = empty({1}, at::kInt, dev);
+  const at::Tensor all = empty({2 * n + 1}, at::kInt, dev);
+  at::Tensor copies = part_of(all, 0, at::kInt, {n, 2}), missing = part_of(all, 8 * n, at::kInt, {1});
   a.copies = copies.data_ptr<int32_t>();
   a.missing = missing.data_ptr<int32_t>();
   check(bozo_paged_fork(&a, at::cuda::getCurrentCUDAStream(dev.index()).stream()), "bozo_paged_fork");
@@ -649,7 +655,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> beam_select(const at::Tensor& log
   a.eos = (int32_t)eos;
   a.scores = scores.data_ptr<float>();
   a.done = d ? static_cast<const uint8_t*>(d->data_ptr()) : nullptr;
-  at::Tensor s = empty({N, K}, at::kFloat, dev), t = empty({N, K}, at::kLong, dev), r = empty({N, K}, at::kInt, dev);
+  const at::Tensor all = empty({N * K * 16}, at::kByte, dev);
+  at::Tensor t = part_of(all, 0, at::kLong, {N, K}), s = part_of(all, 8 * N * K, at::kFloat, {N, K}),
+             r = part_of(all, 12 * N * K, at::kInt, {N, K});
   a.out_scores = s.data_ptr<float>();
   a.out_tokens = t.data_ptr<int64_t>();
   a.out_rows = r.data_ptr<int32_t>();
