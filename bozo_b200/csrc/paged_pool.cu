@@ -17,7 +17,17 @@ namespace {
 
 namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
-constexpr int kSmallPool = 16384;  // pages that one block counts
+// One block does without the cluster's barrier; eight count the pages faster.  In a graph, µs,
+// one | eight, 4 and 64 sequences that all need a page: 1024 pages 4.4, 5.0 | 6.3, 6.9; 8192
+// 5.4, 7.4 | 6.4, 7.4; 16000 5.8, 9.8 | 6.7, 7.9; 64000 12.1, 29.3 | 7.6, 9.0.
+constexpr int kReservePool = 8192;
+// A fork has the table to move as well, every second row a copy: 32 × 64 entries over 2400
+// pages 6.9 | 7.8, over 16000 7.7 | 8.2, over 64000 13.4 | 8.4; 64 × 64 over 16000 8.6 | 8.2
+// (5.5 | 4.1 where nothing forks), 128 × 64 11.6 | 9.2.
+constexpr int kForkPool = 16384, kForkTable = 2048;
+// Rows whose places the cluster's first kernel writes itself; a second kernel has all SMs but
+// has to start: 1024 rows 4.1 | 6.1, 2048 5.2 | 6.5, 4096 7.4 | 7.1, 16384 21.2 | 10.4.
+constexpr int kPlacesHere = 4096;
 
 // Sums over the block's threads, one barrier each: every warp adds the warps' totals up
 // for itself, and two buffers take turns, so that none is written while it is read.
@@ -416,8 +426,8 @@ cudaError_t launch_after(void (*kern)(P), dim3 grid, int threads, cudaStream_t s
 }  // namespace
 
 cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launches) {
-  const int blocks = p.P <= kSmallPool ? 1 : 8;
-  const bool here = p.rows <= 4096;
+  const int blocks = p.P <= kReservePool ? 1 : 8;
+  const bool here = p.rows <= kPlacesHere;
   cudaError_t e = launch_cluster(paged_reserve, blocks, (size_t)(4 * p.B + 2) * sizeof(int), st, p, here);
   *launches = here ? 1 : 2;
   if (e != cudaSuccess || here) return e;
@@ -427,7 +437,7 @@ cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launch
 
 cudaError_t launch_paged_fork(const ForkP& p, cudaStream_t st) {
   // small tables: one block, whole; else a sector's worth of columns, fewer where the rows are many
-  const bool small = p.P <= kSmallPool && (long long)p.B * p.M <= 8192;
+  const bool small = p.P <= kForkPool && (long long)p.B * p.M <= kForkTable;
   const int tile = small ? p.M : p.B <= 2048 ? 8 : p.B <= 4096 ? 2 : 1;
   return launch_cluster(paged_fork, small ? 1 : 8, ((size_t)6 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
                         make_fastdiv((unsigned)tile));
