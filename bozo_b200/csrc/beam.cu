@@ -522,12 +522,18 @@ cudaError_t launch(const BeamP& p, int log_parts, int blocks, cudaStream_t st) {
 
 template <int DT, bool AL>
 cudaError_t launch(const BeamP& p, int sms, cudaStream_t st) {
-  // a row is shared out where there are fewer rows than SMs, while 256 threads have a piece each
+  // A row is shared out where there are fewer rows than SMs; rows up to 32 KB are not worth the
+  // larger cluster.  In a graph, µs, whole | parts:
+  // bf16 1 × 1 × 8192 4.4 | 5.6, 1 × 4 × 16384 5.6 | 5.7, 1 × 4 × 32768 7.6 | 6.4, 1 × 1 × 32768
+  // 6.3 | 5.6; fp32 1 × 1 × 8192 4.6 | 5.3, 1 × 4 × 16384 6.8 | 5.9.
   int parts = 1, log_parts = 0;
-  while (parts * 2 * p.K <= kParts && p.N * p.K * parts * 2 <= sms && p.V > parts * 256 * Vec<DT>::N) parts *= 2, ++log_parts;
+  while (p.V > 2048 * Vec<DT>::N && parts * 2 * p.K <= kParts && p.N * p.K * parts * 2 <= sms) parts *= 2, ++log_parts;
   const int blocks = std::min(p.K * parts, kCluster);
-  // long rows in few blocks: more threads
-  if (2 * p.N * blocks <= sms && p.V / parts >= 4096 * Vec<DT>::N) return launch<DT, 1024, AL>(p, log_parts, blocks, st);
+  // Long rows in few blocks: more threads, which also share the elements above the bound out,
+  // many with many hypotheses.  256 | 1024 threads, bf16: 1 × 8 × 32768 7.2 | 8.0, × 98304
+  // 11.3 | 12.4, × 131072 13.2 | 11.8; 1 × 16 × 32768 15.9 | 11.3, 1 × 32 × 16384 15.3 | 15.2;
+  // 4 × 4 × 131072 in two parts 9.0 | 9.8, × 262144 15.7 | 13.0; in 64 blocks (16 × 4 × 32768) 7.0 | 14.3.
+  if (2 * p.N * blocks <= sms && p.V / parts >= (p.K > 8 ? 4096 : 16384) * Vec<DT>::N) return launch<DT, 1024, AL>(p, log_parts, blocks, st);
   return launch<DT, 256, AL>(p, log_parts, blocks, st);
 }
 
