@@ -153,6 +153,15 @@ int check_aux(const A* a) {
   return BOZO_OK;
 }
 
+// The group scales of 4-bit pages.  A caller that knows no such pages may pass a block
+// that ends before them: they are read for such pages only.
+struct PagedGroups {
+  uint8_t *k = nullptr, *v = nullptr;
+  template <typename A> explicit PagedGroups(const A* a) {
+    if (a->cache.dtype == BOZO_DT_F4E2M1) k = a->k_group, v = a->v_group;
+  }
+};
+
 }  // namespace
 }  // namespace bozo
 
@@ -502,7 +511,7 @@ int bozo_tension_decode(const bozo_tension_decode_args* a, void* stream) {
   return BOZO_OK;
 }
 
-static int check_paged(const bozo_paged_cache& c, const uint8_t* kg, const uint8_t* vg) {
+static int check_paged(const bozo_paged_cache& c, const PagedGroups& g) {
   if (c.pages <= 0 || c.kv_heads <= 0 || c.page_size <= 0 || c.HD <= 0 || c.batch <= 0 ||
       c.width <= 0 || c.table_stride < 0)
     return BOZO_ERR_BAD_SHAPE;
@@ -516,11 +525,11 @@ static int check_paged(const bozo_paged_cache& c, const uint8_t* kg, const uint8
     return BOZO_ERR_UNSUPPORTED;
   if (!c.k_pages || !c.v_pages || !c.table || !c.lengths) return BOZO_ERR_NULL;
   if (scaled && (!c.k_scale || !c.v_scale)) return BOZO_ERR_NULL;
-  if (four && (!kg || !vg)) return BOZO_ERR_NULL;
+  if (four && (!g.k || !g.v)) return BOZO_ERR_NULL;
   if (!scaled && (c.k_scale || c.v_scale)) return BOZO_ERR_BAD_SHAPE;
   if ((reinterpret_cast<uintptr_t>(c.k_pages) | reinterpret_cast<uintptr_t>(c.v_pages)) & 15)
     return BOZO_ERR_ALIGNMENT;
-  if (four && ((reinterpret_cast<uintptr_t>(kg) | reinterpret_cast<uintptr_t>(vg) |
+  if (four && ((reinterpret_cast<uintptr_t>(g.k) | reinterpret_cast<uintptr_t>(g.v) |
                 reinterpret_cast<uintptr_t>(c.k_scale) | reinterpret_cast<uintptr_t>(c.v_scale)) & 15))
     return BOZO_ERR_ALIGNMENT;
   return BOZO_OK;
@@ -535,8 +544,9 @@ static int check_rope(int len, const float* cos, const float* sin, int HD) {
 
 int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
+  const PagedGroups groups(a);
   int st;
-  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
+  if ((st = check_paged(a->cache, groups))) return st;
   if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
     return BOZO_ERR_BAD_SHAPE;
   if ((st = check_rope(a->rope_len, a->rope_cos, a->rope_sin, a->cache.HD))) return st;
@@ -545,7 +555,7 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
   DeviceRestore restore;
   cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
-  PagedP p = paged_params(a->cache, a->k_group, a->v_group);
+  PagedP p = paged_params(a->cache, groups.k, groups.v);
   p.rows = a->rows; p.cu = a->cu_rows;
   p.rope_len = a->rope_len;
   p.cos = a->rope_len ? a->rope_cos : nullptr;
@@ -561,8 +571,9 @@ int bozo_paged_write(const bozo_paged_write_args* a, void* stream) {
 
 int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   if (!a) return BOZO_ERR_NULL;
+  const PagedGroups groups(a);
   int st;
-  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
+  if ((st = check_paged(a->cache, groups))) return st;
   if (a->rows < 0 || a->rows > 0x7fffffffLL || (!a->cu_rows && a->rows != a->cache.batch))
     return BOZO_ERR_BAD_SHAPE;
   if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
@@ -571,7 +582,7 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
   DeviceRestore restore;
   cudaError_t e = a->cache.device_current ? cudaSuccess : bind_device(a->cache.k_pages, restore);
   if (e != cudaSuccess) return cuda_fail(e);
-  PagedP p = paged_params(a->cache, a->k_group, a->v_group);
+  PagedP p = paged_params(a->cache, groups.k, groups.v);
   p.rows = a->rows; p.cu = a->cu_rows;
   p.k_out = a->k_out; p.v_out = a->v_out; p.out_dt = a->out_dtype;
   if (!(p.err = error_word(&e))) return cuda_fail(e);
@@ -585,8 +596,9 @@ int bozo_paged_read(const bozo_paged_read_args* a, void* stream) {
 // The decode step's parameters (no device needed): checks first.
 static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
   if (!a) return BOZO_ERR_NULL;
+  const PagedGroups groups(a);
   int st;
-  if ((st = check_paged(a->cache, a->k_group, a->v_group))) return st;
+  if ((st = check_paged(a->cache, groups))) return st;
   const bozo_paged_cache& c = a->cache;
   if (a->H <= 0 || a->H % c.kv_heads) return BOZO_ERR_BAD_SHAPE;
   if ((long long)c.batch * a->H > 0x7fffffffLL / 4096) return BOZO_ERR_UNSUPPORTED;
@@ -606,7 +618,7 @@ static int paged_decode_params(const bozo_paged_decode_args* a, PagedP& p) {
   if (!dtype_ok(a->out_dtype)) return BOZO_ERR_BAD_DTYPE;
   if (a->tau && (!dtype_ok(a->tau_dtype) || a->tau_width < 1)) return BOZO_ERR_BAD_SHAPE;
   if (a->mode == BOZO_MODE_LOCAL && a->tau && a->tau_width != a->window) return BOZO_ERR_BAD_SHAPE;
-  p = paged_params(c, a->k_group, a->v_group);
+  p = paged_params(c, groups.k, groups.v);
   p.rows = c.batch;
   p.rope_len = a->rope_len;
   p.cos = a->rope_len ? a->rope_cos : nullptr;

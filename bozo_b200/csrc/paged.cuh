@@ -47,7 +47,7 @@ struct PagedP {
 
 inline PagedP paged_params(const bozo_paged_cache& c, unsigned char* kg, unsigned char* vg) {
   PagedP p{};
-  if (c.dtype == BOZO_DT_F4E2M1) p.kg = kg, p.vg = vg;
+  p.kg = kg; p.vg = vg;
   p.k = c.k_pages; p.v = c.v_pages; p.ks = c.k_scale; p.vs = c.v_scale;
   p.dt = c.dtype; p.P = c.pages; p.Hk = c.kv_heads; p.page = c.page_size; p.HD = c.HD;
   p.B = c.batch; p.M = c.width;
