@@ -1,5 +1,5 @@
 // paged_mma.cuh — the tensor-core kernel of a decode step over a paged cache:
-// 16- and 8-bit pages, head widths 32, 64 and 128.
+// 16-, 8- and 4-bit pages, head widths 32, 64 and 128.
 //
 // One block per (b, key head, up to 8 of its query heads, piece).  Each warp walks
 // tiles of its own through a ring in shared memory that 16-byte asynchronous
@@ -136,9 +136,11 @@ __device__ __forceinline__ unsigned group_pair(unsigned x) {
   return w;
 }
 __device__ __forceinline__ float2 halves(unsigned x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
-// τ · unit · kGroupUnit times a group's scale (≤ 448) stays under 65504, and keeps 2^-24
-// of it where the scale is 2^-6 of the row's largest.
-constexpr float kGroupUnit = 0x1p-6f;
+// τ · unit · kGroupUnit times a group's scale (≤ 448) stays under 65504.  Its rest beside
+// the half goes in times kRest, in a column of its own: with the smallest group scale, 2^-9,
+// the largest τ of a head gives at least 2^-15, which is then held to 2^-36 (without kRest to
+// 2^-25: columns whose groups are far below their rows' largest were off by up to 2^-10).
+constexpr float kGroupUnit = 0x1p-6f, kRest = 0x1p11f;
 __device__ __forceinline__ unsigned two_halves(float x, float y) {
   unsigned w;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(y), "f"(x));
@@ -916,7 +918,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP, KEYS>::block
               const float x = __uint_as_float(pk[0]) * f.x, y = __uint_as_float(pk[1]) * f.y;
               const unsigned hi = two_halves(x, y);
               const float2 h = halves(hi);
-              const unsigned lo = two_halves(x - h.x, y - h.y);
+              const unsigned lo = two_halves((x - h.x) * kRest, (y - h.y) * kRest);
               const unsigned got = __shfl_xor_sync(0xffffffffu, odd ? hi : lo, 4);
               b0 = odd ? got : hi;
               b1 = odd ? lo : got;
@@ -1059,14 +1061,14 @@ __global__ void __launch_bounds__(kWarps * 32 + 32, Geo<DT, HD, GP, KEYS>::block
   } else if constexpr (TURN) {
     // this lane's columns: of these elements' group, or of head c
     if ((LONE ? c == (GB == 2 ? g >> 2 : g >> 1) : c < Gh) && warp < kWarps) {
-      const float back = 1.f / (LONE ? unit[0] * kGroupUnit : unit[0]);
+      const float back = 1.f / (LONE ? unit[0] * kGroupUnit : unit[0]), rest = LONE ? 1.f / kRest : 1.f;
       constexpr int kBytes = GB == 2 ? 2 : 4;
 #pragma unroll
       for (int j = 0; j < kAcc; ++j) {
         const int d = j / kBytes * 64 + 2 * kBytes * g + 2 * (j % kBytes);
         float* to = part + (warp * Gh + (LONE ? 0 : c)) * HD + d;
-        to[0] = (acc[j][0] + acc[j][1]) * back;
-        to[1] = (acc[j][2] + acc[j][3]) * back;
+        to[0] = fmaf(acc[j][1], rest, acc[j][0]) * back;
+        to[1] = fmaf(acc[j][3], rest, acc[j][2]) * back;
       }
     }
   } else if (hrow < Gh && warp < kWarps) {

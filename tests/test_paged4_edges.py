@@ -1,10 +1,25 @@
-"""4-bit paged caches at the edges of their interface: argument blocks of hosts that know no
-group scales."""
+"""4-bit paged caches at their edges: argument blocks of hosts that know no group scales,
+rows whose groups are of very different sizes."""
 import ctypes as C
+import math
 import subprocess
 import sys
 
-from bozo_b200 import _capi
+import pytest
+import torch
+
+from bozo_b200 import _capi, paged
+from oracle import paged_oracle as orc
+from test_paged import history, int32, offsets
+from test_paged4 import Pool4
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def seeded():
+    torch.manual_seed(0)
+
 
 ENTRY = {"write": ("bozo_paged_write", _capi.PagedWriteArgs), "read": ("bozo_paged_read", _capi.PagedReadArgs),
          "decode": ("bozo_paged_decode", _capi.PagedDecodeArgs),
@@ -57,3 +72,53 @@ def test_blocks_of_other_pages_may_end_before_the_group_scales():
     # all checks passed, up to the pointers, which are not a device's (the query needs no device)
     for entry in ("write", "read", "decode"):
         assert [int(x) for x in got[entry].split()] == [BOZO_ERR_CUDA] * len(OTHERS), entry
+
+
+# ── groups of different sizes in one row ──
+
+def sized_rows(rows, Hk, HD, small, mixed, seed):
+    """Normal rows whose groups but one are 2^-small of it (`mixed`: that one changes from
+    key to key, so every group is large somewhere)."""
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(rows, Hk, HD // 16, 16, generator=g, device="cuda")
+    large = torch.zeros(rows, dtype=torch.long, device="cuda")
+    if mixed:
+        large = torch.randint(0, HD // 16, (rows,), generator=g, device="cuda")
+    size = torch.full((rows, HD // 16), 2.0 ** -small, device="cuda").scatter_(1, large[:, None], 1.0)
+    return (x * size[:, None, :, None]).flatten(-2)
+
+
+@gpu
+@pytest.mark.parametrize("small", [4, 8, 11, 14, 17])
+@pytest.mark.parametrize("H,Hk", [(2, 2), (4, 2), (8, 2), (7, 1)])
+@pytest.mark.parametrize("HD,page", [(64, 16), (32, 16), (128, 16), (64, 8), (128, 5), (32, 5), (48, 16)])
+def test_small_groups_keep_their_precision(HD, page, H, Hk, small):
+    """|err| ≤ 1e-5 · the column's own largest |v|, whatever the row's other groups hold.
+
+    Queries of a quarter keep Σ|q·k| / √HD under 2, so with mass normalisation the parts are:
+    q as two halfs, 2^-23 of each term, and a score's sums, a dozen additions of 2^-23: dz <
+    3e-6, which moves τ by (1 − τ)·dz and the quotient by twice that, < 4.5e-6; the sigmoid's
+    two approximations, 2^-21, twice: 1e-6; τ (times the row's scale) as two halfs, 2^-21 of
+    the largest, which is at most 3 times the mean: 1.5e-6; sums of products, of warps and
+    pieces, a dozen additions: 1.5e-6; the result's own 2^-24.  Below 1e-5 together."""
+    lengths = [0, 39, 299]
+    pool = Pool4(3, Hk, HD, page, -(-300 // page))
+    counts = [n + 1 for n in lengths]
+    for mixed in (False, True):
+        k = sized_rows(sum(counts), Hk, HD, small, mixed, HD + small)
+        v = sized_rows(sum(counts), Hk, HD, small, mixed, HD + small + 1)
+        paged.write_kv(k, v, *pool.cache, int32([0] * 3), cu_rows=int32(offsets(counts)), **pool.scales)
+        hist = history(pool, counts, Hk, HD)
+        q = torch.randn(3, H, HD, device="cuda") * 0.25
+        for window in (None, 24):
+            out = paged.paged_tension(q, *pool.cache, int32(lengths), window=window, **pool.scales)
+            ref, _ = orc.decode(q.cpu().double(), hist, lengths, window=window, capacity=pool.cap, scale=math.sqrt(HD),
+                                normalize="mass", tau_width=0)
+            for b, t in enumerate(lengths):
+                lo, end = (0, t + 1) if window is None else (max(0, t - window), t)
+                if end == lo:
+                    assert (out[b] == 0).all()
+                    continue
+                top = hist[b][1][lo:end].abs().amax(0).repeat_interleave(H // Hk, dim=0)   # [H, HD]
+                err = (out[b].cpu().double() - ref[b]).abs()
+                assert bool((err <= 1e-5 * top).all()), (b, float((err / top.clamp(min=1e-30)).max()))
