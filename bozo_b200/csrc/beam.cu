@@ -480,17 +480,16 @@ __global__ void __launch_bounds__(kThreads, 1024 / kThreads) beam_select(BeamP p
     if (tid < L * K) kept[tid] = item(my_list, my_item, kind[my_list >> log_parts] ? 0. : log_of(my_list >> log_parts));
     if (tid == 0) n = L * K;
   } else {
-    // of many items those that the K-th of the lists' first ones does not come before
+    // of many items, of hypotheses that are not shared out in parts, those that the K-th of
+    // the lists' first ones does not come before
+    static_assert(kParts * kParts <= 256, "up to kParts lists of as many items");
+    if (tid < K) heads[tid] = item(tid, 0, lse[tid]);
     __syncthreads();
-    if (tid < K && parts > 1 && kind[tid] == 0) lse[tid] = log_of(tid);
-    __syncthreads();
-    if (tid < L) heads[tid] = item(tid, 0, lse[tid >> log_parts]);
-    __syncthreads();
-    for_ranks<kThreads>(L, [&](int i, int j) { return ahead(heads[j], heads[i]) || (j < i && !ahead(heads[i], heads[j])); },
+    for_ranks<kThreads>(K, [&](int i, int j) { return ahead(heads[j], heads[i]) || (j < i && !ahead(heads[i], heads[j])); },
                         [&](int i, int r) { if (r == K - 1) limit = heads[i]; });
     __syncthreads();
-    for (int i = tid; i < L * K; i += kThreads) {
-      const Item it = item(i / K, i % K, lse[i / K >> log_parts]);
+    for (int i = tid; i < K * K; i += kThreads) {
+      const Item it = item(i / K, i % K, lse[i / K]);
       if (it.key && !ahead(limit, it)) kept[atomicAdd(&n, 1)] = it;
     }
   }
