@@ -368,6 +368,7 @@ class PagedStepGraph:
 
     def __init__(self, state: PagedState, export: bool = False, warmup: int = 2):
         self.state = state
+        state._grow({})  # refused by states that are not fed slot by slot
         dev = state.lengths.device
         self.tokens = torch.zeros(state.slots, dtype=torch.long, device=dev)
         held = state.lengths.clone()
@@ -457,7 +458,9 @@ class BeamState(PagedState):
     ``paged.fork``): hypotheses share the full pages of what they have in common, and
     the rings of local layers move or are copied with them.  ``start`` takes the
     prompts, ``advance`` adds a token to every hypothesis (a replayed CUDA graph unless
-    ``graph=False``), ``results`` reads what was found.
+    ``graph=False``), ``results`` reads what was found.  The calls for single slots
+    (``admit``, ``extend``, ``step``, ``PagedStepGraph``, ``release`` and the like) are
+    refused.
 
     max_len : longest prompt with its new tokens; with global layers at most
               ``max_seq_len``, since shared pages cannot be rings.
@@ -505,8 +508,15 @@ class BeamState(PagedState):
             self._graph = captured
         self.taken = 0
 
-    def release(self, slot: int) -> None:
-        raise RuntimeError("a beam search's slots are given up together: start() takes new prompts")
+    # What counts slots and pages on the host (admit, extend, step, PagedStepGraph, release)
+    # knows nothing of the device's counts.
+
+    def _together(self, *_) -> None:
+        raise RuntimeError("a beam search's slots are taken, fed and given up together: start() takes new "
+                           "prompts, advance() adds a token to all")
+
+    length = release = _grow = _together
+    idle = free_pages = property(_together)
 
     @torch.no_grad()
     def start(self, prompts: Sequence[Sequence[int]]) -> None:
