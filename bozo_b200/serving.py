@@ -506,7 +506,6 @@ class BeamState(PagedState):
             with torch.cuda.graph(captured):
                 self._advance()
             self._graph = captured
-        self.taken = 0
 
     # What counts slots and pages on the host (admit, extend, step, PagedStepGraph, release)
     # knows nothing of the device's counts.
@@ -530,6 +529,7 @@ class BeamState(PagedState):
         T = max(lens)
         ids = torch.tensor([list(p) + [0] * (T - m) for p, m in zip(prompts, lens)], device=dev)
         n = torch.tensor(lens, device=dev)
+        self.taken = 0  # a call that fails from here on leaves nothing to advance
         for g in self.pools:
             self.tables[g].fill_(-1)
             self.refs[g].zero_()
@@ -547,19 +547,24 @@ class BeamState(PagedState):
         if self.done is not None:
             self.done.zero_()
         self.steps.zero_()
-        self.taken, self.longest = 0, T
+        self.longest = T
         self._choose(logits.repeat_interleave(K, 0))
+        self.taken = 1
+
+    def _started(self) -> None:
+        if not self.taken:
+            raise RuntimeError("nothing is searched: start() takes the prompts first")
 
     def advance(self) -> None:
         """Feed every hypothesis its token and choose the best continuations."""
-        if not self.taken:
-            raise RuntimeError("advance: start() takes the prompts first")
+        self._started()
         self._check(self.longest + self.taken)
+        taken, self.taken = self.taken, 0  # as in start()
         if self._graph is not None:
             self._graph.replay()
-            self.taken += 1
         else:
             self._advance()
+        self.taken = taken + 1
         ops.check_device_error(self.lengths.device)
 
     def _reserve(self, glob: bool, tokens: Optional[Tensor], rows: Optional[int] = None) -> paged.Plan:
@@ -585,13 +590,12 @@ class BeamState(PagedState):
         self.tokens.copy_(tokens.view(-1))
         self.chosen.index_copy_(0, self.steps, torch.stack([self.tokens, at]).unsqueeze(0))
         self.steps += 1
-        if not torch.cuda.is_current_stream_capturing():
-            self.taken += 1
 
     def results(self, length_penalty: float = 0.0) -> List[List[Tuple[List[int], float]]]:
         """For each prompt its hypotheses' new ids (up to and with ``eos``) and scores, each
         the sum of log probabilities over (number of new ids) ^ ``length_penalty``, best
         first."""
+        self._started()
         tokens, rows = self.chosen[:self.taken].cpu().unbind(1)
         scores, out = self.scores.tolist(), []
         for n in range(self.prompts):

@@ -36,3 +36,47 @@ def test_calls_for_single_slots_are_refused(name):
                 call()
         assert all(torch.equal(a, b) for a, b in zip(held(state), before))
     state.advance()
+
+
+@gpu
+@pytest.mark.parametrize("graph", [False, True])
+def test_a_state_without_prompts_has_nothing_to_say(graph, monkeypatch):
+    """Before ``start``, and after a call that failed midway, there is nothing to advance or to
+    return; refused prompts leave the running search as it was."""
+    model = make("rope_global")
+    state = serving.BeamState(model, 2, 3, 40, graph=graph)
+    prompts = [ids(7, 1, 60), ids(20, 2, 60)]
+
+    def empty():
+        for call in (state.advance, state.results, lambda: state.results(1.0)):
+            with pytest.raises(RuntimeError, match="start"):
+                call()
+
+    empty()
+    state.start(prompts)
+    state.advance()
+    want = state.results()
+    with pytest.raises(ValueError, match="prompts"):
+        state.start(prompts[:1])
+    assert state.results() == want
+
+    def fails(*args):
+        raise MemoryError("no room")
+
+    with monkeypatch.context() as m:
+        m.setattr(serving, "_prefill", fails)
+        with pytest.raises(MemoryError):
+            state.start(prompts)
+    empty()
+    state.start(prompts)
+    state.advance()
+    assert state.results() == want
+    if not graph:
+        with monkeypatch.context() as m:
+            m.setattr(serving.paged, "copy_pages", fails)      # tables moved, pages not
+            with pytest.raises(MemoryError):
+                state.advance()
+        empty()
+        state.start(prompts)
+        state.advance()
+        assert state.results() == want
