@@ -619,11 +619,11 @@ def beam_search(model, prompts: Sequence[Sequence[int]], beams: int = 4, max_new
                 page_size: int = 16, graph: bool = True) -> List[List[Tuple[List[int], float]]]:
     """The ``beams`` best continuations of each prompt by beam search, ``batch`` prompts at
     a time: for each prompt ``(new ids, score)``, best first, as ``BeamState.results``
-    returns them.  Prompts longer than ``max_seq_len − max_new`` keep their last ids where
-    the model has global layers or learned positions."""
+    returns them.  Longer prompts keep their last ``max_seq_len`` ids, or their last
+    ``max_seq_len − max_new + 1`` where the model has global layers or learned positions."""
     model.eval()
-    if max_new < 1:
-        raise ValueError("max_new must be at least 1")
+    if max_new < 1 or batch < 1:
+        raise ValueError("max_new and batch must be at least 1")
     cfg, out = model.cfg, []
     bounded = not cfg.use_rope or any(b.global_layer for b in model.blocks)
     limit = cfg.max_seq_len - max_new + 1 if bounded else cfg.max_seq_len

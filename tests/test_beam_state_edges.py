@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from bozo_b200 import serving
-from test_beam_search import ids, make, plain_matmuls  # noqa: F401 (the fixture)
+from test_beam_search import CFGS, ids, make, plain_matmuls  # noqa: F401 (the fixture)
 
 gpu = pytest.mark.gpu
 
@@ -80,3 +80,27 @@ def test_a_state_without_prompts_has_nothing_to_say(graph, monkeypatch):
         state.start(prompts)
         state.advance()
         assert state.results() == want
+
+
+@gpu
+def test_search_refuses_batches_of_nothing():
+    model = make("all_global")
+    for batch in (0, -1, -16):                     # −1 returned no result for any prompt
+        with pytest.raises(ValueError, match="batch must be at least 1"):
+            serving.beam_search(model, [[1, 2], [3]], 2, 4, batch=batch)
+
+
+@gpu
+@pytest.mark.parametrize("name,bounded", [("rope_global", True), ("norope_osc", True), ("rope_local", False)])
+def test_long_prompts_keep_their_last_ids(name, bounded, monkeypatch):
+    """The last id that is fed takes the last position: max_seq_len − max_new + 1 ids of the
+    prompt where positions are bounded, max_seq_len else."""
+    monkeypatch.setitem(CFGS, "rope_local", dict(CFGS["rope_global"], global_every=0))
+    model = make(name)
+    limit, vocab, steps = model.cfg.max_seq_len, model.cfg.vocab_size, 6
+    keep = limit - steps + 1 if bounded else limit
+    taken, start = [], serving.BeamState.start
+    monkeypatch.setattr(serving.BeamState, "start", lambda self, p: (taken.append(p), start(self, p))[1])
+    prompts = [ids(n, n, vocab) for n in (limit + 9, keep, keep + 1, 5)]
+    found = serving.beam_search(model, prompts, 2, steps, graph=False)
+    assert taken == [[p[-keep:] for p in prompts]] and all(len(new) == steps for f in found for new, _ in f)
