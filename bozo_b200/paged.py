@@ -188,8 +188,9 @@ def fork(page_table: Tensor, lengths: Tensor, parents: Tensor, refs: Tensor, pag
 
     Returns ``copies`` (int32, ``[B, 2]`` or ``[B · M, 2]``: page to copy and its copy, −1
     where there is none) for ``copy_pages``, and ``missing [1]``: pages that were not there
-    (the last rows then lack theirs).  As long as no more rows hold a sequence than before
-    the pages given up suffice.  Free pages are given in ascending order."""
+    (the last rows then lack theirs; never where the pool has a page for every entry of the
+    table, though where rows share pages a fork may want more than it gives up).  Free pages
+    are given in ascending order."""
     return _capi.ext().paged_fork(page_table, lengths, parents, refs, page_size, share)
 
 

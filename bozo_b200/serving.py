@@ -580,6 +580,7 @@ class BeamState(PagedState):
         scores, tokens, rows = beam.select(logits, self.scores, done=self.done, eos=self.eos)
         rows = rows.view(-1)
         for g, pools in self.pools.items():
+            # none is missing: both pools have a page for every entry of their table
             copies, _ = paged.fork(self.tables[g], self.lengths, rows, self.refs[g], self.page_size, share=g)
             paged.copy_pages(pools, copies)
         at = rows.long()

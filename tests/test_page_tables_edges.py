@@ -1,0 +1,50 @@
+"""Page tables at their edges: pages that a fork may lack."""
+import random
+
+import pytest
+
+from oracle import paged_oracle as orc
+from test_page_tables import check_fork
+
+gpu = pytest.mark.gpu
+
+# rows of 16 and 17 tokens on pages of 16, the first page shared, both to follow the second
+SHARED = ([[0, -1], [0, 1]], [16, 17], [1, 1], [2, 1], 16)
+
+
+def test_as_many_rows_may_want_a_page_more():
+    """The counterexample by hand: the shared page stays, so nothing is given up."""
+    table, refs, copies, missing = orc.fork(*SHARED, True)
+    assert missing == 1 and refs == [2, 1] and table == [[0, 1], [0, -1]] and copies == [(-1, -1)] * 2
+
+
+@gpu
+def test_fork_reports_the_page_that_sharing_lacks():
+    assert check_fork(*SHARED, True)[3] == 1
+    table, lengths, parents, refs, page = SHARED
+    assert check_fork(table, lengths, parents, refs + [0], page, True)[3] == 0
+
+
+@gpu
+@pytest.mark.parametrize("share", [True, False])
+def test_a_page_for_every_entry_is_enough(share):
+    """Generations of forks that multiply one row at its fullest, with no spare page."""
+    rng = random.Random(7)
+    B, M, page = 6, 4, 5
+    table, lengths = [[-1] * M for _ in range(B)], [-1] * B
+    refs = [0] * (B * M)
+    lengths[0] = 0
+    for gen in range(40):
+        tokens = [rng.randint(0, min(6, M * page - t)) if t >= 0 else 0 for t in lengths]
+        table, refs, _, missing, _ = orc.reserve(table, lengths, tokens, refs, page, 0)
+        assert missing == 0
+        lengths = [t + n if t >= 0 else t for t, n in zip(lengths, tokens)]
+        alive = [b for b in range(B) if lengths[b] >= 0]
+        parents = [rng.choice(alive[:1 + gen % len(alive)]) for _ in range(B)]
+        table, refs, _, missing = check_fork(table, lengths, parents, refs, page, share)
+        assert missing == 0
+        lengths = [lengths[x] for x in parents]
+        if all(t == M * page for t in lengths):                 # full: all but one go, and begin again
+            table, refs, _, _ = check_fork(table, lengths, [-1] * B, refs, page, share)
+            lengths = [0] + [-1] * (B - 1)
+            assert sum(refs) == 0
