@@ -3,7 +3,7 @@ state does not serve, failed calls, and what is held after its pages move."""
 import pytest
 import torch
 
-from bozo_b200 import serving
+from bozo_b200 import ops, paged, serving
 from test_beam_search import CFGS, ids, make, plain_matmuls  # noqa: F401 (the fixture)
 
 gpu = pytest.mark.gpu
@@ -104,3 +104,48 @@ def test_long_prompts_keep_their_last_ids(name, bounded, monkeypatch):
     prompts = [ids(n, n, vocab) for n in (limit + 9, keep, keep + 1, 5)]
     found = serving.beam_search(model, prompts, 2, steps, graph=False)
     assert taken == [[p[-keep:] for p in prompts]] and all(len(new) == steps for f in found for new, _ in f)
+
+
+def cached_rows(state, lengths):
+    """Each slot's cached rows as they are held, a list of (k, v) by layer and slot: the last ones
+    that the layer's pages reach."""
+    res = []
+    for li, lay in enumerate(state.layers):
+        table = state.table(li)
+        counts = [min(max(t, 0), table.shape[1] * state.page_size) for t in lengths]
+        cu = torch.tensor([0] + counts, device="cuda").cumsum(0).int()
+        start = torch.tensor([t - n if t >= 0 else -1 for t, n in zip(lengths, counts)], dtype=torch.int32, device="cuda")
+        k, v = paged.read_kv(lay.k, lay.v, table, start, cu, sum(counts), dtype=torch.float32, **lay.scales)
+        res.append(list(zip(k.split(counts), v.split(counts))))
+    return res
+
+
+@gpu
+@pytest.mark.parametrize("cache", [torch.bfloat16, torch.float8_e4m3fn, torch.int8, torch.float4_e2m1fn_x2])
+@pytest.mark.parametrize("page", [16, 8, 3])
+def test_every_hypothesis_holds_its_parents_rows(cache, page):
+    """What a hypothesis' pages hold after they were shared, moved and copied is what its parent's
+    held before, bit for bit, in every layer: codes, scales and group scales."""
+    model = make("rope_global", torch.bfloat16, sharp=2.0)
+    state = serving.BeamState(model, 2, 5, 23 + 40, page_size=page, cache_dtype=cache, graph=False)
+    choose, forks = state._choose, []
+
+    def watched(logits):
+        lengths = state.lengths.tolist()
+        before = cached_rows(state, lengths)
+        choose(logits)
+        parents = state.chosen[int(state.steps) - 1, 1].tolist()
+        lengths = [lengths[x] for x in parents]
+        assert state.lengths.tolist() == lengths
+        for li, (was, now) in enumerate(zip(before, cached_rows(state, lengths))):
+            for r, x in enumerate(parents):
+                for a, b in zip(was[x], now[r]):
+                    assert torch.equal(a.view(torch.int32), b.view(torch.int32)), (li, r, x)
+        forks.append(len(set(parents)) < len(parents))
+
+    state._choose = watched
+    state.start([ids(23, 1, 97), ids(2, 2, 97)])
+    for _ in range(40):
+        state.advance()
+    assert len(forks) == 41 and sum(forks) > 20
+    ops.poll_device_error("cuda")
