@@ -10,6 +10,8 @@
 // prefix sums, so nothing depends on an order of atomics.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "pool.cuh"
 
 namespace bozo {
@@ -389,11 +391,21 @@ __global__ void __launch_bounds__(kCopyThreads) paged_copy(const __grid_constant
   }
 }
 
-template <typename K, typename P, typename... A>
-cudaError_t launch_cluster(K kern, int blocks, size_t smem, cudaStream_t st, const P& p, A... a) {
+// Shared memory of the largest call (a fork's tile of one column): allowed once a device, never
+// a call's own size, which another thread's smaller call would take back before the launch.
+constexpr size_t kMostShared = (7 * (size_t)kMaxTableRows + 1) * sizeof(int);
+template <auto kern, typename P, typename... A>
+cudaError_t launch_cluster(int blocks, size_t smem, cudaStream_t st, const P& p, A... a) {
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
+      if (e != cudaSuccess) return e;
+      if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
@@ -428,7 +440,7 @@ cudaError_t launch_after(void (*kern)(P), dim3 grid, int threads, cudaStream_t s
 cudaError_t launch_paged_reserve(const ReserveP& p, cudaStream_t st, int* launches) {
   const int blocks = p.P <= kReservePool ? 1 : 8;
   const bool here = p.rows <= kPlacesHere;
-  cudaError_t e = launch_cluster(paged_reserve, blocks, (size_t)(4 * p.B + 2) * sizeof(int), st, p, here);
+  cudaError_t e = launch_cluster<paged_reserve>(blocks, (size_t)(4 * p.B + 2) * sizeof(int), st, p, here);
   *launches = here ? 1 : 2;
   if (e != cudaSuccess || here) return e;
   return launch_after(paged_places, dim3((unsigned)((p.rows + 4 * kPlaceThreads - 1) / (4 * kPlaceThreads))),
@@ -439,7 +451,7 @@ cudaError_t launch_paged_fork(const ForkP& p, cudaStream_t st) {
   // small tables: one block, whole; else a sector's worth of columns, fewer where the rows are many
   const bool small = p.P <= kForkPool && (long long)p.B * p.M <= kForkTable;
   const int tile = small ? p.M : p.B <= 2048 ? 8 : p.B <= 4096 ? 2 : 1;
-  return launch_cluster(paged_fork, small ? 1 : 8, ((size_t)6 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
+  return launch_cluster<paged_fork>(small ? 1 : 8, ((size_t)6 * p.B + 1 + (size_t)p.B * tile) * sizeof(int), st, p, tile,
                         make_fastdiv((unsigned)tile));
 }
 

@@ -1,8 +1,12 @@
-"""Page tables at their edges: pages that a fork may lack."""
+"""Page tables at their edges: pages that a fork may lack, calls of two threads at once."""
+import ctypes as C
 import random
+import threading
 
 import pytest
+import torch
 
+from bozo_b200 import _capi
 from oracle import paged_oracle as orc
 from test_page_tables import check_fork
 
@@ -48,3 +52,45 @@ def test_a_page_for_every_entry_is_enough(share):
             table, refs, _, _ = check_fork(table, lengths, [-1] * B, refs, page, share)
             lengths = [0] + [-1] * (B - 1)
             assert sum(refs) == 0
+
+
+def idle_call(name, B, M, P=20000, page=4):
+    """An argument block over idle rows, and what it points to."""
+    int32 = lambda *shape, value=-1: torch.full(shape, value, dtype=torch.int32, device="cuda")
+    t = {"table": int32(B, M), "lengths": int32(B), "refs": int32(P, value=0), "missing": int32(1)}
+    if name == "fork":
+        a = _capi.PagedForkArgs()
+        a.share, t["parents"], t["copies"] = 1, int32(B), int32(B, 2)
+    else:
+        a = _capi.PagedReserveArgs()
+        t["cu_rows"] = int32(B + 1)
+    a.batch, a.width, a.table_stride, a.page_size, a.pages = B, M, M, page, P
+    for field, x in t.items():
+        setattr(a, field, x.data_ptr())
+    return a, t
+
+
+@gpu
+@pytest.mark.parametrize("name", ["fork", "reserve"])
+def test_calls_of_several_sizes_from_two_threads(name):
+    """The C entries from two threads (which ctypes lets run), each with tables of its own that
+    want different amounts of shared memory: every call is launched."""
+    call = getattr(_capi.lib(), f"bozo_paged_{name}")
+    blocks = [idle_call(name, 8192, 2), idle_call(name, 1500 if name == "fork" else 4000, 8)]
+    status = [set(), set()]
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        for _ in range(3000):
+            status[i].add(call(C.byref(blocks[i][0]), stream.cuda_stream))
+        stream.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert status == [{0}, {0}]
+    for a, t in blocks:
+        assert int(t["missing"]) == 0 and (t["table"] == -1).all() and (t["refs"] == 0).all()
