@@ -71,15 +71,15 @@ __device__ __forceinline__ int find(const int* sums, int n, int x) {
 // The pool is shared out in order: a run of consecutive pages a warp, in words of 32 that
 // all its lanes read together.
 struct Run {
-  int from, to, words;
+  unsigned from, to, words;  // pages past 2^31 − 32 would pass an int's range in a loop's last step
   __device__ Run(int pages, unsigned rank, unsigned blocks) {
     const long long warps = (long long)blocks * (kThreads / 32), warp = (long long)rank * (kThreads / 32) + (threadIdx.x >> 5);
-    words = (int)((pages + warps * 32 - 1) / (warps * 32));
-    from = (int)min((long long)pages, warp * words * 32);
-    to = (int)min((long long)pages, from + (long long)words * 32);
+    words = (unsigned)((pages + warps * 32 - 1) / (warps * 32));
+    from = (unsigned)min((long long)pages, warp * words * 32);
+    to = (unsigned)min((long long)pages, from + (long long)words * 32);
   }
-  __device__ unsigned word(const int* refs, int p) const {
-    const int lane = threadIdx.x & 31;
+  __device__ unsigned word(const int* refs, unsigned p) const {
+    const unsigned lane = threadIdx.x & 31;
     return __ballot_sync(0xffffffffu, p + lane < to && refs[p + lane] == 0);
   }
   // the warp's free pages; `mask`: which of word `lane` are
@@ -87,7 +87,7 @@ struct Run {
     int n = 0, i = 0;
     mask = 0;
 #pragma unroll 8
-    for (int p = from; p < to; p += 32, ++i) {
+    for (unsigned p = from; p < to; p += 32, ++i) {
       const unsigned b = word(refs, p);
       n += __popc(b);
       if (i == (int)(threadIdx.x & 31)) mask = b;
@@ -99,10 +99,11 @@ struct Run {
   __device__ void give(const int* refs, unsigned mask, int n, int before, int want, F f) const {
     const int lane = threadIdx.x & 31;
     if (n == 0) return;
-    for (int p = from, i = 0; p < to && before < want; p += 32, ++i) {
+    int i = 0;
+    for (unsigned p = from; p < to && before < want; p += 32, ++i) {
       const unsigned b = i < 32 ? __shfl_sync(0xffffffffu, mask, i) : word(refs, p);
       const int rank = before + __popc(b & ((1u << lane) - 1u));
-      if (b >> lane & 1 && rank < want) f(rank, p + lane);
+      if (b >> lane & 1 && rank < want) f(rank, (int)(p + lane));
       before += __popc(b);
     }
   }
@@ -283,11 +284,12 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
   const int rank = (int)cl.block_rank(), blocks = (int)cl.num_blocks();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the copies' kernel, which waits for this one
   // the old entries of columns c0 …: thread i has every kThreads-th of a tile's B · tile
-  auto load = [&](int c0) {
+  auto load = [&](unsigned c0) {
 #pragma unroll 4
     for (int i = threadIdx.x; i < p.B * tile; i += kThreads) {
-      const int r = (int)fast_div((unsigned)i, div_tile), c = c0 + i - r * tile;
-      old[i] = c < p.M ? __ldcg(p.table + r * p.ts + c) : -1;
+      const int r = (int)fast_div((unsigned)i, div_tile);
+      const unsigned c = c0 + (unsigned)(i - r * tile);
+      old[i] = c < (unsigned)p.M ? __ldcg(p.table + r * p.ts + c) : -1;
     }
   };
   const int x0 = (int)threadIdx.x < p.B ? p.parents[threadIdx.x] : 0, t0 = (int)threadIdx.x < p.B ? p.lengths[threadIdx.x] : 0;
@@ -329,16 +331,17 @@ __global__ void __launch_bounds__(kThreads) paged_fork(ForkP p, int tile, FastDi
   const int want = (int)carry;
   if (threadIdx.x == 0) off[p.B] = want;
   // whole columns at a time: their old entries are read before any is written
-  for (int c0 = rank * tile; c0 < p.M; c0 += blocks * tile) {
-    if (c0 != rank * tile) {
+  for (unsigned c0 = (unsigned)(rank * tile); c0 < (unsigned)p.M; c0 += (unsigned)(blocks * tile)) {
+    if (c0 != (unsigned)(rank * tile)) {
       __syncthreads();
       load(c0);
       __syncthreads();
     }
 #pragma unroll 4
     for (int i = threadIdx.x; i < p.B * tile; i += kThreads) {
-      const int r = (int)fast_div((unsigned)i, div_tile), j = i - r * tile, c = c0 + j, x = parent[r];
-      if (c >= p.M) continue;
+      const int r = (int)fast_div((unsigned)i, div_tile), j = i - r * tile, x = parent[r];
+      if (c0 + (unsigned)j >= (unsigned)p.M) continue;
+      const int c = (int)(c0 + (unsigned)j);
       p.table[r * p.ts + c] = x >= 0 && (eldest[x] == r || c < full[x]) ? old[x * tile + j] : -1;
       // what the old row gives up, or its further children take
       const int was = old[i], n = children[r], d = (c < full[r] ? n : min(n, 1)) - 1;

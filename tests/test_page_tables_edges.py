@@ -6,9 +6,9 @@ import threading
 import pytest
 import torch
 
-from bozo_b200 import _capi
+from bozo_b200 import _capi, paged
 from oracle import paged_oracle as orc
-from test_page_tables import check_fork
+from test_page_tables import check_fork, int32
 
 gpu = pytest.mark.gpu
 
@@ -94,3 +94,25 @@ def test_calls_of_several_sizes_from_two_threads(name):
     assert status == [{0}, {0}]
     for a, t in blocks:
         assert int(t["missing"]) == 0 and (t["table"] == -1).all() and (t["refs"] == 0).all()
+
+
+@gpu
+def test_the_last_pages_that_31_bits_number():
+    """A pool of 2^31 − 1 pages, all taken but three of its last: its last word of 32 pages ends
+    where an int does."""
+    P = 2 ** 31 - 1
+    try:
+        refs = torch.ones(P, dtype=torch.int32, device="cuda")
+    except torch.cuda.OutOfMemoryError:
+        pytest.skip("needs 9 GB of free device memory")
+    refs[[-40, -7, -1]] = 0
+    table = int32([[5, -1, -1], [-1, -1, -1]])
+    plan = paged.reserve(table, int32([1, -1]), int32([2, 0]), refs, 1, rows=3)
+    assert table.tolist() == [[5, P - 40, P - 7], [-1] * 3] and plan.missing.item() == 0
+    assert plan.slot.tolist() == [P - 40, P - 7, -1]
+    plan = paged.reserve(table, int32([3, 0]), int32([0, 2]), refs, 1)
+    assert plan.missing.item() == 1 and table[1].tolist() == [-1] * 3      # one is left
+    copies, missing = paged.fork(table, int32([3, -1]), int32([0, 0]), refs, 1, share=False)
+    assert missing.item() == 2 and table.tolist() == [[5, P - 40, P - 7], [P - 1, -1, -1]]
+    assert copies.tolist() == [[-1, -1]] * 3 + [[5, P - 1], [-1, -1], [-1, -1]]
+    assert refs[-40:].sum().item() == 40
