@@ -135,10 +135,10 @@ __device__ __forceinline__ void sync_all() {
 
 // Where row i of the packed new tokens goes: sequence b, which has the rows [first, next).
 __device__ __forceinline__ void place(const ReserveP& p, int i, int b, int len, int first, int next, int& at, int& slot) {
-  const long long t = len, pos = t + (i - first);
-  at = (int)pos;
+  const long long t = len, pos = t + (i - first), end = min(t + (next - first), 1LL << 31);
+  at = pos < end ? (int)pos : -1;  // positions end at 2^31 − 1
   slot = -1;
-  if (pos < t + (next - first) - (long long)p.cap || pos > 0x7fffffffLL) return;
+  if (pos < end - (long long)p.cap || pos >= end) return;
   const unsigned s = (unsigned)pos - fast_div((unsigned)pos, p.div_cap) * p.cap, j = fast_div(s, p.div_page);
   const int page = __ldcg(p.table + b * p.ts + j);
   if ((unsigned)page < (unsigned)p.P) slot = page * p.page + (int)(s - j * p.page);
@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(kThreads) paged_reserve(ReserveP p, bool place
         atomicCAS(p.err, 0, kErrPaged | 1);
         n = 0;
       }
+      if (n && (unsigned)t + (unsigned)n > 0x80000000u) atomicCAS(p.err, 0, kErrPaged | 1);
       if (n) {
         have = pages_of(p, t);
         const int need = pages_of(p, (unsigned)t + (unsigned)n);

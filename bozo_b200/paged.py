@@ -159,7 +159,8 @@ def reserve(page_table: Tensor, lengths: Tensor, tokens: Optional[Tensor], refs:
                  updated in place.
     rows       : also say where the first ``rows`` packed new tokens go (``seq``, ``pos``,
                  ``slot``; −1 behind the last).  A token whose place a later one of this
-                 call takes (a ring) has slot −1.
+                 call takes (a ring) has slot −1, one past position 2^31 − 1 has neither
+                 (and is reported as an index error).
 
     Columns from ⌈lengths / page_size⌉ on are filled from the first empty one, up to
     ⌈(lengths + tokens) / page_size⌉ and M, so pages reserved before are kept.  Free

@@ -338,7 +338,8 @@ int bozo_paged_decode(const bozo_paged_decode_args* args, void* stream);
  * cu_rows[b] ≤ n < cu_rows[b+1], is token pos[n] = lengths[b] + n − cu_rows[b] of
  * sequence seq[n] = b, at slot[n] = page · page_size + pos mod page_size of its table's
  * page, or −1 where there is none or a later token of the same call takes its place;
- * all three are −1 for rows from cu_rows[batch] on. */
+ * pos and slot are −1 past position 2^31 − 1 (BOZO_ERR_DEVICE_INDEX), and all three
+ * for rows from cu_rows[batch] on. */
 typedef struct {
   int32_t* table;         /* [batch, width], rows table_stride apart; updated */
   int64_t table_stride;

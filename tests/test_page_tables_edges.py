@@ -6,7 +6,7 @@ import threading
 import pytest
 import torch
 
-from bozo_b200 import _capi, paged
+from bozo_b200 import _capi, ops, paged
 from oracle import paged_oracle as orc
 from test_page_tables import check_fork, int32
 
@@ -116,3 +116,23 @@ def test_the_last_pages_that_31_bits_number():
     assert missing.item() == 2 and table.tolist() == [[5, P - 40, P - 7], [P - 1, -1, -1]]
     assert copies.tolist() == [[-1, -1]] * 3 + [[5, P - 1], [-1, -1], [-1, -1]]
     assert refs[-40:].sum().item() == 40
+
+
+@gpu
+@pytest.mark.parametrize("rows", [9, 5000])      # places by the first kernel, and by their own
+def test_positions_end_at_31_bits(rows):
+    """Tokens behind the last position that an int holds have none (they had negative ones)."""
+    last = 2 ** 31 - 1
+    table, refs = int32([[3, 1], [0, 2], [-1, -1]]), int32([1, 1, 1, 1])
+    ops.poll_device_error("cuda")
+    plan = paged.reserve(table, int32([last - 2, last - 1, 0]), int32([3, 2, 0]), refs, 16, rows=rows)
+    ops.poll_device_error("cuda")                  # the last position is one
+    slots = [1 * 16 + 13, 1 * 16 + 14, 1 * 16 + 15, 2 * 16 + 14, 2 * 16 + 15]   # 2^31 − 1 = 31 mod 32
+    assert plan.pos[:5].tolist() == [last - 2, last - 1, last, last - 1, last] and plan.slot[:5].tolist() == slots
+    plan = paged.reserve(table, int32([last - 2, last, -1]), int32([5, 1, 3]), refs, 16, rows=rows)
+    with pytest.raises(RuntimeError, match="outside"):
+        ops.poll_device_error("cuda")
+    assert plan.cu_rows.tolist() == [0, 5, 6, 6] and plan.seq[:7].tolist() == [0] * 5 + [1, -1]
+    assert plan.pos[:7].tolist() == [last - 2, last - 1, last, -1, -1, last, -1]
+    assert plan.slot[:7].tolist() == [29, 30, 31, -1, -1, 47, -1]
+    assert (plan.pos[7:] == -1).all() and plan.missing.item() == 0 and table.tolist() == [[3, 1], [0, 2], [-1, -1]]
