@@ -36,5 +36,5 @@ def select(logits: Tensor, scores: Tensor, *, done: Optional[Tensor] = None,
 
     Returns ``scores [N, K]`` (float32, best first), ``tokens [N, K]`` (int64) and
     ``rows [N, K]`` (int32): the row of ``logits`` that each continues.  K up to 32, V
-    from K to 2^20.  No gradients."""
+    from K to 2^20, N · K up to 65535.  No gradients."""
     return _capi.ext().beam_select(logits, scores, done, -1 if eos is None else int(eos))

@@ -473,6 +473,8 @@ class BeamState(PagedState):
         cfg = model.cfg
         if prompts < 1 or not 1 <= beams <= 32 or beams > cfg.vocab_size:
             raise ValueError("beam search takes at least one prompt and 1 to 32 beams, no more than tokens")
+        if prompts * beams > 8192:
+            raise ValueError(f"beam search holds up to 8192 hypotheses, not {prompts} prompts of {beams}")
         if eos is not None and not 0 <= eos < cfg.vocab_size:
             raise ValueError(f"eos must be a token, got {eos}")
         if any(b.global_layer for b in model.blocks) and max_len > cfg.max_seq_len:

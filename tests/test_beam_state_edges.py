@@ -83,6 +83,15 @@ def test_a_state_without_prompts_has_nothing_to_say(graph, monkeypatch):
 
 
 @gpu
+def test_more_hypotheses_than_a_table_has_rows_are_refused():
+    """Before anything is held: the table's kernels refused it, in the middle of start()."""
+    model = make("all_global")
+    for prompts, beams in ((8193, 1), (2049, 4), (257, 32)):
+        with pytest.raises(ValueError, match="8192"):
+            serving.BeamState(model, prompts, beams, 8, graph=False)
+
+
+@gpu
 def test_search_refuses_batches_of_nothing():
     model = make("all_global")
     for batch in (0, -1, -16):                     # −1 returned no result for any prompt
