@@ -29,7 +29,7 @@ def select(logits: Tensor, scores: Tensor, *, done: Optional[Tensor] = None,
     A continuation is worth score + logit − log Σ exp(logits), added up and compared in 64
     bits; of equal ones the lower hypothesis comes first, of one hypothesis the higher logit,
     then the lower token.  The exponentials are summed from 32-bit ones: log Σ exp is off by
-    a few 1e-7, and by (55 + 2.3 ln V) · 2^-24 at most, so continuations of two hypotheses
+    a few 1e-7, and by (79 + 2.3 ln V) · 2^-24 at most, so continuations of two hypotheses
     closer than that may come in either order.  A masked token (logit −∞), and every token of a row with a NaN or
     +∞, of a row of −∞ only, or of a hypothesis whose score is not finite, is worth −∞:
     those come last, lowest token first.

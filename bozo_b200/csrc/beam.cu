@@ -12,7 +12,7 @@
 //   * every block's K best keys and sum go to the first block's shared memory, which
 //     finds the prompt's best among them in 64 bits.
 // Bound by the logits' bytes where rows are many, by the chain of these steps where
-// they are few: 64 prompts × 8 hypotheses × 32768 tokens in bf16 14.4 µs in a graph (29.4
+// they are few: 64 prompts × 8 hypotheses × 32768 tokens in bf16 14.3 µs in a graph (29.4
 // MB without the ended ones, 4.5 µs; the loop over them 6), 1 × 4 × 8192 in fp32 5.3.  Rows
 // that are not all aligned to 16 bytes take a kernel of their own, 20.0 µs for the former
 // with 32767 tokens (as branches of one kernel they cost aligned rows 1.2 µs).
@@ -218,30 +218,33 @@ __device__ __forceinline__ void for_ranks(int n, B is_before, P put) {
   }
 }
 
-// What a sum relative to m is worth relative to a larger `to`: few batches need it, and inside
-// the loop its registers are spilled (32 × 8 rows of 50257 that are not aligned 18.8 µs, 21.4).
-__device__ __noinline__ double raised(double s, float m, float to) { return s * exp((double)m - (double)to); }
-
-// A thread's pieces into its largest logit m and s = Σ exp(x − m): 32 bits for a batch, 64
-// beyond, so that the error does not grow with the row, nor with how often m rises (128 rows
-// of 2^20 fp32 logits: 2e-7, in 32 bits throughout 1.5e-5; 145 µs for 134).  In all log Σ exp
-// is off by (55 + 2.3 ln V) · 2^-24 at most: exponentials of 2^-22, a batch's additions, and
-// those of warps, blocks and parts.
+// A thread's largest logit m, and s + rest = Σ exp(x − ref): what adding a batch to s leaves over
+// is kept, so that the error does not grow with the row (128 rows of 2^20 fp32 logits: 2e-7,
+// without it 1.5e-5; 64 × 8 × 32768 in bf16 14.7 µs for 14.4, with doubles 15.1).  The
+// reference follows m in steps of kStep or more: what is rescaled, to 2^-22, is then at most
+// exp(−kStep) of itself, and however often m rises that adds up to 4.5 · 2^-22.  In all
+// log Σ exp is off by (79 + 2.3 ln V) · 2^-24 at most: exponentials of 2^-22, a batch's
+// additions, and those of warps, blocks and parts.
+constexpr float kStep = 0.25f;
+struct Sum {
+  float m = -INFINITY, ref = -INFINITY, s = 0.f, rest = 0.f;
+};
 template <int DT, int U>
-__device__ __forceinline__ void take(const Vec<DT>* v, float& m, double& s) {
+__device__ __forceinline__ void take(const Vec<DT>* v, Sum& t) {
   constexpr int N = Vec<DT>::N;
-  float to = m;
 #pragma unroll
-  for (int j = 0; j < U; ++j) to = fmaxf(to, v[j].most());
-  const float ref = finite_or_0(to);
+  for (int j = 0; j < U; ++j) t.m = fmaxf(t.m, v[j].most());
+  const float to = t.m >= t.ref + kStep ? t.m : t.ref, ref = finite_or_0(to);
   float a[2] = {0.f, 0.f}, b[2] = {0.f, 0.f};
 #pragma unroll
   for (int j = 0; j < U; ++j)
 #pragma unroll
     for (int i = 0; i < N; i += 2) add_pow2(a[i / 2 % 2], b[i / 2 % 2], v[j].at(i), v[j].at(i + 1), ref);
-  if (to > m && m > -INFINITY) s = raised(s, m, to);
-  s += (double)((a[0] + a[1]) + (b[0] + b[1]));
-  m = to;
+  const float f = rescale(t.ref, to), s = t.s * f, x = (a[0] + a[1]) + (b[0] + b[1]);
+  t.s = __fadd_rn(s, x);
+  const float y = __fsub_rn(t.s, s);  // of x; the rest of it and of s (Knuth's sum of two)
+  t.rest = t.rest * f + (__fsub_rn(s, __fsub_rn(t.s, y)) + __fsub_rn(x, y));
+  t.ref = to;
 }
 
 // A thread's batch of pieces q, q + kThreads, … below q1: whole pieces are nothing but loads,
@@ -280,24 +283,24 @@ __device__ __forceinline__ void scan(const Row<DT, AL>& row, int q0, int q1, int
                                      float& M, float& S, double& lse) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   constexpr int kWarps = kThreads / 32, N = Vec<DT>::N;
-  float m = -INFINITY;
-  double sum = 0.;
+  Sum sum;
   if (q1 - q0 <= kBatch / 2 * kThreads) {
-    take<DT, kBatch / 2>(v, m, sum);
+    take<DT, kBatch / 2>(v, sum);
   } else {
     for (int q = q0 + tid;;) {
-      take<DT, kBatch>(v, m, sum);
+      take<DT, kBatch>(v, sum);
       q += kBatch * kThreads;
       if (q >= q1) break;
       batch<DT, kThreads>(row, q, q1, v);
     }
   }
+  const float m = sum.m;
   float g = m;
 #pragma unroll
   for (int o = 1; o < kThreads / kGroups; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
   const float wm = warp_most(m);
   if (tid % (kThreads / kGroups) == 0) sc.top[tid / (kThreads / kGroups)] = g;
-  const float s = warp_sum((float)sum * rescale(m, wm));
+  const float s = warp_sum((sum.s + sum.rest) * rescale(sum.ref, wm));
   if (lane == 0) {
     sc.wm[warp] = wm;
     sc.ws[warp] = s;

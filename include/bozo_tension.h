@@ -403,7 +403,7 @@ int bozo_paged_copy(const bozo_paged_copy_args* args, void* stream);
  * has row n·beams + k of `logits`; continuing it with token v is worth
  * scores[n][k] + logits[v] − log Σ exp(logits), added up and compared in 64 bits; the
  * exponentials are summed from 32-bit ones, so that log Σ exp is off by a few 1e-7, and by
- * (55 + 2.3 ln vocab) · 2^-24 at most, and continuations of two hypotheses closer than that
+ * (79 + 2.3 ln vocab) · 2^-24 at most, and continuations of two hypotheses closer than that
  * may come in either order.  A hypothesis
  * that has ended (done) goes on as itself only: token eos, its score unchanged.
  * Higher values come first; of equal ones the lower hypothesis, of one hypothesis the

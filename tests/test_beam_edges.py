@@ -17,11 +17,13 @@ def seeded():
 
 def log_error(V):
     """Bound of log Σ exp's error.  In units of 2^-24 of the sum: 4 for the exponential of a term
-    (2^-22); (x − m)·log2 e rounded three times, 2.3 · (m − x), which over the sum's terms is at
-    most 2.3 ln V on average (their entropy is); 18 additions of a batch; 1 for the thread's sum
-    in 32 bits (it is held in 64); thread to warp, warp to block and part to row an exponential
-    and a product each, 15; their 5 + 5 + 7 additions.  The logarithm itself 1.4e-9."""
-    return (4 + 18 + 1 + 15 + 17 + 2.3 * math.log(V)) * 2.0 ** -24 + 1.4e-9
+    (2^-22); (x − ref)·log2 e rounded three times, 2.3 · (m − x), which over the sum's terms is at
+    most 2.3 (ln V + ¼) on average (their entropy is); 18 additions of a batch; the thread's
+    sum keeps what its additions leave over, but where its reference rises, by ¼ or more, it is
+    multiplied by an exponential, 5, of which a row of rises adds 1 / (1 − e^-¼) = 4.5; 1 for the
+    two parts' sum; thread to warp, warp to block and part to row an exponential and a product
+    each, 15; their 5 + 5 + 7 additions.  The logarithm itself 1.4e-9."""
+    return (4 + 18 + 22.5 + 1 + 15 + 17 + 2.3 * (math.log(V) + 0.25)) * 2.0 ** -24 + 1.4e-9
 
 
 def check(logits, scores):
