@@ -291,13 +291,14 @@ int head_groups(const PagedP& p) {
 
 // Pieces of a row.  About three blocks an SM keep the memory busy (16 rows of
 // 120002 keys: 76.4 µs at 18 pieces, 75.3 at 24, 75.9 at 28, 78.5 at 37; four of 4-bit
-// pages, 46.1 µs at 27, 43.9 at 37, 50 at 92).  Sequences
+// pages, 42.9 µs at 18, 38.2 at 27, 37.3 at 37, 37.7 at 46, 44.2 at 92).  Sequences
 // of different lengths want smaller pieces to even out — twelve an SM, of 2048 keys
 // at least (1024 rows of up to 8192 keys: 164 µs in two to four; 512 rows of up to
 // 16384 keys in e4m3: 199 µs in three, 192 in four, 190 in six, 195 in eight).  4-bit
 // pages' blocks take the longest sequences first, which evens them out by itself: six an
-// SM (1024 rows of up to 8192 keys 80 µs in one piece, 88 in two; 512 rows of up to 16384
-// with four heads 135 in two, 141 in four, 228 in one).
+// SM (two draws of lengths: 1024 rows of up to 8192 keys 81 and 75 µs in one piece or two,
+// 88 and 82 in three; 512 rows of up to 16384, 128 wide with four heads, 184 and 141 in two,
+// 169 and 152 in four, 264 in one; 64 wide 120 and 93 in two, 114 and 104 in four).
 // Up to eight pieces are joined inside a cluster, which saves a second kernel's
 // 2-3 µs of a call, where the clusters all find their place at once (12 rows of 1024
 // keys in eight: 5.9 µs and 8.2 a call, 6.1 and 10.1 with a second kernel; 192 rows of up

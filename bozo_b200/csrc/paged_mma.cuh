@@ -43,9 +43,9 @@
 // keys 75.6 µs (0.99); e4m3, 128 wide, four heads a key head: 189 µs for 1106 MB
 // (0.89).  Tiles of 8 KB and half the blocks: 193 µs for the first.  4-bit rows: 180
 // instructions for 16 keys of 1.3 KB, many of them conversions and selections that run at
-// half rate, bound them (a head each, 64 ragged sequences × 16 heads: 79 µs for 337 MB, 0.65
-// of a copy; 66 with no page read at all; with scaled codes 83).  128 wide, four heads: 179
-// µs for 658 MB.
+// half rate, bound them (a head each, 64 ragged sequences × 16 heads: 77 µs for 337 MB, 0.67
+// of a copy; before the last steps 79, then 66 with no page read at all, 83 with scaled codes;
+// 91 where the new rows are written).  128 wide, four heads: 178 µs for 658 MB.
 #pragma once
 
 #include <limits.h>
@@ -224,7 +224,9 @@ __device__ __forceinline__ float ld_peer(unsigned addr, unsigned rank) {
 
 constexpr int kWarps = 4;
 // Windows up to here take tiles of 32 4-bit rows, for more of the warps (16 sequences × 12
-// heads, 64 keys: 4.6 µs a call, with 64 rows 5.3; 128 keys 5.5 and 5.3, 256 keys 6.4 and 7.0).
+// heads that write their new rows, as a model's step does, in a graph: 64 keys 6.3 µs, with
+// tiles of 64 rows 7.1; 128 keys 6.8 and 7.2, 256 8.1 and 8.8, 512 9.8 and 9.7; without new rows
+// 4.8 and 5.6, 5.7 and 5.5, 6.6 and 7.3, 8.7 and 8.3).
 constexpr int kShortWindow = 256;
 
 
