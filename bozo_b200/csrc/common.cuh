@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "bozo_block_ops.h"
 #include "bozo_graph_bias.h"
 #include "bozo_tau_aux.h"
@@ -192,6 +194,23 @@ inline FastDiv make_fastdiv(uint32_t d) {
 __device__ __forceinline__ uint32_t fast_div(uint32_t n, FastDiv f) {
   const uint32_t t = __umulhi(f.m, n);
   return (t + ((n - t) >> f.s1)) >> f.s2;
+}
+
+// Lets a kernel have all the dynamic shared memory that a block may, once a device: a call's
+// own amount would be taken back by another thread's smaller call before the launch.
+template <auto kern>
+cudaError_t allow_shared() {
+  static std::atomic<unsigned long long> allowed{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && (allowed.load(std::memory_order_relaxed) >> dev & 1)) return cudaSuccess;
+  cudaFuncAttributes a{};
+  e = cudaFuncGetAttributes(&a, kern);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)a.sharedSizeBytes);
+  if (e == cudaSuccess && dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return e;
 }
 
 struct AuxShape {

@@ -330,25 +330,30 @@ __global__ void __launch_bounds__(kW * 32) decode_kernel_vec(DecodeP p) {
   }
 }
 
-template <typename E>
+template <auto kern>
+cudaError_t launch_kernel(const DecodeP& p, int threads, size_t smem, cudaStream_t st) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = allow_shared<kern>();
+    if (e != cudaSuccess) return e;
+  }
+  kern<<<p.B * p.H, threads, smem, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename E, int HD>
 cudaError_t launch_vec(const DecodeP& p, size_t smem, cudaStream_t st) {
   // a long cache (global layers, wide windows) gets 32 warps per (b, h):
   // four times the loads in flight per step of its short dependent chain
   const bool wide = (p.mode == BOZO_MODE_GLOBAL ? p.C : p.W) > 256;
-  const int threads = (wide ? kWideWarps : kFastWarps) * 32;
-  auto go = [&](auto kern) {
-    if (smem > 48 * 1024) {
-      cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-      if (e != cudaSuccess) return e;
-    }
-    kern<<<p.B * p.H, threads, smem, st>>>(p);
-    return cudaGetLastError();
-  };
+  return wide ? launch_kernel<decode_kernel_vec<E, HD, kWideWarps>>(p, kWideWarps * 32, smem, st)
+              : launch_kernel<decode_kernel_vec<E, HD, kFastWarps>>(p, kFastWarps * 32, smem, st);
+}
+template <typename E>
+cudaError_t launch_vec(const DecodeP& p, size_t smem, cudaStream_t st) {
   switch (p.HD) {
-    case 32: return wide ? go(decode_kernel_vec<E, 32, kWideWarps>) : go(decode_kernel_vec<E, 32, kFastWarps>);
-    case 64: return wide ? go(decode_kernel_vec<E, 64, kWideWarps>) : go(decode_kernel_vec<E, 64, kFastWarps>);
-    default:
-      return wide ? go(decode_kernel_vec<E, 128, kWideWarps>) : go(decode_kernel_vec<E, 128, kFastWarps>);
+    case 32: return launch_vec<E, 32>(p, smem, st);
+    case 64: return launch_vec<E, 64>(p, smem, st);
+    default: return launch_vec<E, 128>(p, smem, st);
   }
 }
 
@@ -376,13 +381,7 @@ cudaError_t launch_decode(const DecodeP& p, cudaStream_t st) {
       default: return launch_vec<__half>(p, smem, st);
     }
   }
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  decode_kernel<<<p.B * p.H, kDecThreads, smem, st>>>(p);
-  return cudaGetLastError();
+  return launch_kernel<decode_kernel>(p, kDecThreads, smem, st);
 }
 
 }  // namespace bozo

@@ -10,8 +10,6 @@
 // prefix sums, so nothing depends on an order of atomics.
 #include <cooperative_groups.h>
 
-#include <atomic>
-
 #include "pool.cuh"
 
 namespace bozo {
@@ -395,21 +393,11 @@ __global__ void __launch_bounds__(kCopyThreads) paged_copy(const __grid_constant
   }
 }
 
-// Shared memory of the largest call (a fork's tile of one column): allowed once a device, never
-// a call's own size, which another thread's smaller call would take back before the launch.
-constexpr size_t kMostShared = (7 * (size_t)kMaxTableRows + 1) * sizeof(int);
 template <auto kern, typename P, typename... A>
 cudaError_t launch_cluster(int blocks, size_t smem, cudaStream_t st, const P& p, A... a) {
   if (smem > 48 * 1024) {
-    static std::atomic<unsigned long long> allowed{0};  // devices where the kernel may use that much
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
+    const cudaError_t e = allow_shared<kern>();
     if (e != cudaSuccess) return e;
-    if (dev >= 64 || !(allowed.load(std::memory_order_relaxed) >> dev & 1)) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostShared);
-      if (e != cudaSuccess) return e;
-      if (dev < 64) allowed.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);

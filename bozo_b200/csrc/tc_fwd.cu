@@ -622,8 +622,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <bool kBias, bool kTau, int kNKV, bool kF32>
 cudaError_t launch_variant(const CUtensorMap* m, const FwdTC& a, size_t smem, int grid,
                            cudaStream_t st) {
-  auto kern = tc_fwd_kernel<kBias, kTau, kNKV, kF32>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  constexpr auto kern = tc_fwd_kernel<kBias, kTau, kNKV, kF32>;
+  const cudaError_t e = allow_shared<kern>();
   if (e != cudaSuccess) return e;
   kern<<<grid, kThreads, smem, st>>>(m[0], m[1], m[2], m[3], m[4], m[5], a);
   return cudaGetLastError();

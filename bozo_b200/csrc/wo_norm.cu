@@ -344,7 +344,7 @@ cudaError_t launch_wo_norm(const bozo_wo_add_rmsnorm_args& a, int* err, cudaStre
     return cudaErrorInvalidValue;
   const size_t smem = (size_t)p.stages * stage_bytes(p.Nc) + tile_bytes(p.Nc, esz) + fixed_bytes();
   auto kern = bf ? wo_norm_kernel<true> : wo_norm_kernel<false>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaError_t e = bf ? allow_shared<wo_norm_kernel<true>>() : allow_shared<wo_norm_kernel<false>>();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(p.CN, (unsigned)((p.M + kRows - 1) / kRows), 1);
